@@ -180,6 +180,162 @@ int jal_op_gqa_attention(const float *q, const float *k, const float *v,
                          void *stream);
 
 /* ========================================================================
+ * Paged batch operators (no counterpart in the reference)
+ *
+ * What a server runs around the projections when it serves a ragged batch
+ * from one paged cache: new keys and values rotated and appended, attention
+ * over the pages, attention with a prefix that sequences share, beam search's
+ * selection and the reordering of its page tables.  All pointers are device
+ * pointers of the current device (JAL_ERR_INVALID_ARGUMENT otherwise),
+ * everything is enqueued on `stream`, nothing is allocated and nothing
+ * synchronises, so every call can be captured in a graph.  A workspace belongs
+ * to the caller: it needs no initial content, holds nothing between calls, and
+ * must not be used by two calls whose GPU work can overlap.
+ *
+ * Lengths and tables are read on the device.  Values that contradict each
+ * other there are not reported, but nothing is read or written outside the
+ * pools, the tables and the rows that the arguments describe.
+ * ====================================================================== */
+
+/* A paged cache: element (page, kv head, slot, dim) of a pool lies at
+ * page * page_stride + head * head_stride + slot * slot_stride + dim.
+ * Position t of sequence s is slot t % page_size of page
+ * page_table[s * max_pages + t / page_size].  An entry outside [0, n_pages)
+ * means "no page": nothing is appended there and its keys count as masked
+ * (pages behind a window may be given back). */
+typedef struct jal_paged_kv {
+  void *k, *v;               /* pools, 16-byte aligned */
+  const int32_t *page_table; /* [n_seqs][max_pages] */
+  uint64_t n_pages, page_size, n_heads_kv;
+  uint64_t head_dim; /* multiple of 8, at most 256 */
+  uint64_t n_seqs, max_pages; /* max_pages * page_size < 2^31 - 2^16 */
+  /* elements, multiples of 8; all three 0 = [page][kv_head][slot][head_dim],
+   * a layer of jal_kv_cache */
+  uint64_t page_stride, head_stride, slot_stride;
+  int32_t dtype; /* JAL_F32, JAL_F16 or JAL_BF16 */
+} jal_paged_kv;
+
+/* The new rows of a batch: sequence s has token rows [q_start[s],
+ * q_start[s + 1]) (ascending), the last of them at position kv_len[s] - 1 and
+ * the others at the positions before.  A sequence may have no row.  Rows
+ * before q_start[0] and from q_start[n_seqs] on belong to none and are left
+ * as they were, as are a sequence's rows past the first max_q_len. */
+typedef struct jal_ragged_batch {
+  const int32_t *q_start; /* [n_seqs + 1] */
+  const int32_t *kv_len;  /* [n_seqs], the new rows included */
+  uint64_t n_seqs;        /* at most the cache's */
+  uint64_t n_rows;        /* rows of the row buffers */
+  uint64_t max_q_len;     /* no sequence has more new rows */
+  uint64_t max_kv_len;    /* about the largest kv_len: how the work is cut up
+                             follows from it, results do not depend on it */
+} jal_ragged_batch;
+
+/* Sequences that share a prefix: group g is the sequences [group_start[g],
+ * group_start[g + 1]) (ascending), whose first prefix_len[g] positions are
+ * the same; they are read through the page-table row of its first sequence.
+ * A sequence outside every group has its own keys alone. */
+typedef struct jal_prefix_groups {
+  const int32_t *group_start; /* [n_groups + 1] */
+  const int32_t *prefix_len;  /* [n_groups] */
+  uint64_t n_groups;
+  uint64_t max_group;      /* no group has more sequences */
+  uint64_t max_prefix_len; /* no prefix is longer; 0 = there is none */
+} jal_prefix_groups;
+
+/* Rotates and appends: for every token row of the batch, K[position] =
+ * rotate(k row), V[position] = v row and, where q is given, q_out row =
+ * rotate(q row).  k and v rows are [n_heads_kv][head_dim] of `dtype`, kv_stride
+ * elements apart; q rows [n_heads_q][head_dim], q_stride / q_out_stride
+ * elements apart (0 = dense; slices of one fused projection row are strided);
+ * q_out may be q.  dtype is the cache's or JAL_F32.  The first rotary_dim
+ * dims are rotated (0 = none, iRoPE layers): neox = 0 pairs (2i, 2i + 1), 1
+ * pairs (i, i + rotary_dim / 2), by position * inv_freq[i] (device,
+ * rotary_dim / 2 floats).  That angle is formed in 64 bits; jal_op_rope and
+ * the contexts round it to f32 as the reference does, which differs at far
+ * positions.  A position of a sequence occurs once in a batch by
+ * construction; two sequences must not append to the same slot. */
+int jal_op_rope_kv_append(const jal_paged_kv *kv, const jal_ragged_batch *batch,
+                          int dtype, const void *k, const void *v,
+                          size_t kv_stride, const float *inv_freq,
+                          size_t rotary_dim, int neox, const void *q,
+                          void *q_out, size_t n_heads_q, size_t q_stride,
+                          size_t q_out_stride, void *stream);
+
+/* Causal grouped-query attention of the batch's token rows over the cache:
+ * out row = sum over visible t of softmax(scale * q . K[t]) V[t].  A row at
+ * position p sees t <= p; with sliding_window > 0 only t > p - sliding_window
+ * and the first n_sink positions.  A row that sees nothing (no position, no
+ * page) is 0, keys and values that a row does not see have no effect on it
+ * whatever they hold, and a row that sees a NaN or an infinity follows the
+ * formula (scores of -inf count as masked).  dtype (q and out): the
+ * cache's or JAL_F32.  Sums and softmax are f32; with 16-bit q the softmax
+ * weights are rounded to that type for the product with V.  n_heads_q is a
+ * multiple of n_heads_kv.  Strides as in jal_op_rope_kv_append; out may be q.
+ * The workspace has to be as large as jal_op_paged_attention_workspace says
+ * for the same arguments (JAL_ERR_TENSOR_BOUNDS), 16-byte aligned. */
+int jal_op_paged_attention(const jal_paged_kv *kv, const jal_ragged_batch *batch,
+                           int dtype, const void *q, size_t n_heads_q,
+                           size_t q_stride, float scale, size_t sliding_window,
+                           size_t n_sink, void *out, size_t out_stride,
+                           void *workspace, size_t workspace_len, void *stream);
+int jal_op_paged_attention_workspace(const jal_paged_kv *kv,
+                                     const jal_ragged_batch *batch, int dtype,
+                                     size_t n_heads_q, size_t sliding_window,
+                                     size_t n_sink, size_t *bytes);
+
+/* jal_op_paged_attention without a window, for a batch whose sequences share
+ * prefixes: the keys of each prefix are read once for all rows of its group,
+ * every sequence's further keys for its own rows, and the two are joined.
+ * The result is that of jal_op_paged_attention over the same positions. */
+int jal_op_shared_prefix_attention(const jal_paged_kv *kv,
+                                   const jal_ragged_batch *batch,
+                                   const jal_prefix_groups *groups, int dtype,
+                                   const void *q, size_t n_heads_q,
+                                   size_t q_stride, float scale, void *out,
+                                   size_t out_stride, void *workspace,
+                                   size_t workspace_len, void *stream);
+int jal_op_shared_prefix_attention_workspace(const jal_paged_kv *kv,
+                                             const jal_ragged_batch *batch,
+                                             const jal_prefix_groups *groups,
+                                             int dtype, size_t n_heads_q,
+                                             size_t *bytes);
+
+/* Beam search's selection: of all continuations (beam b, token t) of a
+ * sequence, scored cum[b] + log_softmax(logits[b])[t], the k best in
+ * descending order; equal scores go to the lowest b * vocab + t.  logits:
+ * [n_seqs * n_beams] rows of `dtype` (JAL_F32 / F16 / BF16), row_stride elements
+ * apart (0 = vocab); cum: [n_seqs][n_beams].  Scores are formed and compared
+ * in 64 bits, within a beam in the order of the logits.  A NaN logit counts as
+ * -inf; a beam whose cum is not finite or whose logits hold +inf or nothing
+ * above -inf scores -inf throughout (finished and empty beams).  k <= 64,
+ * k <= n_beams * vocab.  Outputs [n_seqs][k]. */
+int jal_op_beam_select(const void *logits, int dtype, size_t row_stride,
+                       const float *cum, size_t n_seqs, size_t n_beams,
+                       size_t vocab, size_t k, float *scores, int32_t *parents,
+                       int32_t *tokens, void *workspace, size_t workspace_len,
+                       void *stream);
+int jal_op_beam_select_workspace(size_t n_seqs, size_t n_beams, size_t vocab,
+                                 size_t k, size_t *bytes);
+
+/* The beams' caches in the order of their parents: row r = (sequence, beam)
+ * continues row p = (sequence, parents[r]) of the cache's tables.
+ * new_len[r] = kv_len[p]; new_table[r] holds p's whole pages, then the page
+ * that takes position new_len[r], then -1.  That page is p's own unfinished
+ * page for the first row that continues p, and fresh_pages[r] for the others,
+ * with the unfinished page's filled slots copied in every layer; where p has
+ * no unfinished page it is fresh_pages[r] for every row.  Row r of a parent
+ * outside [0, n_beams) becomes empty.  fresh_pages: [n_seqs * n_beams]
+ * distinct pages that no row uses; the caller takes back those that new_table
+ * does not name.  Layer i of the pools starts i * layer_stride elements
+ * after the first (0 = n_pages * page_stride).  new_table and new_len must
+ * not overlap the old ones. */
+int jal_op_beam_reorder(const jal_paged_kv *kv, size_t n_layers,
+                        size_t layer_stride, const int32_t *kv_len,
+                        const int32_t *parents, const int32_t *fresh_pages,
+                        size_t n_seqs, size_t n_beams, int32_t *new_table,
+                        int32_t *new_len, void *stream);
+
+/* ========================================================================
  * recipe.rs -- LlamaRecipe
  * ====================================================================== */
 typedef struct jal_recipe jal_recipe;

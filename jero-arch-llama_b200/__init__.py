@@ -124,6 +124,24 @@ class TpPlanFields(C.Structure):
                                           "v_lo", "v_n", "v_pad")]
 
 
+class PagedKvFields(C.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("page_table", _P),
+                ("n_pages", C.c_uint64), ("page_size", C.c_uint64), ("n_heads_kv", C.c_uint64),
+                ("head_dim", C.c_uint64), ("n_seqs", C.c_uint64), ("max_pages", C.c_uint64),
+                ("page_stride", C.c_uint64), ("head_stride", C.c_uint64), ("slot_stride", C.c_uint64),
+                ("dtype", C.c_int32)]
+
+
+class RaggedBatchFields(C.Structure):
+    _fields_ = [("q_start", _P), ("kv_len", _P), ("n_seqs", C.c_uint64), ("n_rows", C.c_uint64),
+                ("max_q_len", C.c_uint64), ("max_kv_len", C.c_uint64)]
+
+
+class PrefixGroupsFields(C.Structure):
+    _fields_ = [("group_start", _P), ("prefix_len", _P), ("n_groups", C.c_uint64), ("max_group", C.c_uint64),
+                ("max_prefix_len", C.c_uint64)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "jal_last_error": (C.c_char_p, []),
@@ -148,6 +166,14 @@ _SIGS = {
     "jal_op_rope": (C.c_int, [_P, _SZ, _SZ, _SZ, _SZ, C.c_int, _SZ, _P, _P]),
     "jal_op_swiglu": (C.c_int, [_P, _P, _SZ, _P, _P]),
     "jal_op_gqa_attention": (C.c_int, [_P, _P, _P, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, C.c_float, _P, _P]),
+    "jal_op_rope_kv_append": (C.c_int, [_P, _P, C.c_int, _P, _P, _SZ, _P, _SZ, C.c_int, _P, _P, _SZ, _SZ, _SZ, _P]),
+    "jal_op_paged_attention": (C.c_int, [_P, _P, C.c_int, _P, _SZ, _SZ, C.c_float, _SZ, _SZ, _P, _SZ, _P, _SZ, _P]),
+    "jal_op_paged_attention_workspace": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, C.POINTER(_SZ)]),
+    "jal_op_shared_prefix_attention": (C.c_int, [_P, _P, _P, C.c_int, _P, _SZ, _SZ, C.c_float, _P, _SZ, _P, _SZ, _P]),
+    "jal_op_shared_prefix_attention_workspace": (C.c_int, [_P, _P, _P, C.c_int, _SZ, C.POINTER(_SZ)]),
+    "jal_op_beam_select": (C.c_int, [_P, C.c_int, _SZ, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, _P, _P, _SZ, _P]),
+    "jal_op_beam_select_workspace": (C.c_int, [_SZ, _SZ, _SZ, _SZ, C.POINTER(_SZ)]),
+    "jal_op_beam_reorder": (C.c_int, [_P, _SZ, _SZ, _P, _P, _P, _SZ, _SZ, _P, _P, _P]),
     "jal_recipe_new": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "jal_recipe_from_gguf": (C.c_int, [_P, _SZ, C.POINTER(_P)]),
     "jal_recipe_free": (None, [_P]),
@@ -379,6 +405,109 @@ def gqa_attention(q, k, v, m, n_heads_q, n_heads_kv, head_dim, total_seq, start_
                   stream=None) -> None:
     _check(lib().jal_op_gqa_attention(_ptr(q), _ptr(k), _ptr(v), m, n_heads_q, n_heads_kv, head_dim, total_seq,
                                       start_pos, sliding_window, scale, _ptr(out), _stream(stream)))
+
+
+# ---- paged batch operators (include/jal.h) -----------------------------------
+class PagedKv:
+    """A paged cache as the operators take it (jal_paged_kv): device pools, the
+    page table [n_seqs, max_pages] of int32, and the pools' layout.  `strides`:
+    (page, head, slot) in elements; None = [page][kv_head][slot][head_dim].
+    Keeps the tensors alive; a view is made once and used for many calls."""
+
+    def __init__(self, k, v, page_table, dtype: int, n_pages: int, page_size: int, n_heads_kv: int, head_dim: int,
+                 n_seqs: int, max_pages: int, strides=None):
+        self._keep = (k, v, page_table)
+        self.fields = PagedKvFields(_ptr(k), _ptr(v), _ptr(page_table), n_pages, page_size, n_heads_kv, head_dim,
+                                    n_seqs, max_pages, *(strides or (0, 0, 0)), dtype)
+        self._as_parameter_ = C.addressof(self.fields)
+
+
+class RaggedBatch:
+    """The new rows of a batch (jal_ragged_batch): int32 device arrays q_start
+    [n_seqs + 1] and kv_len [n_seqs]."""
+
+    def __init__(self, q_start, kv_len, n_seqs: int, n_rows: int, max_q_len: int, max_kv_len: int):
+        self._keep = (q_start, kv_len)
+        self.fields = RaggedBatchFields(_ptr(q_start), _ptr(kv_len), n_seqs, n_rows, max_q_len, max_kv_len)
+        self._as_parameter_ = C.addressof(self.fields)
+
+
+class PrefixGroups:
+    """Sequences that share prefixes (jal_prefix_groups): int32 device arrays
+    group_start [n_groups + 1] and prefix_len [n_groups]."""
+
+    def __init__(self, group_start, prefix_len, n_groups: int, max_group: int, max_prefix_len: int):
+        self._keep = (group_start, prefix_len)
+        self.fields = PrefixGroupsFields(_ptr(group_start), _ptr(prefix_len), n_groups, max_group, max_prefix_len)
+        self._as_parameter_ = C.addressof(self.fields)
+
+
+def rope_kv_append(kv: PagedKv, batch: RaggedBatch, k, v, inv_freq, dtype: int, rotary_dim: int, neox: bool = False,
+                   kv_stride: int = 0, q=None, q_out=None, n_heads_q: int = 0, q_stride: int = 0,
+                   q_out_stride: int = 0, stream=None) -> None:
+    """Rotates the batch's k (and q) rows and appends k and v to the cache."""
+    _check(lib().jal_op_rope_kv_append(kv, batch, dtype, _ptr(k), _ptr(v), kv_stride, _ptr(inv_freq), rotary_dim,
+                                       1 if neox else 0, _ptr(q), _ptr(q_out), n_heads_q, q_stride, q_out_stride,
+                                       _stream(stream)))
+
+
+def paged_attention(kv: PagedKv, batch: RaggedBatch, q, out, n_heads_q: int, scale: float, dtype: int,
+                    sliding_window: int = 0, n_sink: int = 0, q_stride: int = 0, out_stride: int = 0, workspace=None,
+                    workspace_len: int = 0, stream=None) -> None:
+    """Causal attention of the batch's rows over the cache; with a window, the
+    first n_sink positions stay visible."""
+    _check(lib().jal_op_paged_attention(kv, batch, dtype, _ptr(q), n_heads_q, q_stride, scale, sliding_window, n_sink,
+                                        _ptr(out), out_stride, _ptr(workspace), workspace_len, _stream(stream)))
+
+
+def paged_attention_workspace(kv: PagedKv, batch: RaggedBatch, n_heads_q: int, dtype: int, sliding_window: int = 0,
+                              n_sink: int = 0) -> int:
+    """Workspace bytes of the same paged_attention call."""
+    n = _SZ()
+    _check(lib().jal_op_paged_attention_workspace(kv, batch, dtype, n_heads_q, sliding_window, n_sink, C.byref(n)))
+    return n.value
+
+
+def shared_prefix_attention(kv: PagedKv, batch: RaggedBatch, groups: PrefixGroups, q, out, n_heads_q: int,
+                            scale: float, dtype: int, q_stride: int = 0, out_stride: int = 0, workspace=None,
+                            workspace_len: int = 0, stream=None) -> None:
+    """paged_attention of sequences that share prefixes, each prefix read once
+    for its group."""
+    _check(lib().jal_op_shared_prefix_attention(kv, batch, groups, dtype, _ptr(q), n_heads_q, q_stride, scale,
+                                                _ptr(out), out_stride, _ptr(workspace), workspace_len,
+                                                _stream(stream)))
+
+
+def shared_prefix_attention_workspace(kv: PagedKv, batch: RaggedBatch, groups: PrefixGroups, n_heads_q: int,
+                                      dtype: int) -> int:
+    """Workspace bytes of the same shared_prefix_attention call."""
+    n = _SZ()
+    _check(lib().jal_op_shared_prefix_attention_workspace(kv, batch, groups, dtype, n_heads_q, C.byref(n)))
+    return n.value
+
+
+def beam_select(logits, cum, scores, parents, tokens, n_seqs: int, n_beams: int, vocab: int, k: int, dtype: int = F32,
+                row_stride: int = 0, workspace=None, workspace_len: int = 0, stream=None) -> None:
+    """The k best continuations of each sequence's beams: scores f32, parents
+    and tokens int32, [n_seqs, k]."""
+    _check(lib().jal_op_beam_select(_ptr(logits), dtype, row_stride, _ptr(cum), n_seqs, n_beams, vocab, k,
+                                    _ptr(scores), _ptr(parents), _ptr(tokens), _ptr(workspace), workspace_len,
+                                    _stream(stream)))
+
+
+def beam_select_workspace(n_seqs: int, n_beams: int, vocab: int, k: int) -> int:
+    """Workspace bytes of the same beam_select call."""
+    n = _SZ()
+    _check(lib().jal_op_beam_select_workspace(n_seqs, n_beams, vocab, k, C.byref(n)))
+    return n.value
+
+
+def beam_reorder(kv: PagedKv, kv_len, parents, fresh_pages, new_table, new_len, n_seqs: int, n_beams: int,
+                 n_layers: int = 1, layer_stride: int = 0, stream=None) -> None:
+    """The beams' page tables and lengths in the order of their parents, with
+    the unfinished pages of further children copied in every layer."""
+    _check(lib().jal_op_beam_reorder(kv, n_layers, layer_stride, _ptr(kv_len), _ptr(parents), _ptr(fresh_pages),
+                                     n_seqs, n_beams, _ptr(new_table), _ptr(new_len), _stream(stream)))
 
 
 # ---- LlamaRecipe (recipe.rs:110-547) ----------------------------------------

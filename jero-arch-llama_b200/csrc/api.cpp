@@ -44,11 +44,6 @@ struct jal_kv_cache {
   std::unique_ptr<KvCache> kv;
 };
 
-#define NEED(p)                                                  \
-  do {                                                           \
-    if (!(p)) fail(JAL_ERR_INVALID_ARGUMENT, "null argument: %s", #p); \
-  } while (0)
-
 static cudaStream_t as_stream(void *s) { return (cudaStream_t)s; }
 
 extern "C" {

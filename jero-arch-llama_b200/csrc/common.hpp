@@ -54,3 +54,8 @@ int guard(F &&f) {
       ::jal::fail(JAL_ERR_CUDA, "%s failed: %s (%s:%d)", #call,              \
                   cudaGetErrorString(err__), __FILE__, __LINE__);             \
   } while (0)
+
+#define NEED(p)                                                                       \
+  do {                                                                                \
+    if (!(p)) ::jal::fail(JAL_ERR_INVALID_ARGUMENT, "null argument: %s", #p);         \
+  } while (0)

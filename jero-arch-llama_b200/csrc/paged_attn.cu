@@ -1,0 +1,338 @@
+// Attention of a ragged batch over a paged cache: the plan of a call, the f32
+// kernel, and the joining of the pieces that the keys were cut into.
+#include <algorithm>
+
+#include "common.hpp"
+#include "paged_dev.cuh"
+
+namespace jal {
+
+namespace {
+
+using namespace paged;
+
+// Which tile a block of the flat grid works on: first the shared prefixes'
+// (piece fastest, then tile, head, group), then the sequences'.
+__device__ __forceinline__ bool block_tile(const AttnParams &p, int rt, int key_align, Tile &t) {
+  int64_t b = blockIdx.x;
+  const int64_t np = (int64_t)p.prefix_splits * p.prefix_tiles * p.kv.hkv * p.n_groups;
+  const bool prefix = b < np;
+  if (!prefix) b -= np;
+  const int splits = prefix ? p.prefix_splits : p.splits, tiles = prefix ? p.prefix_tiles : p.tiles;
+  const int piece = (int)(b % splits);
+  b /= splits;
+  const int tile = (int)(b % tiles);
+  b /= tiles;
+  return make_tile(p, prefix, (int)(b / p.kv.hkv), (int)(b % p.kv.hkv), tile, piece, rt, key_align, t);
+}
+
+// ---- the f32 kernel ---------------------------------------------------------
+// One pass over the tile's keys with the running maximum and sum of each row:
+// K and V tiles of KT keys widened to f32 in shared memory, scores and output
+// on the CUDA cores in f32, 128 threads as 8 row groups x 16 key (or dim)
+// groups.
+constexpr int kF32Threads = 128;
+constexpr int kF32Keys = 32;
+
+template <int HD, int RT>
+struct F32Smem {
+  float q[RT][HD + 4];
+  float k[kF32Keys][HD + 4];
+  float v[kF32Keys][HD];
+  float s[RT][kF32Keys + 4];
+  RowMask mask[RT];
+  float corr[RT];
+  int poison;
+};
+
+template <class TK, int HD, int RT>
+__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const AttnParams p, const bool direct) {
+  extern __shared__ __align__(16) char smem_raw[];
+  auto &sm = *(F32Smem<HD, RT> *)smem_raw;
+  pdl_trigger();
+  Tile t;
+  if (!block_tile(p, RT, kF32Keys, t)) return;
+  constexpr int R = RT / 8, KC = kF32Keys / 16, DC = HD / 16;
+  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int hd = p.kv.hd;
+  for (int i = tid; i < RT * HD; i += kF32Threads) {
+    const int j = i / HD, d = i % HD;
+    sm.q[j][d] = j < t.rows && d < hd ? load_as_f32(p.q, q_offset(p, t, j) + d, p.act) * p.scale_log2 : 0.0f;
+  }
+  for (int j = tid; j < RT; j += kF32Threads)
+    sm.mask[j] = j < t.rows ? row_mask(p, t, j) : RowMask{0, 0};
+  if (tid == 0) sm.poison = 0;
+  float o[R][DC], m[R], l[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DC; c++) o[i][c] = 0.0f;
+  }
+  bool bad = false;
+  for (int u = t.u0; u < t.u1; u += kF32Keys) {
+    __syncthreads();
+    const int n = min(kF32Keys, t.u1 - u);
+    for (int i = tid; i < kF32Keys * (HD / 8); i += kF32Threads) {
+      const int r = i / (HD / 8), d = (i % (HD / 8)) * 8;
+      float a[8] = {}, b[8] = {};
+      if (r < n && d < hd) {
+        const int64_t at = slot_offset(p.kv, t.table, t.head, t.key(u + r));
+        if (at >= 0) {
+          load8((const TK *)p.kv.k + at + d, a);
+          load8((const TK *)p.kv.v + at + d, b);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) bad |= !isfinite(b[e]);
+      store8(&sm.k[r][d], a);
+      store8(&sm.v[r][d], b);
+    }
+    __syncthreads();
+    float s[R][KC];
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int c = 0; c < KC; c++) s[i][c] = 0.0f;
+    for (int d = 0; d < HD; d += 4) {
+      float4 a[R], b[KC];
+#pragma unroll
+      for (int i = 0; i < R; i++) a[i] = *(const float4 *)&sm.q[ty + 8 * i][d];
+#pragma unroll
+      for (int c = 0; c < KC; c++) b[c] = *(const float4 *)&sm.k[tx + 16 * c][d];
+#pragma unroll
+      for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+          s[i][c] = fmaf(a[i].x, b[c].x, s[i][c]);
+          s[i][c] = fmaf(a[i].y, b[c].y, s[i][c]);
+          s[i][c] = fmaf(a[i].z, b[c].z, s[i][c]);
+          s[i][c] = fmaf(a[i].w, b[c].w, s[i][c]);
+        }
+    }
+    // An unmapped page's keys are masked for every row.
+    bool there[KC];
+    int key[KC];
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+      const int r = tx + 16 * c;
+      key[c] = r < n ? t.key(u + r) : 0;
+      there[c] = r < n && slot_offset(p.kv, t.table, t.head, key[c]) >= 0;
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const RowMask mk = sm.mask[ty + 8 * i];
+      float top = m[i];
+#pragma unroll
+      for (int c = 0; c < KC; c++) {
+        if (!there[c] || !mk.sees(key[c], p.n_sink)) s[i][c] = -INFINITY;
+        top = fmaxf(top, s[i][c]);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float safe = top == -INFINITY ? 0.0f : top;
+      const float corr = exp2f(m[i] - safe);
+      float sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < KC; c++) {
+        const float e = exp2f(s[i][c] - safe);
+        sum += e;
+        sm.s[ty + 8 * i][tx + 16 * c] = e;
+      }
+      l[i] = l[i] * corr + sum;
+      m[i] = top;
+#pragma unroll
+      for (int c = 0; c < DC; c++) o[i][c] *= corr;
+    }
+    __syncwarp();  // a row group's weights are written and read by one warp
+    for (int r = 0; r < kF32Keys; r += 4) {
+      float4 w[R];
+#pragma unroll
+      for (int i = 0; i < R; i++) w[i] = *(const float4 *)&sm.s[ty + 8 * i][r];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float v[DC];
+#pragma unroll
+        for (int c = 0; c < DC; c += 4) *(float4 *)&v[c] = *(const float4 *)&sm.v[r + e][tx * 4 + (c / 4) * 64];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+          const float we = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+#pragma unroll
+          for (int c = 0; c < DC; c++) o[i][c] = fmaf(we, v[c], o[i][c]);
+        }
+      }
+    }
+  }
+  if (__syncthreads_or(bad)) {
+    for (int j = tid / 32; j < t.rows; j += kF32Threads / 32) attend_row_alone(p, t, j, direct);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int j = ty + 8 * i;
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+    if (j >= t.rows) continue;
+    const int64_t oo = out_offset(p, t, j), pi = part_index(p, t, j);
+    const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    if (!direct && tx == 0) p.part_ml[pi] = make_float2(m[i], l[i]);
+#pragma unroll
+    for (int c = 0; c < DC; c++) {
+      const int d = tx * 4 + (c / 4) * 64 + c % 4;
+      if (d >= hd) continue;
+      if (direct)
+        store_from_f32(p.out, oo + d, p.act, o[i][c] * inv);
+      else
+        p.part_o[pi * hd + d] = o[i][c];
+    }
+  }
+}
+
+// ---- joining the pieces -----------------------------------------------------
+// Row by row, one warp for each (token row, query head): the pieces' sums
+// rescaled to the largest of their maxima and added in the order of the
+// pieces.  A piece without a visible key has sum 0 and is not read.
+constexpr int kJoinWarps = 4;
+
+__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(const AttnParams p, const int prefix_rows) {
+  pdl_wait();
+  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31, head = (int)(id % p.hq);
+  const int64_t tok = id / p.hq;
+  const int s = (int)(tok / p.max_q), i = (int)(tok % p.max_q);
+  if (s >= p.n_seqs) return;
+  int beg, end;
+  seq_rows(p.q_start, p.n_rows, s, beg, end);
+  if (i >= end - beg) return;
+  const int row = beg + i;
+  int first = p.prefix_splits;  // a sequence outside every group has its own keys alone
+  if (p.prefix_splits) {
+    const int g = seq_of_row(p.group_start, 0, p.n_groups, s);
+    if (p.group_start[g] <= s && s < p.group_start[g + 1]) {
+      first = 0;
+      const int gb = min(max(p.q_start[min(max(p.group_start[g], 0), p.n_seqs)], 0), p.n_rows);
+      if ((int64_t)(row - gb + 1) * p.G > (int64_t)p.prefix_tiles * prefix_rows) return;  // past max_group: not computed
+    }
+  }
+  const int n = p.prefix_splits + p.splits;
+  const int64_t stride = (int64_t)p.n_rows * p.hq, at = (int64_t)row * p.hq + head;
+  constexpr int W = kPagedMaxSplits * 2 / 32;
+  float mw[W], lw[W], top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int k = 0; k < W; k++) {
+    const int piece = k * 32 + lane;
+    mw[k] = -INFINITY;
+    lw[k] = 0.0f;
+    if (piece >= first && piece < n) {
+      const float2 ml = p.part_ml[piece * stride + at];
+      mw[k] = ml.x;
+      lw[k] = ml.y;
+    }
+    nan |= mw[k] != mw[k];
+    top = fmaxf(top, mw[k]);
+  }
+  top = warp_max(top);
+  const float safe = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f;
+#pragma unroll
+  for (int k = 0; k < W; k++) {
+    mw[k] = lw[k] == 0.0f ? 0.0f : exp2f(mw[k] - safe);  // from here the piece's weight
+    total += mw[k] * lw[k];
+  }
+  total = warp_sum(total);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  float o[kPagedMaxHeadDim / 32];
+#pragma unroll
+  for (int c = 0; c < kPagedMaxHeadDim / 32; c++) o[c] = 0.0f;
+  const int hd = p.kv.hd;
+#pragma unroll
+  for (int k = 0; k < W; k++) {
+    for (int q = 0; q < 32 && k * 32 + q < n; q++) {
+      const float w = __shfl_sync(0xffffffffu, mw[k], q);
+      if (w == 0.0f) continue;
+      const float *po = p.part_o + ((k * 32 + q) * stride + at) * hd;
+#pragma unroll
+      for (int c = 0; c < kPagedMaxHeadDim / 32; c++)
+        if (lane + 32 * c < hd) o[c] = fmaf(w, po[lane + 32 * c], o[c]);
+    }
+  }
+  const int64_t oo = (int64_t)row * p.out_stride + (int64_t)head * hd;
+#pragma unroll
+  for (int c = 0; c < kPagedMaxHeadDim / 32; c++)
+    if (lane + 32 * c < hd) store_from_f32(p.out, oo + lane + 32 * c, p.act, o[c] * inv);
+}
+
+template <class TK, int HD, int RT>
+void run_f32(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  const int smem = (int)sizeof(F32Smem<HD, RT>);
+  JAL_CUDA(cudaFuncSetAttribute(k_paged_attn_f32<TK, HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t blocks = (int64_t)p.kv.hkv * ((int64_t)p.prefix_splits * p.prefix_tiles * p.n_groups +
+                                              (int64_t)p.splits * p.tiles * p.n_seqs);
+  k_paged_attn_f32<TK, HD, RT><<<(unsigned)blocks, kF32Threads, smem, s>>>(p, plan.direct);
+  JAL_CUDA(cudaGetLastError());
+}
+template <class TK, int HD>
+void run_f32_rows(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  if (plan.rows == 8) run_f32<TK, HD, 8>(p, plan, s);
+  else run_f32<TK, HD, 32>(p, plan, s);
+}
+template <class TK>
+void run_f32_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  if (p.kv.hd <= 64) run_f32_rows<TK, 64>(p, plan, s);
+  else if (p.kv.hd <= 128) run_f32_rows<TK, 128>(p, plan, s);
+  else run_f32_rows<TK, 256>(p, plan, s);
+}
+
+int pieces(int64_t blocks, int64_t keys, int64_t wanted, int64_t least) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / least));
+  return (int)std::min(most, std::max<int64_t>(1, wanted / std::max<int64_t>(1, blocks)));
+}
+
+}  // namespace
+
+AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const jal_prefix_groups *g, size_t hq,
+                        int act, size_t window, size_t n_sink) {
+  (void)act;
+  AttnPlan a = {};
+  const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv;
+  const int64_t pairs = (int64_t)b.max_q_len * G;
+  const int64_t group_pairs = g ? (int64_t)g->max_group * pairs : 0;
+  a.rows = std::max(pairs, group_pairs) <= 8 ? 8 : 32;
+  a.tiles = (int)((pairs + a.rows - 1) / a.rows);
+  int64_t keys = (int64_t)b.max_kv_len;
+  if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
+  const int64_t wanted = 2 * kPagedSMs;
+  if (g && g->n_groups && g->max_prefix_len) {
+    a.prefix_rows = a.rows;
+    a.prefix_tiles = (int)((group_pairs + a.rows - 1) / a.rows);
+    a.prefix_splits = pieces(a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len, wanted, 128);
+    keys = std::max<int64_t>(1, keys - (int64_t)g->max_prefix_len);
+  }
+  a.splits = pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, wanted, 128);
+  a.direct = a.splits + a.prefix_splits == 1;
+  if (!a.direct)
+    a.bytes = (size_t)(a.splits + a.prefix_splits) * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;
+  return a;
+}
+
+void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) {
+  if (p.kv.dtype == JAL_F32) run_f32_hd<float>(p, plan, s);
+  else if (p.kv.dtype == JAL_F16) run_f32_hd<__half>(p, plan, s);
+  else run_f32_hd<__nv_bfloat16>(p, plan, s);
+  if (plan.direct) return;
+  const int64_t warps = (int64_t)p.n_seqs * p.max_q * p.hq;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  JAL_CUDA(cudaLaunchKernelEx(&cfg, k_paged_attn_join, p, plan.prefix_rows));
+}
+
+}  // namespace jal
