@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "paged_attn_mma.cuh"
 #include "paged_dev.cuh"
 
 namespace jal {
@@ -10,21 +11,6 @@ namespace jal {
 namespace {
 
 using namespace paged;
-
-// Which tile a block of the flat grid works on: first the shared prefixes'
-// (piece fastest, then tile, head, group), then the sequences'.
-__device__ __forceinline__ bool block_tile(const AttnParams &p, int rt, int key_align, Tile &t) {
-  int64_t b = blockIdx.x;
-  const int64_t np = (int64_t)p.prefix_splits * p.prefix_tiles * p.kv.hkv * p.n_groups;
-  const bool prefix = b < np;
-  if (!prefix) b -= np;
-  const int splits = prefix ? p.prefix_splits : p.splits, tiles = prefix ? p.prefix_tiles : p.tiles;
-  const int piece = (int)(b % splits);
-  b /= splits;
-  const int tile = (int)(b % tiles);
-  b /= tiles;
-  return make_tile(p, prefix, (int)(b / p.kv.hkv), (int)(b % p.kv.hkv), tile, piece, rt, key_align, t);
-}
 
 // ---- the f32 kernel ---------------------------------------------------------
 // One pass over the tile's keys with the running maximum and sum of each row:
@@ -285,6 +271,22 @@ void run_f32_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
   else run_f32_rows<TK, 256>(p, plan, s);
 }
 
+template <class T, int NS, int HD>
+void run_mma(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  constexpr int smem = MmaShape<NS, HD>::smem;
+  JAL_CUDA(cudaFuncSetAttribute(k_paged_attn_mma<T, NS, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t blocks = (int64_t)p.kv.hkv * ((int64_t)p.prefix_splits * p.prefix_tiles * p.n_groups +
+                                              (int64_t)p.splits * p.tiles * p.n_seqs);
+  k_paged_attn_mma<T, NS, HD><<<(unsigned)blocks, kMmaThreads, smem, s>>>(p, plan.direct);
+  JAL_CUDA(cudaGetLastError());
+}
+template <class T, int NS>
+void run_mma_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  if (p.kv.hd <= 64) run_mma<T, NS, 64>(p, plan, s);
+  else if (p.kv.hd <= 128) run_mma<T, NS, 128>(p, plan, s);
+  else run_mma<T, NS, 256>(p, plan, s);
+}
+
 int pieces(int64_t blocks, int64_t keys, int64_t wanted, int64_t least) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / least));
   return (int)std::min(most, std::max<int64_t>(1, wanted / std::max<int64_t>(1, blocks)));
@@ -296,21 +298,22 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
                         int act, size_t window, size_t n_sink) {
   (void)act;
   AttnPlan a = {};
+  a.mma = kv.dtype != JAL_F32;
   const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv;
   const int64_t pairs = (int64_t)b.max_q_len * G;
   const int64_t group_pairs = g ? (int64_t)g->max_group * pairs : 0;
-  a.rows = std::max(pairs, group_pairs) <= 8 ? 8 : 32;
+  a.rows = a.mma ? kMmaRows : std::max(pairs, group_pairs) <= 8 ? 8 : 32;
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
   int64_t keys = (int64_t)b.max_kv_len;
   if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
-  const int64_t wanted = 2 * kPagedSMs;
+  const int64_t wanted = 8 * kPagedSMs;
   if (g && g->n_groups && g->max_prefix_len) {
     a.prefix_rows = a.rows;
     a.prefix_tiles = (int)((group_pairs + a.rows - 1) / a.rows);
-    a.prefix_splits = pieces(a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len, wanted, 128);
+    a.prefix_splits = pieces(a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len, wanted, 256);
     keys = std::max<int64_t>(1, keys - (int64_t)g->max_prefix_len);
   }
-  a.splits = pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, wanted, 128);
+  a.splits = pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, wanted, 256);
   a.direct = a.splits + a.prefix_splits == 1;
   if (!a.direct)
     a.bytes = (size_t)(a.splits + a.prefix_splits) * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;
@@ -318,9 +321,11 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
 }
 
 void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) {
-  if (p.kv.dtype == JAL_F32) run_f32_hd<float>(p, plan, s);
-  else if (p.kv.dtype == JAL_F16) run_f32_hd<__half>(p, plan, s);
-  else run_f32_hd<__nv_bfloat16>(p, plan, s);
+  if (!plan.mma) run_f32_hd<float>(p, plan, s);
+  else if (p.act == JAL_F16) run_mma_hd<__half, 1>(p, plan, s);
+  else if (p.act == JAL_BF16) run_mma_hd<__nv_bfloat16, 1>(p, plan, s);
+  else if (p.kv.dtype == JAL_F16) run_mma_hd<__half, 2>(p, plan, s);
+  else run_mma_hd<__nv_bfloat16, 3>(p, plan, s);
   if (plan.direct) return;
   const int64_t warps = (int64_t)p.n_seqs * p.max_q * p.hq;
   cudaLaunchConfig_t cfg = {};

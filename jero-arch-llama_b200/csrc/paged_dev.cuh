@@ -179,6 +179,21 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
   return true;
 }
 
+// Which tile a block of the flat grid works on: first the shared prefixes'
+// (piece fastest, then tile, head, group), then the sequences'.
+__device__ __forceinline__ bool block_tile(const AttnParams &p, int rt, int key_align, Tile &t) {
+  int64_t b = blockIdx.x;
+  const int64_t np = (int64_t)p.prefix_splits * p.prefix_tiles * p.kv.hkv * p.n_groups;
+  const bool prefix = b < np;
+  if (!prefix) b -= np;
+  const int splits = prefix ? p.prefix_splits : p.splits, tiles = prefix ? p.prefix_tiles : p.tiles;
+  const int piece = (int)(b % splits);
+  b /= splits;
+  const int tile = (int)(b % tiles);
+  b /= tiles;
+  return make_tile(p, prefix, (int)(b / p.kv.hkv), (int)(b % p.kv.hkv), tile, piece, rt, key_align, t);
+}
+
 // What row j of the tile may see: keys t < lim with t >= wlo or t < sink.
 struct RowMask {
   int lim, wlo;
