@@ -45,7 +45,6 @@ struct AttnParams {
 
 // How one call is cut; the workspace size follows from it.
 struct AttnPlan {
-  bool mma;                    // a 16-bit cache: matrix instructions
   int rows;                    // query rows of a tile (a sequence's own keys)
   int prefix_rows;             // query rows of a tile (shared prefixes; 0 = none)
   int tiles, prefix_tiles, splits, prefix_splits;

@@ -4,6 +4,7 @@
 
 #include "common.hpp"
 #include "paged_attn_mma.cuh"
+#include "paged_attn_tc.cuh"
 #include "paged_dev.cuh"
 
 namespace jal {
@@ -32,12 +33,12 @@ struct F32Smem {
 };
 
 template <class TK, int HD, int RT>
-__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const AttnParams p, const bool direct) {
+__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const AttnParams p, const int part, const bool direct) {
   extern __shared__ __align__(16) char smem_raw[];
   auto &sm = *(F32Smem<HD, RT> *)smem_raw;
   pdl_trigger();
   Tile t;
-  if (!block_tile(p, RT, kF32Keys, t)) return;
+  if (!block_tile(p, part, RT, kF32Keys, t)) return;
   constexpr int R = RT / 8, KC = kF32Keys / 16, DC = HD / 16;
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int hd = p.kv.hd;
@@ -250,70 +251,98 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(const AttnP
     if (lane + 32 * c < hd) store_from_f32(p.out, oo + lane + 32 * c, p.act, o[c] * inv);
 }
 
-template <class TK, int HD, int RT>
-void run_f32(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
-  const int smem = (int)sizeof(F32Smem<HD, RT>);
-  JAL_CUDA(cudaFuncSetAttribute(k_paged_attn_f32<TK, HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int64_t blocks = (int64_t)p.kv.hkv * ((int64_t)p.prefix_splits * p.prefix_tiles * p.n_groups +
-                                              (int64_t)p.splits * p.tiles * p.n_seqs);
-  k_paged_attn_f32<TK, HD, RT><<<(unsigned)blocks, kF32Threads, smem, s>>>(p, plan.direct);
+int64_t blocks_of(const AttnParams &p, int part) {
+  const int64_t prefix = (int64_t)p.prefix_splits * p.prefix_tiles * p.n_groups;
+  const int64_t own = (int64_t)p.splits * p.tiles * p.n_seqs;
+  return p.kv.hkv * ((part == kOwn ? 0 : prefix) + (part == kPrefix ? 0 : own));
+}
+template <class F>
+void run_kernel(F kernel, const AttnParams &p, int part, bool direct, int threads, int smem, cudaStream_t s) {
+  const int64_t blocks = blocks_of(p, part);
+  if (!blocks) return;
+  JAL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<(unsigned)blocks, threads, smem, s>>>(p, part, direct);
   JAL_CUDA(cudaGetLastError());
-}
-template <class TK, int HD>
-void run_f32_rows(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
-  if (plan.rows == 8) run_f32<TK, HD, 8>(p, plan, s);
-  else run_f32<TK, HD, 32>(p, plan, s);
-}
-template <class TK>
-void run_f32_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
-  if (p.kv.hd <= 64) run_f32_rows<TK, 64>(p, plan, s);
-  else if (p.kv.hd <= 128) run_f32_rows<TK, 128>(p, plan, s);
-  else run_f32_rows<TK, 256>(p, plan, s);
 }
 
+template <class TK, int HD>
+void run_f32(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  if (plan.rows == 8)
+    run_kernel(k_paged_attn_f32<TK, HD, 8>, p, kBoth, plan.direct, kF32Threads, (int)sizeof(F32Smem<HD, 8>), s);
+  else
+    run_kernel(k_paged_attn_f32<TK, HD, 32>, p, kBoth, plan.direct, kF32Threads, (int)sizeof(F32Smem<HD, 32>), s);
+}
 template <class T, int NS, int HD>
-void run_mma(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
-  constexpr int smem = MmaShape<NS, HD>::smem;
-  JAL_CUDA(cudaFuncSetAttribute(k_paged_attn_mma<T, NS, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int64_t blocks = (int64_t)p.kv.hkv * ((int64_t)p.prefix_splits * p.prefix_tiles * p.n_groups +
-                                              (int64_t)p.splits * p.tiles * p.n_seqs);
-  k_paged_attn_mma<T, NS, HD><<<(unsigned)blocks, kMmaThreads, smem, s>>>(p, plan.direct);
-  JAL_CUDA(cudaGetLastError());
+void run_16bit(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  const int tc = plan.rows == kTcRows ? plan.prefix_rows != kMmaRows ? kBoth : kOwn : kPrefix;
+  if constexpr (HD <= 128 && NS <= 2) {
+    if (plan.rows == kTcRows || plan.prefix_rows == kTcRows)
+      run_kernel(k_paged_attn_tc<T, NS, HD>, p, tc, plan.direct, kTcThreads, TcShape<NS, HD>::smem, s);
+  }
+  if (plan.rows == kMmaRows || plan.prefix_rows == kMmaRows) {
+    const int part = plan.rows != kMmaRows ? kPrefix : plan.prefix_rows == kTcRows ? kOwn : kBoth;
+    run_kernel(k_paged_attn_mma<T, NS, HD>, p, part, plan.direct, kMmaThreads, MmaShape<NS, HD>::smem, s);
+  }
 }
 template <class T, int NS>
-void run_mma_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
-  if (p.kv.hd <= 64) run_mma<T, NS, 64>(p, plan, s);
-  else if (p.kv.hd <= 128) run_mma<T, NS, 128>(p, plan, s);
-  else run_mma<T, NS, 256>(p, plan, s);
+void run_16bit_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  if (p.kv.hd <= 64) run_16bit<T, NS, 64>(p, plan, s);
+  else if (p.kv.hd <= 128) run_16bit<T, NS, 128>(p, plan, s);
+  else run_16bit<T, NS, 256>(p, plan, s);
 }
 
-int pieces(int64_t blocks, int64_t keys, int64_t wanted, int64_t least) {
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / least));
-  return (int)std::min(most, std::max<int64_t>(1, wanted / std::max<int64_t>(1, blocks)));
+// Into how many pieces the keys of `blocks` blocks' rows go.  `slots` blocks
+// run at once; the time is that of the rounds it takes, each as long as a
+// piece's keys and what a block costs besides (a start and an end worth
+// kBlockKeys keys of reading).  A second kernel joins the pieces: worth
+// kJoinKeys.  Measured on one 131071-key row over 8 KV heads: 37 pieces (one
+// full round of 296 blocks) XX us, 64 pieces (1.7 rounds) 150 us.
+constexpr int64_t kTcLeast = 64;
+constexpr int64_t kBlockKeys = 128, kJoinKeys = 256, kLeastKeys = 128;
+int pieces(int64_t blocks, int64_t keys, int64_t slots) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / kLeastKeys));
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = 1; s <= most; s++) {
+    const int64_t rounds = (blocks * s + slots - 1) / slots;
+    const int64_t cost = rounds * ((keys + s - 1) / s + kBlockKeys) + (s > 1 ? kJoinKeys : 0);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return (int)best;
 }
 
 }  // namespace
 
 AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const jal_prefix_groups *g, size_t hq,
                         int act, size_t window, size_t n_sink) {
-  (void)act;
   AttnPlan a = {};
-  a.mma = kv.dtype != JAL_F32;
   const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv;
   const int64_t pairs = (int64_t)b.max_q_len * G;
   const int64_t group_pairs = g ? (int64_t)g->max_group * pairs : 0;
-  a.rows = a.mma ? kMmaRows : std::max(pairs, group_pairs) <= 8 ? 8 : 32;
+  // Which kernel: f32 caches on the CUDA cores; 16-bit ones on mma.sync in
+  // tiles of 16 rows, or on tcgen05 in tiles of 256 where enough rows share
+  // their keys (three bf16 parts of f32 rows, and head dims above 128, do not
+  // fit its shared memory).
+  const bool tc = kv.dtype != JAL_F32 && kv.head_dim <= 128 && !(act == JAL_F32 && kv.dtype == JAL_BF16);
+  auto rows_for = [&](int64_t n) {
+    if (kv.dtype == JAL_F32) return std::max(pairs, group_pairs) <= 8 ? 8 : 32;
+    return tc && n > kTcLeast ? kTcRows : kMmaRows;
+  };
+  auto slots_for = [&](int rows) { return rows == kTcRows ? (int64_t)kPagedSMs : 2 * (int64_t)kPagedSMs; };
+  a.rows = rows_for(pairs);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
   int64_t keys = (int64_t)b.max_kv_len;
   if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
-  const int64_t wanted = 8 * kPagedSMs;
   if (g && g->n_groups && g->max_prefix_len) {
-    a.prefix_rows = a.rows;
-    a.prefix_tiles = (int)((group_pairs + a.rows - 1) / a.rows);
-    a.prefix_splits = pieces(a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len, wanted, 256);
+    a.prefix_rows = rows_for(group_pairs);
+    a.prefix_tiles = (int)((group_pairs + a.prefix_rows - 1) / a.prefix_rows);
+    a.prefix_splits = pieces(a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len,
+                             slots_for(a.prefix_rows));
     keys = std::max<int64_t>(1, keys - (int64_t)g->max_prefix_len);
   }
-  a.splits = pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, wanted, 256);
+  a.splits = pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, slots_for(a.rows));
   a.direct = a.splits + a.prefix_splits == 1;
   if (!a.direct)
     a.bytes = (size_t)(a.splits + a.prefix_splits) * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;
@@ -321,11 +350,19 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
 }
 
 void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) {
-  if (!plan.mma) run_f32_hd<float>(p, plan, s);
-  else if (p.act == JAL_F16) run_mma_hd<__half, 1>(p, plan, s);
-  else if (p.act == JAL_BF16) run_mma_hd<__nv_bfloat16, 1>(p, plan, s);
-  else if (p.kv.dtype == JAL_F16) run_mma_hd<__half, 2>(p, plan, s);
-  else run_mma_hd<__nv_bfloat16, 3>(p, plan, s);
+  if (p.kv.dtype == JAL_F32) {
+    if (p.kv.hd <= 64) run_f32<float, 64>(p, plan, s);
+    else if (p.kv.hd <= 128) run_f32<float, 128>(p, plan, s);
+    else run_f32<float, 256>(p, plan, s);
+  } else if (p.act == JAL_F16) {
+    run_16bit_hd<__half, 1>(p, plan, s);
+  } else if (p.act == JAL_BF16) {
+    run_16bit_hd<__nv_bfloat16, 1>(p, plan, s);
+  } else if (p.kv.dtype == JAL_F16) {
+    run_16bit_hd<__half, 2>(p, plan, s);
+  } else {
+    run_16bit_hd<__nv_bfloat16, 3>(p, plan, s);
+  }
   if (plan.direct) return;
   const int64_t warps = (int64_t)p.n_seqs * p.max_q * p.hq;
   cudaLaunchConfig_t cfg = {};

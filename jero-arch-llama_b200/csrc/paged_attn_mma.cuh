@@ -87,7 +87,7 @@ struct MmaShape {
 };
 
 template <class T, int NS, int HD>
-__global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnParams p, const bool direct) {
+__global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnParams p, const int part, const bool direct) {
   using S = MmaShape<NS, HD>;
   extern __shared__ __align__(128) char smem_raw[];
   __shared__ RowMask masks[kMmaRows];
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
   __shared__ uint32_t present[kMmaWarps][S::stages];
   pdl_trigger();
   Tile t;
-  if (!block_tile(p, kMmaRows, kMmaWarps * kMmaKeys, t)) return;
+  if (!block_tile(p, part, kMmaRows, kMmaWarps * kMmaKeys, t)) return;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, hd = p.kv.hd;
   const uint32_t sq = smem_u32(smem_raw), ring = sq + S::q_bytes + warp * (S::stages * 2 * S::half);
   char *const q_sm = smem_raw;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
     n0 = fmaxf(top0, fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2)));
     n1 = fmaxf(top1, fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2)));
     if (__any_sync(0xffffffffu, n0 != top0 || n1 != top1)) {
-      const float c0 = n0 == top0 ? 1.0f : exp2f(top0 - n0), c1 = n1 == top1 ? 1.0f : exp2f(top1 - n1);
+      const float c0 = n0 == top0 ? 1.0f : exp2_fast(top0 - n0), c1 = n1 == top1 ? 1.0f : exp2_fast(top1 - n1);
       top0 = n0;
       top1 = n1;
       l0 *= c0;
@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
     for (int n = 0; n < 2; n++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        s[n][e] = exp2f(s[n][e] - b0);
-        s[n][2 + e] = exp2f(s[n][2 + e] - b1);
+        s[n][e] = exp2_fast(s[n][e] - b0);
+        s[n][2 + e] = exp2_fast(s[n][2 + e] - b1);
         l0 += s[n][e];
         l1 += s[n][2 + e];
       }

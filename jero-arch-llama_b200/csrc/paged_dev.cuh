@@ -78,6 +78,14 @@ __device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
   ((float4 *)p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// 2^x by the special-function unit: relative error 2^-22, results below 2^-126
+// are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Element offset of position t's row of `head`, or -1 where the table names no
 // page of the pool (such a key counts as masked and is not read).
 __device__ __forceinline__ int64_t slot_offset(const PagedView &kv, const int32_t *table_row, int head, int t) {
@@ -179,17 +187,19 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
   return true;
 }
 
+// Which tiles a launch works on.
+enum Part { kBoth, kPrefix, kOwn };
 // Which tile a block of the flat grid works on: first the shared prefixes'
 // (piece fastest, then tile, head, group), then the sequences'.
-__device__ __forceinline__ bool block_tile(const AttnParams &p, int rt, int key_align, Tile &t) {
+__device__ __forceinline__ bool block_tile(const AttnParams &p, int part, int rt, int key_align, Tile &t) {
   int64_t b = blockIdx.x;
-  const int64_t np = (int64_t)p.prefix_splits * p.prefix_tiles * p.kv.hkv * p.n_groups;
+  const int64_t np = part == kOwn ? 0 : (int64_t)p.prefix_splits * p.prefix_tiles * p.kv.hkv * p.n_groups;
   const bool prefix = b < np;
   if (!prefix) b -= np;
   const int splits = prefix ? p.prefix_splits : p.splits, tiles = prefix ? p.prefix_tiles : p.tiles;
   const int piece = (int)(b % splits);
   b /= splits;
-  const int tile = (int)(b % tiles);
+  const int tile = tiles - 1 - (int)(b % tiles);  // the last rows see the most keys: first
   b /= tiles;
   return make_tile(p, prefix, (int)(b / p.kv.hkv), (int)(b % p.kv.hkv), tile, piece, rt, key_align, t);
 }
