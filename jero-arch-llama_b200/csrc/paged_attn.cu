@@ -33,7 +33,7 @@ struct F32Smem {
 };
 
 template <class TK, int HD, int RT>
-__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const AttnParams p, const int part, const bool direct) {
+__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_constant__ AttnParams p, const int part, const bool direct) {
   extern __shared__ __align__(16) char smem_raw[];
   auto &sm = *(F32Smem<HD, RT> *)smem_raw;
   pdl_trigger();
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const AttnParams
 // pieces.  A piece without a visible key has sum 0 and is not read.
 constexpr int kJoinWarps = 4;
 
-__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(const AttnParams p, const int prefix_rows) {
+__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(const __grid_constant__ AttnParams p, const int prefix_rows) {
   pdl_wait();
   const int64_t id = (int64_t)blockIdx.x * kJoinWarps + threadIdx.x / 32;
   const int lane = threadIdx.x & 31, head = (int)(id % p.hq);
@@ -298,6 +298,12 @@ void run_16bit_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
 // kJoinKeys.  Measured on one 131071-key row over 8 KV heads: 37 pieces (one
 // full round of 296 blocks) XX us, 64 pieces (1.7 rounds) 150 us.
 constexpr int64_t kTcLeast = 64;
+// Blocks of the tcgen05 kernel fill an SM each and write 256 rows of partial
+// results, so its keys are cut only as far as that gives idle SMs work.
+int tc_pieces(int64_t blocks, int64_t keys) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / (2 * kTcKeys)));
+  return (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
+}
 constexpr int64_t kBlockKeys = 128, kJoinKeys = 256, kLeastKeys = 128;
 int pieces(int64_t blocks, int64_t keys, int64_t slots) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / kLeastKeys));
@@ -330,7 +336,9 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
     if (kv.dtype == JAL_F32) return std::max(pairs, group_pairs) <= 8 ? 8 : 32;
     return tc && n > kTcLeast ? kTcRows : kMmaRows;
   };
-  auto slots_for = [&](int rows) { return rows == kTcRows ? (int64_t)kPagedSMs : 2 * (int64_t)kPagedSMs; };
+  auto pieces_for = [&](int rows, int64_t blocks, int64_t keys) {
+    return rows == kTcRows ? tc_pieces(blocks, keys) : pieces(blocks, keys, 2 * kPagedSMs);
+  };
   a.rows = rows_for(pairs);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
   int64_t keys = (int64_t)b.max_kv_len;
@@ -338,11 +346,10 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
   if (g && g->n_groups && g->max_prefix_len) {
     a.prefix_rows = rows_for(group_pairs);
     a.prefix_tiles = (int)((group_pairs + a.prefix_rows - 1) / a.prefix_rows);
-    a.prefix_splits = pieces(a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len,
-                             slots_for(a.prefix_rows));
+    a.prefix_splits = pieces_for(a.prefix_rows, a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len);
     keys = std::max<int64_t>(1, keys - (int64_t)g->max_prefix_len);
   }
-  a.splits = pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, slots_for(a.rows));
+  a.splits = pieces_for(a.rows, a.tiles * hkv * (int64_t)b.n_seqs, keys);
   a.direct = a.splits + a.prefix_splits == 1;
   if (!a.direct)
     a.bytes = (size_t)(a.splits + a.prefix_splits) * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;

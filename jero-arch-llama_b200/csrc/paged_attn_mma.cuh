@@ -87,7 +87,7 @@ struct MmaShape {
 };
 
 template <class T, int NS, int HD>
-__global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnParams p, const int part, const bool direct) {
+__global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const __grid_constant__ AttnParams p, const int part, const bool direct) {
   using S = MmaShape<NS, HD>;
   extern __shared__ __align__(128) char smem_raw[];
   __shared__ RowMask masks[kMmaRows];
@@ -104,30 +104,36 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
   // This warp's keys: chunks of 16 of [u0, u1), every fourth.  Lanes 0..15
   // look up where a chunk's keys lie one chunk ahead of its copies.
   const int n_chunks = (t.u1 - t.u0 + kMmaKeys - 1) / kMmaKeys;
-  auto locate = [&](int c) -> int64_t {
+  auto locate = [&](int c) -> Slot {
     const int u = t.u0 + c * kMmaKeys + lane;
-    return lane < kMmaKeys && c < n_chunks && u < t.u1 ? slot_offset(p.kv, t.table, t.head, t.key(u)) : -1;
+    return lane < kMmaKeys && c < n_chunks && u < t.u1 ? slot_of(p.kv, t.table, t.key(u)) : Slot{-1, 0};
   };
-  auto copy = [&](int64_t at, int stage) {
+  auto copy = [&](const Slot &where, int stage) {
+    const int64_t at = slot_offset(p.kv, where, t.head);
     const uint32_t dst = ring + stage * 2 * S::half;
     const uint32_t bits = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
     if (lane == 0) present[warp][stage] = bits;
+    // Eight lanes copy 128 bytes of a row; a lane has the rows lane / 8 + 4 i.
+    const int c8 = lane % 8, r8 = lane / 8;
 #pragma unroll
-    for (int i = 0; i < kMmaKeys * S::chunks / 32; i++) {
-      const int r = (i * 32 + lane) / S::chunks, ch = (i * 32 + lane) % S::chunks;
-      const int64_t o = __shfl_sync(0xffffffffu, at, r);
-      const bool there = o >= 0 && ch * 8 < hd;
-      const int64_t e = there ? o + ch * 8 : 0;
-      const uint32_t d = dst + r * (HD * 2) + ((ch ^ (r & 7)) * 16);
-      copy16(d, (const T *)p.kv.k + e, there);
-      copy16(d + S::half, (const T *)p.kv.v + e, there);
+    for (int i = 0; i < kMmaKeys / 4; i++) {
+      const int64_t o = __shfl_sync(0xffffffffu, at, r8 + 4 * i);
+      const int r = r8 + 4 * i;
+      const uint32_t d = dst + r * (HD * 2) + ((c8 ^ (r & 7)) * 16);
+      const int64_t e = o >= 0 ? o + c8 * 8 : 0;
+#pragma unroll
+      for (int h = 0; h < HD / 64; h++) {
+        const bool there = o >= 0 && h * 64 + c8 * 8 < hd;
+        copy16(d + h * 128, (const T *)p.kv.k + (there ? e + h * 64 : 0), there);
+        copy16(d + S::half + h * 128, (const T *)p.kv.v + (there ? e + h * 64 : 0), there);
+      }
     }
     copies_done();
   };
-  int64_t next = locate(warp);
+  Slot next = locate(warp);
 #pragma unroll
   for (int i = 0; i < S::stages - 1; i++) {
-    const int64_t at = next;
+    const Slot at = next;
     next = locate(warp + (i + 1) * kMmaWarps);
     copy(at, i);
   }
@@ -180,7 +186,10 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
 
   // Rows lane/4 and lane/4 + 8 are this lane's.
   const int r0 = lane / 4;
-  const RowMask m0 = masks[r0], m1 = masks[r0 + 8];
+  // Rows that do not exist see everything: they have no say in what is masked.
+  const RowSpan every = {0x7fffffff, 0, 0};
+  const RowSpan m0 = r0 < t.rows ? row_span(p, t, masks[r0]) : every;
+  const RowSpan m1 = r0 + 8 < t.rows ? row_span(p, t, masks[r0 + 8]) : every;
   const float f0 = q_scale[r0], f1 = q_scale[r0 + 8];
   int lim_lo = 0x7fffffff, lim_hi = 0, wlo_lo = 0x7fffffff, wlo_hi = 0;
   for (int j = 0; j < t.rows; j++) {
@@ -194,12 +203,12 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float top0 = -INFINITY, top1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-  bool bad = false;
+  uint32_t bad = 0;
 
   int stage = 0;
   for (int c = warp; c < n_chunks; c += kMmaWarps) {
     {  // the copies of the chunk stages - 1 ahead
-      const int64_t at = next;
+      const Slot at = next;
       const int ahead = c + (S::stages - 1) * kMmaWarps;
       next = locate(ahead + kMmaWarps);
       int ns = stage + S::stages - 1;
@@ -226,8 +235,9 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
         mma16816<T>(s[1], a, b[2], b[3]);
       }
     }
-    const int u = t.u0 + c * kMmaKeys, first = t.key(u), last = t.key(min(u + kMmaKeys, t.u1) - 1);
-    const bool masked = bits != 0xffffu || first < wlo_hi || last >= lim_lo;
+    const int u = t.u0 + c * kMmaKeys;
+    const bool masked = __any_sync(0xffffffffu, bits != 0xffffu || !m0.all(u, kMmaKeys) || !m1.all(u, kMmaKeys));
+    const uint32_t see0 = bits & m0.bits(u), see1 = bits & m1.bits(u);
 #pragma unroll
     for (int n = 0; n < 2; n++) {
 #pragma unroll
@@ -235,25 +245,20 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
         s[n][e] *= f0;
         s[n][2 + e] *= f1;
         if (masked) {
-          const int i = n * 8 + (lane & 3) * 2 + e, key = t.key(u + i);
-          const bool there = (bits >> i) & 1;
-          if (!there || !m0.sees(key, p.n_sink)) s[n][e] = -INFINITY;
-          if (!there || !m1.sees(key, p.n_sink)) s[n][2 + e] = -INFINITY;
+          const int i = n * 8 + (lane & 3) * 2 + e;
+          if (!((see0 >> i) & 1)) s[n][e] = -INFINITY;
+          if (!((see1 >> i) & 1)) s[n][2 + e] = -INFINITY;
         }
       }
     }
     if (masked && mixed) {  // a value that some rows must not meet
 #pragma unroll
       for (int i = 0; i < kMmaKeys * S::chunks / 32; i++) {
-        uint32_t w[4];
+        uint4 w;
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                      : "r"(vb + (i * 32 + lane) * 16));
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 f = unpack2<T>(w[e]);
-          bad |= !isfinite(f.x) || !isfinite(f.y);
-        }
+        watch8<T>(bad, w);
       }
     }
     float n0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const AttnPar
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
   l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-  if (__syncthreads_or(bad)) {  // (also: no warp reads its ring any more)
+  if (__syncthreads_or(watched_bad<T>(bad))) {  // (also: no warp reads its ring any more)
     for (int j = warp; j < t.rows; j += kMmaWarps) attend_row_alone(p, t, j, direct);
     return;
   }

@@ -34,6 +34,7 @@ namespace jal {
 namespace paged {
 
 constexpr int kTcRows = 256, kTcKeys = 128, kTcThreads = 512;
+constexpr int kPoly = 4;
 constexpr float kTcSlack = 8.0f;  // growth of a maximum (base 2) that is let stand
 
 template <int NS, int HD>
@@ -41,11 +42,62 @@ struct TcShape {
   static constexpr int tile = kTcKeys * HD * 2;            // bytes of a K or V tile
   static constexpr int q_tile = 128 * HD * 2;              // of one part of a row tile
   static constexpr int buffers = HD == 64 ? 6 : NS == 1 ? 5 : 3;
-  // Groups of copies that may be under way when the loader waits for a free
-  // buffer: freeing a V tile takes the next K tile, so buffers - 2 at most.
-  static constexpr int pending = buffers == 3 ? 1 : 2;
   static constexpr int smem = 1024 + 2 * NS * q_tile + buffers * tile;
 };
+
+// ---- pairs of f32 in one instruction
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair(float a, float b) {
+  pair_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpair(pair_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+  pair_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+  pair_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
+// 2^x of a pair on the multiply-add units: x = n + r with n whole and |r| <=
+// 1/2, 2^r by a polynomial whose coefficients were fitted for the least largest
+// relative error on that range (degree 3: 7.5e-5, 4: 2.6e-6, 5: 7.5e-8), n
+// added to the exponent.  x below -126 gives about 2^-126; x is finite.
+template <int DEG>
+__device__ __forceinline__ void exp2_poly(pair_t x2, float &a, float &b) {
+  constexpr float c3[] = {0.9999280728f, 0.6932609870f, 0.2426111351f, 0.05517166682f};
+  constexpr float c4[] = {0.9999992614f, 0.6931218145f, 0.2402474485f, 0.05591786210f, 0.009570101653f};
+  constexpr float c5[] = {1.0000000717f, 0.6931469671f, 0.2402211972f, 0.05550713276f, 0.009675541540f, 0.001327647173f};
+  const float *const c = DEG == 3 ? c3 : DEG == 4 ? c4 : c5;
+  unpair(x2, a, b);
+  x2 = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  constexpr float whole = 12582912.0f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
+  const pair_t t = add2(x2, pair(whole, whole));
+  const pair_t r = add2(x2, fma2(t, pair(-1.0f, -1.0f), pair(whole, whole)));
+  pair_t y = pair(c[DEG], c[DEG]);
+#pragma unroll
+  for (int i = DEG - 1; i >= 0; i--) y = fma2(y, r, pair(c[i], c[i]));
+  float ya, yb, ta, tb;
+  unpair(y, ya, yb);
+  unpair(t, ta, tb);
+  a = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(tb) << 23));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 
 // ---- tcgen05 ----------------------------------------------------------------
 __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead_bytes, uint32_t stride_bytes) {
@@ -106,18 +158,19 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t *r) {
 #undef JAL_I8
 
 struct TcSync {
-  uint64_t q_full;
+  uint64_t q_full, loaded;
   uint64_t kv_full[6], kv_empty[6];
   uint64_t present_full[8];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
   uint32_t tmem;
   int given_up, poison;
   int lim_lo, lim_hi, wlo_lo, wlo_hi;
-  uint32_t present[8][4];  // which keys of tile j exist, by j % 8
+  float q_factor[kTcRows];  // NS = 2: what a row's scores are still to be multiplied by
+  alignas(16) uint32_t present[8][4];  // which keys of tile j exist, by j % 8
 };
 
 template <class T, int NS, int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParams p, const int part, const bool direct) {
+__global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_constant__ AttnParams p, const int part, const bool direct) {
   using S = TcShape<NS, HD>;
   extern __shared__ char smem_raw[];
   __shared__ TcSync sy;
@@ -132,6 +185,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
 
   if (tid == 0) {
     mbar_init(&sy.q_full, 256);
+    mbar_init(&sy.loaded, 128);
     for (int i = 0; i < S::buffers; i++) {
       mbar_init(&sy.kv_full[i], 128);
       mbar_init(&sy.kv_empty[i], 1);
@@ -139,6 +193,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
     for (int i = 0; i < 8; i++) mbar_init(&sy.present_full[i], 4);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sy.s_full[i], 1);
+      mbar_init(&sy.p_half[i], 128);
       mbar_init(&sy.p_full[i], 128);
       mbar_init(&sy.o_full[i], 1);
     }
@@ -170,126 +225,165 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
     if (warp < 12) {
       // ---- the loader
       const int w = warp - 8;
-      auto locate = [&](int j) -> int64_t {
+      auto locate = [&](int j) -> Slot {
         const int u = t.u0 + j * kTcKeys + w * 32 + lane;
-        return j < n_tiles && u < t.u1 ? slot_offset(p.kv, t.table, t.head, t.key(u)) : -1;
+        return j < n_tiles && u < t.u1 ? slot_of(p.kv, t.table, t.key(u)) : Slot{-1, 0};
       };
-      constexpr int CH = HD / 8, N = 32 * CH / 32;
-      bool ok = true, bad = false;
-      int arrived = 0;
-      // Group g (K tile g / 2 when even, V tile when odd) has landed: rows that
-      // some queries must not meet are looked through, then it is handed over.
-      auto hand_over = [&](int g) {
-        const int b = g % S::buffers;
-        if (g & 1) {
-          const int u = t.u0 + (g >> 1) * kTcKeys, first = t.key(u), last = t.key(min(u + kTcKeys, t.u1) - 1);
-          if (g == 1) ok = ok && wait(&sy.q_full, 0);
-          const bool mixed = (first < sy.wlo_hi && sy.wlo_lo != sy.wlo_hi) || (last >= sy.lim_lo && sy.lim_lo != sy.lim_hi);
-          if (mixed) {
-            const char *rows = base_p + 2 * NS * S::q_tile + b * S::tile + (w * 32) * 128;
-#pragma unroll 4
-            for (int i = 0; i < HD / 64 * 8; i++) {  // 32 rows x 128 bytes x (HD / 64) of this warp
-              const uint4 x = *(const uint4 *)(rows + (i / 8) * (kTcKeys * 128) + ((i % 8) * 32 + lane) * 16);
-              const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+      // Eight lanes copy 128 bytes of a row; a lane has the rows lane / 8 + 4 i
+      // of the warp's 32.  Their addresses are passed round once for K and V.
+      const int c8 = lane % 8, r8 = lane / 8;
+      const uint32_t to_even = (w * 32 + r8) * 128 + ((c8 ^ r8) * 16), to_odd = (w * 32 + r8) * 128 + ((c8 ^ (r8 + 4)) * 16);
+      // Copies arrive on the buffer's barrier by themselves; the thread that
+      // issues the products puts the fence between them and the tensor cores.
+      uint32_t bad = 0;
+      bool ok = true, ranges = false;
+      int b = 0, parity = 1;  // of the buffer's "empty" phase before this use: the first use finds it free
+      auto copy = [&](const void *pool_v, const int64_t (&from)[8]) {
+        ok = __all_sync(0xffffffffu, ok && wait(&sy.kv_empty[b], parity));
+        if (!ok) return;
+        const char *const pool = (const char *)pool_v + c8 * 16;
+        const uint32_t dst = ring + b * S::tile;
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const float2 f = unpack2<T>(v[e]);
-                bad |= !isfinite(f.x) || !isfinite(f.y);
-              }
-            }
-            if (bad) sy.poison = 1;
+        for (int i = 0; i < 8; i++) {
+          const char *const src = pool + from[i] * 2;
+          const uint32_t to = dst + (i & 1 ? to_odd : to_even) + i * 512;
+#pragma unroll
+          for (int h = 0; h < HD / 64; h++) {
+            const bool there = from[i] >= 0 && h * 64 + c8 * 8 < hd;
+            copy16(to + h * (kTcKeys * 128), there ? src + h * 128 : (const char *)pool_v, there);
           }
         }
-        fence_proxy_async();
-        mbar_arrive(&sy.kv_full[b]);
-        arrived = g + 1;
+        copies_done();
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sy.kv_full[b])) : "memory");
+        if (++b == S::buffers) {
+          b = 0;
+          parity ^= 1;
+        }
       };
-      int64_t next = locate(0);
-      for (int j = 0; j < n_tiles && ok; j++) {
-        const int64_t at = next;
+      // Looks through the V tile in buffer vb for values that some queries must not meet.
+      auto scan = [&](int vb) {
+        const char *rows = base_p + 2 * NS * S::q_tile + vb * S::tile + (w * 32) * 128;
+#pragma unroll 4
+        for (int i = 0; i < HD / 64 * 8; i++)  // 32 rows x 128 bytes x (HD / 64) of this warp
+          watch8<T>(bad, *(const uint4 *)(rows + (i / 8) * (kTcKeys * 128) + ((i % 8) * 32 + lane) * 16));
+      };
+      Slot next = locate(0);
+      int scan_b = -1;
+#pragma unroll 1
+      for (int j = 0; j < n_tiles; j++) {
+        const int64_t at = slot_offset(p.kv, next, t.head);
         const uint32_t bits = __ballot_sync(0xffffffffu, at >= 0);
         next = locate(j + 1);
+        int64_t from[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) from[i] = __shfl_sync(0xffffffffu, at, r8 + 4 * i);
         if (lane == 0) {  // tile j + 8 comes long after the softmax has read tile j's
           sy.present[j & 7][w] = bits;
           mbar_arrive(&sy.present_full[j & 7]);
         }
-#pragma unroll 1
-        for (int kv = 0; kv < 2 && ok; kv++) {
-          const int g = 2 * j + kv, b = g % S::buffers;
-          if (g >= S::buffers) ok = wait(&sy.kv_empty[b], (g / S::buffers - 1) & 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const T *pool = (const T *)(kv ? p.kv.v : p.kv.k);
-          const uint32_t dst = ring + b * S::tile;
-#pragma unroll
-          for (int i = 0; i < N; i++) {
-            const int r = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH, row = w * 32 + r;
-            const int64_t o = __shfl_sync(0xffffffffu, at, r);
-            const bool there = o >= 0 && c * 8 < hd;
-            copy16(dst + (c / 8) * (kTcKeys * 128) + row * 128 + (((c % 8) ^ (row & 7)) * 16),
-                   pool + (there ? o + c * 8 : 0), there);
-          }
-          copies_done();
-          if (g >= S::pending) {
-            copies_wait<S::pending>();
-            hand_over(g - S::pending);
-          }
+        copy(p.kv.k, from);
+        const int vb = b;
+        copy(p.kv.v, from);
+        if (!ok) break;
+        if (scan_b >= 0) {  // the tile before; its buffer is not filled again before the next round
+          copies_wait<2>();
+          __syncwarp();
+          scan(scan_b);
         }
+        if (!ranges) {
+          ok = __all_sync(0xffffffffu, wait(&sy.q_full, 0));
+          ranges = true;
+        }
+        const int u = t.u0 + j * kTcKeys, first = t.key(u), last = t.key(min(u + kTcKeys, t.u1) - 1);
+        const bool mixed = (first < sy.wlo_hi && sy.wlo_lo != sy.wlo_hi) || (last >= sy.lim_lo && sy.lim_lo != sy.lim_hi);
+        scan_b = mixed ? vb : -1;
       }
       copies_wait<0>();
-      if (ok) {
-#pragma unroll 1
-        for (int g = arrived; g < 2 * n_tiles; g++) hand_over(g);
-      }
-    } else if (warp == 12 && lane == 0) {
-      // ---- the products
+      __syncwarp();
+      if (scan_b >= 0) scan(scan_b);
+      if (watched_bad<T>(bad)) sy.poison = 1;
+      mbar_arrive(&sy.loaded);
+    } else if (warp == 12) {
+      // ---- the products: the whole warp runs the loop, so that addresses stay
+      // uniform, and one lane issues
+      const bool leader = elect_one();
       constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t id = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);
       constexpr uint32_t id_s = id | ((kTcKeys >> 3) << 17), id_o = id | (1u << 16) | ((HD >> 3) << 17);
-      auto scores = [&](int i, int j) {
-        const uint32_t kb = ring + ((2 * j) % S::buffers) * S::tile;
+      const uint64_t q_desc = tc_desc(sq, 16, 1024), k_desc = tc_desc(ring, 16, 1024),
+                     v_desc = tc_desc(ring, kTcKeys * 128, 1024);
+      auto scores = [&](int i, int kb) {
+        if (leader) {
+          const uint64_t a = q_desc + (uint32_t)(i * NS * (S::q_tile >> 4)), b = k_desc + (uint32_t)(kb * (S::tile >> 4));
 #pragma unroll
-        for (int s = 0; s < NS; s++)
+          for (int s = 0; s < NS; s++)
 #pragma unroll
-          for (int k = 0; k < HD / 16; k++) {
-            const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-            tc_mma_ss(tmem + i * 128, tc_desc(sq + (i * NS + s) * S::q_tile + off, 16, 1024), tc_desc(kb + off, 16, 1024),
-                      id_s, s + k > 0);
-          }
-        tc_commit(&sy.s_full[i]);
+            for (int k = 0; k < HD / 16; k++) {
+              const uint32_t off = ((k / 4) * (128 * 128) + (k % 4) * 32) >> 4;
+              tc_mma_ss(tmem + i * 128, a + (uint32_t)(s * (S::q_tile >> 4) + off), b + off, id_s, s + k > 0);
+            }
+          tc_commit(&sy.s_full[i]);
+        }
+        __syncwarp();
       };
-      auto output = [&](int i, int j) {
-        const uint32_t vb = ring + ((2 * j + 1) % S::buffers) * S::tile;
+      auto output = [&](int i, int vb, bool first, int half) {  // 64 of the keys
+        if (leader) {
+          const uint64_t b = v_desc + (uint32_t)(vb * (S::tile >> 4) + half * 4 * (2048 >> 4));
+          const uint32_t a = tmem + i * 128 + half * 32;
 #pragma unroll
-        for (int s = 0; s < NS; s++)
+          for (int s = 0; s < NS; s++)
 #pragma unroll
-          for (int k = 0; k < kTcKeys / 16; k++)
-            tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + s * 64 + k * 8, tc_desc(vb + k * 2048, kTcKeys * 128, 1024), id_o,
-                      j > 0 || s + k > 0);
+            for (int q = 0; q < 4; q++)
+              tc_mma_ts(tmem + 256 + i * 128, a + s * 64 + q * 8, b + (uint32_t)(q * (2048 >> 4)), id_o,
+                        !first || s + q > 0);
+        }
+        __syncwarp();
       };
-      auto full = [&](int g) { return wait(&sy.kv_full[g % S::buffers], (g / S::buffers) & 1); };
-      bool ok = n_tiles == 0 || (wait(&sy.q_full, 0) && full(0));
+      auto release = [&](int b) {
+        if (leader) tc_commit(&sy.kv_empty[b]);
+        __syncwarp();
+      };
+      int b = 0, parity = 0;  // the next buffer to be taken
+      auto take = [&](int &got) {
+        const bool there = wait(&sy.kv_full[b], parity);
+        fence_proxy_async();  // the rows were written by cp.async, the tensor cores read them by the async proxy
+        got = b;
+        if (++b == S::buffers) {
+          b = 0;
+          parity ^= 1;
+        }
+        return there;
+      };
+      int kb = 0, vb = 0;
+      bool ok = n_tiles == 0 || (wait(&sy.q_full, 0) && take(kb));
       if (ok && n_tiles) {
         tc_fence_after();
-        scores(0, 0);
-        scores(1, 0);
-        tc_commit(&sy.kv_empty[0]);
+        scores(0, kb);
+        scores(1, kb);
+        release(kb);
       }
+#pragma unroll 1
       for (int j = 0; j < n_tiles && ok; j++) {
-        for (int i = 0; i < 2 && ok; i++) {
-          ok = (i || full(2 * j + 1)) && wait(&sy.p_full[i], j & 1);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          ok = ok && (i || take(vb)) && wait(&sy.p_half[i], j & 1);
           if (!ok) break;
           tc_fence_after();
-          output(i, j);
-          if (i) tc_commit(&sy.kv_empty[(2 * j + 1) % S::buffers]);
+          output(i, vb, j == 0, 0);
+          ok = wait(&sy.p_full[i], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          output(i, vb, false, 1);
+          if (i) release(vb);
           if (j + 1 < n_tiles) {
-            ok = i || full(2 * j + 2);
+            ok = i || take(kb);
             if (!ok) break;
             tc_fence_after();
-            scores(i, j + 1);
-            if (i) tc_commit(&sy.kv_empty[(2 * j + 2) % S::buffers]);
+            scores(i, kb);
+            if (i) release(kb);
           } else {
-            tc_commit(&sy.o_full[i]);
+            if (leader) tc_commit(&sy.o_full[i]);
+            __syncwarp();
           }
         }
       }
@@ -308,46 +402,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
       char *const dst_p = base_p + i * NS * S::q_tile;
       const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
       const bool take = real && p.scale_log2 != 0.0f;
-      float a = 1.0f, b = 1.0f;
-      if (NS == 2) {
-        float top = 0.0f;
-        for (int d = 0; real && d < hd; d += 8) {
-          float v[8];
-          load8((const float *)p.q + qo + d, v);
+      // The 32 rows of a warp are read by all its lanes, neighbouring lanes
+      // neighbouring pieces of eight elements.
+      constexpr int CH = HD / 8;
+      const int64_t qt = take ? qo : -1;
+      const int i_row = row & ~31;  // the warp's first row
+      if constexpr (NS == 1) {
+        const int c8 = lane % 8, r8 = lane / 8;
+        uint4 w[8][HD / 64];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int64_t o = __shfl_sync(0xffffffffu, qt, r8 + 4 * k);
+#pragma unroll
+          for (int h = 0; h < HD / 64; h++)
+            w[k][h] = o >= 0 && h * 64 + c8 * 8 < hd ? *(const uint4 *)((const T *)p.q + o + h * 64 + c8 * 8)
+                                                     : make_uint4(0, 0, 0, 0);
+        }
+        char *const even = dst_p + ((r & ~31) + r8) * 128 + ((c8 ^ r8) * 16);
+        char *const odd = dst_p + ((r & ~31) + r8) * 128 + ((c8 ^ (r8 + 4)) * 16);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+#pragma unroll
+          for (int h = 0; h < HD / 64; h++) {
+            const uint4 x = w[k][h];
+            *(uint4 *)((k & 1 ? odd : even) + k * 512 + h * (128 * 128)) =
+                make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+          }
+      } else {
+#pragma unroll 4
+        for (int i = 0; i < CH; i++) {
+          const int k = (i * 32 + lane) / CH, c = lane % CH;
+          const int64_t o = __shfl_sync(0xffffffffu, qt, k);
+          float v[8] = {}, top = 0.0f;
+          if (o >= 0 && c * 8 < hd) load8((const float *)p.q + o + c * 8, v);
 #pragma unroll
           for (int e = 0; e < 8; e++)
             if (fabsf(v[e]) < INFINITY) top = fmaxf(top, fabsf(v[e]));
-        }
-        const int e = top > 0.0f ? 13 - ilogbf(top) : 0;
-        a = exp2f((float)(e / 2));
-        b = exp2f((float)(e - e / 2));
-        scale *= (1.0f / a) / b;
-        if (flip) a = -a;
-      }
-#pragma unroll 4
-      for (int c = 0; c < HD / 8; c++) {
-        uint4 out[NS];
-        if (NS == 1) {
-          out[0] = make_uint4(0, 0, 0, 0);
-          if (take && c * 8 < hd) {
-            out[0] = *(const uint4 *)((const T *)p.q + qo + c * 8);
-            out[0].x ^= flip;
-            out[0].y ^= flip;
-            out[0].z ^= flip;
-            out[0].w ^= flip;
-          }
-        } else {
-          float v[8] = {};
-          if (take && c * 8 < hd) load8((const float *)p.q + qo + c * 8, v);
+#pragma unroll
+          for (int x = CH / 2; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const int e = top > 0.0f ? 13 - ilogbf(top) : 0;
+          const float a = (flip ? -1.0f : 1.0f) * exp2f((float)(e / 2)), b = exp2f((float)(e - e / 2));
           uint32_t part2[4][NS];
 #pragma unroll
-          for (int e = 0; e < 4; e++) split2<T, NS>(v[2 * e] * a * b, v[2 * e + 1] * a * b, part2[e]);
+          for (int q = 0; q < 4; q++) split2<T, NS>(v[2 * q] * a * b, v[2 * q + 1] * a * b, part2[q]);
+          const int kr = (r & ~31) + k;
 #pragma unroll
-          for (int s = 0; s < NS; s++) out[s] = make_uint4(part2[0][s], part2[1][s], part2[2][s], part2[3][s]);
+          for (int s = 0; s < NS; s++)
+            *(uint4 *)(dst_p + s * S::q_tile + (c / 8) * (128 * 128) + kr * 128 + (((c % 8) ^ (kr & 7)) * 16)) =
+                make_uint4(part2[0][s], part2[1][s], part2[2][s], part2[3][s]);
+          if (c == 0) sy.q_factor[i_row + k] = (1.0f / fabsf(a)) / b;
         }
-#pragma unroll
-        for (int s = 0; s < NS; s++)
-          *(uint4 *)(dst_p + s * S::q_tile + (c / 8) * (128 * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16)) = out[s];
+        __syncwarp();
+        scale *= sy.q_factor[row];
       }
       int lo = real ? mk.lim : 0x7fffffff, hi = real ? mk.lim : 0, wl = real ? mk.wlo : 0x7fffffff, wh = real ? mk.wlo : 0;
       lo = __reduce_min_sync(0xffffffffu, lo);
@@ -365,6 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
     }
     const uint32_t quarter = (uint32_t)(warp % 4) << 21;  // lane 32 (warp % 4) of the tensor memory
     const uint32_t ts = tmem + i * 128 + quarter, to = tmem + 256 + i * 128 + quarter;
+    const RowSpan span = row_span(p, t, mk);
     float m = -INFINITY, l = 0.0f;  // m: what the weights refer to, scaled to base 2
     bool ok = true;
     for (int j = 0; j < n_tiles; j++) {
@@ -375,23 +482,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
 #pragma unroll
       for (int c = 0; c < 4; c++) tc_ld32(ts + c * 32, (uint32_t *)s + c * 32);
       tc_wait_ld();
-      const int u = t.u0 + j * kTcKeys, first = t.key(u), last = t.key(min(u + kTcKeys, t.u1) - 1);
-      const uint32_t *here = sy.present[j & 7];
-      const bool whole = (here[0] & here[1] & here[2] & here[3]) == 0xffffffffu && first >= mk.wlo && last < mk.lim;
-      if (!__all_sync(0xffffffffu, whole || !real)) {
+      const int u = t.u0 + j * kTcKeys;
+      const uint4 here = *(const uint4 *)sy.present[j & 7];
+      const bool whole = (here.x & here.y & here.z & here.w) == 0xffffffffu && span.all(u, kTcKeys);
+      const bool masked = !__all_sync(0xffffffffu, whole || !real);
+      if (masked) {
+        const uint32_t bits[4] = {here.x & span.bits(u), here.y & span.bits(u + 32), here.z & span.bits(u + 64),
+                                  here.w & span.bits(u + 96)};
 #pragma unroll
         for (int c = 0; c < 128; c++)
-          if (!((here[c / 32] >> (c % 32)) & 1) || !mk.sees(t.key(u + c), p.n_sink)) s[c] = -INFINITY;
+          if (!((bits[c / 32] >> (c % 32)) & 1)) s[c] = -INFINITY;
       }
       float x[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < 128; c += 4) {
-        x[0] = fmaxf(x[0], s[c]);
-        x[1] = fmaxf(x[1], s[c + 1]);
-        x[2] = fmaxf(x[2], s[c + 2]);
-        x[3] = fmaxf(x[3], s[c + 3]);
+      for (int c = 4; c < 124; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = max3_nan(x[e], s[c + 2 * e], s[c + 2 * e + 1]);
       }
-      const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * scale;
+      const float top = max3_nan(max3_nan(x[0], x[1], s[124]), max3_nan(x[2], x[3], s[125]), max3_nan(s[126], s[127], s[127])) * scale;
+      // A NaN or an infinite score makes the row NaN, as the formula does; it
+      // need not come through the weights.
+      if (!(top < INFINITY)) l = NAN;
       // Raise the reference of the rows that need it (the first tile's all).
       // O is at rest: its products up to tile j - 1 were done before S.
       const bool raise = top > m + kTcSlack || (m == -INFINITY && top > m);
@@ -412,42 +523,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
         }
       }
       const float ref = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {};
+      // The weights.  The special-function units would be the slowest part, so
+      // where nothing is masked every kPoly-th pair goes by the polynomial.
+      pair_t sum[2] = {0, 0};
+      const pair_t scale2 = pair(scale, scale), ref2 = pair(-ref, -ref);
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t w[NS][16];
+        for (int c = 0; c < 4; c++) {
+          uint32_t w[NS][16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float a = exp2_fast(fmaf(s[c * 32 + 2 * e], scale, -ref)), b = exp2_fast(fmaf(s[c * 32 + 2 * e + 1], scale, -ref));
-          sum[e % 4] += a + b;
-          uint32_t part2[NS];
-          split2<T, NS>(a, b, part2);
+          for (int e = 0; e < 16; e++) {
+            const pair_t x2 = fma2(pair(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), scale2, ref2);
+            float a, b;
+            if (poly && e % kPoly == kPoly - 1) {
+              exp2_poly<NS == 2 ? 5 : std::is_same<T, __half>::value ? 4 : 3>(x2, a, b);
+            } else {
+              unpair(x2, a, b);
+              a = exp2_fast(a);
+              b = exp2_fast(b);
+            }
+            sum[e % 2] = add2(sum[e % 2], pair(a, b));
+            uint32_t part2[NS];
+            split2<T, NS>(a, b, part2);
 #pragma unroll
-          for (int q = 0; q < NS; q++) w[q][e] = part2[q];
+            for (int q = 0; q < NS; q++) w[q][e] = part2[q];
+          }
+#pragma unroll
+          for (int q = 0; q < NS; q++) tc_st16(ts + q * 64 + c * 16, w[q]);
+          if (c == 1) {  // the products of the first half of the keys can start
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sy.p_half[i]);
+          }
         }
-#pragma unroll
-        for (int q = 0; q < NS; q++) tc_st16(ts + q * 64 + c * 16, w[q]);
+      };
+      if (masked) weights(std::false_type{});
+      else weights(std::true_type{});
+      {
+        float a, b;
+        unpair(add2(sum[0], sum[1]), a, b);
+        l += a + b;
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&sy.p_full[i]);
     }
     // ---- the result
-    // Poison is final once the loader has handed over the last V tile.
-    const int last_v = 2 * n_tiles - 1;
-    if (ok && n_tiles)
-      ok = __all_sync(0xffffffffu, wait(&sy.o_full[i], 0) &&
-                                       wait(&sy.kv_full[last_v % S::buffers], (last_v / S::buffers) & 1));
+    // Poison is final once the loader is through.
+    ok = __all_sync(0xffffffffu, ok && (!n_tiles || wait(&sy.o_full[i], 0)) && wait(&sy.loaded, 0));
     tc_fence_after();
     if (!ok || *given_up || *(volatile int *)&sy.poison) {
       for (int k = warp * 32; k < min(warp * 32 + 32, t.rows); k++) attend_row_alone(p, t, k, direct);
     } else {
-      const int64_t oo = real ? out_offset(p, t, row) : 0, pi = real ? part_index(p, t, row) : 0;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      if (real && !direct) p.part_ml[pi] = make_float2(m, l);
+      // 32 dims at a time through the warp's 4 KB of the query tiles' memory
+      // (no product reads it any more), so that rows are stored in whole lines.
+      if (!n_tiles) wait(&sy.q_full, 0);
+      const int64_t at = !real ? -1 : direct ? out_offset(p, t, row) : part_index(p, t, row) * hd;
+      const float inv = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+      if (real && !direct) p.part_ml[part_index(p, t, row)] = make_float2(m, l);
+      char *const stage = base_p + warp * 4096;
+      const bool wide = !direct || NS == 2;  // f32 rows
 #pragma unroll 1
-      for (int d = 0; d < HD; d += 32) {
+      for (int d = 0; d < HD && d < hd; d += 32) {
         float o[32];
         __syncwarp();
         if (n_tiles) {
@@ -458,14 +595,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const AttnParam
           for (int e = 0; e < 32; e++) o[e] = 0.0f;
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (!real || d + e >= hd) continue;
-          float v[8];
+        for (int e = 0; e < 32; e++) o[e] *= inv;
+        if (wide) {
 #pragma unroll
-          for (int k = 0; k < 8; k++) v[k] = direct ? o[e + k] * inv : o[e + k];
-          if (!direct) store8(p.part_o + pi * hd + d + e, v);
-          else if (NS == 2) store8((float *)p.out + oo + d + e, v);
-          else store8((T *)p.out + oo + d + e, v);
+          for (int c = 0; c < 8; c++)
+            *(float4 *)(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
+                make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+            *(uint4 *)(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
+                make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
+                           pack2<T>(o[8 * c + 4], o[8 * c + 5]), pack2<T>(o[8 * c + 6], o[8 * c + 7]));
+        }
+        __syncwarp();
+        if (wide) {
+          float *const out = direct ? (float *)p.out : p.part_o;
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            const int rr = k * 4 + lane / 8, c = lane % 8;
+            const int64_t o2 = __shfl_sync(0xffffffffu, at, rr);
+            const float4 v = *(const float4 *)(stage + rr * 128 + ((c ^ (rr & 7)) * 16));
+            if (o2 >= 0 && d + c * 4 < hd) *(float4 *)(out + o2 + d + c * 4) = v;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int rr = k * 8 + lane / 4, c = lane % 4;
+            const int64_t o2 = __shfl_sync(0xffffffffu, at, rr);
+            const uint4 v = *(const uint4 *)(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) * 16));
+            if (o2 >= 0 && d + c * 8 < hd) *(uint4 *)((T *)p.out + o2 + d + c * 8) = v;
+          }
         }
       }
     }

@@ -68,6 +68,26 @@ __device__ __forceinline__ void load8<float>(const float *p, float (&v)[8]) {
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
+// Adds x * 0 of eight 16-bit elements: NaN in acc once an element was not finite.
+template <class T>
+__device__ __forceinline__ void watch8(uint32_t &acc, const uint4 &x);
+template <>
+__device__ __forceinline__ void watch8<__half>(uint32_t &acc, const uint4 &x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w[i]), "r"(0u));
+}
+template <>
+__device__ __forceinline__ void watch8<__nv_bfloat16>(uint32_t &acc, const uint4 &x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w[i]), "r"(0u));
+}
+template <class T>
+__device__ __forceinline__ bool watched_bad(uint32_t acc) {
+  const float2 f = unpack2<T>(acc);
+  return f.x != f.x || f.y != f.y;
+}
 template <class T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
   *(uint4 *)p = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
@@ -86,27 +106,39 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Element offset of position t's row of `head`, or -1 where the table names no
-// page of the pool (such a key counts as masked and is not read).
-__device__ __forceinline__ int64_t slot_offset(const PagedView &kv, const int32_t *table_row, int head, int t) {
+// Where position t's row of `head` lies.  In two steps, so that the table entry
+// can be asked for long before it is needed: `page` is the entry as found.
+struct Slot {
+  int page, slot;
+};
+__device__ __forceinline__ Slot slot_of(const PagedView &kv, const int32_t *table_row, int t) {
   const int pi = kv.page_shift >= 0 ? t >> kv.page_shift : t / kv.page_size;
-  const int slot = kv.page_shift >= 0 ? t & (kv.page_size - 1) : t - pi * kv.page_size;
-  const int page = __ldg(table_row + pi);
-  if ((unsigned)page >= (unsigned)kv.n_pages) return -1;
-  return (int64_t)page * kv.page_stride + (int64_t)head * kv.head_stride + (int64_t)slot * kv.slot_stride;
+  int page;  // (volatile: the load stays where it is asked for)
+  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(page) : "l"(table_row + pi));
+  return {page, kv.page_shift >= 0 ? t & (kv.page_size - 1) : t - pi * kv.page_size};
+}
+// The element offset, or -1 where the entry is no page of the pool (such a
+// key counts as masked and is not read).
+__device__ __forceinline__ int64_t slot_offset(const PagedView &kv, const Slot &s, int head) {
+  const int64_t at = (int64_t)s.page * kv.page_stride + (int64_t)head * kv.head_stride + (int64_t)s.slot * kv.slot_stride;
+  return (unsigned)s.page < (unsigned)kv.n_pages ? at : -1;
+}
+__device__ __forceinline__ int64_t slot_offset(const PagedView &kv, const int32_t *table_row, int head, int t) {
+  return slot_offset(kv, slot_of(kv, table_row, t), head);
 }
 
 // Rows [beg, end) of sequence s, kept inside the batch whatever q_start says.
 __device__ __forceinline__ void seq_rows(const int32_t *q_start, int n_rows, int s, int &beg, int &end) {
-  beg = min(max(q_start[s], 0), n_rows);
-  end = min(max(q_start[s + 1], beg), n_rows);
+  const int b = __ldg(q_start + s), e = __ldg(q_start + s + 1);
+  beg = min(max(b, 0), n_rows);
+  end = min(max(e, beg), n_rows);
 }
 // The sequence in [lo, hi) that holds row r (q_start ascending): the last one
 // that starts at or before it.
 __device__ __forceinline__ int seq_of_row(const int32_t *q_start, int lo, int hi, int r) {
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (q_start[mid] <= r) lo = mid; else hi = mid;
+    if (__ldg(q_start + mid) <= r) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -126,17 +158,21 @@ struct Tile {
   int slot;              // partial slot the results go to
   int limit;             // prefix tiles: keys end here for every row
   int seq_lo, seq_hi;    // sequences whose rows these are
+  int64_t shift;         // one sequence: a token row's position is row + shift
   __device__ __forceinline__ int key(int u) const { return u < ns ? u : lo + (u - ns); }
 };
 
-// Position of token row r, and -1 - (what it is) below zero for rows that see
-// nothing.
+// Position of token row r: -1 before the first position (such a row sees
+// nothing), at most the last position of the table.
+__device__ __forceinline__ int clamp_position(const AttnParams &p, int64_t pos) {
+  return pos < 0 ? -1 : pos >= p.kv.cap ? p.kv.cap - 1 : (int)pos;
+}
 __device__ __forceinline__ int row_position(const AttnParams &p, const Tile &t, int r) {
-  const int s = t.seq_hi - t.seq_lo > 1 ? seq_of_row(p.q_start, t.seq_lo, t.seq_hi, r) : t.seq_lo;
+  if (t.seq_hi - t.seq_lo == 1) return clamp_position(p, r + t.shift);
+  const int s = seq_of_row(p.q_start, t.seq_lo, t.seq_hi, r);
   int b, e;
   seq_rows(p.q_start, p.n_rows, s, b, e);
-  const int64_t pos = (int64_t)p.kv_len[s] - (e - r);
-  return pos < 0 ? -1 : pos >= p.kv.cap ? p.kv.cap - 1 : (int)pos;
+  return clamp_position(p, (int64_t)__ldg(p.kv_len + s) - (e - r));
 }
 
 // Tile `tile` (of `rt` rows) and piece `piece` of block (seq or group) `z`;
@@ -147,14 +183,21 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
   t.head = head;
   t.seq_lo = z;
   t.seq_hi = z + 1;
+  int prefix_len = 0;
   if (prefix) {
-    t.seq_lo = min(max(p.group_start[z], 0), p.n_seqs);
-    t.seq_hi = min(max(p.group_start[z + 1], t.seq_lo), p.n_seqs);
+    const int a = __ldg(p.group_start + z), b = __ldg(p.group_start + z + 1);
+    prefix_len = __ldg(p.prefix_len + z);
+    t.seq_lo = min(max(a, 0), p.n_seqs);
+    t.seq_hi = min(max(b, t.seq_lo), p.n_seqs);
     if (t.seq_lo == t.seq_hi) return false;
   }
-  int e;
+  const int len = __ldg(p.kv_len + t.seq_lo);  // (independent of the rows' loads)
   seq_rows(p.q_start, p.n_rows, t.seq_lo, t.beg, t.end);
-  if (t.seq_hi - t.seq_lo > 1) seq_rows(p.q_start, p.n_rows, t.seq_hi - 1, e, t.end);
+  t.shift = (int64_t)len - t.end;
+  if (t.seq_hi - t.seq_lo > 1) {
+    int e;
+    seq_rows(p.q_start, p.n_rows, t.seq_hi - 1, e, t.end);
+  }
   int n_tok = t.end - t.beg;
   if (!prefix) n_tok = min(n_tok, p.max_q);
   t.first = tile * rt;
@@ -165,7 +208,7 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
   t.slot = (prefix ? 0 : p.prefix_splits) + piece;
   t.limit = 0x7fffffff;
   if (prefix) {
-    t.limit = min(max(p.prefix_len[z], 0), p.kv.cap);
+    t.limit = min(max(prefix_len, 0), p.kv.cap);
     t.ns = t.lo = 0;
     t.hi = t.limit;
   } else {
@@ -174,14 +217,15 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
     t.lo = p.window > 0 ? max(0, pf + 1 - p.window) : 0;
     if (p.n_groups) {  // the keys behind the shared prefix of the sequence's group
       const int g = seq_of_row(p.group_start, 0, p.n_groups, t.seq_lo);
-      const bool in = p.group_start[g] <= t.seq_lo && t.seq_lo < p.group_start[g + 1];
-      t.lo = in ? min(max(p.prefix_len[g], 0), p.kv.cap) : 0;
+      const int a = __ldg(p.group_start + g), b = __ldg(p.group_start + g + 1), n = __ldg(p.prefix_len + g);
+      t.lo = a <= t.seq_lo && t.seq_lo < b ? min(max(n, 0), p.kv.cap) : 0;
     }
     t.lo = min(t.lo, t.hi);
     t.ns = min(p.n_sink, t.lo);
   }
   const int total = t.ns + (t.hi - t.lo);
-  const int per = (int)(((int64_t)total + (int64_t)splits * key_align - 1) / ((int64_t)splits * key_align)) * key_align;
+  const uint32_t step = (uint32_t)splits * key_align;  // (total + step stays below 2^32)
+  const int per = (int)(((uint32_t)total + step - 1) / step) * key_align;
   t.u0 = (int)min((int64_t)total, (int64_t)piece * per);
   t.u1 = (int)min((int64_t)total, (int64_t)t.u0 + per);
   return true;
@@ -192,16 +236,18 @@ enum Part { kBoth, kPrefix, kOwn };
 // Which tile a block of the flat grid works on: first the shared prefixes'
 // (piece fastest, then tile, head, group), then the sequences'.
 __device__ __forceinline__ bool block_tile(const AttnParams &p, int part, int rt, int key_align, Tile &t) {
-  int64_t b = blockIdx.x;
-  const int64_t np = part == kOwn ? 0 : (int64_t)p.prefix_splits * p.prefix_tiles * p.kv.hkv * p.n_groups;
+  uint32_t b = blockIdx.x;  // (32-bit divisions: the grid is below 2^31)
+  const uint32_t np = part == kOwn ? 0 : (uint32_t)(p.prefix_splits * p.prefix_tiles) * (uint32_t)(p.kv.hkv * p.n_groups);
   const bool prefix = b < np;
   if (!prefix) b -= np;
-  const int splits = prefix ? p.prefix_splits : p.splits, tiles = prefix ? p.prefix_tiles : p.tiles;
-  const int piece = (int)(b % splits);
-  b /= splits;
-  const int tile = tiles - 1 - (int)(b % tiles);  // the last rows see the most keys: first
-  b /= tiles;
-  return make_tile(p, prefix, (int)(b / p.kv.hkv), (int)(b % p.kv.hkv), tile, piece, rt, key_align, t);
+  const uint32_t splits = prefix ? p.prefix_splits : p.splits, tiles = prefix ? p.prefix_tiles : p.tiles, hkv = p.kv.hkv;
+  uint32_t rest = b / splits;
+  const int piece = (int)(b - rest * splits);
+  b = rest;
+  rest = b / tiles;
+  const int tile = (int)(tiles - 1 - (b - rest * tiles));  // the last rows see the most keys: first
+  const uint32_t z = rest / hkv;
+  return make_tile(p, prefix, (int)z, (int)(rest - z * hkv), tile, piece, rt, key_align, t);
 }
 
 // What row j of the tile may see: keys t < lim with t >= wlo or t < sink.
@@ -215,6 +261,25 @@ __device__ __forceinline__ RowMask row_mask(const AttnParams &p, const Tile &t, 
   m.lim = min(pos + 1, t.limit);
   m.wlo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
   return m;
+}
+// The same over the key numbers u of the tile: a row sees u < end with u <
+// sink or u >= near, whose bounds do not depend on u.
+struct RowSpan {
+  int end, sink, near;
+  // Is all of [u, u + n) seen?
+  __device__ __forceinline__ bool all(int u, int n) const { return u + n <= end && (u >= near || u + n <= sink); }
+  // Which of the 32 keys from u on are seen.
+  __device__ __forceinline__ uint32_t bits(int u) const {
+    return below(end - u) & (below(sink - u) | ~below(near - u));
+  }
+  static __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+};
+__device__ __forceinline__ RowSpan row_span(const AttnParams &p, const Tile &t, const RowMask &m) {
+  RowSpan s;
+  s.end = m.lim > t.lo ? t.ns + (m.lim - t.lo) : min(m.lim, t.ns);
+  s.sink = t.ns + max(0, p.n_sink - t.lo);
+  s.near = t.ns + max(0, m.wlo - t.lo);
+  return s;
 }
 __device__ __forceinline__ int64_t q_offset(const AttnParams &p, const Tile &t, int j) {
   const int pair = t.first + j;
