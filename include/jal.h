@@ -308,7 +308,8 @@ int jal_op_shared_prefix_attention_workspace(const jal_paged_kv *kv,
  * in 64 bits, within a beam in the order of the logits.  A NaN logit counts as
  * -inf; a beam whose cum is not finite or whose logits hold +inf or nothing
  * above -inf scores -inf throughout (finished and empty beams).  k <= 64,
- * k <= n_beams * vocab.  Outputs [n_seqs][k]. */
+ * k <= n_beams * vocab, n_beams <= 256, n_beams * k <= 8192, vocab <= 2^20
+ * (JAL_ERR_CAPABILITY_MISMATCH).  Outputs [n_seqs][k]. */
 int jal_op_beam_select(const void *logits, int dtype, size_t row_stride,
                        const float *cum, size_t n_seqs, size_t n_beams,
                        size_t vocab, size_t k, float *scores, int32_t *parents,

@@ -13,15 +13,19 @@ using namespace paged;
 
 // Selection in two kernels.  Scores of one beam are in the order of its
 // logits, so the k best of a row are found on the logits themselves: each
-// block takes one chunk of a row, keeps its k best (logit, index) pairs and
-// the chunk's maximum and sum of exponentials.  The second kernel joins the
-// chunks: log-sum-exp of each row in 64 bits, the candidates' scores
-// cum + (x - lse) in 64 bits, and the k best of the sequence.
+// block takes one chunk of a row, keeps its k best (logit, index) pairs in
+// order, and the chunk's maximum and sum of exponentials.  The second kernel
+// joins them, a warp for each beam: log-sum-exp of the row in 64 bits, the
+// chunks' lists merged from their heads, scores cum + (x - lse) in 64 bits;
+// then one warp merges the beams' lists.  One pass over the logits, so the
+// first kernel is bound by reading them.
 constexpr int kSelThreads = 256;
-constexpr int kSelPer = 32;                       // logits of a chunk per thread
-constexpr int kSelChunk = kSelThreads * kSelPer;  // 8192
-constexpr int kJoinThreads = 512;
 constexpr int kMaxK = 64;
+constexpr int kSelList = 1024;  // candidates that are ranked without a second threshold
+constexpr int kJoinThreads = 512;
+constexpr int kJoinLists = 4;   // chunk lists a lane merges at most: 128 chunks a row
+constexpr int kMaxBeams = 256;  // eight lists a lane in the last merge
+constexpr size_t kJoinSmem = 96 * 1024;
 
 // A key whose unsigned order is (value descending -> larger first, then index
 // ascending): NaN counts as -inf, and -0 as +0.
@@ -42,155 +46,242 @@ struct ChunkHead {  // what a chunk leaves beside its k keys
   float top, sum;
 };
 
-template <class T>
-__global__ void __launch_bounds__(kSelThreads) k_beam_chunk(const BeamParams p, uint64_t *keys, ChunkHead *heads) {
-  __shared__ uint64_t best[kSelThreads];
-  __shared__ uint64_t cand[kMaxK * kSelPer];
-  __shared__ float red[2][kSelThreads / 32];
-  __shared__ uint64_t floor_key;
-  __shared__ int n_cand;
+// PER logits a thread, in pieces of 16 bytes where the rows are so aligned.
+template <class T, int PER>
+__global__ void __launch_bounds__(kSelThreads) k_beam_chunk(const BeamParams p, const bool wide, uint64_t *keys,
+                                                           ChunkHead *heads) {
+  constexpr int VEC = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
+  __shared__ uint64_t list[kMaxK * PER > kSelList ? kMaxK * PER : kSelList];
+  __shared__ uint64_t floors[kSelThreads / 32];
+  __shared__ float2 sums[kSelThreads / 32];
+  __shared__ int n_list;
   pdl_trigger();
-  const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
-  const T *x = (const T *)p.logits + row * p.row_stride;
-  const int v0 = chunk * kSelChunk;
+  const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  uint64_t *const out = keys + ((int64_t)row * p.chunks + chunk) * p.k;
+  ChunkHead *const head = heads + (int64_t)row * p.chunks + chunk;
   const float cum = p.cum[row];
-  const bool dead = !(cum > -INFINITY && cum < INFINITY);
-  uint64_t mine = 0;  // below every real key
-  float v[kSelPer], top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kSelPer; i++) {
-    const int at = v0 + i * kSelThreads + tid;
-    v[i] = -INFINITY;
-    if (at < p.vocab) {
-      v[i] = load_as_f32(x, at, p.dtype);
-      if (dead || v[i] != v[i]) v[i] = -INFINITY;
-      mine = max(mine, key_of(v[i], at));
-    }
-    top = fmaxf(top, v[i]);
+  if (!(cum > -INFINITY && cum < INFINITY)) {  // a dead beam: nothing of it is looked at
+    if (tid == 0) *head = {-INFINITY, 0.0f};
+    return;
   }
-  top = warp_max(top);
-  if (tid % 32 == 0) red[0][tid / 32] = top;
-  best[tid] = mine;
-  if (tid == 0) { n_cand = 0; floor_key = 0; }
+  const T *const x = (const T *)p.logits + row * p.row_stride;
+  const int v0 = chunk * (kSelThreads * PER);
+  auto place = [&](int i) { return v0 + ((i / VEC) * kSelThreads + tid) * VEC + i % VEC; };
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i += VEC) {
+    const int at = place(i);
+    if (wide && at + VEC <= p.vocab) {
+      if constexpr (VEC == 8) {
+        float w[8];
+        load8(x + at, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[i + e] = w[e];
+      } else {
+        const float4 w = *(const float4 *)(x + at);
+        v[i] = w.x; v[i + 1] = w.y; v[i + 2] = w.z; v[i + 3] = w.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) v[i + e] = at + e < p.vocab ? load_as_f32(x, at + e, p.dtype) : -INFINITY;
+    }
+  }
+  // The thread's best: the first of its largest.  A NaN is -inf.
+  float top = -INFINITY;
+  int first = -1;
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    v[i] = fmaxf(v[i], -INFINITY);
+    if (v[i] > top) {
+      top = v[i];
+      first = i;
+    }
+  }
+  if (first < 0 && place(0) < p.vocab) first = 0;  // all -inf
+  const uint64_t mine = first < 0 ? 0 : key_of(top, (uint32_t)place(first));  // 0: below every key
+  {
+    const float safe = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; i++) sum += __expf(v[i] - safe);
+    const float all = warp_max(top);
+    sum *= all == -INFINITY ? 0.0f : __expf(top - all);
+    sum = warp_sum(sum);
+    if (lane == 0) sums[warp] = make_float2(all, sum);
+  }
+  // At least k groups of threads: the least of the groups' best keys is below
+  // k keys at least, so the k best are not below it.
+  const int width = p.k <= 8 ? 32 : p.k <= 16 ? 16 : p.k <= 32 ? 8 : 4;
+  uint64_t best = mine;
+  for (int o = 1; o < width; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  for (int o = width; o < 32; o <<= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) floors[warp] = best;
+  if (tid == 0) n_list = 0;
   __syncthreads();
+  uint64_t least = floors[0];
 #pragma unroll
-  for (int w = 0; w < kSelThreads / 32; w++) top = fmaxf(top, red[0][w]);
-  const float safe = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
+  for (int w = 1; w < kSelThreads / 32; w++) least = min(least, floors[w]);
+  least = max(least, (uint64_t)1);
+  auto collect = [&](int room) {
+    if (mine < least) return;
 #pragma unroll
-  for (int i = 0; i < kSelPer; i++) sum += __expf(v[i] - safe);
-  sum = warp_sum(sum);
-  if (tid % 32 == 0) red[1][tid / 32] = sum;
-  // The k-th largest of the threads' best keys: the k best keys of the chunk
-  // are not below it, and only k threads hold such keys, at most kSelPer each.
-  int above = 0;
-  for (int i = 0; i < kSelThreads; i++) above += best[i] > mine;
-  if (above == p.k - 1) floor_key = mine;
-  __syncthreads();
-  const uint64_t least = max(floor_key, (uint64_t)1);
-  if (mine >= least) {
-#pragma unroll
-    for (int i = 0; i < kSelPer; i++) {
-      const int at = v0 + i * kSelThreads + tid;
+    for (int i = 0; i < PER; i++) {
+      const int at = place(i);
       if (at >= p.vocab) continue;
-      const uint64_t key = key_of(v[i], at);
-      if (key >= least) cand[atomicAdd(&n_cand, 1)] = key;
+      const uint64_t key = key_of(v[i], (uint32_t)at);
+      if (key >= least) {
+        const int n = atomicAdd(&n_list, 1);
+        if (n < room) list[n] = key;
+      }
     }
-  }
+  };
+  collect(kSelList);
   __syncthreads();
-  const int n = n_cand;
-  uint64_t *out = keys + ((int64_t)row * p.chunks + chunk) * p.k;
+  int n = n_list;
+  if (n > kSelList) {
+    // Unevenly spread: from the k-th largest of the threads' best keys on, which
+    // k threads reach, with PER keys each at most.
+    __syncthreads();
+    list[tid] = mine;
+    if (tid == 0) {
+      n_list = 0;
+      floors[0] = 1;
+    }
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < kSelThreads; i++) above += list[i] > mine;
+    if (above == p.k - 1 && mine) floors[0] = mine;
+    __syncthreads();
+    least = floors[0];
+    collect(kMaxK * PER);
+    __syncthreads();
+    n = n_list;
+  }
   for (int i = tid; i < n; i += kSelThreads) {
-    const uint64_t key = cand[i];
+    const uint64_t key = list[i];
     int rank = 0;
-    for (int j = 0; j < n; j++) rank += cand[j] > key;
+    for (int j = 0; j < n; j++) rank += list[j] > key;
     if (rank < p.k) out[rank] = key;
   }
-  for (int i = tid; i < p.k; i += kSelThreads)
-    if (i >= n) out[i] = 0;
+  for (int i = tid + n; i < p.k; i += kSelThreads) out[i] = 0;
   if (tid == 0) {
-    float all = 0.0f;
-    for (int w = 0; w < kSelThreads / 32; w++) all += red[1][w];
-    heads[(int64_t)row * p.chunks + chunk] = {top, all};
+    float all = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSelThreads / 32; w++) all = fmaxf(all, sums[w].x);
+#pragma unroll
+    for (int w = 0; w < kSelThreads / 32; w++) sum += sums[w].x == -INFINITY ? 0.0f : sums[w].y * __expf(sums[w].x - all);
+    *head = {all, sum};
   }
 }
 
-// (score, flat index): larger score first, then the lower index.
-struct Cand {
-  double score;
-  int64_t at;
-};
-__device__ __forceinline__ bool ahead(const Cand &a, const Cand &b) {
-  return a.score > b.score || (a.score == b.score && a.at < b.at);
+// The largest of the lanes' 64-bit values.
+__device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return ((uint64_t)hi << 32) | lo;
+}
+// A key in the order of x.
+__device__ __forceinline__ uint64_t order_of(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double score_of(uint64_t o) {
+  return __longlong_as_double((long long)(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
 }
 
 __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, const uint64_t *keys,
-                                                           const ChunkHead *heads, const int take) {
+                                                           const ChunkHead *heads, const bool staged) {
   extern __shared__ __align__(16) char smem_raw[];
-  Cand *cand = (Cand *)smem_raw;               // [k * take]
-  Cand *best = cand + (int64_t)p.k * take;     // [kJoinThreads]
-  double *lse = (double *)(best + kJoinThreads);  // [n_beams]
-  __shared__ int n_cand;
-  __shared__ Cand floor_cand;
+  uint64_t *const order = (uint64_t *)smem_raw;                // [n_beams][k] scores, in the order of order_of
+  int32_t *const token = (int32_t *)(order + p.n_beams * p.k);  // [n_beams][k]
   pdl_wait();
-  const int seq = blockIdx.x, tid = threadIdx.x;
-  for (int b = tid / 32; b < p.n_beams; b += kJoinThreads / 32) {
-    const ChunkHead *h = heads + ((int64_t)seq * p.n_beams + b) * p.chunks;
+  const int seq = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int per_beam = p.chunks * p.k, each = min(p.k, p.vocab);
+  uint64_t *const stage = (uint64_t *)(smem_raw + (((int64_t)p.n_beams * p.k * 12 + 15) & ~15)) + warp * per_beam;
+  for (int b = warp; b < p.n_beams; b += kJoinThreads / 32) {
+    const int row = seq * p.n_beams + b;
+    const ChunkHead *const h = heads + (int64_t)row * p.chunks;
+    const uint64_t *list = keys + (int64_t)row * per_beam;
+    if (staged) {
+      __syncwarp();
+      for (int i = lane; i < per_beam; i += 32) stage[i] = list[i];
+      __syncwarp();
+      list = stage;
+    }
+    const double cum = p.cum[row];
     float top = -INFINITY;
-    for (int c = tid % 32; c < p.chunks; c += 32) top = fmaxf(top, h[c].top);
+    for (int c = lane; c < p.chunks; c += 32) top = fmaxf(top, h[c].top);
     top = warp_max(top);
+    // No log-sum-exp: nothing but -inf, or a +inf among them.
+    const bool dead = !(cum > -INFINITY && cum < INFINITY && top > -INFINITY && top < INFINITY);
+    if (dead) {  // -inf throughout, in the order of the index
+      for (int j = lane; j < each; j += 32) {
+        order[b * p.k + j] = order_of(-INFINITY);
+        token[b * p.k + j] = j;
+      }
+      continue;
+    }
     double sum = 0.0;
-    if (top > -INFINITY && top < INFINITY)
-      for (int c = tid % 32; c < p.chunks; c += 32) sum += exp((double)h[c].top - (double)top) * (double)h[c].sum;
+    for (int c = lane; c < p.chunks; c += 32)
+      if (h[c].sum > 0.0f) sum += exp((double)h[c].top - (double)top) * (double)h[c].sum;
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    // no finite log-sum-exp (nothing but -inf, or a +inf): the beam is dead
-    if (tid % 32 == 0) lse[b] = top > -INFINITY && top < INFINITY ? (double)top + log(sum) : INFINITY;
-  }
-  if (tid == 0) { n_cand = 0; floor_cand = {-INFINITY, INT64_MAX}; }
-  __syncthreads();
-  const int per_beam = p.chunks * p.k, total = p.n_beams * per_beam;
-  auto get = [&](int i) -> Cand {
-    const int b = i / per_beam, j = i % per_beam;
-    const double l = lse[b];
-    const double cum = p.cum[seq * p.n_beams + b];
-    if (l == INFINITY || !(cum > -INFINITY && cum < INFINITY)) {
-      // All of a dead beam's scores are -inf: in the order of the index.
-      if (j >= min(p.k, p.vocab)) return {-INFINITY, INT64_MAX};
-      return {-INFINITY, (int64_t)b * p.vocab + j};
+    const double lse = (double)top + log(sum);
+    uint64_t head[kJoinLists];
+    int pos[kJoinLists];
+#pragma unroll
+    for (int i = 0; i < kJoinLists; i++) {
+      const int c = lane + 32 * i;
+      pos[i] = 0;
+      head[i] = c < p.chunks ? list[c * p.k] : 0;
     }
-    const uint64_t key = keys[((int64_t)seq * p.n_beams + b) * per_beam + j];
-    if (key == 0) return {-INFINITY, INT64_MAX};
-    return {cum + ((double)value_of(key) - l), (int64_t)b * p.vocab + index_of(key)};
-  };
-  Cand mine = {-INFINITY, INT64_MAX};
-  for (int i = tid; i < total; i += kJoinThreads) {
-    const Cand c = get(i);
-    if (ahead(c, mine)) mine = c;
-  }
-  best[tid] = mine;
-  __syncthreads();
-  int above = 0;
-  for (int i = 0; i < kJoinThreads; i++) above += ahead(best[i], mine);
-  if (above == p.k - 1 && mine.at != INT64_MAX) floor_cand = mine;
-  __syncthreads();
-  const Cand least = floor_cand;
-  if (mine.at != INT64_MAX && !ahead(least, mine)) {
-    for (int i = tid; i < total; i += kJoinThreads) {
-      const Cand c = get(i);
-      if (c.at != INT64_MAX && !ahead(least, c)) cand[atomicAdd(&n_cand, 1)] = c;
+    for (int j = 0; j < each; j++) {
+      uint64_t mine = head[0];
+#pragma unroll
+      for (int i = 1; i < kJoinLists; i++) mine = max(mine, head[i]);
+      const uint64_t best = warp_max64(mine);
+      if (mine == best) {  // keys are distinct: one lane
+#pragma unroll
+        for (int i = 0; i < kJoinLists; i++)
+          if (head[i] == best) {
+            pos[i]++;
+            head[i] = pos[i] < p.k ? list[(lane + 32 * i) * p.k + pos[i]] : 0;
+          }
+        order[b * p.k + j] = order_of(cum + ((double)value_of(best) - lse));
+        token[b * p.k + j] = (int32_t)index_of(best);
+      }
     }
   }
   __syncthreads();
-  const int n = n_cand;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const Cand c = cand[i];
-    int rank = 0;
-    for (int j = 0; j < n; j++) rank += ahead(cand[j], c);
-    if (rank < p.k) {
-      const int64_t o = (int64_t)seq * p.k + rank;
-      p.scores[o] = (float)c.score;
-      p.parents[o] = (int32_t)(c.at / p.vocab);
-      p.tokens[o] = (int32_t)(c.at % p.vocab);
+  if (warp) return;
+  // The beams' lists from their heads: the larger score, then the lower beam.
+  constexpr int N = kMaxBeams / 32;
+  int pos[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) pos[i] = 0;
+  for (int j = 0; j < p.k; j++) {
+    uint64_t mine = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int b = lane + 32 * i;
+      if (b >= p.n_beams || pos[i] >= each) continue;
+      const uint64_t o = order[b * p.k + pos[i]];
+      if (o > mine) {
+        mine = o;
+        at = i;
+      }
+    }
+    const uint64_t best = warp_max64(mine);
+    const int beam = (int)__reduce_min_sync(0xffffffffu, mine == best ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
+    if (mine == best && beam == lane + 32 * at) {
+      int taken = 0;
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (i == at) taken = pos[i]++;
+      const int64_t o = (int64_t)seq * p.k + j;
+      p.scores[o] = (float)score_of(best);
+      p.parents[o] = beam;
+      p.tokens[o] = token[beam * p.k + taken];
     }
   }
 }
@@ -227,30 +318,58 @@ __global__ void __launch_bounds__(kReorderThreads) k_beam_reorder(const ReorderP
   if (!takes || fill == 0) return;
   const int from = old[full], to = p.fresh[row];
   if ((unsigned)from >= (unsigned)kv.n_pages || (unsigned)to >= (unsigned)kv.n_pages) return;
-  const int chunks = kv.hd * elem / 16;  // 16-byte pieces of a slot's row
-  const int total = kv.hkv * fill * chunks;
-  for (int i = tid; i < 2 * total; i += kReorderThreads) {
-    const bool is_v = i >= total;
-    const int j = is_v ? i - total : i, c = j % chunks, slot = j / chunks % fill, head = j / chunks / fill;
-    const int64_t at = layer * p.layer_stride + head * kv.head_stride + slot * kv.slot_stride;
-    const char *src = (const char *)(is_v ? kv.v : kv.k) + (at + from * kv.page_stride) * elem + c * 16;
-    char *dst = (char *)(is_v ? p.vw : p.kw) + (at + to * kv.page_stride) * elem + c * 16;
-    *(uint4 *)dst = *(const uint4 *)src;
+  // A warp for each head of K and of V in turn; four 16-byte pieces a lane are
+  // on their way at a time.
+  const int chunks = kv.hd * elem / 16, total = fill * chunks, lane = tid % 32;
+  const bool dense = kv.slot_stride == kv.hd;
+  for (int seg = tid / 32; seg < 2 * kv.hkv; seg += kReorderThreads / 32) {
+    const bool is_v = seg >= kv.hkv;
+    const int64_t at = layer * p.layer_stride + (int64_t)(is_v ? seg - kv.hkv : seg) * kv.head_stride;
+    const char *const src = (const char *)(is_v ? kv.v : kv.k) + (at + from * kv.page_stride) * elem;
+    char *const dst = (char *)(is_v ? p.vw : p.kw) + (at + to * kv.page_stride) * elem;
+    for (int i = lane; i < total; i += 128) {
+      uint4 w[4];
+      int64_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int k = i + 32 * e;
+        o[e] = dense ? (int64_t)k * 16 : (int64_t)(k / chunks) * kv.slot_stride * elem + (k % chunks) * 16;
+        if (k < total) w[e] = *(const uint4 *)(src + o[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (i + 32 * e < total) *(uint4 *)(dst + o[e]) = w[e];
+    }
   }
 }
 
-int join_take(size_t n_beams, size_t chunks, size_t k) {
-  return (int)((n_beams * chunks * k + kJoinThreads - 1) / kJoinThreads);
+// Logits a thread of the first kernel takes.  A few rows are cut finer, so that
+// they spread over the SMs (4 rows of 4096: 8 blocks instead of 4).
+int per_thread(size_t n_rows, size_t vocab) {
+  const size_t blocks = n_rows * ((vocab + kSelThreads * 32 - 1) / (kSelThreads * 32));
+  return blocks < 2 * (size_t)kPagedSMs && vocab <= (size_t)kSelThreads * 8 * 32 * kJoinLists ? 8 : 32;
 }
-size_t join_smem(size_t n_beams, size_t chunks, size_t k) {
-  return (k * join_take(n_beams, chunks, k) + kJoinThreads) * sizeof(Cand) + n_beams * sizeof(double);
+size_t join_lists(size_t n_beams, size_t k) { return (n_beams * k * 12 + 15) / 16 * 16; }
+size_t join_stage(size_t chunks, size_t k) { return kJoinThreads / 32 * chunks * k * sizeof(uint64_t); }
+
+template <class T>
+void run_chunks(const BeamParams &p, uint64_t *keys, ChunkHead *heads, cudaStream_t s) {
+  const size_t rows = (size_t)p.n_seqs * p.n_beams;
+  const bool wide = (uintptr_t)p.logits % 16 == 0 && p.row_stride * sizeof(T) % 16 == 0;
+  const dim3 grid((unsigned)p.chunks, (unsigned)rows);
+  if (per_thread(rows, p.vocab) == 8) k_beam_chunk<T, 8><<<grid, kSelThreads, 0, s>>>(p, wide, keys, heads);
+  else k_beam_chunk<T, 32><<<grid, kSelThreads, 0, s>>>(p, wide, keys, heads);
+  JAL_CUDA(cudaGetLastError());
 }
 
 }  // namespace
 
-int beam_chunks(size_t, size_t vocab) { return (int)((vocab + kSelChunk - 1) / kSelChunk); }
+int beam_chunks(size_t n_rows, size_t vocab) {
+  const size_t chunk = (size_t)kSelThreads * per_thread(n_rows, vocab);
+  return (int)((vocab + chunk - 1) / chunk);
+}
 bool beam_fits(size_t n_beams, size_t vocab, size_t k, size_t n_rows) {
-  return join_smem(n_beams, (size_t)beam_chunks(n_rows, vocab), k) <= 200 * 1024;
+  return beam_chunks(n_rows, vocab) <= 32 * kJoinLists && n_beams <= (size_t)kMaxBeams && join_lists(n_beams, k) <= kJoinSmem;
 }
 size_t beam_workspace(size_t n_seqs, size_t n_beams, size_t vocab, size_t k) {
   const size_t chunks = n_seqs * n_beams * (size_t)beam_chunks(n_seqs * n_beams, vocab);
@@ -261,13 +380,13 @@ void launch_beam_select(const BeamParams &p, cudaStream_t s) {
   const int64_t rows = (int64_t)p.n_seqs * p.n_beams;
   uint64_t *keys = (uint64_t *)p.ws;
   ChunkHead *heads = (ChunkHead *)(keys + rows * p.chunks * p.k);
-  const dim3 grid((unsigned)p.chunks, (unsigned)rows);
-  if (p.dtype == JAL_F32) k_beam_chunk<float><<<grid, kSelThreads, 0, s>>>(p, keys, heads);
-  else if (p.dtype == JAL_F16) k_beam_chunk<__half><<<grid, kSelThreads, 0, s>>>(p, keys, heads);
-  else k_beam_chunk<__nv_bfloat16><<<grid, kSelThreads, 0, s>>>(p, keys, heads);
-  JAL_CUDA(cudaGetLastError());
-  const size_t smem = join_smem((size_t)p.n_beams, (size_t)p.chunks, (size_t)p.k);
-  JAL_CUDA(cudaFuncSetAttribute(k_beam_join, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (p.dtype == JAL_F32) run_chunks<float>(p, keys, heads, s);
+  else if (p.dtype == JAL_F16) run_chunks<__half>(p, keys, heads, s);
+  else run_chunks<__nv_bfloat16>(p, keys, heads, s);
+  const size_t lists = join_lists((size_t)p.n_beams, (size_t)p.k), stage = join_stage((size_t)p.chunks, (size_t)p.k);
+  const bool staged = lists + stage <= kJoinSmem;
+  const size_t smem = lists + (staged ? stage : 0);
+  JAL_CUDA(cudaFuncSetAttribute(k_beam_join, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kJoinSmem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.n_seqs);
   cfg.blockDim = dim3(kJoinThreads);
@@ -278,8 +397,7 @@ void launch_beam_select(const BeamParams &p, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  JAL_CUDA(cudaLaunchKernelEx(&cfg, k_beam_join, p, (const uint64_t *)keys, (const ChunkHead *)heads,
-                              join_take((size_t)p.n_beams, (size_t)p.chunks, (size_t)p.k)));
+  JAL_CUDA(cudaLaunchKernelEx(&cfg, k_beam_join, p, (const uint64_t *)keys, (const ChunkHead *)heads, staged));
 }
 
 void launch_beam_reorder(const ReorderParams &p, cudaStream_t s) {

@@ -79,7 +79,7 @@ struct BeamParams {
 // Pieces a row of logits is cut into, and the workspace bytes of a selection.
 int beam_chunks(size_t n_rows, size_t vocab);
 size_t beam_workspace(size_t n_seqs, size_t n_beams, size_t vocab, size_t k);
-// Candidates the joining block of one sequence takes at most.
+// Whether the joining block of one sequence can take that many lists.
 bool beam_fits(size_t n_beams, size_t vocab, size_t k, size_t n_rows);
 void launch_beam_select(const BeamParams &p, cudaStream_t s);
 

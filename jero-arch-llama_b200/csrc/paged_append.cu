@@ -1,5 +1,8 @@
 // New keys and values of a ragged batch into the paged cache, with the
 // position rotation applied on the way (and to the queries).
+#include <algorithm>
+#include <type_traits>
+
 #include "common.hpp"
 #include "paged_dev.cuh"
 
@@ -51,13 +54,117 @@ __device__ __forceinline__ void rotated8(const TA *row, int d, int rotary, int n
   }
 }
 
-// One block per token row.
+// The sequence in [0, n) that holds row r, found by the whole warp: 32 starts at
+// a time, so two rounds for 1024 sequences instead of ten dependent loads.
+__device__ __forceinline__ int warp_seq_of_row(const int32_t *q_start, int n, int r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;  // q_start[lo] <= r (or lo = 0)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + step * lane;
+    const bool before = lane > 0 && at < hi && __ldg(q_start + at) <= r;
+    const int k = __popc(__ballot_sync(0xffffffffu, before));
+    lo += step * k;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// rotary_dim a multiple of 16 (or 0): a warp takes part of a token row's heads,
+// item by item.  An item is eight dims and, in the rotated part, the eight
+// rotary_dim / 2 further on, so both of a pair's elements are in one lane
+// whichever way they are paired, and q_out may be q.  What bounds it: reading
+// the rows and writing the pages once; kItems items of a lane are on their way
+// at a time.
+constexpr int kWarps = 4;
+
+template <class T>
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2 *cs, int d, int half, int neox) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    if (neox) {
+      const float2 c = cs[d + e];
+      const float x = a[e], y = b[e];
+      a[e] = x * c.x - y * c.y;
+      b[e] = x * c.y + y * c.x;
+    } else if (e % 2 == 0) {
+      const float2 c = cs[(d + e) / 2], f = cs[(d + half + e) / 2];
+      const float x = a[e], y = a[e + 1], z = b[e], w = b[e + 1];
+      a[e] = x * c.x - y * c.y;
+      a[e + 1] = x * c.y + y * c.x;
+      b[e] = z * f.x - w * f.y;
+      b[e + 1] = z * f.y + w * f.x;
+    }
+  }
+}
+
+template <class TA, class TK>
+__global__ void __launch_bounds__(kWarps * 32) k_rope_kv_append_pairs(const __grid_constant__ AppendParams p, const int parts) {
+  constexpr int kItems = sizeof(TA) == 4 ? 2 : 4;
+  __shared__ float2 turns[kWarps][kPagedMaxHeadDim / 2];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, unit = blockIdx.x * kWarps + warp;
+  const int row = unit / parts, part = unit - row * parts;
+  if (row >= p.n_rows) return;
+  const int first = __ldg(p.q_start), last = __ldg(p.q_start + p.n_seqs);
+  const int s = warp_seq_of_row(p.q_start, p.n_seqs, row);
+  if (row < first || row >= last) return;
+  int beg, end;
+  seq_rows(p.q_start, p.n_rows, s, beg, end);
+  const int64_t pos64 = (int64_t)__ldg(p.kv_len + s) - (end - row);
+  if (pos64 < 0 || pos64 >= p.kv.cap) return;
+  const int pos = (int)pos64, hd = p.kv.hd, half = p.rotary / 2;
+  const int64_t at = slot_offset(p.kv, p.kv.table + (int64_t)s * p.kv.max_pages, 0, pos);
+  float2 *const cs = turns[warp];
+  for (int i = lane; i < half; i += 32) cs[i] = turn(pos, __ldg(p.inv_freq + i));
+  __syncwarp();
+  const int nq = p.q ? p.hq : 0, items = half / 8 + (hd - p.rotary) / 8, total = (nq + 2 * p.kv.hkv) * items;
+  const int per = (total + parts - 1) / parts, stop = min(total, (part + 1) * per);
+  for (int i = part * per + lane; i < stop; i += 32 * kItems) {
+    float a[kItems][8], b[kItems][8];
+#pragma unroll
+    for (int k = 0; k < kItems; k++) {
+      const int it = i + 32 * k;
+      if (it >= stop) break;
+      const int head = it / items, c = it - head * items;
+      const bool is_q = head < nq, is_k = !is_q && head < nq + p.kv.hkv;
+      const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
+      const TA *const src = (const TA *)(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.q_stride : p.kv_stride) + h * hd;
+      if (c < half / 8) {
+        load8(src + c * 8, a[k]);
+        load8(src + c * 8 + half, b[k]);
+      } else {
+        load8(src + p.rotary + (c - half / 8) * 8, a[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; k++) {
+      const int it = i + 32 * k;
+      if (it >= stop) break;
+      const int head = it / items, c = it - head * items;
+      const bool is_q = head < nq, is_k = !is_q && head < nq + p.kv.hkv;
+      const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
+      const bool rotated = c < half / 8;
+      const int d = rotated ? c * 8 : p.rotary + (c - half / 8) * 8;
+      if (rotated && (is_q || is_k)) turn8<TA>(a[k], b[k], cs, d, half, p.neox);
+      if (is_q) {
+        TA *const dst = (TA *)p.q_out + row * p.q_out_stride + h * hd;
+        store8(dst + d, a[k]);
+        if (rotated) store8(dst + d + half, b[k]);
+      } else if (at >= 0) {
+        TK *const dst = (TK *)(is_k ? p.kw : p.vw) + at + h * p.kv.head_stride;
+        store8(dst + d, a[k]);
+        if (rotated) store8(dst + d + half, b[k]);
+      }
+    }
+  }
+}
+
+// Any rotary_dim: one block per token row.
 template <class TA, class TK>
 __global__ void __launch_bounds__(kAppendThreads) k_rope_kv_append(const AppendParams p, const int lanes) {
   __shared__ float2 cs[kPagedMaxHeadDim / 2];
   const int row = blockIdx.x, hd = p.kv.hd;
   if (row < p.q_start[0] || row >= p.q_start[p.n_seqs]) return;
-  const int s = seq_of_row(p.q_start, 0, p.n_seqs, row);
+  const int s = warp_seq_of_row(p.q_start, p.n_seqs, row);
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   const int64_t pos64 = (int64_t)p.kv_len[s] - (end - row);
@@ -95,9 +202,19 @@ __global__ void __launch_bounds__(kAppendThreads) k_rope_kv_append(const AppendP
 
 template <class TA, class TK>
 void run(const AppendParams &p, cudaStream_t s) {
-  int lanes = 1;
-  while (lanes * 8 < p.kv.hd) lanes *= 2;
-  k_rope_kv_append<TA, TK><<<(unsigned)p.n_rows, kAppendThreads, 0, s>>>(p, lanes);
+  if (p.rotary % 16 == 0) {
+    // Warps enough to fill the SMs, each with a round of items at least.
+    const int heads = (p.q ? p.hq : 0) + 2 * p.kv.hkv, items = heads * (p.rotary / 16 + (p.kv.hd - p.rotary) / 8);
+    const int most = std::max(1, items / (32 * (sizeof(TA) == 4 ? 2 : 4)));
+    const int64_t rows = p.n_rows;
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 32 * kPagedSMs / rows));
+    const unsigned blocks = (unsigned)((rows * parts + kWarps - 1) / kWarps);
+    k_rope_kv_append_pairs<TA, TK><<<blocks, kWarps * 32, 0, s>>>(p, parts);
+  } else {
+    int lanes = 1;
+    while (lanes * 8 < p.kv.hd) lanes *= 2;
+    k_rope_kv_append<TA, TK><<<(unsigned)p.n_rows, kAppendThreads, 0, s>>>(p, lanes);
+  }
   JAL_CUDA(cudaGetLastError());
 }
 

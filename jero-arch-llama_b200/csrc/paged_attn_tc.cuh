@@ -11,10 +11,13 @@
 // 128 exponentials; at HD = 128 the former takes longer, so what bounds the
 // kernel is how gaplessly the products are issued.
 //
-//   warps 0-3, 4-7   softmax of row tile 0, 1 (warp w reads tensor-memory
-//                    lanes 32 (w % 4) ..), and the result
-//   warps 8-11       K and V rows from their pages into the ring, cp.async
-//   warp 12          one thread issues the products
+//   warps 0-15       softmax: four warpgroups, two for each row tile, each with
+//                    64 of the tile's 128 keys (warp w reads tensor-memory lanes
+//                    32 (w % 4) ..), and the result.  One thread a row and half:
+//                    one warp of a tile on a scheduler cannot hide its own
+//                    latencies
+//   warps 16-18      K and V rows from their pages into the ring, cp.async
+//   warp 19          one thread issues the products
 //
 // Pages may hold any number of slots, so rows are copied one by one to their
 // place in the 128-byte swizzle that the matrix descriptors name: K tiles and
@@ -33,16 +36,33 @@
 namespace jal {
 namespace paged {
 
-constexpr int kTcRows = 256, kTcKeys = 128, kTcThreads = 512;
-constexpr int kPoly = 4;
+constexpr int kTcRows = 256, kTcKeys = 128, kTcThreads = 640;
+constexpr int kTcSoftmax = 512, kTcLoaders = 3;  // threads; warps
 constexpr float kTcSlack = 8.0f;  // growth of a maximum (base 2) that is let stand
+
+struct TcSync {
+  uint64_t q_full, loaded;
+  uint64_t kv_full[6], kv_empty[6];
+  uint64_t present_full[8];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int given_up, poison;
+  int lim_lo, lim_hi, wlo_lo, wlo_hi;
+  // Of a row's halves: the largest score of the key tile, and at the end the sum
+  // of the weights.  Before the first tile: what a row's scores are still to be
+  // multiplied by (NS = 2, [256]).  Barriers lie between these uses.
+  float x[2][2][128];
+  alignas(16) uint8_t present[8][16];    // which keys of tile j exist, a bit each, by j % 8
+};
 
 template <int NS, int HD>
 struct TcShape {
   static constexpr int tile = kTcKeys * HD * 2;            // bytes of a K or V tile
   static constexpr int q_tile = 128 * HD * 2;              // of one part of a row tile
   static constexpr int buffers = HD == 64 ? 6 : NS == 1 ? 5 : 3;
-  static constexpr int smem = 1024 + 2 * NS * q_tile + buffers * tile;
+  // The query tiles; at the end 4 KB for each softmax warp.
+  static constexpr int q_area = 2 * NS * q_tile > 65536 ? 2 * NS * q_tile : 65536;
+  static constexpr int ring = q_area, sync = q_area + buffers * tile, smem = sync + (int)sizeof(TcSync);
 };
 
 // ---- pairs of f32 in one instruction
@@ -68,31 +88,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
   return v;
 }
-// 2^x of a pair on the multiply-add units: x = n + r with n whole and |r| <=
-// 1/2, 2^r by a polynomial whose coefficients were fitted for the least largest
-// relative error on that range (degree 3: 7.5e-5, 4: 2.6e-6, 5: 7.5e-8), n
-// added to the exponent.  x below -126 gives about 2^-126; x is finite.
-template <int DEG>
-__device__ __forceinline__ void exp2_poly(pair_t x2, float &a, float &b) {
-  constexpr float c3[] = {0.9999280728f, 0.6932609870f, 0.2426111351f, 0.05517166682f};
-  constexpr float c4[] = {0.9999992614f, 0.6931218145f, 0.2402474485f, 0.05591786210f, 0.009570101653f};
-  constexpr float c5[] = {1.0000000717f, 0.6931469671f, 0.2402211972f, 0.05550713276f, 0.009675541540f, 0.001327647173f};
-  const float *const c = DEG == 3 ? c3 : DEG == 4 ? c4 : c5;
-  unpair(x2, a, b);
-  x2 = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  constexpr float whole = 12582912.0f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
-  const pair_t t = add2(x2, pair(whole, whole));
-  const pair_t r = add2(x2, fma2(t, pair(-1.0f, -1.0f), pair(whole, whole)));
-  pair_t y = pair(c[DEG], c[DEG]);
-#pragma unroll
-  for (int i = DEG - 1; i >= 0; i--) y = fma2(y, r, pair(c[i], c[i]));
-  float ya, yb, ta, tb;
-  unpair(y, ya, yb);
-  unpair(t, ta, tb);
-  a = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(tb) << 23));
-}
-
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
@@ -157,44 +152,31 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t *r) {
 #undef JAL_R8
 #undef JAL_I8
 
-struct TcSync {
-  uint64_t q_full, loaded;
-  uint64_t kv_full[6], kv_empty[6];
-  uint64_t present_full[8];
-  uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-  uint32_t tmem;
-  int given_up, poison;
-  int lim_lo, lim_hi, wlo_lo, wlo_hi;
-  float q_factor[kTcRows];  // NS = 2: what a row's scores are still to be multiplied by
-  alignas(16) uint32_t present[8][4];  // which keys of tile j exist, by j % 8
-};
 
 template <class T, int NS, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_constant__ AttnParams p, const int part, const bool direct) {
   using S = TcShape<NS, HD>;
-  extern __shared__ char smem_raw[];
-  __shared__ TcSync sy;
+  extern __shared__ __align__(1024) char smem_tc[];
+  TcSync &sy = *(TcSync *)(smem_tc + S::sync);
   pdl_trigger();
   Tile t;
   if (!block_tile(p, part, kTcRows, kTcKeys, t)) return;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, hd = p.kv.hd;
-  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
-  char *const base_p = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t sq = base, ring = base + 2 * NS * S::q_tile;
+  char *const base_p = smem_tc;
+  const uint32_t sq = smem_u32(smem_tc), ring = sq + S::ring;
   const int n_tiles = (t.u1 - t.u0 + kTcKeys - 1) / kTcKeys;
 
   if (tid == 0) {
-    mbar_init(&sy.q_full, 256);
-    mbar_init(&sy.loaded, 128);
+    mbar_init(&sy.q_full, kTcSoftmax);
+    mbar_init(&sy.loaded, kTcLoaders * 32);
     for (int i = 0; i < S::buffers; i++) {
-      mbar_init(&sy.kv_full[i], 128);
+      mbar_init(&sy.kv_full[i], kTcLoaders * 32);
       mbar_init(&sy.kv_empty[i], 1);
     }
-    for (int i = 0; i < 8; i++) mbar_init(&sy.present_full[i], 4);
+    for (int i = 0; i < 8; i++) mbar_init(&sy.present_full[i], kTcLoaders);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sy.s_full[i], 1);
-      mbar_init(&sy.p_half[i], 128);
-      mbar_init(&sy.p_full[i], 128);
+      mbar_init(&sy.p_full[i], 256);
       mbar_init(&sy.o_full[i], 1);
     }
     sy.given_up = sy.poison = 0;
@@ -202,7 +184,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     sy.lim_hi = sy.wlo_hi = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 19) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sy.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tc_fence_before();
@@ -215,42 +197,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
   volatile int *given_up = &sy.given_up;
   auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
     if (mbar_try_wait(bar, parity)) return true;
-    if (mbar_wait_bounded(bar, parity)) return true;
+    if (!*given_up && mbar_wait_bounded(bar, parity)) return true;
     *given_up = 1;
     return false;
   };
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp < 12) {
+  // 640 threads of 96 registers: 512 x 104 + 128 x 64.
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp < 16 + kTcLoaders) {
       // ---- the loader
-      const int w = warp - 8;
-      auto locate = [&](int j) -> Slot {
-        const int u = t.u0 + j * kTcKeys + w * 32 + lane;
-        return j < n_tiles && u < t.u1 ? slot_of(p.kv, t.table, t.key(u)) : Slot{-1, 0};
+      // The 16 groups of 8 rows of a tile go round the warps; a lane looks up
+      // two of its warp's (up to) 48 rows, one tile ahead.
+      const int w = warp - 16;
+      constexpr int kGroups = (16 + kTcLoaders - 1) / kTcLoaders;
+      auto group = [&](int k) { return w + k * kTcLoaders; };
+      auto locate = [&](int j, int k) -> Slot {
+        const int gr = group(k + lane / 8), u = t.u0 + j * kTcKeys + gr * 8 + lane % 8;
+        return j < n_tiles && k + lane / 8 < kGroups && gr < 16 && u < t.u1 ? slot_of(p.kv, t.table, t.key(u)) : Slot{-1, 0};
       };
-      // Eight lanes copy 128 bytes of a row; a lane has the rows lane / 8 + 4 i
-      // of the warp's 32.  Their addresses are passed round once for K and V.
+      // Eight lanes copy 128 bytes of a row; a lane has rows lane / 8 and lane / 8
+      // + 4 of each group.  Their addresses are passed round once for K and V.
       const int c8 = lane % 8, r8 = lane / 8;
-      const uint32_t to_even = (w * 32 + r8) * 128 + ((c8 ^ r8) * 16), to_odd = (w * 32 + r8) * 128 + ((c8 ^ (r8 + 4)) * 16);
+      const uint32_t to0 = r8 * 128 + ((c8 ^ r8) * 16), to1 = (r8 + 4) * 128 + ((c8 ^ (r8 + 4)) * 16);
       // Copies arrive on the buffer's barrier by themselves; the thread that
       // issues the products puts the fence between them and the tensor cores.
       uint32_t bad = 0;
       bool ok = true, ranges = false;
       int b = 0, parity = 1;  // of the buffer's "empty" phase before this use: the first use finds it free
-      auto copy = [&](const void *pool_v, const int64_t (&from)[8]) {
+      auto copy = [&](const void *pool_v, const int64_t (&from)[kGroups][2]) {
         ok = __all_sync(0xffffffffu, ok && wait(&sy.kv_empty[b], parity));
         if (!ok) return;
         const char *const pool = (const char *)pool_v + c8 * 16;
         const uint32_t dst = ring + b * S::tile;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const char *const src = pool + from[i] * 2;
-          const uint32_t to = dst + (i & 1 ? to_odd : to_even) + i * 512;
+        for (int k = 0; k < kGroups; k++) {
+          if (group(k) >= 16) break;
 #pragma unroll
-          for (int h = 0; h < HD / 64; h++) {
-            const bool there = from[i] >= 0 && h * 64 + c8 * 8 < hd;
-            copy16(to + h * (kTcKeys * 128), there ? src + h * 128 : (const char *)pool_v, there);
+          for (int e = 0; e < 2; e++) {
+            const char *const src = pool + from[k][e] * 2;
+            const uint32_t to = dst + group(k) * 1024 + (e ? to1 : to0);
+#pragma unroll
+            for (int h = 0; h < HD / 64; h++) {
+              const bool there = from[k][e] >= 0 && h * 64 + c8 * 8 < hd;
+              copy16(to + h * (kTcKeys * 128), there ? src + h * 128 : (const char *)pool_v, there);
+            }
           }
         }
         copies_done();
@@ -262,25 +253,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       };
       // Looks through the V tile in buffer vb for values that some queries must not meet.
       auto scan = [&](int vb) {
-        const char *rows = base_p + 2 * NS * S::q_tile + vb * S::tile + (w * 32) * 128;
-#pragma unroll 4
-        for (int i = 0; i < HD / 64 * 8; i++)  // 32 rows x 128 bytes x (HD / 64) of this warp
-          watch8<T>(bad, *(const uint4 *)(rows + (i / 8) * (kTcKeys * 128) + ((i % 8) * 32 + lane) * 16));
+        const char *const rows = base_p + S::ring + vb * S::tile;
+#pragma unroll
+        for (int k = 0; k < kGroups; k++)  // the rows that this warp has copied
+#pragma unroll
+          for (int h = 0; h < HD / 64 * 2; h++)
+            if (group(k) < 16)
+              watch8<T>(bad, *(const uint4 *)(rows + (h / 2) * (kTcKeys * 128) + group(k) * 1024 + (h % 2) * 512 + lane * 16));
       };
-      Slot next = locate(0);
+      Slot next0 = locate(0, 0), next1 = locate(0, 4);
       int scan_b = -1;
 #pragma unroll 1
       for (int j = 0; j < n_tiles; j++) {
-        const int64_t at = slot_offset(p.kv, next, t.head);
-        const uint32_t bits = __ballot_sync(0xffffffffu, at >= 0);
-        next = locate(j + 1);
-        int64_t from[8];
+        const int64_t at0 = slot_offset(p.kv, next0, t.head), at1 = slot_offset(p.kv, next1, t.head);
+        const uint32_t bits0 = __ballot_sync(0xffffffffu, at0 >= 0), bits1 = __ballot_sync(0xffffffffu, at1 >= 0);
+        next0 = locate(j + 1, 0);
+        next1 = locate(j + 1, 4);
+        int64_t from[kGroups][2];
 #pragma unroll
-        for (int i = 0; i < 8; i++) from[i] = __shfl_sync(0xffffffffu, at, r8 + 4 * i);
-        if (lane == 0) {  // tile j + 8 comes long after the softmax has read tile j's
-          sy.present[j & 7][w] = bits;
-          mbar_arrive(&sy.present_full[j & 7]);
-        }
+        for (int k = 0; k < kGroups; k++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            from[k][e] = __shfl_sync(0xffffffffu, k < 4 ? at0 : at1, (k % 4) * 8 + r8 + 4 * e);
+        if (lane < kGroups && group(lane) < 16)  // tile j + 8 comes long after the softmax has read tile j's
+          sy.present[j & 7][group(lane)] = (uint8_t)((lane < 4 ? bits0 : bits1) >> (lane % 4 * 8));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sy.present_full[j & 7]);
         copy(p.kv.k, from);
         const int vb = b;
         copy(p.kv.v, from);
@@ -303,7 +301,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       if (scan_b >= 0) scan(scan_b);
       if (watched_bad<T>(bad)) sy.poison = 1;
       mbar_arrive(&sy.loaded);
-    } else if (warp == 12) {
+    } else {
       // ---- the products: the whole warp runs the loop, so that addresses stay
       // uniform, and one lane issues
       const bool leader = elect_one();
@@ -326,16 +324,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         }
         __syncwarp();
       };
-      auto output = [&](int i, int vb, bool first, int half) {  // 64 of the keys
+      auto output = [&](int i, int vb, bool first) {
         if (leader) {
-          const uint64_t b = v_desc + (uint32_t)(vb * (S::tile >> 4) + half * 4 * (2048 >> 4));
-          const uint32_t a = tmem + i * 128 + half * 32;
+          const uint64_t b = v_desc + (uint32_t)(vb * (S::tile >> 4));
 #pragma unroll
           for (int s = 0; s < NS; s++)
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-              tc_mma_ts(tmem + 256 + i * 128, a + s * 64 + q * 8, b + (uint32_t)(q * (2048 >> 4)), id_o,
-                        !first || s + q > 0);
+            for (int k = 0; k < kTcKeys / 16; k++)
+              tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + (k / 4) * 64 + s * 32 + (k % 4) * 8,
+                        b + (uint32_t)(k * (2048 >> 4)), id_o, !first || s + k > 0);
         }
         __syncwarp();
       };
@@ -366,14 +363,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       for (int j = 0; j < n_tiles && ok; j++) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          ok = ok && (i || take(vb)) && wait(&sy.p_half[i], j & 1);
+          ok = ok && (i || take(vb)) && wait(&sy.p_full[i], j & 1);
           if (!ok) break;
           tc_fence_after();
-          output(i, vb, j == 0, 0);
-          ok = wait(&sy.p_full[i], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          output(i, vb, false, 1);
+          output(i, vb, j == 0);
           if (i) release(vb);
           if (j + 1 < n_tiles) {
             ok = i || take(kb);
@@ -389,50 +382,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ---- softmax: thread r of warpgroup i has row i * 128 + r
-    const int i = warp / 4, r = tid % 128, row = i * 128 + r;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---- softmax: threads r of the warpgroups 2 i and 2 i + 1 have row i * 128 + r
+    const int i = warp / 8, half = warp / 4 % 2, r = tid % 128, row = i * 128 + r;
     const bool real = row < t.rows;
     const RowMask mk = real ? row_mask(p, t, row) : RowMask{0, 0};
     // Weights are formed with a positive factor: a negative one turns q round,
     // none makes it 0.
     float scale = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
-    {  // its query row into shared memory
-      const int64_t qo = real ? q_offset(p, t, row) : 0;
-      char *const dst_p = base_p + i * NS * S::q_tile;
+    auto tile_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory"); };
+    {  // the query rows into shared memory, 16 rows a warp, neighbouring lanes neighbouring pieces
+      const int first = warp % 8 * 16;  // of the row tile
+      char *const dst = base_p + i * NS * S::q_tile;
       const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-      const bool take = real && p.scale_log2 != 0.0f;
-      // The 32 rows of a warp are read by all its lanes, neighbouring lanes
-      // neighbouring pieces of eight elements.
+      const int mine = i * 128 + first + lane % 16;
+      const int64_t qt = mine < t.rows && p.scale_log2 != 0.0f ? q_offset(p, t, mine) : -1;
       constexpr int CH = HD / 8;
-      const int64_t qt = take ? qo : -1;
-      const int i_row = row & ~31;  // the warp's first row
       if constexpr (NS == 1) {
         const int c8 = lane % 8, r8 = lane / 8;
-        uint4 w[8][HD / 64];
+        uint4 w[4][HD / 64];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < 4; k++) {
           const int64_t o = __shfl_sync(0xffffffffu, qt, r8 + 4 * k);
 #pragma unroll
           for (int h = 0; h < HD / 64; h++)
             w[k][h] = o >= 0 && h * 64 + c8 * 8 < hd ? *(const uint4 *)((const T *)p.q + o + h * 64 + c8 * 8)
                                                      : make_uint4(0, 0, 0, 0);
         }
-        char *const even = dst_p + ((r & ~31) + r8) * 128 + ((c8 ^ r8) * 16);
-        char *const odd = dst_p + ((r & ~31) + r8) * 128 + ((c8 ^ (r8 + 4)) * 16);
 #pragma unroll
-        for (int k = 0; k < 8; k++)
+        for (int k = 0; k < 4; k++)
 #pragma unroll
           for (int h = 0; h < HD / 64; h++) {
+            const int kr = first + r8 + 4 * k;
             const uint4 x = w[k][h];
-            *(uint4 *)((k & 1 ? odd : even) + k * 512 + h * (128 * 128)) =
+            *(uint4 *)(dst + h * (128 * 128) + kr * 128 + ((c8 ^ (kr & 7)) * 16)) =
                 make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
           }
       } else {
-#pragma unroll 4
-        for (int i = 0; i < CH; i++) {
-          const int k = (i * 32 + lane) / CH, c = lane % CH;
-          const int64_t o = __shfl_sync(0xffffffffu, qt, k);
+#pragma unroll 2
+        for (int k = 0; k < CH / 2; k++) {
+          const int kr = (k * 32 + lane) / CH, c = lane % CH;
+          const int64_t o = __shfl_sync(0xffffffffu, qt, kr);
           float v[8] = {}, top = 0.0f;
           if (o >= 0 && c * 8 < hd) load8((const float *)p.q + o + c * 8, v);
 #pragma unroll
@@ -445,15 +435,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
           uint32_t part2[4][NS];
 #pragma unroll
           for (int q = 0; q < 4; q++) split2<T, NS>(v[2 * q] * a * b, v[2 * q + 1] * a * b, part2[q]);
-          const int kr = (r & ~31) + k;
 #pragma unroll
           for (int s = 0; s < NS; s++)
-            *(uint4 *)(dst_p + s * S::q_tile + (c / 8) * (128 * 128) + kr * 128 + (((c % 8) ^ (kr & 7)) * 16)) =
+            *(uint4 *)(dst + s * S::q_tile + (c / 8) * (128 * 128) + (first + kr) * 128 + (((c % 8) ^ (kr & 7)) * 16)) =
                 make_uint4(part2[0][s], part2[1][s], part2[2][s], part2[3][s]);
-          if (c == 0) sy.q_factor[i_row + k] = (1.0f / fabsf(a)) / b;
+          if (c == 0) (&sy.x[0][0][0])[i * 128 + first + kr] = (1.0f / fabsf(a)) / b;
         }
-        __syncwarp();
-        scale *= sy.q_factor[row];
+        tile_sync();
+        scale *= (&sy.x[0][0][0])[row];
       }
       int lo = real ? mk.lim : 0x7fffffff, hi = real ? mk.lim : 0, wl = real ? mk.wlo : 0x7fffffff, wh = real ? mk.wlo : 0;
       lo = __reduce_min_sync(0xffffffffu, lo);
@@ -470,38 +459,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       mbar_arrive(&sy.q_full);
     }
     const uint32_t quarter = (uint32_t)(warp % 4) << 21;  // lane 32 (warp % 4) of the tensor memory
-    const uint32_t ts = tmem + i * 128 + quarter, to = tmem + 256 + i * 128 + quarter;
+    const uint32_t ts = tmem + i * 128 + half * 64 + quarter, to = tmem + 256 + i * 128 + quarter;
     const RowSpan span = row_span(p, t, mk);
-    float m = -INFINITY, l = 0.0f;  // m: what the weights refer to, scaled to base 2
+    float m = -INFINITY, l = 0.0f;  // m: what the weights refer to, scaled to base 2; l: this half's sum
     bool ok = true;
+#pragma unroll 1
     for (int j = 0; j < n_tiles; j++) {
-      ok = __all_sync(0xffffffffu, wait(&sy.present_full[j & 7], (j >> 3) & 1) && wait(&sy.s_full[i], j & 1));
-      if (!ok) break;
+      // (A wait that gave up does not leave the loop: the other half waits below.)
+      ok = wait(&sy.present_full[j & 7], (j >> 3) & 1) && ok;
+      ok = wait(&sy.s_full[i], j & 1) && ok;
+      __syncwarp();
       tc_fence_after();
-      float s[128];
-#pragma unroll
-      for (int c = 0; c < 4; c++) tc_ld32(ts + c * 32, (uint32_t *)s + c * 32);
-      tc_wait_ld();
-      const int u = t.u0 + j * kTcKeys;
-      const uint4 here = *(const uint4 *)sy.present[j & 7];
-      const bool whole = (here.x & here.y & here.z & here.w) == 0xffffffffu && span.all(u, kTcKeys);
+      float s[2][32];
+      tc_ld32(ts, (uint32_t *)s[0]);
+      tc_ld32(ts + 32, (uint32_t *)s[1]);
+      const int u = t.u0 + j * kTcKeys + half * 64;
+      const uint2 here = *(const uint2 *)&sy.present[j & 7][half * 8];
+      const bool whole = (here.x & here.y) == 0xffffffffu && span.all(u, 64);
       const bool masked = !__all_sync(0xffffffffu, whole || !real);
+      tc_wait_ld();
       if (masked) {
-        const uint32_t bits[4] = {here.x & span.bits(u), here.y & span.bits(u + 32), here.z & span.bits(u + 64),
-                                  here.w & span.bits(u + 96)};
+        const uint32_t bits[2] = {here.x & span.bits(u), here.y & span.bits(u + 32)};
 #pragma unroll
-        for (int c = 0; c < 128; c++)
-          if (!((bits[c / 32] >> (c % 32)) & 1)) s[c] = -INFINITY;
+        for (int e = 0; e < 64; e++)
+          if (!((bits[e / 32] >> (e % 32)) & 1)) s[e / 32][e % 32] = -INFINITY;
       }
-      float x[4] = {s[0], s[1], s[2], s[3]};
+      float x[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
-      for (int c = 4; c < 124; c += 8) {
+      for (int e = 4; e < 60; e += 8)
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = max3_nan(x[e], s[c + 2 * e], s[c + 2 * e + 1]);
-      }
-      const float top = max3_nan(max3_nan(x[0], x[1], s[124]), max3_nan(x[2], x[3], s[125]), max3_nan(s[126], s[127], s[127])) * scale;
-      // A NaN or an infinite score makes the row NaN, as the formula does; it
-      // need not come through the weights.
+        for (int k = 0; k < 4; k++) x[k] = max3_nan(x[k], s[(e + 2 * k) / 32][(e + 2 * k) % 32], s[(e + 2 * k + 1) / 32][(e + 2 * k + 1) % 32]);
+      const float mine = max3_nan(max3_nan(x[0], x[1], s[1][28]), max3_nan(x[2], x[3], s[1][29]),
+                                  max3_nan(s[1][30], s[1][31], s[1][31]));
+      sy.x[i][half][r] = mine;
+      tile_sync();
+      const float top = max3_nan(mine, sy.x[i][half ^ 1][r], mine) * scale;
+      // A NaN or an infinite score makes the row NaN, as the formula does.
       if (!(top < INFINITY)) l = NAN;
       // Raise the reference of the rows that need it (the first tile's all).
       // O is at rest: its products up to tile j - 1 were done before S.
@@ -510,55 +503,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         const float c = raise ? exp2_fast(m - top) : 1.0f;
         if (raise) m = top;
         l *= c;
-        if (j > 0) {
+        if (j > 0) {  // this half of O's columns
 #pragma unroll 1
-          for (int d = 0; d < HD; d += 32) {
-            float o[32];
-            tc_ld32(to + d, (uint32_t *)o);
+          for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 32) {
+            uint32_t o[32];
+            tc_ld32(to + d, o);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] *= c;
-            tc_st32(to + d, (const uint32_t *)o);
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+            tc_st32(to + d, o);
           }
         }
       }
       const float ref = m == -INFINITY ? 0.0f : m;
-      // The weights.  The special-function units would be the slowest part, so
-      // where nothing is masked every kPoly-th pair goes by the polynomial.
+      // The weights, over this half's own scores: part q of the 64 keys' in the
+      // columns 32 q .. of the half.
       pair_t sum[2] = {0, 0};
       const pair_t scale2 = pair(scale, scale), ref2 = pair(-ref, -ref);
-      auto weights = [&](auto poly) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t w[NS][16];
+      for (int c = 0; c < 2; c++) {
+        uint32_t w[NS][16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const pair_t x2 = fma2(pair(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), scale2, ref2);
-            float a, b;
-            if (poly && e % kPoly == kPoly - 1) {
-              exp2_poly<NS == 2 ? 5 : std::is_same<T, __half>::value ? 4 : 3>(x2, a, b);
-            } else {
-              unpair(x2, a, b);
-              a = exp2_fast(a);
-              b = exp2_fast(b);
-            }
-            sum[e % 2] = add2(sum[e % 2], pair(a, b));
-            uint32_t part2[NS];
-            split2<T, NS>(a, b, part2);
+        for (int e = 0; e < 16; e++) {
+          float a, b;
+          const pair_t x2 = fma2(pair(s[c][2 * e], s[c][2 * e + 1]), scale2, ref2);
+          unpair(x2, a, b);
+          a = exp2_fast(a);
+          b = exp2_fast(b);
+          sum[e % 2] = add2(sum[e % 2], pair(a, b));
+          uint32_t part2[NS];
+          split2<T, NS>(a, b, part2);
 #pragma unroll
-            for (int q = 0; q < NS; q++) w[q][e] = part2[q];
-          }
-#pragma unroll
-          for (int q = 0; q < NS; q++) tc_st16(ts + q * 64 + c * 16, w[q]);
-          if (c == 1) {  // the products of the first half of the keys can start
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sy.p_half[i]);
-          }
+          for (int q = 0; q < NS; q++) w[q][e] = part2[q];
         }
-      };
-      if (masked) weights(std::false_type{});
-      else weights(std::true_type{});
+#pragma unroll
+        for (int q = 0; q < NS; q++) tc_st16(ts + q * 32 + c * 16, w[q]);
+      }
       {
         float a, b;
         unpair(add2(sum[0], sum[1]), a, b);
@@ -570,21 +550,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     }
     // ---- the result
     // Poison is final once the loader is through.
-    ok = __all_sync(0xffffffffu, ok && (!n_tiles || wait(&sy.o_full[i], 0)) && wait(&sy.loaded, 0));
+    if (n_tiles) ok = wait(&sy.o_full[i], 0) && ok;
+    else ok = wait(&sy.q_full, 0) && ok;
+    ok = wait(&sy.loaded, 0) && ok;
+    __syncwarp();
     tc_fence_after();
-    if (!ok || *given_up || *(volatile int *)&sy.poison) {
-      for (int k = warp * 32; k < min(warp * 32 + 32, t.rows); k++) attend_row_alone(p, t, k, direct);
+    sy.x[i][half][r] = l;
+    tile_sync();
+    if (*given_up || *(volatile int *)&sy.poison) {
+      for (int k = warp * 16; k < min(warp * 16 + 16, t.rows); k++) attend_row_alone(p, t, k, direct);
     } else {
       // 32 dims at a time through the warp's 4 KB of the query tiles' memory
       // (no product reads it any more), so that rows are stored in whole lines.
-      if (!n_tiles) wait(&sy.q_full, 0);
+      l += sy.x[i][half ^ 1][r];
       const int64_t at = !real ? -1 : direct ? out_offset(p, t, row) : part_index(p, t, row) * hd;
       const float inv = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-      if (real && !direct) p.part_ml[part_index(p, t, row)] = make_float2(m, l);
-      char *const stage = base_p + warp * 4096;
+      if (real && !direct && half == 0) p.part_ml[part_index(p, t, row)] = make_float2(m, l);
       const bool wide = !direct || NS == 2;  // f32 rows
+      char *const stage = base_p + warp * (wide ? 4096 : 2048);
 #pragma unroll 1
-      for (int d = 0; d < HD && d < hd; d += 32) {
+      for (int d = half * (HD / 2); d < (half + 1) * (HD / 2) && d < hd; d += 32) {
         float o[32];
         __syncwarp();
         if (n_tiles) {
@@ -633,7 +618,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == 19) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 }  // namespace paged
