@@ -19,7 +19,7 @@ using namespace paged;
 // chunks' lists merged from their heads, scores cum + (x - lse) in 64 bits;
 // then one warp merges the beams' lists.  One pass over the logits, so the
 // first kernel is bound by reading them.
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 256, kSelBlocks = 4, kSelPer = 16;
 constexpr int kMaxK = 64;
 constexpr int kSelList = 1024;  // candidates that are ranked without a second threshold
 constexpr int kJoinThreads = 512;
@@ -42,16 +42,21 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
 
-struct ChunkHead {  // what a chunk leaves beside its k keys
-  float top, sum;
+constexpr float kLog2e = 1.44269504f;
+struct ChunkHead {  // what a chunk leaves beside its k keys: the sum of 2^(x kLog2e - ref)
+  float ref, sum;
 };
 
-// PER logits a thread, in pieces of 16 bytes where the rows are so aligned.
+// A block reads its chunk piece by piece, PER logits a thread, 16 bytes at a time
+// where the rows are so aligned.  The first piece gives a threshold that k keys
+// reach; from then on a thread only looks for a logit above it, which is rare,
+// and keeps a running maximum and sum.
 template <class T, int PER>
-__global__ void __launch_bounds__(kSelThreads) k_beam_chunk(const BeamParams p, const bool wide, uint64_t *keys,
-                                                           ChunkHead *heads) {
-  constexpr int VEC = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
-  __shared__ uint64_t list[kMaxK * PER > kSelList ? kMaxK * PER : kSelList];
+__global__ void __launch_bounds__(kSelThreads, kSelBlocks) k_beam_chunk(const BeamParams p, const int span, const bool wide,
+                                                           uint64_t *keys, ChunkHead *heads) {
+  constexpr int VEC = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER, kPiece = kSelThreads * PER;
+  constexpr int kList = kMaxK * (PER + 1) > kSelList ? kMaxK * (PER + 1) : kSelList;
+  __shared__ uint64_t list[kList];
   __shared__ uint64_t floors[kSelThreads / 32];
   __shared__ float2 sums[kSelThreads / 32];
   __shared__ int n_list;
@@ -65,112 +70,175 @@ __global__ void __launch_bounds__(kSelThreads) k_beam_chunk(const BeamParams p, 
     return;
   }
   const T *const x = (const T *)p.logits + row * p.row_stride;
-  const int v0 = chunk * (kSelThreads * PER);
-  auto place = [&](int i) { return v0 + ((i / VEC) * kSelThreads + tid) * VEC + i % VEC; };
+  const int begin = chunk * span, end = min(begin + span, p.vocab);
+  auto place = [&](int piece, int i) { return piece + ((i / VEC) * kSelThreads + tid) * VEC + i % VEC; };
   float v[PER];
+  auto load = [&](int piece) {
+    if (wide && piece + kPiece <= end) {  // (one branch for all, so that the loads are on their way together)
 #pragma unroll
-  for (int i = 0; i < PER; i += VEC) {
-    const int at = place(i);
-    if (wide && at + VEC <= p.vocab) {
-      if constexpr (VEC == 8) {
-        float w[8];
-        load8(x + at, w);
+      for (int i = 0; i < PER; i += VEC) {
+        if constexpr (VEC == 8) {
+          float w[8];
+          load8(x + place(piece, i), w);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[i + e] = w[e];
-      } else {
-        const float4 w = *(const float4 *)(x + at);
-        v[i] = w.x; v[i + 1] = w.y; v[i + 2] = w.z; v[i + 3] = w.w;
+          for (int e = 0; e < 8; e++) v[i + e] = w[e];
+        } else {
+          const float4 w = *(const float4 *)(x + place(piece, i));
+          v[i] = w.x; v[i + 1] = w.y; v[i + 2] = w.z; v[i + 3] = w.w;
+        }
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) v[i + e] = at + e < p.vocab ? load_as_f32(x, at + e, p.dtype) : -INFINITY;
-    }
-  }
-  // The thread's best: the first of its largest.  A NaN is -inf.
-  float top = -INFINITY;
-  int first = -1;
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    v[i] = fmaxf(v[i], -INFINITY);
-    if (v[i] > top) {
-      top = v[i];
-      first = i;
-    }
-  }
-  if (first < 0 && place(0) < p.vocab) first = 0;  // all -inf
-  const uint64_t mine = first < 0 ? 0 : key_of(top, (uint32_t)place(first));  // 0: below every key
-  {
-    const float safe = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; i++) sum += __expf(v[i] - safe);
-    const float all = warp_max(top);
-    sum *= all == -INFINITY ? 0.0f : __expf(top - all);
-    sum = warp_sum(sum);
-    if (lane == 0) sums[warp] = make_float2(all, sum);
-  }
-  // At least k groups of threads: the least of the groups' best keys is below
-  // k keys at least, so the k best are not below it.
-  const int width = p.k <= 8 ? 32 : p.k <= 16 ? 16 : p.k <= 32 ? 8 : 4;
-  uint64_t best = mine;
-  for (int o = 1; o < width; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  for (int o = width; o < 32; o <<= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) floors[warp] = best;
-  if (tid == 0) n_list = 0;
-  __syncthreads();
-  uint64_t least = floors[0];
-#pragma unroll
-  for (int w = 1; w < kSelThreads / 32; w++) least = min(least, floors[w]);
-  least = max(least, (uint64_t)1);
-  auto collect = [&](int room) {
-    if (mine < least) return;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int at = place(i);
-      if (at >= p.vocab) continue;
-      const uint64_t key = key_of(v[i], (uint32_t)at);
-      if (key >= least) {
-        const int n = atomicAdd(&n_list, 1);
-        if (n < room) list[n] = key;
+      for (int i = 0; i < PER; i++) {
+        const int at = place(piece, i);
+        const float w = load_as_f32(x, min(at, end - 1), p.dtype);
+        v[i] = at < end ? w : -INFINITY;
       }
     }
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = fmaxf(v[i], -INFINITY);  // a NaN counts as -inf
   };
-  collect(kSelList);
+  // The best key of the thread's logits of a piece, the first of the largest;
+  // 0, below every key, where it has none.
+  auto best_of = [&](int piece, float top) -> uint64_t {
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; i--) {
+      const int at = place(piece, i);
+      if (at < end && v[i] == top) best = key_of(top, (uint32_t)at);
+    }
+    return best;
+  };
+  // The keys of the piece from `least` on into the list, as far as there is
+  // room.  Few logits reach `bar`: a mask of them costs less than a test and a
+  // branch for each, and the value is read again.
+  auto collect = [&](int piece, uint64_t least, float bar, int room) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) found |= v[i] >= bar ? 1u << i : 0u;
+    while (found) {
+      const int i = __ffs(found) - 1, at = place(piece, i);
+      found &= found - 1;
+      if (at >= end) continue;
+      const uint64_t key = key_of(load_as_f32(x, at, p.dtype), (uint32_t)at);
+      if (key < least) continue;
+      const int n = atomicAdd(&n_list, 1);
+      if (n < room) list[n] = key;
+    }
+  };
+  // Sums of 2^(v log2 e - ref), with log2 e as it is in f32 throughout: the
+  // quotient by the same number at the end makes that an error of 10^-8 of the
+  // entropy.  One multiply-add, one exponential and one addition a logit.
+  float top = -INFINITY, ref = 0.0f, sum = 0.0f, bar = -INFINITY;
+  uint64_t least = 1;
+  for (int piece = begin; piece < end; piece += kPiece) {
+    load(piece);
+    float mine = v[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) mine = fmaxf(mine, v[i]);
+    if (mine > top) {
+      const float next = mine * kLog2e;
+      sum *= top == -INFINITY ? 0.0f : exp2_fast(ref - next);
+      top = mine;
+      ref = next;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) sum += exp2_fast(fmaf(v[i], kLog2e, -ref));
+    if (piece == begin) {
+      // At least k groups of threads: the least of the groups' best keys is
+      // below k keys at least, so the k best are not below it.
+      const int width = p.k <= 8 ? 32 : p.k <= 16 ? 16 : p.k <= 32 ? 8 : 4;
+      uint64_t best = best_of(piece, mine);
+      for (int o = 1; o < width; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      for (int o = width; o < 32; o <<= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (lane == 0) floors[warp] = best;
+      if (tid == 0) n_list = 0;
+      __syncthreads();
+      least = floors[0];
+#pragma unroll
+      for (int w = 1; w < kSelThreads / 32; w++) least = min(least, floors[w]);
+      least = max(least, (uint64_t)1);
+      bar = least == 1 ? -INFINITY : value_of(least);
+      if (mine >= bar) collect(piece, least, bar, kSelList);
+      if (begin + kPiece < end) {  // the exact threshold of the first piece for the others
+        __syncthreads();
+        const int n = n_list;
+        if (n <= kSelThreads) {
+          if (tid < n) {
+            const uint64_t key = list[tid];
+            int rank = 0;
+            for (int j = 0; j < n; j++) rank += list[j] > key;
+            if (rank == p.k - 1) floors[0] = key;
+          }
+          __syncthreads();
+          if (n >= p.k) least = floors[0];
+          bar = least == 1 ? -INFINITY : value_of(least);
+        }
+      }
+    } else if (mine >= bar) {
+      collect(piece, least, bar, kSelList);
+    }
+  }
+  {
+    const float all = warp_max(top == -INFINITY ? -INFINITY : ref);
+    const float part = warp_sum(top == -INFINITY ? 0.0f : sum * exp2_fast(ref - all));
+    if (lane == 0) sums[warp] = make_float2(all, part);
+  }
   __syncthreads();
   int n = n_list;
   if (n > kSelList) {
-    // Unevenly spread: from the k-th largest of the threads' best keys on, which
-    // k threads reach, with PER keys each at most.
-    __syncthreads();
-    list[tid] = mine;
-    if (tid == 0) {
-      n_list = 0;
-      floors[0] = 1;
+    // Rows in order, or with many equal logits.  Piece by piece once more: the
+    // k-th largest of the threads' best keys is a threshold that k threads
+    // reach, with PER keys each at most; those and the k best so far are ranked.
+    n = 0;
+    for (int piece = begin; piece < end; piece += kPiece) {
+      __syncthreads();
+      const uint64_t kept = tid < min(n, p.k) ? out[tid] : 0;
+      load(piece);
+      float mine = v[0];
+#pragma unroll
+      for (int i = 1; i < PER; i++) mine = fmaxf(mine, v[i]);
+      const uint64_t best = best_of(piece, mine);
+      list[tid] = best;
+      if (tid == 0) {
+        n_list = 0;
+        floors[0] = 1;
+      }
+      __syncthreads();
+      int above = 0;
+      for (int i = 0; i < kSelThreads; i++) above += list[i] > best;
+      if (above == p.k - 1 && best) floors[0] = best;
+      __syncthreads();
+      least = floors[0];
+      if (best >= least) collect(piece, least, -INFINITY, kList);
+      if (kept) list[atomicAdd(&n_list, 1)] = kept;
+      __syncthreads();
+      n = n_list;
+      for (int i = tid; i < n; i += kSelThreads) {
+        const uint64_t key = list[i];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += list[j] > key;
+        if (rank < p.k) out[rank] = key;
+      }
+      __threadfence_block();
     }
-    __syncthreads();
-    int above = 0;
-    for (int i = 0; i < kSelThreads; i++) above += list[i] > mine;
-    if (above == p.k - 1 && mine) floors[0] = mine;
-    __syncthreads();
-    least = floors[0];
-    collect(kMaxK * PER);
-    __syncthreads();
-    n = n_list;
-  }
-  for (int i = tid; i < n; i += kSelThreads) {
-    const uint64_t key = list[i];
-    int rank = 0;
-    for (int j = 0; j < n; j++) rank += list[j] > key;
-    if (rank < p.k) out[rank] = key;
+  } else {
+    for (int i = tid; i < n; i += kSelThreads) {
+      const uint64_t key = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; j++) rank += list[j] > key;
+      if (rank < p.k) out[rank] = key;
+    }
   }
   for (int i = tid + n; i < p.k; i += kSelThreads) out[i] = 0;
   if (tid == 0) {
-    float all = -INFINITY, sum = 0.0f;
+    float all = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kSelThreads / 32; w++) all = fmaxf(all, sums[w].x);
 #pragma unroll
-    for (int w = 0; w < kSelThreads / 32; w++) sum += sums[w].x == -INFINITY ? 0.0f : sums[w].y * __expf(sums[w].x - all);
-    *head = {all, sum};
+    for (int w = 0; w < kSelThreads / 32; w++)
+      total += sums[w].x == -INFINITY ? 0.0f : sums[w].y * exp2_fast(sums[w].x - all);
+    *head = {all, total};
   }
 }
 
@@ -195,6 +263,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
   uint64_t *const order = (uint64_t *)smem_raw;                // [n_beams][k] scores, in the order of order_of
   int32_t *const token = (int32_t *)(order + p.n_beams * p.k);  // [n_beams][k]
   pdl_wait();
+  pdl_trigger();
   const int seq = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int per_beam = p.chunks * p.k, each = min(p.k, p.vocab);
   uint64_t *const stage = (uint64_t *)(smem_raw + (((int64_t)p.n_beams * p.k * 12 + 15) & ~15)) + warp * per_beam;
@@ -210,7 +279,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
     }
     const double cum = p.cum[row];
     float top = -INFINITY;
-    for (int c = lane; c < p.chunks; c += 32) top = fmaxf(top, h[c].top);
+    for (int c = lane; c < p.chunks; c += 32) top = fmaxf(top, h[c].ref);
     top = warp_max(top);
     // No log-sum-exp: nothing but -inf, or a +inf among them.
     const bool dead = !(cum > -INFINITY && cum < INFINITY && top > -INFINITY && top < INFINITY);
@@ -223,9 +292,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
     }
     double sum = 0.0;
     for (int c = lane; c < p.chunks; c += 32)
-      if (h[c].sum > 0.0f) sum += exp((double)h[c].top - (double)top) * (double)h[c].sum;
+      if (h[c].sum > 0.0f) sum += exp2((double)h[c].ref - (double)top) * (double)h[c].sum;
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double lse = (double)top + log(sum);
+    const double lse = ((double)top + log2(sum)) / (double)kLog2e;
     uint64_t head[kJoinLists];
     int pos[kJoinLists];
 #pragma unroll
@@ -287,67 +356,88 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
 }
 
 // One block per (beam row, layer): the row's page list from its parent's, and
-// this layer's copy of the unfinished page where the row needs its own.
-constexpr int kReorderThreads = 256;
+// this layer's copy of the unfinished page where the row needs its own.  Bound by
+// reading and writing those pages once: 128 beams in 32 layers, 44 rows copied,
+// 322 MB written and 116 MB read from DRAM in 69 us, the measured copy rate.
+// (Bulk copies through shared memory took 73 us, eight layers a block 83 us.)
+constexpr int kRowThreads = 256;
 
-__global__ void __launch_bounds__(kReorderThreads) k_beam_reorder(const ReorderParams p, const int elem) {
+// One head's filled slots, by a warp; `dense`: they lie one after another.
+__device__ __forceinline__ void copy_head(const char *src, char *dst, int fill, int chunks, int64_t slot_bytes,
+                                          bool dense) {
+  constexpr int kPieces = 4;
+  const int total = fill * chunks, lane = threadIdx.x % 32;
+  for (int i = lane; i < total; i += 32 * kPieces) {
+    uint4 w[kPieces];
+    int64_t o[kPieces];
+#pragma unroll
+    for (int e = 0; e < kPieces; e++) {
+      const int k = i + 32 * e;
+      o[e] = dense ? (int64_t)k * 16 : (int64_t)(k / chunks) * slot_bytes + (k % chunks) * 16;
+      if (k < total) w[e] = *(const uint4 *)(src + o[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < kPieces; e++)
+      if (i + 32 * e < total) *(uint4 *)(dst + o[e]) = w[e];
+  }
+}
+
+__global__ void __launch_bounds__(kRowThreads) k_beam_reorder(const __grid_constant__ ReorderParams p, const int elem) {
+  pdl_wait();  // (the parents may come from a selection just before)
   const int row = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x;
   const int seq = row / p.n_beams, beam = row % p.n_beams;
   const int32_t *parents = p.parents + (int64_t)seq * p.n_beams;
   const int parent = parents[beam];
+  bool heir = true;
+  for (int j = 0; j < beam; j++) heir &= parents[j] != parent;
+  if (heir && layer) return;
   const PagedView &kv = p.kv;
   int32_t *out = p.new_table + (int64_t)row * kv.max_pages;
   if ((unsigned)parent >= (unsigned)p.n_beams) {  // no such beam: an empty row
     if (layer) return;
-    for (int j = tid; j < kv.max_pages; j += kReorderThreads) out[j] = -1;
+    for (int j = tid; j < kv.max_pages; j += kRowThreads) out[j] = -1;
     if (tid == 0) p.new_len[row] = 0;
     return;
   }
-  const int source = seq * p.n_beams + parent;
+  const int source = seq * p.n_beams + parent, to = p.fresh[row];
   const int32_t *old = kv.table + (int64_t)source * kv.max_pages;
   const int len = min(max(p.kv_len[source], 0), kv.cap);
   const int full = len / kv.page_size, fill = len - full * kv.page_size;
-  bool heir = true;
-  for (int j = 0; j < beam; j++) heir &= parents[j] != parent;
+  const int from = fill ? old[full] : -1;  // (a table that is full has no unfinished page)
   const bool takes = !heir || fill == 0;
   if (layer == 0) {
-    for (int j = tid; j < kv.max_pages; j += kReorderThreads)
-      out[j] = j < full ? old[j] : j > full ? -1 : takes ? p.fresh[row] : old[j];
+    for (int j = tid; j < kv.max_pages; j += kRowThreads)
+      out[j] = j < full ? old[j] : j > full ? -1 : takes ? to : from;
     if (tid == 0) p.new_len[row] = len;
   }
   if (!takes || fill == 0) return;
-  const int from = old[full], to = p.fresh[row];
   if ((unsigned)from >= (unsigned)kv.n_pages || (unsigned)to >= (unsigned)kv.n_pages) return;
-  // A warp for each head of K and of V in turn; four 16-byte pieces a lane are
-  // on their way at a time.
-  const int chunks = kv.hd * elem / 16, total = fill * chunks, lane = tid % 32;
-  const bool dense = kv.slot_stride == kv.hd;
-  for (int seg = tid / 32; seg < 2 * kv.hkv; seg += kReorderThreads / 32) {
-    const bool is_v = seg >= kv.hkv;
-    const int64_t at = layer * p.layer_stride + (int64_t)(is_v ? seg - kv.hkv : seg) * kv.head_stride;
-    const char *const src = (const char *)(is_v ? kv.v : kv.k) + (at + from * kv.page_stride) * elem;
-    char *const dst = (char *)(is_v ? p.vw : p.kw) + (at + to * kv.page_stride) * elem;
-    for (int i = lane; i < total; i += 128) {
-      uint4 w[4];
-      int64_t o[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int k = i + 32 * e;
-        o[e] = dense ? (int64_t)k * 16 : (int64_t)(k / chunks) * kv.slot_stride * elem + (k % chunks) * 16;
-        if (k < total) w[e] = *(const uint4 *)(src + o[e]);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (i + 32 * e < total) *(uint4 *)(dst + o[e]) = w[e];
-    }
-  }
+  const int heads = 2 * kv.hkv;
+  auto place = [&](int h, int page) {  // byte offset of head h (of K, then of V) in a page of this layer
+    return (layer * p.layer_stride + (h >= kv.hkv ? h - kv.hkv : h) * kv.head_stride + page * kv.page_stride) * elem;
+  };
+  auto pool = [&](int h) { return (char *)(h >= kv.hkv ? p.vw : p.kw); };
+  for (int h = tid / 32; h < heads; h += kRowThreads / 32)
+    copy_head(pool(h) + place(h, from), pool(h) + place(h, to), fill, kv.hd * elem / 16, kv.slot_stride * elem,
+              kv.slot_stride == kv.hd);
 }
 
-// Logits a thread of the first kernel takes.  A few rows are cut finer, so that
-// they spread over the SMs (4 rows of 4096: 8 blocks instead of 4).
-int per_thread(size_t n_rows, size_t vocab) {
-  const size_t blocks = n_rows * ((vocab + kSelThreads * 32 - 1) / (kSelThreads * 32));
-  return blocks < 2 * (size_t)kPagedSMs && vocab <= (size_t)kSelThreads * 8 * 32 * kJoinLists ? 8 : 32;
+// How a selection is cut: logits a thread takes at a time, and blocks a row.
+// kSelBlocks blocks run on an SM: one round of them where there are rows enough;
+// few rows go to more and smaller blocks.
+struct SelPlan {
+  int per, chunks, span;
+};
+SelPlan sel_plan(size_t n_rows, size_t vocab) {
+  SelPlan a;
+  const size_t slots = kSelBlocks * (size_t)kPagedSMs, wide = (vocab + kSelThreads * kSelPer - 1) / (kSelThreads * kSelPer);
+  a.per = n_rows * wide < slots / 2 ? 8 : kSelPer;
+  const size_t pieces = (vocab + kSelThreads * a.per - 1) / (kSelThreads * a.per);
+  const size_t wanted = std::max<size_t>(1, std::min<size_t>(pieces, slots / std::max<size_t>(1, n_rows)));
+  const size_t chunks = std::min<size_t>(wanted, 32 * kJoinLists);
+  a.span = (int)((((vocab + chunks - 1) / chunks) + 7) / 8 * 8);
+  a.chunks = (int)((vocab + a.span - 1) / a.span);
+  return a;
 }
 size_t join_lists(size_t n_beams, size_t k) { return (n_beams * k * 12 + 15) / 16 * 16; }
 size_t join_stage(size_t chunks, size_t k) { return kJoinThreads / 32 * chunks * k * sizeof(uint64_t); }
@@ -357,19 +447,18 @@ void run_chunks(const BeamParams &p, uint64_t *keys, ChunkHead *heads, cudaStrea
   const size_t rows = (size_t)p.n_seqs * p.n_beams;
   const bool wide = (uintptr_t)p.logits % 16 == 0 && p.row_stride * sizeof(T) % 16 == 0;
   const dim3 grid((unsigned)p.chunks, (unsigned)rows);
-  if (per_thread(rows, p.vocab) == 8) k_beam_chunk<T, 8><<<grid, kSelThreads, 0, s>>>(p, wide, keys, heads);
-  else k_beam_chunk<T, 32><<<grid, kSelThreads, 0, s>>>(p, wide, keys, heads);
+  const SelPlan a = sel_plan(rows, (size_t)p.vocab);
+  if (a.per == 8) k_beam_chunk<T, 8><<<grid, kSelThreads, 0, s>>>(p, a.span, wide, keys, heads);
+  else k_beam_chunk<T, kSelPer><<<grid, kSelThreads, 0, s>>>(p, a.span, wide, keys, heads);
   JAL_CUDA(cudaGetLastError());
 }
 
 }  // namespace
 
-int beam_chunks(size_t n_rows, size_t vocab) {
-  const size_t chunk = (size_t)kSelThreads * per_thread(n_rows, vocab);
-  return (int)((vocab + chunk - 1) / chunk);
-}
+int beam_chunks(size_t n_rows, size_t vocab) { return sel_plan(n_rows, vocab).chunks; }
 bool beam_fits(size_t n_beams, size_t vocab, size_t k, size_t n_rows) {
-  return beam_chunks(n_rows, vocab) <= 32 * kJoinLists && n_beams <= (size_t)kMaxBeams && join_lists(n_beams, k) <= kJoinSmem;
+  (void)n_rows;
+  return vocab <= (1u << 20) && n_beams <= (size_t)kMaxBeams && join_lists(n_beams, k) <= kJoinSmem;
 }
 size_t beam_workspace(size_t n_seqs, size_t n_beams, size_t vocab, size_t k) {
   const size_t chunks = n_seqs * n_beams * (size_t)beam_chunks(n_seqs * n_beams, vocab);
@@ -402,8 +491,16 @@ void launch_beam_select(const BeamParams &p, cudaStream_t s) {
 
 void launch_beam_reorder(const ReorderParams &p, cudaStream_t s) {
   const int elem = p.kv.dtype == JAL_F32 ? 4 : 2;
-  k_beam_reorder<<<dim3((unsigned)(p.n_seqs * p.n_beams), (unsigned)p.n_layers), kReorderThreads, 0, s>>>(p, elem);
-  JAL_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.n_seqs * p.n_beams), (unsigned)p.n_layers);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  JAL_CUDA(cudaLaunchKernelEx(&cfg, k_beam_reorder, p, elem));
 }
 
 }  // namespace jal

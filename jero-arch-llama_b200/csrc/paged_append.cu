@@ -97,8 +97,33 @@ __device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2
   }
 }
 
+// Eight elements as they are in memory.
+template <class T>
+struct Raw8 {
+  uint4 w;
+  __device__ __forceinline__ void load(const T *p) { w = *(const uint4 *)p; }
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = unpack2<T>(u[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+template <>
+struct Raw8<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float *p) { load8(p, v); }
+  __device__ __forceinline__ void widen(float (&o)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = v[i];
+  }
+};
+
 template <class TA, class TK>
-__global__ void __launch_bounds__(kWarps * 32) k_rope_kv_append_pairs(const __grid_constant__ AppendParams p, const int parts) {
+__global__ void __launch_bounds__(kWarps * 32, 7) k_rope_kv_append_pairs(const __grid_constant__ AppendParams p, const int parts) {
   constexpr int kItems = sizeof(TA) == 4 ? 2 : 4;
   __shared__ float2 turns[kWarps][kPagedMaxHeadDim / 2];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, unit = blockIdx.x * kWarps + warp;
@@ -119,7 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_rope_kv_append_pairs(const __gr
   const int nq = p.q ? p.hq : 0, items = half / 8 + (hd - p.rotary) / 8, total = (nq + 2 * p.kv.hkv) * items;
   const int per = (total + parts - 1) / parts, stop = min(total, (part + 1) * per);
   for (int i = part * per + lane; i < stop; i += 32 * kItems) {
-    float a[kItems][8], b[kItems][8];
+    Raw8<TA> ra[kItems], rb[kItems];
 #pragma unroll
     for (int k = 0; k < kItems; k++) {
       const int it = i + 32 * k;
@@ -129,10 +154,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_rope_kv_append_pairs(const __gr
       const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
       const TA *const src = (const TA *)(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.q_stride : p.kv_stride) + h * hd;
       if (c < half / 8) {
-        load8(src + c * 8, a[k]);
-        load8(src + c * 8 + half, b[k]);
+        ra[k].load(src + c * 8);
+        rb[k].load(src + c * 8 + half);
       } else {
-        load8(src + p.rotary + (c - half / 8) * 8, a[k]);
+        ra[k].load(src + p.rotary + (c - half / 8) * 8);
       }
     }
 #pragma unroll
@@ -144,15 +169,18 @@ __global__ void __launch_bounds__(kWarps * 32) k_rope_kv_append_pairs(const __gr
       const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
       const bool rotated = c < half / 8;
       const int d = rotated ? c * 8 : p.rotary + (c - half / 8) * 8;
-      if (rotated && (is_q || is_k)) turn8<TA>(a[k], b[k], cs, d, half, p.neox);
+      float a[8], b[8];
+      ra[k].widen(a);
+      rb[k].widen(b);
+      if (rotated && (is_q || is_k)) turn8<TA>(a, b, cs, d, half, p.neox);
       if (is_q) {
         TA *const dst = (TA *)p.q_out + row * p.q_out_stride + h * hd;
-        store8(dst + d, a[k]);
-        if (rotated) store8(dst + d + half, b[k]);
+        store8(dst + d, a);
+        if (rotated) store8(dst + d + half, b);
       } else if (at >= 0) {
         TK *const dst = (TK *)(is_k ? p.kw : p.vw) + at + h * p.kv.head_stride;
-        store8(dst + d, a[k]);
-        if (rotated) store8(dst + d + half, b[k]);
+        store8(dst + d, a);
+        if (rotated) store8(dst + d + half, b);
       }
     }
   }
