@@ -137,10 +137,11 @@ jal_prefix_groups checked_groups(const jal_prefix_groups *in, const jal_paged_kv
   return g;
 }
 
-void check_grid(const AttnPlan &a, const jal_paged_kv &kv, const jal_ragged_batch &b, const jal_prefix_groups *g) {
+void check_grid(const AttnPlan &a, const jal_paged_kv &kv, const jal_ragged_batch &b, const jal_prefix_groups *g,
+                size_t hq) {
   const double blocks = (double)kv.n_heads_kv * ((double)a.tiles * a.splits * (double)b.n_seqs +
                                                  (g ? (double)a.prefix_tiles * a.prefix_splits * (double)g->n_groups : 0));
-  if (blocks > 2e9 || (double)b.n_seqs * (double)b.max_q_len > 2e9)
+  if (blocks > 2e9 || (!a.direct && (double)b.n_seqs * (double)b.max_q_len * (double)hq > 2e9))
     fail(JAL_ERR_CAPABILITY_MISMATCH, "batch too large for one launch");
 }
 
@@ -164,7 +165,7 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   aligned16(out, "out");
   if (b.n_seqs == 0 || b.n_rows == 0 || b.max_q_len == 0) return;
   const AttnPlan plan = plan_attention(kv, b, g.n_groups ? &g : nullptr, hq, dtype, window, n_sink);
-  check_grid(plan, kv, b, g.n_groups ? &g : nullptr);
+  check_grid(plan, kv, b, g.n_groups ? &g : nullptr, hq);
   if (plan.bytes) {
     NEED(ws);
     aligned16(ws, "workspace");

@@ -177,18 +177,20 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
 }
 
 // ---- joining the pieces -----------------------------------------------------
-// Row by row, one warp for each (token row, query head): the pieces' sums
-// rescaled to the largest of their maxima and added in the order of the
-// pieces.  A piece without a visible key has sum 0 and is not read.
-constexpr int kJoinWarps = 4;
+// One block for each (token row, query head): the pieces' sums rescaled to the
+// largest of their maxima and added, each warp every fourth piece with eight
+// pieces' loads under way, the warps in order at the end.  A piece without a
+// visible key has sum 0 and is not read.
+constexpr int kJoinWarps = 4, kJoinThreads = kJoinWarps * 32;
+static_assert(2 * kPagedMaxSplits <= kJoinThreads, "a thread looks at one piece's maximum and sum");
 
-__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(const __grid_constant__ AttnParams p, const int prefix_rows) {
+__global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(const __grid_constant__ AttnParams p, const int prefix_rows) {
+  __shared__ float weight[kJoinThreads];
+  __shared__ float red[kJoinWarps];
+  __shared__ float4 part[kJoinWarps][kPagedMaxHeadDim / 4];
   pdl_wait();
-  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31, head = (int)(id % p.hq);
-  const int64_t tok = id / p.hq;
-  const int s = (int)(tok / p.max_q), i = (int)(tok % p.max_q);
-  if (s >= p.n_seqs) return;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, head = blockIdx.x % p.hq;
+  const int tok = blockIdx.x / p.hq, s = tok / p.max_q, i = tok - s * p.max_q;
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   if (i >= end - beg) return;
@@ -202,53 +204,61 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_attn_join(const __gri
       if ((int64_t)(row - gb + 1) * p.G > (int64_t)p.prefix_tiles * prefix_rows) return;  // past max_group: not computed
     }
   }
-  const int n = p.prefix_splits + p.splits;
+  const int n = p.prefix_splits + p.splits, hd = p.kv.hd;
   const int64_t stride = (int64_t)p.n_rows * p.hq, at = (int64_t)row * p.hq + head;
-  constexpr int W = kPagedMaxSplits * 2 / 32;
-  float mw[W], lw[W], top = -INFINITY;
-  bool nan = false;
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (tid >= first && tid < n) ml = p.part_ml[tid * stride + at];
+  float top = warp_max(ml.x);
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < W; k++) {
-    const int piece = k * 32 + lane;
-    mw[k] = -INFINITY;
-    lw[k] = 0.0f;
-    if (piece >= first && piece < n) {
-      const float2 ml = p.part_ml[piece * stride + at];
-      mw[k] = ml.x;
-      lw[k] = ml.y;
+  for (int w = 0; w < kJoinWarps; w++) top = fmaxf(top, red[w]);
+  const float w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+  weight[tid] = w;
+  float total = warp_sum(w * ml.y);
+  __syncthreads();
+  if (lane == 0) red[warp] = total;
+  __syncthreads();
+  total = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kJoinWarps; k++) total += red[k];
+  const int chunks = hd / 4;  // float4 pieces of a row: two a lane at most
+  float4 o[2] = {};
+  for (int k = warp; k < n; k += kJoinWarps * 8) {
+    float4 v[8][2];
+    float c[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int piece = k + e * kJoinWarps;
+      c[e] = piece < n ? weight[piece] : 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        v[e][h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c[e] != 0.0f && lane + 32 * h < chunks)
+          v[e][h] = *((const float4 *)(p.part_o + (piece * stride + at) * hd) + lane + 32 * h);
+      }
     }
-    nan |= mw[k] != mw[k];
-    top = fmaxf(top, mw[k]);
-  }
-  top = warp_max(top);
-  const float safe = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f;
 #pragma unroll
-  for (int k = 0; k < W; k++) {
-    mw[k] = lw[k] == 0.0f ? 0.0f : exp2f(mw[k] - safe);  // from here the piece's weight
-    total += mw[k] * lw[k];
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        o[h].x = fmaf(c[e], v[e][h].x, o[h].x);
+        o[h].y = fmaf(c[e], v[e][h].y, o[h].y);
+        o[h].z = fmaf(c[e], v[e][h].z, o[h].z);
+        o[h].w = fmaf(c[e], v[e][h].w, o[h].w);
+      }
   }
-  total = warp_sum(total);
+  part[warp][lane] = o[0];
+  part[warp][lane + 32] = o[1];
+  __syncthreads();
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  float o[kPagedMaxHeadDim / 32];
-#pragma unroll
-  for (int c = 0; c < kPagedMaxHeadDim / 32; c++) o[c] = 0.0f;
-  const int hd = p.kv.hd;
-#pragma unroll
-  for (int k = 0; k < W; k++) {
-    for (int q = 0; q < 32 && k * 32 + q < n; q++) {
-      const float w = __shfl_sync(0xffffffffu, mw[k], q);
-      if (w == 0.0f) continue;
-      const float *po = p.part_o + ((k * 32 + q) * stride + at) * hd;
-#pragma unroll
-      for (int c = 0; c < kPagedMaxHeadDim / 32; c++)
-        if (lane + 32 * c < hd) o[c] = fmaf(w, po[lane + 32 * c], o[c]);
-    }
-  }
   const int64_t oo = (int64_t)row * p.out_stride + (int64_t)head * hd;
+  for (int d = tid; d < hd; d += kJoinThreads) {
+    float sum = 0.0f;
 #pragma unroll
-  for (int c = 0; c < kPagedMaxHeadDim / 32; c++)
-    if (lane + 32 * c < hd) store_from_f32(p.out, oo + lane + 32 * c, p.act, o[c] * inv);
+    for (int k = 0; k < kJoinWarps; k++) sum += ((const float *)part[k])[d];
+    store_from_f32(p.out, oo + d, p.act, sum * inv);
+  }
 }
 
 int64_t blocks_of(const AttnParams &p, int part) {
@@ -256,13 +266,30 @@ int64_t blocks_of(const AttnParams &p, int part) {
   const int64_t own = (int64_t)p.splits * p.tiles * p.n_seqs;
   return p.kv.hkv * ((part == kOwn ? 0 : prefix) + (part == kPrefix ? 0 : own));
 }
+// `beside`: may start while the launch before it still runs (it waits for that
+// one's end itself).
+template <class F, class... A>
+void launch(F kernel, int64_t blocks, int threads, int smem, bool beside, cudaStream_t s, const A &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  JAL_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
 template <class F>
-void run_kernel(F kernel, const AttnParams &p, int part, bool direct, int threads, int smem, cudaStream_t s) {
+bool run_kernel(F kernel, const AttnParams &p, int part, bool direct, int threads, int smem, cudaStream_t s,
+                bool beside = false) {
   const int64_t blocks = blocks_of(p, part);
-  if (!blocks) return;
+  if (!blocks) return false;
   JAL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<(unsigned)blocks, threads, smem, s>>>(p, part, direct);
-  JAL_CUDA(cudaGetLastError());
+  launch(kernel, blocks, threads, smem, beside, s, p, part, direct);
+  return true;
 }
 
 template <class TK, int HD>
@@ -274,14 +301,18 @@ void run_f32(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
 }
 template <class T, int NS, int HD>
 void run_16bit(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
+  // Prefixes on tcgen05 and a sequence's own keys on mma.sync: two launches
+  // that do not depend on each other.
   const int tc = plan.rows == kTcRows ? plan.prefix_rows != kMmaRows ? kBoth : kOwn : kPrefix;
+  bool first = false;
   if constexpr (HD <= 128 && NS <= 2) {
     if (plan.rows == kTcRows || plan.prefix_rows == kTcRows)
-      run_kernel(k_paged_attn_tc<T, NS, HD>, p, tc, plan.direct, kTcThreads, TcShape<NS, HD>::smem, s);
+      first = run_kernel(k_paged_attn_tc<T, NS, HD>, p, tc, plan.direct, kTcThreads, TcShape<NS, HD>::smem, s);
   }
   if (plan.rows == kMmaRows || plan.prefix_rows == kMmaRows) {
     const int part = plan.rows != kMmaRows ? kPrefix : plan.prefix_rows == kTcRows ? kOwn : kBoth;
-    run_kernel(k_paged_attn_mma<T, NS, HD>, p, part, plan.direct, kMmaThreads, MmaShape<NS, HD>::smem, s);
+    run_kernel(k_paged_attn_mma<T, NS, HD>, p, part, plan.direct, kMmaThreads, MmaShape<NS, HD>::smem, s,
+               first);
   }
 }
 template <class T, int NS>
@@ -371,17 +402,7 @@ void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) 
     run_16bit_hd<__nv_bfloat16, 3>(p, plan, s);
   }
   if (plan.direct) return;
-  const int64_t warps = (int64_t)p.n_seqs * p.max_q * p.hq;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  JAL_CUDA(cudaLaunchKernelEx(&cfg, k_paged_attn_join, p, plan.prefix_rows));
+  launch(k_paged_attn_join, (int64_t)p.n_seqs * p.max_q * p.hq, kJoinThreads, 0, true, s, p, plan.prefix_rows);
 }
 
 }  // namespace jal

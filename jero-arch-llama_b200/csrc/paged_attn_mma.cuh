@@ -96,7 +96,10 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const __grid_
   __shared__ uint32_t present[kMmaWarps][S::stages];
   pdl_trigger();
   Tile t;
-  if (!block_tile(p, part, kMmaRows, kMmaWarps * kMmaKeys, t)) return;
+  if (!block_tile(p, part, kMmaRows, kMmaWarps * kMmaKeys, t)) {
+    pdl_wait();
+    return;
+  }
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, hd = p.kv.hd;
   const uint32_t sq = smem_u32(smem_raw), ring = sq + S::q_bytes + warp * (S::stages * 2 * S::half);
   char *const q_sm = smem_raw;
@@ -323,9 +326,13 @@ __global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const __grid_
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
   if (__syncthreads_or(watched_bad<T>(bad))) {  // (also: no warp reads its ring any more)
     for (int j = warp; j < t.rows; j += kMmaWarps) attend_row_alone(p, t, j, direct);
+    pdl_wait();
     return;
   }
 
+  // A launch beside another one ends after it, so that what waits for this
+  // launch has waited for both.
+  pdl_wait();
   // The four warps' results, joined through shared memory.
   float *const merge = (float *)(smem_raw + S::q_bytes);
   if ((lane & 3) == 0) {

@@ -52,6 +52,7 @@ struct TcSync {
   // of the weights.  Before the first tile: what a row's scores are still to be
   // multiplied by (NS = 2, [256]).  Barriers lie between these uses.
   float x[2][2][128];
+  float m1[128];  // at the end: what the weights of the second row tile refer to
   alignas(16) uint8_t present[8][16];    // which keys of tile j exist, a bit each, by j % 8
 };
 
@@ -153,6 +154,8 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t *r) {
 #undef JAL_I8
 
 
+static_assert(TcShape<1, 128>::smem <= 232448 && TcShape<2, 128>::smem <= 232448, "shared memory of a block");
+
 template <class T, int NS, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_constant__ AttnParams p, const int part, const bool direct) {
   using S = TcShape<NS, HD>;
@@ -165,6 +168,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
   char *const base_p = smem_tc;
   const uint32_t sq = smem_u32(smem_tc), ring = sq + S::ring;
   const int n_tiles = (t.u1 - t.u0 + kTcKeys - 1) / kTcKeys;
+  // At most 128 rows: both row tiles hold them, the first takes the even key
+  // tiles and the second the odd ones, and their results are joined.
+  const bool twice = t.rows <= 128;
 
   if (tid == 0) {
     mbar_init(&sy.q_full, kTcSoftmax);
@@ -340,51 +346,73 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         if (leader) tc_commit(&sy.kv_empty[b]);
         __syncwarp();
       };
-      int b = 0, parity = 0;  // the next buffer to be taken
-      auto take = [&](int &got) {
-        const bool there = wait(&sy.kv_full[b], parity);
+      // K tile j is copy 2 j, V tile j copy 2 j + 1; copies go round the buffers.
+      auto there = [&](int g) {
+        const bool ok = wait(&sy.kv_full[g % S::buffers], (g / S::buffers) & 1);
         fence_proxy_async();  // the rows were written by cp.async, the tensor cores read them by the async proxy
-        got = b;
-        if (++b == S::buffers) {
-          b = 0;
-          parity ^= 1;
-        }
-        return there;
-      };
-      int kb = 0, vb = 0;
-      bool ok = n_tiles == 0 || (wait(&sy.q_full, 0) && take(kb));
-      if (ok && n_tiles) {
         tc_fence_after();
-        scores(0, kb);
-        scores(1, kb);
-        release(kb);
-      }
+        return ok;
+      };
+      bool ok = n_tiles == 0 || wait(&sy.q_full, 0);
+      if (twice) {
+        for (int j = 0; j < min(n_tiles, 2) && ok; j++) {
+          ok = there(2 * j);
+          if (!ok) break;
+          scores(j, (2 * j) % S::buffers);
+          release((2 * j) % S::buffers);
+        }
 #pragma unroll 1
-      for (int j = 0; j < n_tiles && ok; j++) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          ok = ok && (i || take(vb)) && wait(&sy.p_full[i], j & 1);
+        for (int j = 0; j < n_tiles && ok; j++) {
+          const int i = j & 1, v = 2 * j + 1, k = 2 * j + 4;
+          ok = there(v) && wait(&sy.p_full[i], (j >> 1) & 1);
           if (!ok) break;
           tc_fence_after();
-          output(i, vb, j == 0);
-          if (i) release(vb);
-          if (j + 1 < n_tiles) {
-            ok = i || take(kb);
+          output(i, v % S::buffers, j < 2);
+          release(v % S::buffers);
+          if (j + 2 < n_tiles) {
+            ok = there(k);
             if (!ok) break;
-            tc_fence_after();
-            scores(i, kb);
-            if (i) release(kb);
+            scores(i, k % S::buffers);
+            release(k % S::buffers);
           } else {
             if (leader) tc_commit(&sy.o_full[i]);
             __syncwarp();
+          }
+        }
+      } else {
+        ok = ok && (n_tiles == 0 || there(0));
+        if (ok && n_tiles) {
+          scores(0, 0);
+          scores(1, 0);
+          release(0);
+        }
+#pragma unroll 1
+        for (int j = 0; j < n_tiles && ok; j++) {
+          const int v = 2 * j + 1, k = 2 * j + 2;
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            ok = ok && (i || there(v)) && wait(&sy.p_full[i], j & 1);
+            if (!ok) break;
+            tc_fence_after();
+            output(i, v % S::buffers, j == 0);
+            if (i) release(v % S::buffers);
+            if (j + 1 < n_tiles) {
+              ok = i || there(k);
+              if (!ok) break;
+              scores(i, k % S::buffers);
+              if (i) release(k % S::buffers);
+            } else {
+              if (leader) tc_commit(&sy.o_full[i]);
+              __syncwarp();
+            }
           }
         }
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    // ---- softmax: threads r of the warpgroups 2 i and 2 i + 1 have row i * 128 + r
-    const int i = warp / 8, half = warp / 4 % 2, r = tid % 128, row = i * 128 + r;
+    // ---- softmax: threads r of the warpgroups 2 i and 2 i + 1 have row r of row tile i
+    const int i = warp / 8, half = warp / 4 % 2, r = tid % 128, base = twice ? 0 : i * 128, row = base + r;
     const bool real = row < t.rows;
     const RowMask mk = real ? row_mask(p, t, row) : RowMask{0, 0};
     // Weights are formed with a positive factor: a negative one turns q round,
@@ -395,7 +423,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       const int first = warp % 8 * 16;  // of the row tile
       char *const dst = base_p + i * NS * S::q_tile;
       const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-      const int mine = i * 128 + first + lane % 16;
+      const int mine = base + first + lane % 16;
       const int64_t qt = mine < t.rows && p.scale_log2 != 0.0f ? q_offset(p, t, mine) : -1;
       constexpr int CH = HD / 8;
       if constexpr (NS == 1) {
@@ -442,7 +470,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
           if (c == 0) (&sy.x[0][0][0])[i * 128 + first + kr] = (1.0f / fabsf(a)) / b;
         }
         tile_sync();
-        scale *= (&sy.x[0][0][0])[row];
+        scale *= (&sy.x[0][0][0])[i * 128 + r];
       }
       int lo = real ? mk.lim : 0x7fffffff, hi = real ? mk.lim : 0, wl = real ? mk.wlo : 0x7fffffff, wh = real ? mk.wlo : 0;
       lo = __reduce_min_sync(0xffffffffu, lo);
@@ -463,11 +491,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     const RowSpan span = row_span(p, t, mk);
     float m = -INFINITY, l = 0.0f;  // m: what the weights refer to, scaled to base 2; l: this half's sum
     bool ok = true;
+    int turn = 0;  // of this row tile
 #pragma unroll 1
-    for (int j = 0; j < n_tiles; j++) {
+    for (int j = twice ? i : 0; j < n_tiles; j += twice ? 2 : 1, turn++) {
       // (A wait that gave up does not leave the loop: the other half waits below.)
       ok = wait(&sy.present_full[j & 7], (j >> 3) & 1) && ok;
-      ok = wait(&sy.s_full[i], j & 1) && ok;
+      ok = wait(&sy.s_full[i], turn & 1) && ok;
       __syncwarp();
       tc_fence_after();
       float s[2][32];
@@ -503,7 +532,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         const float c = raise ? exp2_fast(m - top) : 1.0f;
         if (raise) m = top;
         l *= c;
-        if (j > 0) {  // this half of O's columns
+        if (turn > 0) {  // this half of O's columns
 #pragma unroll 1
           for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 32) {
             uint32_t o[32];
@@ -550,19 +579,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     }
     // ---- the result
     // Poison is final once the loader is through.
-    if (n_tiles) ok = wait(&sy.o_full[i], 0) && ok;
-    else ok = wait(&sy.q_full, 0) && ok;
+    const bool has0 = n_tiles > 0, has1 = n_tiles > (twice ? 1 : 0);
+    if (twice ? has0 : (i ? has1 : has0)) ok = wait(&sy.o_full[twice ? 0 : i], 0) && ok;
+    if (twice && has1) ok = wait(&sy.o_full[1], 0) && ok;
+    if (!has0) ok = wait(&sy.q_full, 0) && ok;
     ok = wait(&sy.loaded, 0) && ok;
     __syncwarp();
     tc_fence_after();
     sy.x[i][half][r] = l;
-    tile_sync();
+    if (i == 1 && half == 0) sy.m1[r] = m;
+    asm volatile("bar.sync 3, 512;" ::: "memory");
     if (*given_up || *(volatile int *)&sy.poison) {
       for (int k = warp * 16; k < min(warp * 16 + 16, t.rows); k++) attend_row_alone(p, t, k, direct);
-    } else {
+    } else if (!twice || i == 0) {
+      // The two halves' sums; twice: the two tiles' results on the larger maximum.
+      l += sy.x[i][half ^ 1][r];
+      float c0 = 1.0f, c1 = 0.0f;
+      if (twice) {
+        const float m1 = sy.m1[r], l1 = sy.x[1][0][r] + sy.x[1][1][r], top = fmaxf(m, m1);
+        c0 = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        c1 = m1 == -INFINITY ? 0.0f : exp2_fast(m1 - top);
+        l = l * c0 + l1 * c1;
+        m = top;
+      }
       // 32 dims at a time through the warp's 4 KB of the query tiles' memory
       // (no product reads it any more), so that rows are stored in whole lines.
-      l += sy.x[i][half ^ 1][r];
       const int64_t at = !real ? -1 : direct ? out_offset(p, t, row) : part_index(p, t, row) * hd;
       const float inv = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
       if (real && !direct && half == 0) p.part_ml[part_index(p, t, row)] = make_float2(m, l);
@@ -578,6 +619,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e++) o[e] = 0.0f;
+        }
+        if (twice) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] *= c0;
+          if (has1) {
+            float o1[32];
+            tc_ld32(to + 128 + d, (uint32_t *)o1);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = fmaf(o1[e], c1, o[e]);
+          }
         }
 #pragma unroll
         for (int e = 0; e < 32; e++) o[e] *= inv;
