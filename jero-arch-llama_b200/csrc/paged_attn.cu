@@ -322,12 +322,15 @@ void run_16bit_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
   else run_16bit<T, NS, 256>(p, plan, s);
 }
 
-// Into how many pieces the keys of `blocks` blocks' rows go.  `slots` blocks
-// run at once; the time is that of the rounds it takes, each as long as a
-// piece's keys and what a block costs besides (a start and an end worth
-// kBlockKeys keys of reading).  A second kernel joins the pieces: worth
-// kJoinKeys.  Measured on one 131071-key row over 8 KV heads: 37 pieces (one
-// full round of 296 blocks) XX us, 64 pieces (1.7 rounds) 150 us.
+// Into how many pieces the keys of `blocks` blocks' rows go: the least of a
+// rough count of the time in keys.  The SM with the most blocks takes longest; it
+// holds `resident` at once, two of them read as fast as its share of the memory
+// allows, and each round of blocks has a start and an end worth kBlockKeys.  The
+// pieces have to be joined, by a second kernel that a call with shared prefixes
+// needs anyway.  Measured: 131071 keys of 8 KV heads in 37 pieces 94 us, in 40 or 55
+// 101 us; 48 rows of up to 4100 keys of 8 KV heads in one piece 132 us, in three
+// 142 us; 128 rows of about 1100 keys of 4 KV heads in two pieces 119 us (with their
+// prefixes), in three 132 us.
 constexpr int64_t kTcLeast = 64;
 // Blocks of the tcgen05 kernel fill an SM each and write 256 rows of partial
 // results, so its keys are cut only as far as that gives idle SMs work.
@@ -335,13 +338,14 @@ int tc_pieces(int64_t blocks, int64_t keys) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / (2 * kTcKeys)));
   return (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
 }
-constexpr int64_t kBlockKeys = 128, kJoinKeys = 256, kLeastKeys = 128;
-int pieces(int64_t blocks, int64_t keys, int64_t slots) {
+constexpr int64_t kBlockKeys = 256, kJoinKeys = 256, kPieceKeys = 24, kLeastKeys = 128;
+int pieces(int64_t blocks, int64_t keys, int resident, bool joined) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / kLeastKeys));
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= most; s++) {
-    const int64_t rounds = (blocks * s + slots - 1) / slots;
-    const int64_t cost = rounds * ((keys + s - 1) / s + kBlockKeys) + (s > 1 ? kJoinKeys : 0);
+    const int64_t n = (blocks * s + kPagedSMs - 1) / kPagedSMs, k = (keys + s - 1) / s;
+    const int64_t time = std::max(k, n * k / 2) + kBlockKeys * ((n + resident - 1) / resident);
+    const int64_t cost = time + (s > 1 ? (joined ? 0 : kJoinKeys) + kPieceKeys * s : 0);
     if (cost < least) {
       least = cost;
       best = s;
@@ -368,7 +372,8 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
     return tc && n > kTcLeast ? kTcRows : kMmaRows;
   };
   auto pieces_for = [&](int rows, int64_t blocks, int64_t keys) {
-    return rows == kTcRows ? tc_pieces(blocks, keys) : pieces(blocks, keys, 2 * kPagedSMs);
+    return rows == kTcRows ? tc_pieces(blocks, keys)
+                           : pieces(blocks, keys, mma_blocks((int)kv.head_dim), g != nullptr);
   };
   a.rows = rows_for(pairs);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);

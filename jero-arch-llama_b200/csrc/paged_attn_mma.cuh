@@ -7,7 +7,7 @@
 // ring of shared memory stages, has its own running maximum, sum and output,
 // and never waits for another warp; the four results are joined at the end.
 // Few rows against many keys is bound by reading the cache, so what counts is
-// bytes in flight: kMmaStages stages x 4 warps x 2 blocks on an SM.
+// bytes in flight: the stages of 4 warps x 3 blocks on an SM, 192 KB.
 //
 // f32 rows are not rounded to the cache's type: q is split into the sum of NS
 // 16-bit parts (two f16 parts of q scaled by a power of two per row, 22 bits;
@@ -75,9 +75,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[NS]) {
   }
 }
 
+// Blocks on an SM.  Three, with two stages a warp, read a 131071-key row in 94 us
+// where two with three stages took 99 us: one block's start and end go on beside
+// the others' copies.  (The registers of head dim 256 allow two.)
+constexpr int mma_blocks(int hd) { return hd > 128 ? 2 : 3; }
+
 template <int NS, int HD>
 struct MmaShape {
-  static constexpr int stages = HD == 256 ? 2 : HD == 128 ? 3 : 4;
+  static constexpr int blocks = mma_blocks(HD);
+  static constexpr int stages = HD == 64 ? 4 : 2;
   static constexpr int chunks = HD / 8;              // 16-byte pieces of a row
   static constexpr int half = kMmaKeys * HD * 2;     // bytes of a stage's K (or V)
   static constexpr int ring = kMmaWarps * stages * 2 * half;
@@ -87,7 +93,7 @@ struct MmaShape {
 };
 
 template <class T, int NS, int HD>
-__global__ void __launch_bounds__(kMmaThreads, 2) k_paged_attn_mma(const __grid_constant__ AttnParams p, const int part, const bool direct) {
+__global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged_attn_mma(const __grid_constant__ AttnParams p, const int part, const bool direct) {
   using S = MmaShape<NS, HD>;
   extern __shared__ __align__(128) char smem_raw[];
   __shared__ RowMask masks[kMmaRows];
