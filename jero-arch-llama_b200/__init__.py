@@ -259,12 +259,12 @@ def _check(rc: int) -> None:
 
 def _ptr(x) -> int | None:
     """Device pointer of a torch tensor, an int, or None."""
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or type(x) is int:
         return x
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
+    if isinstance(x, int):
+        return x
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take a pointer of {type(x)}")
@@ -419,7 +419,7 @@ class PagedKv:
         self._keep = (k, v, page_table)
         self.fields = PagedKvFields(_ptr(k), _ptr(v), _ptr(page_table), n_pages, page_size, n_heads_kv, head_dim,
                                     n_seqs, max_pages, *(strides or (0, 0, 0)), dtype)
-        self._as_parameter_ = C.addressof(self.fields)
+        self.ptr = C.addressof(self.fields)
 
 
 class RaggedBatch:
@@ -429,7 +429,7 @@ class RaggedBatch:
     def __init__(self, q_start, kv_len, n_seqs: int, n_rows: int, max_q_len: int, max_kv_len: int):
         self._keep = (q_start, kv_len)
         self.fields = RaggedBatchFields(_ptr(q_start), _ptr(kv_len), n_seqs, n_rows, max_q_len, max_kv_len)
-        self._as_parameter_ = C.addressof(self.fields)
+        self.ptr = C.addressof(self.fields)
 
 
 class PrefixGroups:
@@ -439,14 +439,14 @@ class PrefixGroups:
     def __init__(self, group_start, prefix_len, n_groups: int, max_group: int, max_prefix_len: int):
         self._keep = (group_start, prefix_len)
         self.fields = PrefixGroupsFields(_ptr(group_start), _ptr(prefix_len), n_groups, max_group, max_prefix_len)
-        self._as_parameter_ = C.addressof(self.fields)
+        self.ptr = C.addressof(self.fields)
 
 
 def rope_kv_append(kv: PagedKv, batch: RaggedBatch, k, v, inv_freq, dtype: int, rotary_dim: int, neox: bool = False,
                    kv_stride: int = 0, q=None, q_out=None, n_heads_q: int = 0, q_stride: int = 0,
                    q_out_stride: int = 0, stream=None) -> None:
     """Rotates the batch's k (and q) rows and appends k and v to the cache."""
-    _check(lib().jal_op_rope_kv_append(kv, batch, dtype, _ptr(k), _ptr(v), kv_stride, _ptr(inv_freq), rotary_dim,
+    _check(lib().jal_op_rope_kv_append(kv.ptr, batch.ptr, dtype, _ptr(k), _ptr(v), kv_stride, _ptr(inv_freq), rotary_dim,
                                        1 if neox else 0, _ptr(q), _ptr(q_out), n_heads_q, q_stride, q_out_stride,
                                        _stream(stream)))
 
@@ -456,7 +456,7 @@ def paged_attention(kv: PagedKv, batch: RaggedBatch, q, out, n_heads_q: int, sca
                     workspace_len: int = 0, stream=None) -> None:
     """Causal attention of the batch's rows over the cache; with a window, the
     first n_sink positions stay visible."""
-    _check(lib().jal_op_paged_attention(kv, batch, dtype, _ptr(q), n_heads_q, q_stride, scale, sliding_window, n_sink,
+    _check(lib().jal_op_paged_attention(kv.ptr, batch.ptr, dtype, _ptr(q), n_heads_q, q_stride, scale, sliding_window, n_sink,
                                         _ptr(out), out_stride, _ptr(workspace), workspace_len, _stream(stream)))
 
 
@@ -464,7 +464,7 @@ def paged_attention_workspace(kv: PagedKv, batch: RaggedBatch, n_heads_q: int, d
                               n_sink: int = 0) -> int:
     """Workspace bytes of the same paged_attention call."""
     n = _SZ()
-    _check(lib().jal_op_paged_attention_workspace(kv, batch, dtype, n_heads_q, sliding_window, n_sink, C.byref(n)))
+    _check(lib().jal_op_paged_attention_workspace(kv.ptr, batch.ptr, dtype, n_heads_q, sliding_window, n_sink, C.byref(n)))
     return n.value
 
 
@@ -473,7 +473,7 @@ def shared_prefix_attention(kv: PagedKv, batch: RaggedBatch, groups: PrefixGroup
                             workspace_len: int = 0, stream=None) -> None:
     """paged_attention of sequences that share prefixes, each prefix read once
     for its group."""
-    _check(lib().jal_op_shared_prefix_attention(kv, batch, groups, dtype, _ptr(q), n_heads_q, q_stride, scale,
+    _check(lib().jal_op_shared_prefix_attention(kv.ptr, batch.ptr, groups.ptr, dtype, _ptr(q), n_heads_q, q_stride, scale,
                                                 _ptr(out), out_stride, _ptr(workspace), workspace_len,
                                                 _stream(stream)))
 
@@ -482,7 +482,7 @@ def shared_prefix_attention_workspace(kv: PagedKv, batch: RaggedBatch, groups: P
                                       dtype: int) -> int:
     """Workspace bytes of the same shared_prefix_attention call."""
     n = _SZ()
-    _check(lib().jal_op_shared_prefix_attention_workspace(kv, batch, groups, dtype, n_heads_q, C.byref(n)))
+    _check(lib().jal_op_shared_prefix_attention_workspace(kv.ptr, batch.ptr, groups.ptr, dtype, n_heads_q, C.byref(n)))
     return n.value
 
 
@@ -506,7 +506,7 @@ def beam_reorder(kv: PagedKv, kv_len, parents, fresh_pages, new_table, new_len, 
                  n_layers: int = 1, layer_stride: int = 0, stream=None) -> None:
     """The beams' page tables and lengths in the order of their parents, with
     the unfinished pages of further children copied in every layer."""
-    _check(lib().jal_op_beam_reorder(kv, n_layers, layer_stride, _ptr(kv_len), _ptr(parents), _ptr(fresh_pages),
+    _check(lib().jal_op_beam_reorder(kv.ptr, n_layers, layer_stride, _ptr(kv_len), _ptr(parents), _ptr(fresh_pages),
                                      n_seqs, n_beams, _ptr(new_table), _ptr(new_len), _stream(stream)))
 
 

@@ -139,14 +139,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
     }
     copies_done();
   };
-  Slot next = locate(warp);
-#pragma unroll
-  for (int i = 0; i < S::stages - 1; i++) {
-    const Slot at = next;
-    next = locate(warp + (i + 1) * kMmaWarps);
-    copy(at, i);
-  }
-
+  Slot next;
   // Query rows into shared memory, in their NS parts, in the swizzle of the
   // key rows.  f16 parts: the row times 2^e, so that the largest element lies
   // in [2^13, 2^14) and the second part keeps its bits.
@@ -157,17 +150,30 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
     const int64_t qo = real ? q_offset(p, t, j) : 0;
     float v[2 * N], factor = 1.0f;
     float top = 0.0f;
+    uint32_t raw[NS == 1 ? N : 1];  // (asked for before the copies, looked at behind them)
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int d = (tid % 8) * 2 + i * 16;
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        v[2 * i + e] = real && d < hd ? load_as_f32(p.q, qo + d + e, p.act) : 0.0f;
-        const float a = fabsf(v[2 * i + e]);
-        if (a < INFINITY) top = fmaxf(top, a);
+      if constexpr (NS == 1) {
+        raw[i] = real && d < hd ? *(const uint32_t *)((const T *)p.q + qo + d) : 0u;
+      } else {
+        const float2 f = real && d < hd ? *(const float2 *)((const float *)p.q + qo + d) : make_float2(0.0f, 0.0f);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
       }
     }
+    next = locate(warp);
+#pragma unroll
+    for (int i = 0; i < S::stages - 1; i++) {
+      const Slot at = next;
+      next = locate(warp + (i + 1) * kMmaWarps);
+      copy(at, i);
+    }
+
     if (NS == 2) {
+#pragma unroll
+      for (int i = 0; i < 2 * N; i++)
+        if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const int e = top > 0.0f ? 13 - ilogbf(top) : 0;
@@ -184,7 +190,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
 #pragma unroll
     for (int i = 0; i < N; i++) {
       uint32_t part[NS];
-      split2<T, NS>(v[2 * i], v[2 * i + 1], part);
+      if constexpr (NS == 1) part[0] = raw[i];
+      else split2<T, NS>(v[2 * i], v[2 * i + 1], part);
       const int ch = 2 * i + (tid % 8) / 4;
 #pragma unroll
       for (int s = 0; s < NS; s++)
@@ -200,14 +207,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
   const RowSpan m0 = r0 < t.rows ? row_span(p, t, masks[r0]) : every;
   const RowSpan m1 = r0 + 8 < t.rows ? row_span(p, t, masks[r0 + 8]) : every;
   const float f0 = q_scale[r0], f1 = q_scale[r0 + 8];
-  int lim_lo = 0x7fffffff, lim_hi = 0, wlo_lo = 0x7fffffff, wlo_hi = 0;
-  for (int j = 0; j < t.rows; j++) {
-    lim_lo = min(lim_lo, masks[j].lim);
-    lim_hi = max(lim_hi, masks[j].lim);
-    wlo_lo = min(wlo_lo, masks[j].wlo);
-    wlo_hi = max(wlo_hi, masks[j].wlo);
-  }
-  const bool mixed = lim_lo != lim_hi || wlo_lo != wlo_hi;
+  const RowMask mine = masks[lane < t.rows ? lane : 0];  // (a tile has a row)
+  const bool mixed = __any_sync(0xffffffffu, mine.lim != masks[0].lim || mine.wlo != masks[0].wlo);
   float o[HD / 8][4];
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
