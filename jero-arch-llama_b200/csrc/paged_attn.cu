@@ -14,41 +14,68 @@ namespace {
 using namespace paged;
 
 // ---- the f32 kernel ---------------------------------------------------------
-// One pass over the tile's keys with the running maximum and sum of each row:
-// K and V tiles of KT keys widened to f32 in shared memory, scores and output
-// on the CUDA cores in f32, 128 threads as 8 row groups x 16 key (or dim)
-// groups.
+// f32 caches: one pass over the tile's keys with the running maximum and sum of
+// each row, everything in f32 on the CUDA cores.  K and V tiles of kF32Keys keys
+// go round two stages of shared memory, each warp copying its quarter of a tile's
+// rows with cp.async one tile ahead; 128 threads work on them as 8 row groups x 16
+// key (or dim) groups.  Few rows are bound by the shared memory reads, 11 of 16
+// bytes a product of four, not by the cache: XX.
 constexpr int kF32Threads = 128;
 constexpr int kF32Keys = 32;
 
 template <int HD, int RT>
 struct F32Smem {
   float q[RT][HD + 4];
-  float k[kF32Keys][HD + 4];
-  float v[kF32Keys][HD];
+  float k[2][kF32Keys][HD + 4];
+  float v[2][kF32Keys][HD];
   float s[RT][kF32Keys + 4];
-  RowMask mask[RT];
-  float corr[RT];
-  int poison;
+  RowSpan span[RT];
+  uint32_t present[2][kF32Threads / 32];
 };
 
-template <class TK, int HD, int RT>
-__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_constant__ AttnParams p, const int part, const bool direct) {
+template <int HD, int RT>
+__global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_constant__ AttnParams p, const int part,
+                                                                const bool direct) {
   extern __shared__ __align__(16) char smem_raw[];
   auto &sm = *(F32Smem<HD, RT> *)smem_raw;
   pdl_trigger();
   Tile t;
   if (!block_tile(p, part, RT, kF32Keys, t)) return;
-  constexpr int R = RT / 8, KC = kF32Keys / 16, DC = HD / 16;
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  constexpr int R = RT / 8, KC = kF32Keys / 16, DC = HD / 16, kMine = kF32Keys / 4;
+  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, warp = tid / 32, lane = tid % 32;
   const int hd = p.kv.hd;
-  for (int i = tid; i < RT * HD; i += kF32Threads) {
-    const int j = i / HD, d = i % HD;
-    sm.q[j][d] = j < t.rows && d < hd ? load_as_f32(p.q, q_offset(p, t, j) + d, p.act) * p.scale_log2 : 0.0f;
+  // This warp's rows of the tile at u: looked up by its first lanes one tile ahead.
+  auto locate = [&](int u) -> Slot {
+    const int k = u + warp * kMine + lane;
+    return lane < kMine && k < t.u1 ? slot_of(p.kv, t.table, t.key(k)) : Slot{-1, 0};
+  };
+  auto copy = [&](const Slot &where, int stage) {
+    const int64_t at = slot_offset(p.kv, where, t.head);
+    const uint32_t bits = __ballot_sync(0xffffffffu, at >= 0);
+    if (lane == 0) sm.present[stage][warp] = bits & ((1u << kMine) - 1);
+#pragma unroll
+    for (int i = 0; i < kMine * (HD / 4) / 32; i++) {
+      const int r = (i * 32 + lane) / (HD / 4), d = (i * 32 + lane) % (HD / 4) * 4;
+      const int64_t o = __shfl_sync(0xffffffffu, at, r);
+      const bool there = o >= 0 && d < hd;
+      const int64_t e = there ? o + d : 0;
+      copy16(smem_u32(&sm.k[stage][warp * kMine + r][d]), (const float *)p.kv.k + e, there);
+      copy16(smem_u32(&sm.v[stage][warp * kMine + r][d]), (const float *)p.kv.v + e, there);
+    }
+    copies_done();
+  };
+  Slot next = locate(t.u0);
+  copy(next, 0);
+  next = locate(t.u0 + kF32Keys);
+  for (int i = tid; i < RT * (HD / 4); i += kF32Threads) {
+    const int j = i / (HD / 4), d = i % (HD / 4) * 4;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (j < t.rows && d < hd) x = *(const float4 *)((const float *)p.q + q_offset(p, t, j) + d);
+    *(float4 *)&sm.q[j][d] =
+        make_float4(x.x * p.scale_log2, x.y * p.scale_log2, x.z * p.scale_log2, x.w * p.scale_log2);
   }
-  for (int j = tid; j < RT; j += kF32Threads)
-    sm.mask[j] = j < t.rows ? row_mask(p, t, j) : RowMask{0, 0};
-  if (tid == 0) sm.poison = 0;
+  for (int j = tid; j < RT; j += kF32Threads)  // (rows that do not exist see everything)
+    sm.span[j] = j < t.rows ? row_span(p, t, row_mask(p, t, j)) : RowSpan{0x7fffffff, 0, 0};
   float o[R][DC], m[R], l[R];
 #pragma unroll
   for (int i = 0; i < R; i++) {
@@ -57,37 +84,33 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
 #pragma unroll
     for (int c = 0; c < DC; c++) o[i][c] = 0.0f;
   }
-  bool bad = false;
-  for (int u = t.u0; u < t.u1; u += kF32Keys) {
-    __syncthreads();
-    const int n = min(kF32Keys, t.u1 - u);
-    for (int i = tid; i < kF32Keys * (HD / 8); i += kF32Threads) {
-      const int r = i / (HD / 8), d = (i % (HD / 8)) * 8;
-      float a[8] = {}, b[8] = {};
-      if (r < n && d < hd) {
-        const int64_t at = slot_offset(p.kv, t.table, t.head, t.key(u + r));
-        if (at >= 0) {
-          load8((const TK *)p.kv.k + at + d, a);
-          load8((const TK *)p.kv.v + at + d, b);
-        }
-      }
+  float bad = 0.0f;
+  int stage = 0;
+  for (int u = t.u0; u < t.u1; u += kF32Keys, stage ^= 1) {
+    copies_wait<0>();
+    __syncthreads();  // the tile is there, and the other stage has been read
+    const Slot at = next;
+    next = locate(u + 2 * kF32Keys);
+    copy(at, stage ^ 1);
+    uint32_t bits = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) bad |= !isfinite(b[e]);
-      store8(&sm.k[r][d], a);
-      store8(&sm.v[r][d], b);
-    }
-    __syncthreads();
+    for (int w = 0; w < kF32Threads / 32; w++) bits |= sm.present[stage][w] << (w * kMine);
+    bool whole = bits == 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < R; i++) whole = whole && sm.span[ty + 8 * i].all(u, kF32Keys);
+    const bool masked = __any_sync(0xffffffffu, !whole);
     float s[R][KC];
 #pragma unroll
     for (int i = 0; i < R; i++)
 #pragma unroll
       for (int c = 0; c < KC; c++) s[i][c] = 0.0f;
+#pragma unroll 8
     for (int d = 0; d < HD; d += 4) {
       float4 a[R], b[KC];
 #pragma unroll
       for (int i = 0; i < R; i++) a[i] = *(const float4 *)&sm.q[ty + 8 * i][d];
 #pragma unroll
-      for (int c = 0; c < KC; c++) b[c] = *(const float4 *)&sm.k[tx + 16 * c][d];
+      for (int c = 0; c < KC; c++) b[c] = *(const float4 *)&sm.k[stage][tx + 16 * c][d];
 #pragma unroll
       for (int i = 0; i < R; i++)
 #pragma unroll
@@ -98,22 +121,13 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
           s[i][c] = fmaf(a[i].w, b[c].w, s[i][c]);
         }
     }
-    // An unmapped page's keys are masked for every row.
-    bool there[KC];
-    int key[KC];
-#pragma unroll
-    for (int c = 0; c < KC; c++) {
-      const int r = tx + 16 * c;
-      key[c] = r < n ? t.key(u + r) : 0;
-      there[c] = r < n && slot_offset(p.kv, t.table, t.head, key[c]) >= 0;
-    }
 #pragma unroll
     for (int i = 0; i < R; i++) {
-      const RowMask mk = sm.mask[ty + 8 * i];
+      const uint32_t see = masked ? bits & sm.span[ty + 8 * i].bits(u) : 0xffffffffu;
       float top = m[i];
 #pragma unroll
       for (int c = 0; c < KC; c++) {
-        if (!there[c] || !mk.sees(key[c], p.n_sink)) s[i][c] = -INFINITY;
+        if (!((see >> (tx + 16 * c)) & 1)) s[i][c] = -INFINITY;
         top = fmaxf(top, s[i][c]);
       }
 #pragma unroll
@@ -132,7 +146,13 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
 #pragma unroll
       for (int c = 0; c < DC; c++) o[i][c] *= corr;
     }
+    if (masked) {  // values that some rows must not meet: x * 0 is NaN where x is not finite
+      for (int r = 0; r < kF32Keys; r++)
+#pragma unroll
+        for (int c = 0; c < DC; c++) bad = fmaf(sm.v[stage][r][tx + 16 * c], 0.0f, bad);
+    }
     __syncwarp();  // a row group's weights are written and read by one warp
+#pragma unroll 4
     for (int r = 0; r < kF32Keys; r += 4) {
       float4 w[R];
 #pragma unroll
@@ -141,7 +161,7 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
       for (int e = 0; e < 4; e++) {
         float v[DC];
 #pragma unroll
-        for (int c = 0; c < DC; c += 4) *(float4 *)&v[c] = *(const float4 *)&sm.v[r + e][tx * 4 + (c / 4) * 64];
+        for (int c = 0; c < DC; c += 4) *(float4 *)&v[c] = *(const float4 *)&sm.v[stage][r + e][tx * 4 + (c / 4) * 64];
 #pragma unroll
         for (int i = 0; i < R; i++) {
           const float we = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
@@ -150,9 +170,11 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
         }
       }
     }
+    __syncwarp();
   }
-  if (__syncthreads_or(bad)) {
-    for (int j = tid / 32; j < t.rows; j += kF32Threads / 32) attend_row_alone(p, t, j, direct);
+  copies_wait<0>();
+  if (__syncthreads_or(bad != bad)) {
+    for (int j = warp; j < t.rows; j += kF32Threads / 32) attend_row_alone(p, t, j, direct);
     return;
   }
 #pragma unroll
@@ -162,16 +184,14 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
     for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
     if (j >= t.rows) continue;
     const int64_t oo = out_offset(p, t, j), pi = part_index(p, t, j);
-    const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    const float inv = !direct ? 1.0f : l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    float *const dst = direct ? (float *)p.out + oo : p.part_o + pi * hd;
     if (!direct && tx == 0) p.part_ml[pi] = make_float2(m[i], l[i]);
 #pragma unroll
-    for (int c = 0; c < DC; c++) {
-      const int d = tx * 4 + (c / 4) * 64 + c % 4;
-      if (d >= hd) continue;
-      if (direct)
-        store_from_f32(p.out, oo + d, p.act, o[i][c] * inv);
-      else
-        p.part_o[pi * hd + d] = o[i][c];
+    for (int c = 0; c < DC; c += 4) {
+      const int d = tx * 4 + (c / 4) * 64;
+      if (d < hd)
+        *(float4 *)(dst + d) = make_float4(o[i][c] * inv, o[i][c + 1] * inv, o[i][c + 2] * inv, o[i][c + 3] * inv);
     }
   }
 }
@@ -292,12 +312,12 @@ bool run_kernel(F kernel, const AttnParams &p, int part, bool direct, int thread
   return true;
 }
 
-template <class TK, int HD>
+template <int HD>
 void run_f32(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
   if (plan.rows == 8)
-    run_kernel(k_paged_attn_f32<TK, HD, 8>, p, kBoth, plan.direct, kF32Threads, (int)sizeof(F32Smem<HD, 8>), s);
+    run_kernel(k_paged_attn_f32<HD, 8>, p, kBoth, plan.direct, kF32Threads, (int)sizeof(F32Smem<HD, 8>), s);
   else
-    run_kernel(k_paged_attn_f32<TK, HD, 32>, p, kBoth, plan.direct, kF32Threads, (int)sizeof(F32Smem<HD, 32>), s);
+    run_kernel(k_paged_attn_f32<HD, 32>, p, kBoth, plan.direct, kF32Threads, (int)sizeof(F32Smem<HD, 32>), s);
 }
 template <class T, int NS, int HD>
 void run_16bit(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
@@ -394,9 +414,9 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
 
 void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) {
   if (p.kv.dtype == JAL_F32) {
-    if (p.kv.hd <= 64) run_f32<float, 64>(p, plan, s);
-    else if (p.kv.hd <= 128) run_f32<float, 128>(p, plan, s);
-    else run_f32<float, 256>(p, plan, s);
+    if (p.kv.hd <= 64) run_f32<64>(p, plan, s);
+    else if (p.kv.hd <= 128) run_f32<128>(p, plan, s);
+    else run_f32<256>(p, plan, s);
   } else if (p.act == JAL_F16) {
     run_16bit_hd<__half, 1>(p, plan, s);
   } else if (p.act == JAL_BF16) {
