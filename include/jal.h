@@ -219,7 +219,9 @@ typedef struct jal_paged_kv {
  * q_start[s + 1]) (ascending), the last of them at position kv_len[s] - 1 and
  * the others at the positions before.  A sequence may have no row.  Rows
  * before q_start[0] and from q_start[n_seqs] on belong to none and are left
- * as they were, as are a sequence's rows past the first max_q_len. */
+ * as they were, as are, in attention, a sequence's rows past the first
+ * max_q_len.  A row before position 0 is not appended and sees nothing; one
+ * past the table's last position is not appended and sees what that sees. */
 typedef struct jal_ragged_batch {
   const int32_t *q_start; /* [n_seqs + 1] */
   const int32_t *kv_len;  /* [n_seqs], the new rows included */
@@ -309,7 +311,8 @@ int jal_op_shared_prefix_attention_workspace(const jal_paged_kv *kv,
  * -inf; a beam whose cum is not finite or whose logits hold +inf or nothing
  * above -inf scores -inf throughout (finished and empty beams).  k <= 64,
  * k <= n_beams * vocab, n_beams <= 256, n_beams * k <= 8192, vocab <= 2^20
- * (JAL_ERR_CAPABILITY_MISMATCH).  Outputs [n_seqs][k]. */
+ * (JAL_ERR_CAPABILITY_MISMATCH).  Outputs [n_seqs][k]; with k = n_beams scores
+ * may be cum. */
 int jal_op_beam_select(const void *logits, int dtype, size_t row_stride,
                        const float *cum, size_t n_seqs, size_t n_beams,
                        size_t vocab, size_t k, float *scores, int32_t *parents,

@@ -62,6 +62,9 @@ jal_paged_kv checked_kv(const jal_paged_kv *in) {
   }
   if (kv.page_stride % 8 || kv.head_stride % 8 || kv.slot_stride % 8)
     fail(JAL_ERR_TENSOR_BOUNDS, "paged cache strides have to be multiples of 8");
+  if (kv.page_size > 1 && kv.slot_stride < kv.head_dim)
+    fail(JAL_ERR_TENSOR_BOUNDS, "slot stride %llu, head_dim %llu", (unsigned long long)kv.slot_stride,
+         (unsigned long long)kv.head_dim);
   const uint64_t most = 1ull << 40;
   if (kv.page_stride > most || kv.head_stride > most || kv.slot_stride > most)
     fail(JAL_ERR_TENSOR_BOUNDS, "paged cache stride above 2^40");
@@ -99,7 +102,7 @@ jal_ragged_batch checked_batch(const jal_ragged_batch *in, const jal_paged_kv &k
   if (b.n_seqs > kv.n_seqs)
     fail(JAL_ERR_TENSOR_BOUNDS, "batch of %llu sequences over a table of %llu", (unsigned long long)b.n_seqs,
          (unsigned long long)kv.n_seqs);
-  if (b.n_rows > kMaxInt) fail(JAL_ERR_TENSOR_BOUNDS, "batch of more than 2^31 rows");
+  if (b.n_rows > kMaxPositions) fail(JAL_ERR_TENSOR_BOUNDS, "batch of 2^31 rows or more");
   if (b.max_q_len > b.n_rows) b.max_q_len = b.n_rows;
   b.max_kv_len = std::min<uint64_t>(std::max<uint64_t>(b.max_kv_len, 1), kv.max_pages * kv.page_size);
   return b;
@@ -118,9 +121,11 @@ int64_t row_stride(size_t stride, size_t width, const char *what) {
   return (int64_t)stride;
 }
 
-void check_heads(size_t hq, const jal_paged_kv &kv) {
+void check_heads(size_t hq, const jal_paged_kv &kv, const jal_ragged_batch &b) {
   if (hq == 0 || hq % kv.n_heads_kv || hq > 65535)
     fail(JAL_ERR_CAPABILITY_MISMATCH, "%zu query heads over %llu KV heads", hq, (unsigned long long)kv.n_heads_kv);
+  if (b.n_rows * (hq / kv.n_heads_kv) > kMaxPositions)  // (row, head of the group) pairs are counted in 32 bits
+    fail(JAL_ERR_TENSOR_BOUNDS, "batch of 2^31 rows times heads of a group or more");
 }
 
 jal_prefix_groups checked_groups(const jal_prefix_groups *in, const jal_paged_kv &kv, const jal_ragged_batch &b) {
@@ -153,7 +158,7 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   jal_prefix_groups g = {};
   if (groups) g = checked_groups(groups, kv, b);
   check_act(dtype, kv);
-  check_heads(hq, kv);
+  check_heads(hq, kv, b);
   NEED(q);
   NEED(out);
   if (!std::isfinite(scale)) fail(JAL_ERR_INVALID_ARGUMENT, "attention scale is not finite");
@@ -164,6 +169,8 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   aligned16(q, "q");
   aligned16(out, "out");
   if (b.n_seqs == 0 || b.n_rows == 0 || b.max_q_len == 0) return;
+  window = std::min<size_t>(window, kMaxInt);
+  n_sink = std::min<size_t>(n_sink, kMaxInt);
   const AttnPlan plan = plan_attention(kv, b, g.n_groups ? &g : nullptr, hq, dtype, window, n_sink);
   check_grid(plan, kv, b, g.n_groups ? &g : nullptr, hq);
   if (plan.bytes) {
@@ -198,8 +205,8 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   p.hq = (int32_t)hq;
   p.G = (int32_t)(hq / kv.n_heads_kv);
   p.act = dtype;
-  p.window = (int32_t)std::min<uint64_t>(window, kMaxInt);
-  p.n_sink = (int32_t)std::min<uint64_t>(n_sink, kMaxInt);
+  p.window = (int32_t)window;
+  p.n_sink = (int32_t)n_sink;
   p.splits = plan.splits;
   p.prefix_splits = plan.prefix_splits;
   p.tiles = plan.tiles;
@@ -303,9 +310,11 @@ static size_t attention_bytes(const jal_paged_kv *kv_in, const jal_ragged_batch 
   jal_prefix_groups g = {};
   if (groups) g = checked_groups(groups, kv, b);
   check_act(dtype, kv);
-  check_heads(hq, kv);
+  check_heads(hq, kv, b);
   if (b.n_seqs == 0 || b.n_rows == 0 || b.max_q_len == 0) return 0;
-  return plan_attention(kv, b, g.n_groups ? &g : nullptr, hq, dtype, window, n_sink).bytes;
+  return plan_attention(kv, b, g.n_groups ? &g : nullptr, hq, dtype, std::min<size_t>(window, kMaxInt),
+                        std::min<size_t>(n_sink, kMaxInt))
+      .bytes;
 }
 
 int jal_op_paged_attention_workspace(const jal_paged_kv *kv, const jal_ragged_batch *batch, int dtype,

@@ -31,7 +31,7 @@ def _batch(jal, **kw):
     (dict(dtype=2), "CAPABILITY"), (dict(head_dim=0), "CAPABILITY"), (dict(head_dim=20), "CAPABILITY"),
     (dict(head_dim=264), "CAPABILITY"), (dict(n_heads_kv=0), "BOUNDS"), (dict(page_size=0), "BOUNDS"),
     (dict(n_pages=0), "BOUNDS"), (dict(max_pages=0), "BOUNDS"), (dict(max_pages=1 << 28), "BOUNDS"),
-    (dict(strides=(2048, 1024, 65)), "BOUNDS"), (dict(k=4100), "BOUNDS"), (dict(n_seqs=2), "BOUNDS"),
+    (dict(strides=(2048, 1024, 65)), "BOUNDS"), (dict(strides=(2048, 1024, 56)), "BOUNDS"), (dict(k=4100), "BOUNDS"), (dict(n_seqs=2), "BOUNDS"),
     (dict(n_heads_kv=3), "CAPABILITY"), (dict(dtype=30), "CAPABILITY"),
 ])
 def test_views_are_refused(jal, kv, code):
@@ -80,6 +80,10 @@ def test_attention_arguments_are_refused(jal):
         with pytest.raises(jal.K3Error) as e:
             jal.paged_attention(long, big, **ok, workspace=ws, workspace_len=n)
         assert e.value.code == err
+    for rows in (1 << 31, 1 << 30):  # rows; rows times the two heads of a group
+        with pytest.raises(jal.K3Error) as e:
+            jal.paged_attention(kv, _batch(jal, n_rows=rows), **ok)
+        assert e.value.code == jal.ERR_TENSOR_BOUNDS
     with pytest.raises(jal.K3Error) as e:
         jal.shared_prefix_attention(kv, b, jal.PrefixGroups(None, 4096, 1, 3, 10), **ok)
     assert e.value.code == jal.ERR_INVALID_ARGUMENT
@@ -223,6 +227,34 @@ def test_append_far_positions_and_missing_pages(jal, torch_cuda):
     assert (q_out[2] == 7).all()  # a row before position 0
 
 
+@pytest.mark.gpu
+def test_append_many_sequences(jal, torch_cuda):
+    """Rows find their sequences among a thousand of 0 to 3 rows, with rows before the first and behind the last."""
+    n, hd, page = 1000, 16, 4
+    g = torch.Generator().manual_seed(6)
+    news = torch.randint(0, 4, (n,), generator=g).tolist()
+    starts = [5]
+    for x in news:
+        starts.append(starts[-1] + x)
+    rows = starts[-1] + 7
+    lens = [x + int(e) for x, e in zip(news, torch.randint(0, 5, (n,), generator=g))]
+    table = torch.randperm(2 * n, generator=g).to(torch.int32).view(n, 2)
+    pools = [torch.zeros(2 * n, 1, page, hd, device=DEV) for _ in range(2)]
+    kv = jal.PagedKv(pools[0], pools[1], table.to(DEV), dtype=jal.F32, n_pages=2 * n, page_size=page, n_heads_kv=1,
+                     head_dim=hd, n_seqs=n, max_pages=2)
+    x = torch.randn(rows, hd, generator=g)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    batch = jal.RaggedBatch(ints(starts), ints(lens), n, rows, 3, 8)
+    jal.rope_kv_append(kv, batch, x.to(DEV), x.to(DEV), None, dtype=jal.F32, rotary_dim=0)
+    want = torch.zeros(2 * n, 1, page, hd)
+    for s in range(n):
+        for i in range(news[s]):
+            pos = lens[s] - news[s] + i
+            if pos < 8:
+                want[int(table[s, pos // page]), 0, pos % page] = x[starts[s] + i]
+    assert torch.equal(pools[0].cpu(), want) and torch.equal(pools[1].cpu(), want)
+
+
 # ---- attention ------------------------------------------------------------------
 def attend(jal, c, scale, window=0, sinks=0, stream=None, out=None):
     ws = jal.paged_attention_workspace(c.kv, c.batch, c.hq, dtype=c.act_type, sliding_window=window, n_sink=sinks)
@@ -282,6 +314,82 @@ def test_attention_long(jal, torch_cuda, length, new, window, sinks, act, cache)
     """Keys cut into many pieces; a second, short sequence leaves most of its pieces empty."""
     c = Case([length, 40], [new, min(new, 40)], 8, 2, 64, act, cache, 64, seed=length).to_device(jal)
     check(c, attend(jal, c, 0.125, window, sinks), 0.125, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 2), (3, 1)])
+@pytest.mark.parametrize("pairs", [16, 17, 64, 65, 127, 128, 129, 255, 256, 257])
+def test_attention_row_tiles(jal, torch_cuda, act, cache, hq, hkv, pairs):
+    """Row counts around the sizes of the row tiles, at lengths around those of the key tiles."""
+    new = -(-pairs // (hq // hkv))
+    c = Case([new + 129, max(new, 128), new], [new, new, max(new - 1, 0)], hq, hkv, 64, act, cache, 32, seed=pairs)
+    c.to_device(jal)
+    check(c, attend(jal, c, 0.125, 0, 0), 0.125, 0, 0)
+    check(c, attend(jal, c, 0.125, 90, 3), 0.125, 90, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_table_ends(jal, torch_cuda, act, cache, new):
+    """A sequence that fills its table to the last slot, and rows past it that see what the last position sees."""
+    c = Case([96, 96], [new, new], 4, 2, 64, act, cache, 16, seed=new).to_device(jal)
+    assert c.width * c.page == 96
+    check(c, attend(jal, c, 0.125), 0.125)
+    full = c.reference(0.125)
+    c.d_kv_len.copy_(torch.tensor([96, 96 + new], dtype=torch.int32))  # the second's rows are all past the table
+    out = attend(jal, c, 0.125)
+    got = out[:2 * new, :256].view(2 * new, 4, 64).double()
+    assert ((got - full[0][:2 * new]).abs() <= c.bound(full)[:2 * new])[:new].all()
+    late = Case([96], [1], 4, 2, 64, act, cache, 16, seed=new)
+    late.k, late.v, late.table, late.n_pages = c.k[1:], c.v[1:], c.table[1:], c.n_pages
+    for r in range(new, 2 * new):
+        late.q = c.q[r:r + 1].repeat(late.n_rows, 1, 1)
+        ref = late.reference(0.125)
+        assert ((got[r] - ref[0][0]).abs() <= late.bound(ref)[0]).all()
+
+
+@pytest.mark.gpu
+def test_attention_two_calls_at_once(jal, torch_cuda):
+    """Calls on two streams, each with its own workspace."""
+    cases = [Case([3000 + 10 * i, 50], [1, 1], 8, 2, 64, "f16", "f16", 64, seed=i).to_device(jal) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    bufs = []
+    for c, st in zip(cases, streams):
+        need = jal.paged_attention_workspace(c.kv, c.batch, 8, dtype=c.act_type)
+        assert need
+        bufs.append((torch.full((need,), 255, dtype=torch.uint8, device=DEV), need,
+                     torch.full((c.n_rows, c.hq * c.hd + 8), 7.0, dtype=c.act, device=DEV)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, st, (ws, need, out) in zip(cases, streams, bufs):
+            jal.paged_attention(c.kv, c.batch, c.d_q, out, 8, 0.125, dtype=c.act_type, out_stride=520, workspace=ws,
+                                workspace_len=need, stream=st)
+    torch.cuda.synchronize()
+    for c, (_, _, out) in zip(cases, bufs):
+        check(c, out.cpu(), 0.125)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_attention_in_place_behind_other_rows(jal, torch_cuda, new):
+    """out = q, and a batch whose first sequence starts behind rows that belong to none."""
+    for act, cache in TYPES:
+        c = Case([300, 140], [new, new], 8, 2, 64, act, cache, 16, seed=new)
+        ref, lim = c.reference(0.125), None
+        lim = c.bound(ref)
+        c.q_start += 3
+        c.q_full = torch.cat([torch.full((3, c.q_stride), 7.0, dtype=c.act), c.q_full])
+        c.n_rows += 3
+        c.to_device(jal)
+        need = jal.paged_attention_workspace(c.kv, c.batch, 8, dtype=c.act_type)
+        ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device=DEV)
+        jal.paged_attention(c.kv, c.batch, c.d_q, c.d_q, 8, 0.125, dtype=c.act_type, workspace=ws, workspace_len=need)
+        got = c.d_q.cpu()
+        n = 2 * new
+        assert (got[:3] == 7).all() and torch.equal(got[3 + n:], c.q_full[3 + n:])
+        assert ((got[3:3 + n].view(n, 8, 64).double() - ref[0][:n]).abs() <= lim[:n]).all()
 
 
 @pytest.mark.gpu
@@ -438,6 +546,7 @@ PREFIXES = [
     ([900, 860, 850], [1, 0, 2], [0, 3], [800], 6, 6, 96, 32),
     ([30, 12, 20], [1, 1, 1], [1, 3], [10], 20, 1, 256, 16),
     ([700 + i for i in range(40)], [1] * 40, [0, 17, 40], [640, 699], 32, 8, 128, 64),
+    ([2600 + i for i in range(9)], [2] * 9, [0, 9], [2590], 12, 2, 64, 64),  # 108 rows, 21 key tiles
 ]
 
 
@@ -530,6 +639,22 @@ def test_beam_select_ties_and_dead_beams(jal, torch_cuda):
     check_beams(select(jal, none, cum, 1, 2, 5), none, cum, 1, 2, 5)
     signs = torch.tensor([[0.0, -0.0, 0.0, -1.0]])  # the zeros are equal
     check_beams(select(jal, signs, torch.zeros(1, 1), 1, 1, 4), signs, torch.zeros(1, 1), 1, 1, 4)
+
+
+@pytest.mark.gpu
+def test_beam_select_over_its_own_scores(jal, torch_cuda):
+    """Long rows, where a block reads several pieces, with scores written over cum."""
+    n, beams, vocab = 60, 16, 20011
+    logits = torch.randn(n * beams, vocab, generator=torch.Generator().manual_seed(8)) * 2
+    logits[5] = torch.arange(vocab).float() / 5000  # ascending: each piece has better ones than all before
+    logits[6] = 0.0
+    cum = torch.randn(n, beams, generator=torch.Generator().manual_seed(9)) - 10
+    need = jal.beam_select_workspace(n, beams, vocab, beams)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+    dev, d_cum = logits.to(DEV), cum.to(DEV)
+    parents, tokens = (torch.zeros(n, beams, dtype=torch.int32, device=DEV) for _ in range(2))
+    jal.beam_select(dev, d_cum, d_cum, parents, tokens, n, beams, vocab, beams, workspace=ws, workspace_len=need)
+    check_beams([d_cum.cpu(), parents.cpu(), tokens.cpu()], logits, cum, n, beams, beams)
 
 
 @pytest.mark.gpu
