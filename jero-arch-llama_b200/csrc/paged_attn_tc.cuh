@@ -8,8 +8,14 @@
 // tensor cores work on one, a warpgroup forms the weights of the other, so a
 // K and a V tile are read once for 256 rows.  Per key tile the tensor cores
 // need 4 x 128 x 128 x HD products and the special-function units 2 x 128 x
-// 128 exponentials; at HD = 128 the former takes longer, so what bounds the
-// kernel is how gaplessly the products are issued.
+// 128 exponentials, 2048 cycles each at HD = 128.  What bounds the kernel is how
+// these follow one another: a key tile takes about 4400 cycles (scores, weights,
+// products, and the waits between the warps that make them; without the exponentials
+// it takes 8% less), and a block's start (rows, table, first K tile) and end 10000 and
+// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 250 us, 0.63
+// PFLOP/s, with the tensor cores busy for 35% of the time.  (A quarter or half of the
+// exponentials as polynomials on the multiply-add units: 5 to 20 us slower.  Seven
+// loader warps, or one softmax warpgroup a row tile: no faster.)
 //
 //   warps 0-15       softmax: four warpgroups, two for each row tile, each with
 //                    64 of the tile's 128 keys (warp w reads tensor-memory lanes
