@@ -36,7 +36,7 @@ struct AttnParams {
   int32_t n_seqs, n_rows, max_q, n_groups;
   int32_t G, hq, act;                       // query heads per KV head, query heads, dtype of q / out
   int32_t window, n_sink;
-  int32_t splits, prefix_splits;            // pieces of a sequence's own keys; of a shared prefix's
+  int32_t splits, prefix_splits;            // pieces of a sequence's own keys; of a shared prefix's (0: read by each)
   int32_t tiles, prefix_tiles;              // row tiles of a sequence; of a group
   float scale_log2;                         // softmax scale * log2(e)
   float *part_o;                            // [slot][n_rows][hq][hd], unnormalised

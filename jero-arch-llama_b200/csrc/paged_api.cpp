@@ -161,7 +161,8 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   check_heads(hq, kv, b);
   NEED(q);
   NEED(out);
-  if (!std::isfinite(scale)) fail(JAL_ERR_INVALID_ARGUMENT, "attention scale is not finite");
+  const float scale_log2 = scale * 1.4426950408889634f;  // softmax by powers of two
+  if (!std::isfinite(scale_log2)) fail(JAL_ERR_INVALID_ARGUMENT, "attention scale is not finite or too large");
   AttnParams p = {};
   p.kv = view_of(kv);
   p.q_stride = row_stride(q_stride, hq * kv.head_dim, "q");
@@ -211,7 +212,7 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   p.prefix_splits = plan.prefix_splits;
   p.tiles = plan.tiles;
   p.prefix_tiles = plan.prefix_tiles;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.part_o = (float *)ws;
   if (plan.bytes)
     p.part_ml = (float2 *)(p.part_o + (size_t)(plan.splits + plan.prefix_splits) * b.n_rows * hq * kv.head_dim);

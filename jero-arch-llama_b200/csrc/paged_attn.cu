@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
   // This warp's rows of the tile at u: looked up by its first lanes one tile ahead.
   auto locate = [&](int u) -> Slot {
     const int k = u + warp * kMine + lane;
-    return lane < kMine && k < t.u1 ? slot_of(p.kv, t.table, t.key(k)) : Slot{-1, 0};
+    return lane < kMine && k < t.u1 ? slot_of(p.kv, t, t.key(k)) : Slot{-1, 0};
   };
   auto copy = [&](const Slot &where, int stage) {
     const int64_t at = slot_offset(p.kv, where, t.head);
@@ -353,6 +353,7 @@ void run_16bit_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
 // 101 us; 48 rows of up to 4100 keys of 8 KV heads in one piece 132 us, in three
 // 142 us; 128 rows of about 1100 keys of 4 KV heads in two pieces 119 us (with their
 // prefixes), in three 132 us.
+constexpr int64_t kApartKeys = 320;
 constexpr int64_t kTcLeast = 64;
 // Blocks of the tcgen05 kernel fill an SM each and write 256 rows of partial
 // results, so its keys are cut only as far as that gives idle SMs work.
@@ -360,7 +361,7 @@ int tc_pieces(int64_t blocks, int64_t keys) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / (2 * kTcKeys)));
   return (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
 }
-constexpr int64_t kBlockKeys = 256, kJoinKeys = 256, kPieceKeys = 24, kLeastKeys = 128;
+constexpr int64_t kBlockKeys = 256, kJoinKeys = 256, kPieceKeys = 4, kLeastKeys = 64;
 int pieces(int64_t blocks, int64_t keys, int resident, bool joined) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / kLeastKeys));
   int64_t best = 1, least = INT64_MAX;
@@ -401,13 +402,17 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
   int64_t keys = (int64_t)b.max_kv_len;
   if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
-  if (g && g->n_groups && g->max_prefix_len) {
+  // A few short sequences: each reads its prefix for itself, in one launch and
+  // without joining (4 sequences of 160 keys of 2 KV heads: 8.7 us instead of 12.2, of
+  // 310: 10.3 instead of 12.1; of 560 the joined form is the faster one).
+  const bool apart = a.tiles * hkv * (int64_t)b.n_seqs <= 2 * kPagedSMs && keys <= kApartKeys && a.rows != kTcRows;
+  if (g && g->n_groups && g->max_prefix_len && !apart) {
     a.prefix_rows = rows_for(group_pairs);
     a.prefix_tiles = (int)((group_pairs + a.prefix_rows - 1) / a.prefix_rows);
     a.prefix_splits = pieces_for(a.prefix_rows, a.prefix_tiles * hkv * (int64_t)g->n_groups, (int64_t)g->max_prefix_len);
     keys = std::max<int64_t>(1, keys - (int64_t)g->max_prefix_len);
   }
-  a.splits = pieces_for(a.rows, a.tiles * hkv * (int64_t)b.n_seqs, keys);
+  a.splits = g && g->n_groups && apart ? 1 : pieces_for(a.rows, a.tiles * hkv * (int64_t)b.n_seqs, keys);
   a.direct = a.splits + a.prefix_splits == 1;
   if (!a.direct)
     a.bytes = (size_t)(a.splits + a.prefix_splits) * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;

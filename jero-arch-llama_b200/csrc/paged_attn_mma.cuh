@@ -65,14 +65,26 @@ __device__ __forceinline__ void copies_wait() {
 }
 
 // The remainder of x after its first part in T, NS times: x = sum of parts.
+// Three bf16 parts are cut off, not rounded: 8 bits each are all 24, and the
+// largest f32 values do not become infinite.
 template <class T, int NS>
 __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[NS]) {
+  if constexpr (NS == 3) {
 #pragma unroll
-  for (int i = 0; i < NS; i++) {
-    part[i] = pack2<T>(a, b);
-    const float2 f = unpack2<T>(part[i]);
-    a -= f.x;
-    b -= f.y;
+    for (int i = 0; i < NS; i++) {
+      const uint32_t x = __float_as_uint(a) & 0xFFFF0000u, y = __float_as_uint(b) & 0xFFFF0000u;
+      part[i] = (x >> 16) | y;
+      a -= __uint_as_float(x);
+      b -= __uint_as_float(y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+      part[i] = pack2<T>(a, b);
+      const float2 f = unpack2<T>(part[i]);
+      a -= f.x;
+      b -= f.y;
+    }
   }
 }
 
@@ -116,7 +128,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
   const int n_chunks = (t.u1 - t.u0 + kMmaKeys - 1) / kMmaKeys;
   auto locate = [&](int c) -> Slot {
     const int u = t.u0 + c * kMmaKeys + lane;
-    return lane < kMmaKeys && c < n_chunks && u < t.u1 ? slot_of(p.kv, t.table, t.key(u)) : Slot{-1, 0};
+    return lane < kMmaKeys && c < n_chunks && u < t.u1 ? slot_of(p.kv, t, t.key(u)) : Slot{-1, 0};
   };
   auto copy = [&](const Slot &where, int stage) {
     const int64_t at = slot_offset(p.kv, where, t.head);

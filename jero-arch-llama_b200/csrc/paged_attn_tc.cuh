@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       auto group = [&](int k) { return w + k * kTcLoaders; };
       auto locate = [&](int j, int k) -> Slot {
         const int gr = group(k + lane / 8), u = t.u0 + j * kTcKeys + gr * 8 + lane % 8;
-        return j < n_tiles && k + lane / 8 < kGroups && gr < 16 && u < t.u1 ? slot_of(p.kv, t.table, t.key(u)) : Slot{-1, 0};
+        return j < n_tiles && k + lane / 8 < kGroups && gr < 16 && u < t.u1 ? slot_of(p.kv, t, t.key(u)) : Slot{-1, 0};
       };
       // Eight lanes copy 128 bytes of a row; a lane has rows lane / 8 and lane / 8
       // + 4 of each group.  Their addresses are passed round once for K and V.

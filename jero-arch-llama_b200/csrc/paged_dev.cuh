@@ -150,6 +150,8 @@ __device__ __forceinline__ int seq_of_row(const int32_t *q_start, int lo, int hi
 // them; a row of position p sees t <= p with t > p - window or t < n_sink.
 struct Tile {
   const int32_t *table;  // the page-table row the keys are read through
+  const int32_t *ahead;  // and the one for positions below `shared` (a prefix that a sequence reads for itself)
+  int shared;
   int beg, end;          // token rows of the sequence / of the group
   int first, rows;       // first (token, head) pair; pairs of this tile
   int head;              // KV head
@@ -161,6 +163,10 @@ struct Tile {
   int64_t shift;         // one sequence: a token row's position is row + shift
   __device__ __forceinline__ int key(int u) const { return u < ns ? u : lo + (u - ns); }
 };
+
+__device__ __forceinline__ Slot slot_of(const PagedView &kv, const Tile &t, int key) {
+  return slot_of(kv, key < t.shared ? t.ahead : t.table, key);
+}
 
 // Position of token row r: -1 before the first position (such a row sees
 // nothing), at most the last position of the table.
@@ -203,7 +209,8 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
   t.first = tile * rt;
   t.rows = min(rt, n_tok * p.G - t.first);
   if (t.rows <= 0) return false;
-  t.table = p.kv.table + (int64_t)t.seq_lo * p.kv.max_pages;
+  t.table = t.ahead = p.kv.table + (int64_t)t.seq_lo * p.kv.max_pages;
+  t.shared = 0;
   const int splits = prefix ? p.prefix_splits : p.splits;
   t.slot = (prefix ? 0 : p.prefix_splits) + piece;
   t.limit = 0x7fffffff;
@@ -218,7 +225,13 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
     if (p.n_groups) {  // the keys behind the shared prefix of the sequence's group
       const int g = seq_of_row(p.group_start, 0, p.n_groups, t.seq_lo);
       const int a = __ldg(p.group_start + g), b = __ldg(p.group_start + g + 1), n = __ldg(p.prefix_len + g);
-      t.lo = a <= t.seq_lo && t.seq_lo < b ? min(max(n, 0), p.kv.cap) : 0;
+      const int len = a <= t.seq_lo && t.seq_lo < b ? min(max(n, 0), p.kv.cap) : 0;
+      if (p.prefix_splits) {
+        t.lo = len;
+      } else {
+        t.shared = len;
+        t.ahead = p.kv.table + (int64_t)min(max(a, 0), p.n_seqs - 1) * p.kv.max_pages;
+      }
     }
     t.lo = min(t.lo, t.hi);
     t.ns = min(p.n_sink, t.lo);
@@ -315,7 +328,7 @@ static __device__ __noinline__ void attend_row_alone(const AttnParams &p, const 
   for (int u = t.u0; u < t.u1; u++) {
     const int key = t.key(u);
     if (!mk.sees(key, p.n_sink)) continue;
-    const int64_t at = slot_offset(p.kv, t.table, t.head, key);
+    const int64_t at = slot_offset(p.kv, slot_of(p.kv, t, key), t.head);
     if (at < 0) continue;
     float s = 0.0f;
 #pragma unroll

@@ -55,7 +55,8 @@ def test_attention_arguments_are_refused(jal):
     kv, b = _view(jal), _batch(jal)
     ok = dict(q=4096, out=4096, n_heads_q=4, scale=0.1, dtype=jal.F16)
     for change, err in [(dict(q=None), jal.ERR_INVALID_ARGUMENT), (dict(out=None), jal.ERR_INVALID_ARGUMENT),
-                        (dict(scale=math.nan), jal.ERR_INVALID_ARGUMENT), (dict(n_heads_q=5), jal.ERR_CAPABILITY_MISMATCH),
+                        (dict(scale=math.nan), jal.ERR_INVALID_ARGUMENT),
+                        (dict(scale=3e38), jal.ERR_INVALID_ARGUMENT), (dict(n_heads_q=5), jal.ERR_CAPABILITY_MISMATCH),
                         (dict(n_heads_q=0), jal.ERR_CAPABILITY_MISMATCH), (dict(dtype=jal.BF16), jal.ERR_CAPABILITY_MISMATCH),
                         (dict(dtype=jal.Q4_0), jal.ERR_CAPABILITY_MISMATCH), (dict(q_stride=64), jal.ERR_TENSOR_BOUNDS),
                         (dict(out_stride=257), jal.ERR_TENSOR_BOUNDS), (dict(q=4098), jal.ERR_TENSOR_BOUNDS),
@@ -443,6 +444,26 @@ def test_attention_large_scores(jal, torch_cuda):
         check(c, attend(jal, c, 40.0), 40.0)
         check(c, attend(jal, c, -3.0), -3.0)
         check(c, attend(jal, c, 0.0), 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_extreme_rows(jal, torch_cuda, act, cache, new):
+    """Rows as large and as small as their type has them, with a scale that brings the scores back."""
+    big = {"f32": 3.3e38, "f16": 6.0e4, "bf16": 3.3e38}[act]
+    for size in (big, 1e-4 if act == "f16" else 1e-30):
+        c = Case([120, 90], [new, new], 4, 2, 64, act, cache, 16, seed=12)
+        q = c.q_full.double()
+        c.q_full = (q / q.abs().max() * size).to(c.act)
+        c.q = c.q_full.view(c.n_rows, 4, 64)
+        for i in range(2):  # keys small enough that no score overflows before it is scaled
+            c.k[i] = (c.k[i].double() / 256).to(c.cache)
+            view = c.pools[0].permute(c.perm)
+            for t in range(c.lens[i]):
+                view[int(c.table[i, t // 16]), :, t % 16] = c.k[i][t]
+        scale = 256 / size
+        check(c.to_device(jal), attend(jal, c, scale), scale)
 
 
 @pytest.mark.gpu
