@@ -12,10 +12,11 @@
 // these follow one another: a key tile takes about 4400 cycles (scores, weights,
 // products, and the waits between the warps that make them; without the exponentials
 // it takes 8% less), and a block's start (rows, table, first K tile) and end 10000 and
-// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 250 us, 0.63
-// PFLOP/s, with the tensor cores busy for 35% of the time.  (A quarter or half of the
+// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 240 us, 0.66
+// PFLOP/s, with the tensor cores busy for 37% of the time.  (A quarter or half of the
 // exponentials as polynomials on the multiply-add units: 5 to 20 us slower.  Seven
-// loader warps, or one softmax warpgroup a row tile: no faster.)
+// loader warps, one softmax warpgroup a row tile, or the query rows asked for before the
+// first barrier: no faster.)
 //
 //   warps 0-15       softmax: four warpgroups, two for each row tile, each with
 //                    64 of the tile's 128 keys (warp w reads tensor-memory lanes
@@ -178,6 +179,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
   // tiles and the second the odd ones, and their results are joined.
   const bool twice = t.rows <= 128;
 
+  // Loader: the 16 groups of 8 rows of a tile go round the warps; a lane looks up
+  // two of its warp's (up to) 48 rows, one tile ahead, the first before anything else.
+  const int w = warp - 16;
+  constexpr int kGroups = (16 + kTcLoaders - 1) / kTcLoaders;
+  auto group = [&](int k) { return w + k * kTcLoaders; };
+  auto locate = [&](int j, int k) -> Slot {
+    const int gr = group(k + lane / 8), u = t.u0 + j * kTcKeys + gr * 8 + lane % 8;
+    return j < n_tiles && k + lane / 8 < kGroups && gr < 16 && u < t.u1 ? slot_of(p.kv, t, t.key(u)) : Slot{-1, 0};
+  };
+  Slot next0 = {-1, 0}, next1 = {-1, 0};
+  if (warp >= 16 && warp < 16 + kTcLoaders) {
+    next0 = locate(0, 0);
+    next1 = locate(0, 4);
+  }
+
   if (tid == 0) {
     mbar_init(&sy.q_full, kTcSoftmax);
     mbar_init(&sy.loaded, kTcLoaders * 32);
@@ -219,15 +235,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < 16 + kTcLoaders) {
       // ---- the loader
-      // The 16 groups of 8 rows of a tile go round the warps; a lane looks up
-      // two of its warp's (up to) 48 rows, one tile ahead.
-      const int w = warp - 16;
-      constexpr int kGroups = (16 + kTcLoaders - 1) / kTcLoaders;
-      auto group = [&](int k) { return w + k * kTcLoaders; };
-      auto locate = [&](int j, int k) -> Slot {
-        const int gr = group(k + lane / 8), u = t.u0 + j * kTcKeys + gr * 8 + lane % 8;
-        return j < n_tiles && k + lane / 8 < kGroups && gr < 16 && u < t.u1 ? slot_of(p.kv, t, t.key(u)) : Slot{-1, 0};
-      };
       // Eight lanes copy 128 bytes of a row; a lane has rows lane / 8 and lane / 8
       // + 4 of each group.  Their addresses are passed round once for K and V.
       const int c8 = lane % 8, r8 = lane / 8;
@@ -273,7 +280,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
             if (group(k) < 16)
               watch8<T>(bad, *(const uint4 *)(rows + (h / 2) * (kTcKeys * 128) + group(k) * 1024 + (h % 2) * 512 + lane * 16));
       };
-      Slot next0 = locate(0, 0), next1 = locate(0, 4);
       int scan_b = -1;
 #pragma unroll 1
       for (int j = 0; j < n_tiles; j++) {
@@ -594,7 +600,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     tc_fence_after();
     sy.x[i][half][r] = l;
     if (i == 1 && half == 0) sy.m1[r] = m;
-    asm volatile("bar.sync 3, 512;" ::: "memory");
+    if (twice) asm volatile("bar.sync 3, 512;" ::: "memory");
+    else tile_sync();
     if (*given_up || *(volatile int *)&sy.poison) {
       for (int k = warp * 16; k < min(warp * 16 + 16, t.rows); k++) attend_row_alone(p, t, k, direct);
     } else if (!twice || i == 0) {
@@ -614,11 +621,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
       const float inv = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
       if (real && !direct && half == 0) p.part_ml[part_index(p, t, row)] = make_float2(m, l);
       const bool wide = !direct || NS == 2;  // f32 rows
-      char *const stage = base_p + warp * (wide ? 4096 : 2048);
-#pragma unroll 1
-      for (int d = half * (HD / 2); d < (half + 1) * (HD / 2) && d < hd; d += 32) {
-        float o[32];
-        __syncwarp();
+      char *const stage = base_p + warp * 4096;
+      // 32 dims of this thread's row, times 1 / sum where they are final.
+      auto result = [&](int d, float (&o)[32]) {
         if (n_tiles) {
           tc_ld32(to + d, (uint32_t *)o);
           tc_wait_ld();
@@ -639,21 +644,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         }
 #pragma unroll
         for (int e = 0; e < 32; e++) o[e] *= inv;
-        if (wide) {
+      };
+      const int first = half * (HD / 2);
+      __syncwarp();
+      if (wide) {
+        float *const out = direct ? (float *)p.out : p.part_o;
+#pragma unroll 1
+        for (int d = first; d < first + HD / 2 && d < hd; d += 32) {
+          float o[32];
+          result(d, o);
 #pragma unroll
           for (int c = 0; c < 8; c++)
             *(float4 *)(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
                 make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; c++)
-            *(uint4 *)(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) * 16)) =
-                make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
-                           pack2<T>(o[8 * c + 4], o[8 * c + 5]), pack2<T>(o[8 * c + 6], o[8 * c + 7]));
-        }
-        __syncwarp();
-        if (wide) {
-          float *const out = direct ? (float *)p.out : p.part_o;
+          __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; k++) {
             const int rr = k * 4 + lane / 8, c = lane % 8;
@@ -661,14 +665,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
             const float4 v = *(const float4 *)(stage + rr * 128 + ((c ^ (rr & 7)) * 16));
             if (o2 >= 0 && d + c * 4 < hd) *(float4 *)(out + o2 + d + c * 4) = v;
           }
-        } else {
+          __syncwarp();
+        }
+      } else {
+        constexpr int PC = HD / 16;  // 16-byte pieces of a half row
+        auto place = [&](int r, int c) { return stage + r * (HD) + ((HD == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) * 16); };
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int rr = k * 8 + lane / 4, c = lane % 4;
-            const int64_t o2 = __shfl_sync(0xffffffffu, at, rr);
-            const uint4 v = *(const uint4 *)(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) * 16));
-            if (o2 >= 0 && d + c * 8 < hd) *(uint4 *)((T *)p.out + o2 + d + c * 8) = v;
-          }
+        for (int q = 0; q < HD / 64; q++) {
+          float o[32];
+          result(first + q * 32, o);
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+            *(uint4 *)place(lane, q * 4 + c) =
+                make_uint4(pack2<T>(o[8 * c], o[8 * c + 1]), pack2<T>(o[8 * c + 2], o[8 * c + 3]),
+                           pack2<T>(o[8 * c + 4], o[8 * c + 5]), pack2<T>(o[8 * c + 6], o[8 * c + 7]));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < PC; k++) {
+          const int rr = k * (32 / PC) + lane / PC, c = lane % PC;
+          const int64_t o2 = __shfl_sync(0xffffffffu, at, rr);
+          const uint4 v = *(const uint4 *)place(rr, c);
+          if (o2 >= 0 && first + c * 8 < hd) *(uint4 *)((T *)p.out + o2 + first + c * 8) = v;
         }
       }
     }
