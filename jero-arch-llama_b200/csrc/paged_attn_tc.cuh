@@ -12,8 +12,8 @@
 // these follow one another: a key tile takes about 4400 cycles (scores, weights,
 // products, and the waits between the warps that make them; without the exponentials
 // it takes 8% less), and a block's start (rows, table, first K tile) and end 10000 and
-// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 240 us, 0.66
-// PFLOP/s, with the tensor cores busy for 37% of the time.  (A quarter or half of the
+// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 238 to
+// 252 us, 0.65 PFLOP/s, with the tensor cores busy for 37% of the time.  (A quarter or half of the
 // exponentials as polynomials on the multiply-add units: 5 to 20 us slower.  Seven
 // loader warps, one softmax warpgroup a row tile, or the query rows asked for before the
 // first barrier: no faster.)

@@ -745,6 +745,79 @@ def test_beam_reorder(jal, torch_cuda, layers, beams, page, lens, layout, cache)
 
 # ---- together ------------------------------------------------------------------
 @pytest.mark.gpu
+@pytest.mark.parametrize("act,cache,beams", [("f32", "f16", 4), ("f16", "f16", 40), ("bf16", "bf16", 64), ("f32", "f32", 5)])
+def test_captured_beam_step(jal, torch_cuda, act, cache, beams):
+    """Selection, reordering, append and shared-prefix attention captured in one graph, replayed with other inputs:
+    the same bits as the calls one by one."""
+    hq, hkv, hd, vocab, page, prefix, length = 8, 2, 64, 5003, 16, 1040, 1049
+    g = torch.Generator().manual_seed(beams)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    shared, width = prefix // page, prefix // page + 2
+    n_pages = shared + 2 * beams
+    rows = [list(range(shared)) + [shared + b, -1] for b in range(beams)]
+    types = {"f32": jal.F32, "f16": jal.F16, "bf16": jal.BF16}
+    base = [torch.randn(n_pages, hkv, page, hd, generator=g).to(NAMES[cache]) for _ in range(2)]
+    inv_freq = (10000.0 ** (-torch.arange(hd // 2, dtype=torch.float64) / (hd // 2))).float().to(DEV)
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return [(torch.randn(beams, vocab, generator=g) * 2).to(DEV), (torch.randn(1, beams, generator=g) - 20).to(DEV),
+                *[torch.randn(beams, n * hd, generator=g).to(NAMES[act]).to(DEV) for n in (hkv, hkv, hq)]]
+
+    class State:
+        def __init__(self):
+            self.pools = [p.to(DEV) for p in base]
+            self.table, self.kv_len = ints(rows), ints([length] * beams)
+            self.fresh = ints([shared + beams + b for b in range(beams)])
+            self.new_table, self.new_len = torch.zeros_like(self.table), torch.zeros_like(self.kv_len)
+            self.lens = torch.zeros_like(self.kv_len)
+            self.scores = torch.zeros(1, beams, device=DEV)
+            self.parents, self.tokens = (torch.zeros(1, beams, dtype=torch.int32, device=DEV) for _ in range(2))
+            self.out = torch.zeros(beams, hq * hd, dtype=NAMES[act], device=DEV)
+            mk = lambda t: jal.PagedKv(*self.pools, t, dtype=types[cache], n_pages=n_pages, page_size=page,  # noqa: E731
+                                       n_heads_kv=hkv, head_dim=hd, n_seqs=beams, max_pages=width)
+            self.old, self.new = mk(self.table), mk(self.new_table)
+            self.batch = jal.RaggedBatch(ints(list(range(beams + 1))), self.lens, beams, beams, 1, length + 1)
+            self.groups = jal.PrefixGroups(ints([0, beams]), ints([prefix]), 1, beams, prefix)
+            self.need = (jal.beam_select_workspace(1, beams, vocab, beams),
+                         jal.shared_prefix_attention_workspace(self.new, self.batch, self.groups, hq, dtype=types[act]))
+            self.ws = [torch.full((n + 16,), 255, dtype=torch.uint8, device=DEV) for n in self.need]
+
+        def step(self, x, stream=None):
+            logits, cum, k, v, q = x
+            jal.beam_select(logits, cum, self.scores, self.parents, self.tokens, 1, beams, vocab, beams,
+                            workspace=self.ws[0], workspace_len=self.need[0], stream=stream)
+            jal.beam_reorder(self.old, self.kv_len, self.parents, self.fresh, self.new_table, self.new_len, 1, beams,
+                             stream=stream)
+            torch.add(self.new_len, 1, out=self.lens)
+            jal.rope_kv_append(self.new, self.batch, k, v, inv_freq, dtype=types[act], rotary_dim=hd, neox=True, q=q,
+                               q_out=self.out, n_heads_q=hq, stream=stream)
+            jal.shared_prefix_attention(self.new, self.batch, self.groups, self.out, self.out, hq, 0.125,
+                                        dtype=types[act], workspace=self.ws[1], workspace_len=self.need[1], stream=stream)
+
+        def results(self):
+            torch.cuda.synchronize()
+            return [t.clone() for t in (self.scores, self.parents, self.tokens, self.new_table, self.lens, self.out, *self.pools)]
+
+    once, kept, x = State(), State(), inputs(1)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        kept.step(x, torch.cuda.current_stream())
+    for seed in (1, 2, 3):
+        y = inputs(seed)
+        for a, b in zip(x, y):
+            a.copy_(b)
+        for p, q, b in zip(once.pools, kept.pools, base):
+            p.copy_(b)
+            q.copy_(b)
+        graph.replay()
+        once.step(y)
+        for a, b in zip(kept.results(), once.results()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act,cache", [("f32", "f32"), ("f32", "f16")])
 def test_beam_search_over_the_paged_cache(jal, torch_cuda, act, cache):
     """A one-layer language model searched with four beams for two prompts: the prompts appended and attended as one
