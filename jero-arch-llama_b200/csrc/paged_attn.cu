@@ -213,18 +213,21 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(const __grid_c
   pdl_wait();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, head = blockIdx.x % p.hq;
   const int tok = blockIdx.x / p.hq, s = tok / p.max_q, i = tok - s * p.max_q;
-  int beg, end;
+  int g_first = 0, g_last = 0, g_row = 0, beg, end;
+  if (p.prefix_splits) {
+    const int g = seq_of_row(p.group_start, 0, p.n_groups, s);
+    g_first = __ldg(p.group_start + g);
+    g_last = __ldg(p.group_start + g + 1);
+    g_row = __ldg(p.q_start + min(max(g_first, 0), p.n_seqs));
+  }
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   if (i >= end - beg) return;
   const int row = beg + i;
   int first = p.prefix_splits;  // a sequence outside every group has its own keys alone
-  if (p.prefix_splits) {
-    const int g = seq_of_row(p.group_start, 0, p.n_groups, s);
-    if (p.group_start[g] <= s && s < p.group_start[g + 1]) {
-      first = 0;
-      const int gb = min(max(p.q_start[min(max(p.group_start[g], 0), p.n_seqs)], 0), p.n_rows);
-      if ((int64_t)(row - gb + 1) * p.G > (int64_t)p.prefix_tiles * prefix_rows) return;  // past max_group: not computed
-    }
+  if (g_first <= s && s < g_last) {
+    first = 0;
+    const int rows = row - min(max(g_row, 0), p.n_rows) + 1;
+    if ((int64_t)rows * p.G > (int64_t)p.prefix_tiles * prefix_rows) return;  // past max_group: not computed
   }
   const int n = p.prefix_splits + p.splits, hd = p.kv.hd;
   const int64_t stride = (int64_t)p.n_rows * p.hq, at = (int64_t)row * p.hq + head;

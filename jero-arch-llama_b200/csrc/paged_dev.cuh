@@ -197,7 +197,15 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
     t.seq_hi = min(max(b, t.seq_lo), p.n_seqs);
     if (t.seq_lo == t.seq_hi) return false;
   }
-  const int len = __ldg(p.kv_len + t.seq_lo);  // (independent of the rows' loads)
+  // (Loads that do not depend on each other, asked for together.)
+  int own_first = 0, own_last = 0, own_prefix = 0;
+  if (!prefix && p.n_groups) {
+    const int g = seq_of_row(p.group_start, 0, p.n_groups, t.seq_lo);
+    own_first = __ldg(p.group_start + g);
+    own_last = __ldg(p.group_start + g + 1);
+    own_prefix = __ldg(p.prefix_len + g);
+  }
+  const int len = __ldg(p.kv_len + t.seq_lo);
   seq_rows(p.q_start, p.n_rows, t.seq_lo, t.beg, t.end);
   t.shift = (int64_t)len - t.end;
   if (t.seq_hi - t.seq_lo > 1) {
@@ -223,14 +231,13 @@ __device__ __forceinline__ bool make_tile(const AttnParams &p, bool prefix, int 
     t.hi = pl + 1;
     t.lo = p.window > 0 ? max(0, pf + 1 - p.window) : 0;
     if (p.n_groups) {  // the keys behind the shared prefix of the sequence's group
-      const int g = seq_of_row(p.group_start, 0, p.n_groups, t.seq_lo);
-      const int a = __ldg(p.group_start + g), b = __ldg(p.group_start + g + 1), n = __ldg(p.prefix_len + g);
-      const int len = a <= t.seq_lo && t.seq_lo < b ? min(max(n, 0), p.kv.cap) : 0;
+      const bool in = own_first <= t.seq_lo && t.seq_lo < own_last;
+      const int shared = in ? min(max(own_prefix, 0), p.kv.cap) : 0;
       if (p.prefix_splits) {
-        t.lo = len;
+        t.lo = shared;
       } else {
-        t.shared = len;
-        t.ahead = p.kv.table + (int64_t)min(max(a, 0), p.n_seqs - 1) * p.kv.max_pages;
+        t.shared = shared;
+        t.ahead = p.kv.table + (int64_t)min(max(own_first, 0), p.n_seqs - 1) * p.kv.max_pages;
       }
     }
     t.lo = min(t.lo, t.hi);
