@@ -581,6 +581,19 @@ def test_shared_prefix(jal, torch_cuda, lens, news, groups, prefixes, hq, hkv, h
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("lens,news,groups,prefixes,hq,hkv,hd,page", PREFIXES)
+def test_shared_prefix_pages_named_once(jal, torch_cuda, lens, news, groups, prefixes, hq, hkv, hd, page, act, cache):
+    """Only the first sequence of a group names the prefix's pages."""
+    c = share(Case(lens, news, hq, hkv, hd, act, cache, page, seed=hd + len(lens)), groups, prefixes).to_device(jal)
+    for g, n in enumerate(prefixes):
+        for s in range(groups[g] + 1, groups[g + 1]):
+            c.d_table[s, :min(n, c.lens[s]) // page] = -1
+    scale = 1 / math.sqrt(hd)
+    check(c, shared(jal, c, groups, prefixes, scale), scale)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act,cache", [("f32", "f16"), ("bf16", "bf16")])
 def test_shared_prefix_bounds_of_the_plan(jal, torch_cuda, act, cache):
     """No groups or an unused prefix is plain attention; a batch behind its stated sizes leaves rows as they were."""
