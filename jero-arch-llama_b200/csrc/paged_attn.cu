@@ -20,8 +20,8 @@ using namespace paged;
 // rows with cp.async one tile ahead; 128 threads work on them as 8 row groups x 16
 // key (or dim) groups.  Few rows are bound by shared memory, which a thread reads
 // three times (16 bytes of q, twice 16 of K) for eight multiply-adds, not by the
-// cache: 48 rows of up to 4100 keys take 538 us, 3.0 TB/s (843 us without the copies
-// ahead).
+// cache: 48 rows of up to 4100 keys take 540 to 590 us, 2.8 TB/s (843 us without the
+// copies ahead).
 constexpr int kF32Threads = 128;
 constexpr int kF32Keys = 32;
 
@@ -355,7 +355,8 @@ void run_16bit_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
 // needs anyway.  Measured: 131071 keys of 8 KV heads in 37 pieces 94 us, in 40 or 55
 // 101 us; 48 rows of up to 4100 keys of 8 KV heads in one piece 132 us, in three
 // 142 us; 128 rows of about 1100 keys of 4 KV heads in two pieces 119 us (with their
-// prefixes), in three 132 us.
+// prefixes), in three 132 us.  An f32 cache's keys take longer, so a start is worth
+// fewer of them: the 48 rows 629 us with 256, 587 us with 48.
 constexpr int64_t kApartKeys = 320;
 constexpr int64_t kTcLeast = 64;
 // Blocks of the tcgen05 kernel fill an SM each and write 256 rows of partial
@@ -364,13 +365,13 @@ int tc_pieces(int64_t blocks, int64_t keys) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / (2 * kTcKeys)));
   return (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
 }
-constexpr int64_t kBlockKeys = 256, kJoinKeys = 256, kPieceKeys = 4, kLeastKeys = 64;
-int pieces(int64_t blocks, int64_t keys, int resident, bool joined) {
+constexpr int64_t kBlockKeys = 256, kF32BlockKeys = 48, kJoinKeys = 256, kPieceKeys = 4, kLeastKeys = 64;
+int pieces(int64_t blocks, int64_t keys, int resident, int64_t start_keys, bool joined) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / kLeastKeys));
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= most; s++) {
     const int64_t n = (blocks * s + kPagedSMs - 1) / kPagedSMs, k = (keys + s - 1) / s;
-    const int64_t time = std::max(k, n * k / 2) + kBlockKeys * ((n + resident - 1) / resident);
+    const int64_t time = std::max(k, n * k / 2) + start_keys * ((n + resident - 1) / resident);
     const int64_t cost = time + (s > 1 ? (joined ? 0 : kJoinKeys) + kPieceKeys * s : 0);
     if (cost < least) {
       least = cost;
@@ -399,7 +400,8 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
   };
   auto pieces_for = [&](int rows, int64_t blocks, int64_t keys) {
     return rows == kTcRows ? tc_pieces(blocks, keys)
-                           : pieces(blocks, keys, mma_blocks((int)kv.head_dim), g != nullptr);
+                           : pieces(blocks, keys, mma_blocks((int)kv.head_dim),
+                                    kv.dtype == JAL_F32 ? kF32BlockKeys : kBlockKeys, g != nullptr);
   };
   a.rows = rows_for(pairs);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
