@@ -45,8 +45,8 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
 
 constexpr float kLog2e = 1.44269504f;
-struct ChunkHead {  // what a chunk leaves beside its k keys: the sum of 2^(x kLog2e - ref)
-  float ref, sum;
+struct ChunkHead {  // what a chunk leaves beside its k keys: its largest logit, the sum of 2^((x - top) kLog2e)
+  float top, sum;
 };
 
 // A block reads its chunk piece by piece, PER logits a thread, 16 bytes at a time
@@ -128,10 +128,12 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) k_beam_chunk(const Be
       if (n < room) list[n] = key;
     }
   };
-  // Sums of 2^(v log2 e - ref), with log2 e as it is in f32 throughout: the
+  // Sums of 2^((v - top) log2 e), with log2 e as it is in f32 throughout: the
   // quotient by the same number at the end makes that an error of 10^-8 of the
-  // entropy.  One multiply-add, one exponential and one addition a logit.
-  float top = -INFINITY, ref = 0.0f, sum = 0.0f, bar = -INFINITY;
+  // entropy.  The difference comes before the product: finite logits as low or
+  // high as the type has them give 0 or -inf there, where a product of the
+  // logit itself would overflow.
+  float top = -INFINITY, ref = 0.0f, sum = 0.0f, bar = -INFINITY;  // ref: top, or 0 while there is none
   uint64_t least = 1;
   for (int piece = begin; piece < end; piece += kPiece) {
     load(piece);
@@ -139,13 +141,11 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) k_beam_chunk(const Be
 #pragma unroll
     for (int i = 1; i < PER; i++) mine = fmaxf(mine, v[i]);
     if (mine > top) {
-      const float next = mine * kLog2e;
-      sum *= top == -INFINITY ? 0.0f : exp2_fast(ref - next);
-      top = mine;
-      ref = next;
+      sum *= exp2_fast((top - mine) * kLog2e);
+      top = ref = mine;
     }
 #pragma unroll
-    for (int i = 0; i < PER; i++) sum += exp2_fast(fmaf(v[i], kLog2e, -ref));
+    for (int i = 0; i < PER; i++) sum += exp2_fast((v[i] - ref) * kLog2e);
     if (piece == begin) {
       // At least k groups of threads: the least of the groups' best keys is
       // below k keys at least, so the k best are not below it.
@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) k_beam_chunk(const Be
     }
   }
   {
-    const float all = warp_max(top == -INFINITY ? -INFINITY : ref);
-    const float part = warp_sum(top == -INFINITY ? 0.0f : sum * exp2_fast(ref - all));
+    const float all = warp_max(top);
+    const float part = warp_sum(top == -INFINITY ? 0.0f : sum * exp2_fast((top - all) * kLog2e));
     if (lane == 0) sums[warp] = make_float2(all, part);
   }
   __syncthreads();
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) k_beam_chunk(const Be
     for (int w = 0; w < kSelThreads / 32; w++) all = fmaxf(all, sums[w].x);
 #pragma unroll
     for (int w = 0; w < kSelThreads / 32; w++)
-      total += sums[w].x == -INFINITY ? 0.0f : sums[w].y * exp2_fast(sums[w].x - all);
+      total += sums[w].x == -INFINITY ? 0.0f : sums[w].y * exp2_fast((sums[w].x - all) * kLog2e);
     *head = {all, total};
   }
 }
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
     }
     const double cum = p.cum[row];
     float top = -INFINITY;
-    for (int c = lane; c < p.chunks; c += 32) top = fmaxf(top, h[c].ref);
+    for (int c = lane; c < p.chunks; c += 32) top = fmaxf(top, h[c].top);
     top = warp_max(top);
     // No log-sum-exp: nothing but -inf, or a +inf among them.
     const bool dead = !(cum > -INFINITY && cum < INFINITY && top > -INFINITY && top < INFINITY);
@@ -294,9 +294,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
     }
     double sum = 0.0;
     for (int c = lane; c < p.chunks; c += 32)
-      if (h[c].sum > 0.0f) sum += exp2((double)h[c].ref - (double)top) * (double)h[c].sum;
+      if (h[c].top > -INFINITY) sum += exp2(((double)h[c].top - (double)top) * (double)kLog2e) * (double)h[c].sum;
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double lse = ((double)top + log2(sum)) / (double)kLog2e;
+    const double lse = log2(sum) / (double)kLog2e;  // of the logits less the largest one
     uint64_t head[kJoinLists];
     int pos[kJoinLists];
 #pragma unroll
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_beam_join(const BeamParams p, 
             pos[i]++;
             head[i] = pos[i] < p.k ? list[(lane + 32 * i) * p.k + pos[i]] : 0;
           }
-        order[b * p.k + j] = order_of(cum + ((double)value_of(best) - lse));
+        order[b * p.k + j] = order_of(cum + (((double)value_of(best) - (double)top) - lse));
         token[b * p.k + j] = (int32_t)index_of(best);
       }
     }
