@@ -271,8 +271,12 @@ int jal_op_rope_kv_append(const jal_paged_kv *kv, const jal_ragged_batch *batch,
  * whatever they hold, and a row that sees a NaN or an infinity follows the
  * formula (scores of -inf count as masked).  dtype (q and out): the
  * cache's or JAL_F32.  Sums and softmax are f32; with 16-bit q the softmax
- * weights are rounded to that type for the product with V.  n_heads_q is a
- * multiple of n_heads_kv.  Strides as in jal_op_rope_kv_append; out may be q.
+ * weights are rounded to that type for the product with V, and f32 q and
+ * weights over a 16-bit cache are carried as parts of 22 bits (f16) or 24
+ * (bf16).  Over an f16 cache a weight is further off by up to 2^-36 of the
+ * row's largest, which shows where one position lies 14 nats or more above the
+ * ones that make the result.  n_heads_q is a multiple of n_heads_kv.  Strides
+ * as in jal_op_rope_kv_append; out may be q.
  * The workspace has to be as large as jal_op_paged_attention_workspace says
  * for the same arguments (JAL_ERR_TENSOR_BOUNDS), 16-byte aligned. */
 int jal_op_paged_attention(const jal_paged_kv *kv, const jal_ragged_batch *batch,

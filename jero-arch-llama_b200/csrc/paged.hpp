@@ -40,7 +40,7 @@ struct AttnParams {
   int32_t tiles, prefix_tiles;              // row tiles of a sequence; of a group
   float scale_log2;                         // softmax scale * log2(e)
   float *part_o;                            // [slot][n_rows][hq][hd], unnormalised
-  float2 *part_ml;                          // [slot][n_rows][hq]: running maximum (base 2), sum
+  float2 *part_ml;                          // [slot][n_rows][hq]: what the weights refer to (base 2), their sum
 };
 
 // How one call is cut; the workspace size follows from it.

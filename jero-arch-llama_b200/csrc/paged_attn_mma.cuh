@@ -16,7 +16,17 @@
 // parts are added in f32.  With 16-bit rows (NS = 1) q is exact and the
 // weights are rounded once, to 2^-11 or 2^-8 of themselves, less than what
 // the rounding of the result costs.
+//
+// f16 has no bits below 2^-24 and few below 2^-14, so f16 weights refer to
+// kHeadroom less than the running maximum (base 2): the largest are near the
+// top of the type, and a key's weight is off by 2^-25 of a unit, 2^-40 of
+// the largest weight, beside its relative error.  One position far above
+// 10^5 others then leaves them their share: 20 nats below the maximum a weight
+// still has its 11 bits, 12 nats below it both parts' 22.  The sum and the
+// output carry the same power of two, which their quotient does not have.
 #pragma once
+
+#include <type_traits>
 
 #include "paged_dev.cuh"
 
@@ -87,6 +97,16 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[NS]) {
     }
   }
 }
+
+// What weights refer to where the running maximum is `top`: SHIFT less, so that
+// the largest weight is 2^SHIFT (of maxima so large that the difference is not
+// exact to a quarter, the maximum itself).
+template <int SHIFT>
+__device__ __forceinline__ float reference_of(float top) {
+  return SHIFT && fabsf(top) < 8388608.0f ? top - (float)SHIFT : top;
+}
+template <class T>
+constexpr int kHeadroom = std::is_same<T, __half>::value ? 15 : 0;  // bf16 has the exponents of f32
 
 // Blocks on an SM.  Three, with two stages a warp, read a 131071-key row in 94 us
 // where two with three stages took 99 us: one block's start and end go on beside
@@ -225,7 +245,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
   float o[HD / 8][4];
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float top0 = -INFINITY, top1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  // Running maxima, what the weights refer to, and their sums.
+  float top0 = -INFINITY, top1 = -INFINITY, ref0 = -INFINITY, ref1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
   uint32_t bad = 0;
 
   int stage = 0;
@@ -291,9 +312,12 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
     n0 = fmaxf(top0, fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2)));
     n1 = fmaxf(top1, fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2)));
     if (__any_sync(0xffffffffu, n0 != top0 || n1 != top1)) {
-      const float c0 = n0 == top0 ? 1.0f : exp2_fast(top0 - n0), c1 = n1 == top1 ? 1.0f : exp2_fast(top1 - n1);
+      const float r0 = reference_of<kHeadroom<T>>(n0), r1 = reference_of<kHeadroom<T>>(n1);
+      const float c0 = n0 == top0 ? 1.0f : exp2_fast(ref0 - r0), c1 = n1 == top1 ? 1.0f : exp2_fast(ref1 - r1);
       top0 = n0;
       top1 = n1;
+      ref0 = r0;
+      ref1 = r1;
       l0 *= c0;
       l1 *= c1;
 #pragma unroll
@@ -304,7 +328,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
         o[i][3] *= c1;
       }
     }
-    const float b0 = top0 == -INFINITY ? 0.0f : top0, b1 = top1 == -INFINITY ? 0.0f : top1;
+    const float b0 = ref0 == -INFINITY ? 0.0f : ref0, b1 = ref1 == -INFINITY ? 0.0f : ref1;
 #pragma unroll
     for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -356,8 +380,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
   // The four warps' results, joined through shared memory.
   float *const merge = (float *)(smem_raw + S::q_bytes);
   if ((lane & 3) == 0) {
-    row_ml[warp][r0] = make_float2(top0, l0);
-    row_ml[warp][r0 + 8] = make_float2(top1, l1);
+    row_ml[warp][r0] = make_float2(ref0, l0);
+    row_ml[warp][r0 + 8] = make_float2(ref1, l1);
   }
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) {

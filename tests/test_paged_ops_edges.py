@@ -81,3 +81,105 @@ def test_beam_select_highest_logits(jal, torch_cuda, dtype, vocab):
     logits = logits.to(NAMES[dtype])
     cum = torch.randn(1, 4, generator=g) - 10
     check_continuations(select(jal, logits, cum, 1, 4, 8), logits, cum, 1, 4, 8)
+
+
+# ---- attention: one key far above a flat tail --------------------------------------
+def flat_rows(act, cache, new, length, group=4, jitter=0.0):
+    """Rows of ones whose scores are about 0: keys of 0, or of `jitter`."""
+    hd, hkv = 64, 2
+    c = Case([length], [new], group * hkv, hkv, hd, act, cache, 64, seed=new + length)
+    g = torch.Generator().manual_seed(length)
+    c.q_full.fill_(1.0)
+    c.q = c.q_full.view(c.n_rows, group * hkv, hd)
+    c.k[0] = (torch.randn(length, hkv, hd, generator=g) * jitter).to(c.cache)
+    c.v[0] *= 256.0  # (f16: the result is then no subnormal)
+    pages, slots = c.table[0, torch.arange(length) // 64].long(), torch.arange(length) % 64
+    for pool, rows in zip(c.pools, (c.k, c.v)):
+        pool.permute(c.perm)[pages, :, slots] = rows[0]
+    return c
+
+
+def lift(c, at, gap):
+    """Puts the key at `at` `gap` above the others; its value is 0, so the result is made of the tail."""
+    for pool, rows, x in ((c.pools[0], c.k, gap / 8), (c.pools[1], c.v, 0.0)):  # 64 dims, scale 1/8: rounded to the cache's type
+        rows[0][at] = x
+        pool.permute(c.perm)[int(c.table[0, at // 64]), :, at % 64] = rows[0][at]
+    return c
+
+
+def tail_reference(c):
+    """(out, largest weight * sum |v|, sum of weight * |v|) of every row, in 64 bits; rows differ in what they see alone."""
+    new, group = c.news[0], c.hq // c.hkv
+    last = torch.arange(c.lens[0] - new, c.lens[0])  # the last key that each row sees; all see the largest
+    out, floor, mag = (torch.zeros(new, c.hq, c.hd, dtype=torch.float64) for _ in range(3))
+    for h in range(c.hkv):
+        k, v = c.k[0][:, h].double(), c.v[0][:, h].double()
+        w = (k.sum(-1) / 8 - (k.sum(-1) / 8).max()).exp()[:, None]
+        total = w.cumsum(0)[last]
+        for x, y in ((out, w * v), (mag, w * v.abs()), (floor, v.abs())):
+            x[:, h * group:(h + 1) * group] = (y.cumsum(0)[last] / total)[:, None]
+    return out, floor, mag
+
+
+def lost_bits(c):
+    """Half of f16's smallest step over the largest weight: up to 64 rows that share their keys go to mma.sync."""
+    return 2.0 ** -25 / 2.0 ** (15 if c.news[0] * c.hq // c.hkv <= 64 else 11)
+
+
+GAPS = [8.0, 10.0, 12.0, 13.0, 14.0, 16.0, 17.4, 20.0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f16", "f16"), ("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("new", [1, 20, 40, 70])  # mma.sync; tcgen05 with both row tiles on the same rows, and with two
+@pytest.mark.parametrize("at", [0, 2000])
+@pytest.mark.parametrize("jitter", [0.0, 0.03125])
+def test_attention_one_key_above_the_tail(jal, torch_cuda, act, cache, new, at, jitter):
+    """The keys far below a row's maximum keep their share of the result.
+
+    The bound, of sum p |v|: a score is off by 64 products and the scaling in f32 (its terms are at most `top` in
+    all: 2 * 70 * 2^-24 * top in the exponent, numerator and denominator), exp2 by 2^-22, weights in two f16 parts
+    by 2^-22 and in three bf16 parts by 2^-23, in one part by half a step.  Sums: a warp or a tile adds 16 keys at
+    a time, 256 times at most, and then 64 warps' and pieces' results, each addition to the last unit (2^-23; the
+    matrix units need not round to nearest).  f16 has no bits below 2^-24 and the largest weights are 2^15 on mma.sync
+    and 2^11 at least on tcgen05: each key is off by up to 2^-40 or 2^-36 of the row's largest weight.  Then the
+    result's own rounding.
+    """
+    e = 2.0 ** -24
+    c = flat_rows(act, cache, new, 4097, jitter=jitter)
+    for gap in GAPS:
+        lift(c, at, gap).to_device(jal)
+        out, floor, mag = tail_reference(c)
+        got = attend(jal, c, 0.125)[:new, :c.hq * c.hd].view(new, c.hq, c.hd).double()
+        top = max(gap, 64 * 4.5 * jitter)  # (sums of |q| |k| / 8: what the score's roundings are relative to)
+        part = half_step(c.act) if act != "f32" else 4 * e
+        rough = 2 * 70 * e * top + 4 * e + part + 2 * (256 + 64) * 2 * e
+        lim = rough * mag + (lost_bits(c) * floor if cache == "f16" else 0.0)
+        lim = lim + half_step(c.act) * (out.abs() + lim + torch.finfo(c.act).smallest_normal)
+        off = (got - out).abs()
+        assert (off <= lim).all(), f"gap {gap}: {float((off / lim).max()):.3f} of the bound, {float((off / mag).max()):.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 20, 70])
+def test_attention_f32_rows_use_both_parts(jal, torch_cuda, new):
+    """f32 rows over an f16 cache: weights that one f16 part would put a quarter of a step off or more.
+
+    Flat keys have one weight, so its rounding to one part would not average out.  The gaps are chosen by that
+    rounding, 2^-12 at least of the weight whatever power of two it is scaled by; the bound is that of the test
+    above without a dominant score to round (the tail's scores are 0)."""
+    e = 2.0 ** -24
+    found, c = 0, flat_rows("f32", "f16", new, 1025)
+    for i in range(65):
+        gap = 4.0 + i / 8
+        w = torch.tensor(math.exp(-gap) * 2.0 ** 13, dtype=torch.float64)
+        if abs(float(w.half().double() / w - 1)) < 2.0 ** -12:
+            continue
+        found += 1
+        lift(c, 0, gap).to_device(jal)
+        out, floor, mag = tail_reference(c)
+        got = attend(jal, c, 0.125)[:new, :c.hq * c.hd].view(new, c.hq, c.hd).double()
+        lim = (2 * 3 * e * gap + 8 * e + 2 * (64 + 16) * 2 * e) * mag + lost_bits(c) * floor + 2.0 ** -24 * out.abs()
+        assert (lim <= 2.0 ** -13 * mag).all()  # one part alone could not meet it
+        assert ((got - out).abs() <= lim).all(), (gap, float(((got - out).abs() / mag).max()))
+    assert found >= 6
