@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
   const RowSpan m1 = r0 + 8 < t.rows ? row_span(p, t, masks[r0 + 8]) : every;
   const float f0 = q_scale[r0], f1 = q_scale[r0 + 8];
   const RowMask mine = masks[lane < t.rows ? lane : 0];  // (a tile has a row)
-  const bool mixed = __any_sync(0xffffffffu, mine.lim != masks[0].lim || mine.wlo != masks[0].wlo);
+  // Are there keys of the tile that some row does not see?  Rows that see the same see all
+  // of it, but for a shared prefix, which goes on behind rows inside it.
+  const bool mixed = __any_sync(0xffffffffu, mine.lim != masks[0].lim || mine.wlo != masks[0].wlo || mine.lim < t.hi);
   float o[HD / 8][4];
 #pragma unroll
   for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<NS, HD>::blocks) k_paged
         }
       }
     }
-    if (masked && mixed) {  // a value that some rows must not meet
+    if (masked && mixed) {  // a value that some row must not meet
 #pragma unroll
       for (int i = 0; i < kMmaKeys * S::chunks / 32; i++) {
         uint4 w;

@@ -63,7 +63,7 @@ struct TcSync {
   uint64_t s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
   int given_up, poison;
-  int lim_lo, lim_hi, wlo_lo, wlo_hi;
+  int lim_lo, wlo_lo, wlo_hi;  // of the tile's rows: the least end, the least and largest window start
   // Of a row's halves: the largest score of the key tile, and at the end the sum
   // of the weights.  Before the first tile: what a row's scores are still to be
   // multiplied by (NS = 2, [256]).  Barriers lie between these uses.
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
     }
     sy.given_up = sy.poison = 0;
     sy.lim_lo = sy.wlo_lo = 0x7fffffff;
-    sy.lim_hi = sy.wlo_hi = 0;
+    sy.wlo_hi = 0;
     fence_barrier_init();
   }
   if (warp == 19) {
@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
           ranges = true;
         }
         const int u = t.u0 + j * kTcKeys, first = t.key(u), last = t.key(min(u + kTcKeys, t.u1) - 1);
-        const bool mixed = (first < sy.wlo_hi && sy.wlo_lo != sy.wlo_hi) || (last >= sy.lim_lo && sy.lim_lo != sy.lim_hi);
+        // (Rows of one window's start have no keys between the first positions and it.)
+        const bool mixed = (first < sy.wlo_hi && sy.wlo_lo != sy.wlo_hi) || last >= sy.lim_lo;
         scan_b = mixed ? vb : -1;
       }
       copies_wait<0>();
@@ -493,14 +494,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
         tile_sync();
         scale *= (&sy.x[0][0][0])[i * 128 + r];
       }
-      int lo = real ? mk.lim : 0x7fffffff, hi = real ? mk.lim : 0, wl = real ? mk.wlo : 0x7fffffff, wh = real ? mk.wlo : 0;
+      int lo = real ? mk.lim : 0x7fffffff, wl = real ? mk.wlo : 0x7fffffff, wh = real ? mk.wlo : 0;
       lo = __reduce_min_sync(0xffffffffu, lo);
-      hi = __reduce_max_sync(0xffffffffu, hi);
       wl = __reduce_min_sync(0xffffffffu, wl);
       wh = __reduce_max_sync(0xffffffffu, wh);
       if (lane == 0) {
         atomicMin(&sy.lim_lo, lo);
-        atomicMax(&sy.lim_hi, hi);
         atomicMin(&sy.wlo_lo, wl);
         atomicMax(&sy.wlo_hi, wh);
       }

@@ -183,3 +183,28 @@ def test_attention_f32_rows_use_both_parts(jal, torch_cuda, new):
         assert (lim <= 2.0 ** -13 * mag).all()  # one part alone could not meet it
         assert ((got - out).abs() <= lim).all(), (gap, float(((got - out).abs() / mag).max()))
     assert found >= 6
+
+
+# ---- shared prefixes: values at prefix positions that a row does not see -----------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("hq,new", [(16, 2), (256, 10)])  # tiles of one token's heads: mma.sync, tcgen05
+def test_shared_prefix_poison_behind_a_row(jal, torch_cuda, hq, new, act, cache, bad):
+    """New rows inside the shared prefix, each tile full of one token's heads, so that its rows see the same keys, and
+    fewer than the prefix has."""
+    prefix, poisoned, length = 400, 399, 400 if new == 2 else 404
+    c = share(Case([length, 420], [new, 1], hq, 1, 64, act, cache, 16, seed=hq), [0, 2], [prefix])
+    clean = c.reference(0.125)
+    lim = c.bound(clean)
+    c.pools[1].permute(c.perm)[int(c.table[0, poisoned // 16]), :, poisoned % 16, 5] = bad
+    c.to_device(jal)
+    c.d_table[1, :prefix // 16] = c.d_table[0, :prefix // 16]
+    out = shared(jal, c, [0, 2], [prefix], 0.125)
+    n, blind = new + 1, poisoned - (length - new)
+    assert 0 < blind < new
+    got = out[:n, :hq * 64].view(n, hq, 64).double()
+    ok = (got - clean[0][:n]).abs() <= lim[:n]
+    assert ok[:blind].all()
+    rest = [d for d in range(64) if d != 5]
+    assert ok[blind:][..., rest].all() and not got[blind:, :, 5].isfinite().any()
