@@ -331,7 +331,9 @@ int jal_op_beam_select_workspace(size_t n_seqs, size_t n_beams, size_t vocab,
  * that takes position new_len[r], then -1.  That page is p's own unfinished
  * page for the first row that continues p, and fresh_pages[r] for the others,
  * with the unfinished page's filled slots copied in every layer; where p has
- * no unfinished page it is fresh_pages[r] for every row.  Row r of a parent
+ * no unfinished page it is fresh_pages[r] for every row, and where p's table
+ * has no page for its unfinished one (an entry outside [0, n_pages)) that entry
+ * is every row's, so that those positions stay masked.  Row r of a parent
  * outside [0, n_beams) becomes empty.  fresh_pages: [n_seqs * n_beams]
  * distinct pages that no row uses; the caller takes back those that new_table
  * does not name.  Layer i of the pools starts i * layer_stride elements

@@ -406,14 +406,15 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_reorder(const __grid_const
   const int len = min(max(p.kv_len[source], 0), kv.cap);
   const int full = len / kv.page_size, fill = len - full * kv.page_size;
   const int from = fill ? old[full] : -1;  // (a table that is full has no unfinished page)
-  const bool takes = !heir || fill == 0;
+  // A row that is not the first takes a page of its own; where the unfinished page
+  // is missing there is nothing to copy, and its positions stay without one.
+  const bool whole = fill == 0, takes = whole || (!heir && (unsigned)from < (unsigned)kv.n_pages);
   if (layer == 0) {
     for (int j = tid; j < kv.max_pages; j += kRowThreads)
       out[j] = j < full ? old[j] : j > full ? -1 : takes ? to : from;
     if (tid == 0) p.new_len[row] = len;
   }
-  if (!takes || fill == 0) return;
-  if ((unsigned)from >= (unsigned)kv.n_pages || (unsigned)to >= (unsigned)kv.n_pages) return;
+  if (!takes || whole || (unsigned)to >= (unsigned)kv.n_pages) return;
   const int heads = 2 * kv.hkv;
   auto place = [&](int h, int page) {  // byte offset of head h (of K, then of V) in a page of this layer
     return (layer * p.layer_stride + (h >= kv.hkv ? h - kv.hkv : h) * kv.head_stride + page * kv.page_stride) * elem;

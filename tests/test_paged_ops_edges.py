@@ -208,3 +208,24 @@ def test_shared_prefix_poison_behind_a_row(jal, torch_cuda, hq, new, act, cache,
     assert ok[:blind].all()
     rest = [d for d in range(64) if d != 5]
     assert ok[blind:][..., rest].all() and not got[blind:, :, 5].isfinite().any()
+
+
+# ---- reordering: a parent whose unfinished page is missing ---------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("hole", [-1, 999])
+def test_beam_reorder_missing_unfinished_page(jal, torch_cuda, hole):
+    """Positions without a page stay without one for every child; no fresh page takes their place."""
+    page, hkv, hd, layers = 16, 2, 24, 2
+    g = torch.Generator().manual_seed(1)
+    table = torch.tensor([[0, 1, hole, -1], [3, 4, 5, -1], [6, 7, 8, -1]], dtype=torch.int32)
+    fresh = torch.tensor([9, 10, 11], dtype=torch.int32)
+    pools = [torch.randn(layers, 12, hkv, page, hd, generator=g) for _ in range(2)]
+    d_pools = [p.to(DEV) for p in pools]
+    kv = jal.PagedKv(*d_pools, table.to(DEV), dtype=jal.F32, n_pages=12, page_size=page, n_heads_kv=hkv, head_dim=hd,
+                     n_seqs=3, max_pages=4)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    new_table, new_len = ints([[55] * 4] * 3), ints([55] * 3)
+    jal.beam_reorder(kv, ints([40, 40, 40]), ints([[0, 0, 0]]), fresh.to(DEV), new_table, new_len, 1, 3, n_layers=layers)
+    assert new_table.cpu().tolist() == [[0, 1, hole, -1]] * 3 and new_len.cpu().tolist() == [40] * 3
+    for a, b in zip(d_pools, pools):
+        assert torch.equal(a.cpu(), b)
