@@ -54,21 +54,6 @@ __device__ __forceinline__ void rotated8(const TA *row, int d, int rotary, int n
   }
 }
 
-// The sequence in [0, n) that holds row r, found by the whole warp: 32 starts at
-// a time, so two rounds for 1024 sequences instead of ten dependent loads.
-__device__ __forceinline__ int warp_seq_of_row(const int32_t *q_start, int n, int r) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = n;  // q_start[lo] <= r (or lo = 0)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + step * lane;
-    const bool before = lane > 0 && at < hi && __ldg(q_start + at) <= r;
-    const int k = __popc(__ballot_sync(0xffffffffu, before));
-    lo += step * k;
-    hi = min(hi, lo + step);
-  }
-  return lo;
-}
-
 // rotary_dim a multiple of 16 (or 0): a warp takes part of a token row's heads,
 // item by item.  An item is eight dims and, in the rotated part, the eight
 // rotary_dim / 2 further on, so both of a pair's elements are in one lane

@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(kF32Threads) k_paged_attn_f32(const __grid_con
 // One block for each (token row, query head): the pieces' sums rescaled to the
 // largest of their maxima and added, each warp every fourth piece with eight
 // pieces' loads under way, the warps in order at the end.  A piece without a
-// visible key has sum 0 and is not read.
+// visible key has sum 0 and is not read.  Whose row it is, is looked up before the
+// wait for the pieces: the batch was there before the launch that makes them.
 constexpr int kJoinWarps = 4, kJoinThreads = kJoinWarps * 32;
 static_assert(2 * kPagedMaxSplits <= kJoinThreads, "a thread looks at one piece's maximum and sum");
 
@@ -210,9 +211,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(const __grid_c
   __shared__ float weight[kJoinThreads];
   __shared__ float red[kJoinWarps];
   __shared__ float4 part[kJoinWarps][kPagedMaxHeadDim / 4];
-  pdl_wait();
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, head = blockIdx.x % p.hq;
-  const int tok = blockIdx.x / p.hq, s = tok / p.max_q, i = tok - s * p.max_q;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, head = blockIdx.x % p.hq, row = blockIdx.x / p.hq;
+  const int batch_first = __ldg(p.q_start), batch_last = __ldg(p.q_start + p.n_seqs);
+  const int s = warp_seq_of_row(p.q_start, p.n_seqs, row);
   int g_first = 0, g_last = 0, g_row = 0, beg, end;
   if (p.prefix_splits) {
     const int g = seq_of_row(p.group_start, 0, p.n_groups, s);
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(const __grid_c
     g_row = __ldg(p.q_start + min(max(g_first, 0), p.n_seqs));
   }
   seq_rows(p.q_start, p.n_rows, s, beg, end);
-  if (i >= end - beg) return;
-  const int row = beg + i;
+  pdl_wait();
+  if (row < batch_first || row >= batch_last || row < beg || row >= end || row - beg >= p.max_q) return;
   int first = p.prefix_splits;  // a sequence outside every group has its own keys alone
   if (g_first <= s && s < g_last) {
     first = 0;
@@ -388,7 +389,9 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
   AttnPlan a = {};
   const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv;
   const int64_t pairs = (int64_t)b.max_q_len * G;
-  const int64_t group_pairs = g ? (int64_t)g->max_group * pairs : 0;
+  // (A group has no more rows than the batch: one long prompt among single rows.)
+  const int64_t group_rows = g ? std::min<int64_t>((int64_t)g->max_group * (int64_t)b.max_q_len, (int64_t)b.n_rows) : 0;
+  const int64_t group_pairs = group_rows * G;
   // Which kernel: f32 caches on the CUDA cores; 16-bit ones on mma.sync in
   // tiles of 16 rows, or on tcgen05 in tiles of 256 where enough rows share
   // their keys (three bf16 parts of f32 rows, and head dims above 128, do not
@@ -439,7 +442,7 @@ void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) 
     run_16bit_hd<__nv_bfloat16, 3>(p, plan, s);
   }
   if (plan.direct) return;
-  launch(k_paged_attn_join, (int64_t)p.n_seqs * p.max_q * p.hq, kJoinThreads, 0, true, s, p, plan.prefix_rows);
+  launch(k_paged_attn_join, (int64_t)p.n_rows * p.hq, kJoinThreads, 0, true, s, p, plan.prefix_rows);
 }
 
 }  // namespace jal

@@ -143,6 +143,21 @@ __device__ __forceinline__ int seq_of_row(const int32_t *q_start, int lo, int hi
   return lo;
 }
 
+// The sequence in [0, n) that holds row r, found by the whole warp: 32 starts at
+// a time, so two rounds for 1024 sequences instead of ten dependent loads.
+__device__ __forceinline__ int warp_seq_of_row(const int32_t *q_start, int n, int r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;  // q_start[lo] <= r (or lo = 0)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + step * lane;
+    const bool before = lane > 0 && at < hi && __ldg(q_start + at) <= r;
+    const int k = __popc(__ballot_sync(0xffffffffu, before));
+    lo += step * k;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
 // One tile of query rows of one KV head, and the keys it reads.  Tile row j
 // is row (first + j) of the (token, head-of-group) pairs counted from token
 // row `beg`.  Its keys are the positions [0, ns) and [lo, hi), numbered

@@ -229,3 +229,47 @@ def test_beam_reorder_missing_unfinished_page(jal, torch_cuda, hole):
     assert new_table.cpu().tolist() == [[0, 1, hole, -1]] * 3 and new_len.cpu().tolist() == [40] * 3
     for a, b in zip(d_pools, pools):
         assert torch.equal(a.cpu(), b)
+
+
+# ---- shared prefixes: one long prompt among single rows ------------------------------
+def test_shared_prefix_of_a_long_prompt_is_not_refused(jal):
+    """Work goes by the rows that there are, not by the longest sequence's times all sequences."""
+    kv = _view(jal, n_heads_kv=8, head_dim=128, n_seqs=256, page_size=64, max_pages=4096, n_pages=1 << 16)
+    batch = _batch(jal, n_seqs=256, n_rows=131072 + 255, max_q_len=131072, max_kv_len=200000)
+    groups = jal.PrefixGroups(4096, 4096, 1, 256, 60000)
+    need = jal.shared_prefix_attention_workspace(kv, batch, groups, 64, dtype=jal.F16)
+    with pytest.raises(jal.K3Error) as e:  # (the addresses are none)
+        jal.shared_prefix_attention(kv, batch, groups, 4096, 4096, 64, 0.1, dtype=jal.F16, workspace=4096, workspace_len=need)
+    assert e.value.code != jal.ERR_CAPABILITY_MISMATCH, str(e.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("at", [0, 17, 39])
+def test_shared_prefix_one_long_prompt_among_single_rows(jal, torch_cuda, act, cache, at):
+    lens, news = [330 + i for i in range(40)], [1] * 40
+    lens[at], news[at] = 500, 150
+    news[(at + 5) % 40] = 0
+    c = share(Case(lens, news, 8, 2, 64, act, cache, 16, seed=at, spare_rows=9), [0, 30, 40], [320, 300]).to_device(jal)
+    check(c, shared(jal, c, [0, 30, 40], [320, 300], 0.125), 0.125)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("bf16", "bf16"), ("f32", "f32")])
+def test_joined_rows_of_an_offset_batch(jal, torch_cuda, act, cache):
+    """Pieces are joined for the rows of the batch alone: not before its first, not past max_q_len, not behind its last."""
+    c = Case([3000, 0, 2500, 40], [1, 0, 3, 2], 8, 2, 64, act, cache, 64, seed=5)
+    ref = c.reference(0.125)
+    lim = c.bound(ref)
+    c.q_start += 4
+    c.q_full = torch.cat([torch.full((4, c.q_stride), 7.0, dtype=c.act), c.q_full])
+    c.n_rows += 4
+    c.to_device(jal)
+    c.batch = jal.RaggedBatch(c.d_q_start, c.d_kv_len, n_seqs=4, n_rows=c.n_rows, max_q_len=2, max_kv_len=3000)
+    need = jal.paged_attention_workspace(c.kv, c.batch, 8, dtype=c.act_type)
+    assert need
+    out = attend(jal, c, 0.125)
+    assert (out[:4] == 7).all() and (out[10:] == 7).all() and (out[:, 512:] == 7).all()
+    got = out[4:10, :512].view(6, 8, 64).double()
+    ok = (got - ref[0][:6]).abs() <= lim[:6]
+    assert ok[[0, 1, 2, 4, 5]].all() and (out[7, :512] == 7).all()  # (the third of three rows, of two at most)
