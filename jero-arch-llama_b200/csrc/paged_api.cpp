@@ -38,6 +38,11 @@ int current_device() {
 void aligned16(const void *p, const char *what) {
   if ((uintptr_t)p % 16) fail(JAL_ERR_TENSOR_BOUNDS, "%s is not 16-byte aligned", what);
 }
+// Arrays that kernels read and write as 4-byte values: an address between two of
+// them would fault.
+void aligned4(const void *p, const char *what) {
+  if ((uintptr_t)p % 4) fail(JAL_ERR_TENSOR_BOUNDS, "%s is not 4-byte aligned", what);
+}
 
 // A cache view with its defaults filled in.
 jal_paged_kv checked_kv(const jal_paged_kv *in) {
@@ -70,6 +75,7 @@ jal_paged_kv checked_kv(const jal_paged_kv *in) {
     fail(JAL_ERR_TENSOR_BOUNDS, "paged cache stride above 2^40");
   aligned16(kv.k, "k pool");
   aligned16(kv.v, "v pool");
+  aligned4(kv.page_table, "page_table");
   return kv;
 }
 
@@ -99,6 +105,8 @@ jal_ragged_batch checked_batch(const jal_ragged_batch *in, const jal_paged_kv &k
   jal_ragged_batch b = *in;
   NEED(b.q_start);
   NEED(b.kv_len);
+  aligned4(b.q_start, "q_start");
+  aligned4(b.kv_len, "kv_len");
   if (b.n_seqs > kv.n_seqs)
     fail(JAL_ERR_TENSOR_BOUNDS, "batch of %llu sequences over a table of %llu", (unsigned long long)b.n_seqs,
          (unsigned long long)kv.n_seqs);
@@ -134,6 +142,8 @@ jal_prefix_groups checked_groups(const jal_prefix_groups *in, const jal_paged_kv
   if (g.n_groups) {
     NEED(g.group_start);
     NEED(g.prefix_len);
+    aligned4(g.group_start, "group_start");
+    aligned4(g.prefix_len, "prefix_len");
   }
   if (g.n_groups > kMaxInt) fail(JAL_ERR_TENSOR_BOUNDS, "more than 2^31 groups");
   g.max_group = std::min<uint64_t>(g.max_group, b.n_seqs);
@@ -235,7 +245,10 @@ int jal_op_rope_kv_append(const jal_paged_kv *kv_in, const jal_ragged_batch *bat
     NEED(v);
     if (rotary_dim % 2 || rotary_dim > kv.head_dim)
       fail(JAL_ERR_CAPABILITY_MISMATCH, "rotary_dim %zu of head_dim %llu", rotary_dim, (unsigned long long)kv.head_dim);
-    if (rotary_dim) NEED(inv_freq);
+    if (rotary_dim) {
+      NEED(inv_freq);
+      aligned4(inv_freq, "inv_freq");
+    }
     AppendParams p = {};
     p.kv = view_of(kv);
     p.kv_stride = row_stride(kv_stride, kv.n_heads_kv * kv.head_dim, "k / v");
@@ -357,6 +370,10 @@ int jal_op_beam_select(const void *logits, int dtype, size_t row_stride_in, cons
     NEED(scores);
     NEED(parents);
     NEED(tokens);
+    aligned4(cum, "cum");
+    aligned4(scores, "scores");
+    aligned4(parents, "parents");
+    aligned4(tokens, "tokens");
     if (!float_type(dtype)) fail(JAL_ERR_CAPABILITY_MISMATCH, "logits of type %d", dtype);
     check_beams(n_seqs, n_beams, vocab, k);
     const size_t stride = row_stride_in ? row_stride_in : vocab;
@@ -411,6 +428,11 @@ int jal_op_beam_reorder(const jal_paged_kv *kv_in, size_t n_layers, size_t layer
     NEED(fresh_pages);
     NEED(new_table);
     NEED(new_len);
+    aligned4(kv_len, "kv_len");
+    aligned4(parents, "parents");
+    aligned4(fresh_pages, "fresh_pages");
+    aligned4(new_table, "new_table");
+    aligned4(new_len, "new_len");
     if (n_beams == 0 || n_layers == 0 || n_layers > 65535)
       fail(JAL_ERR_TENSOR_BOUNDS, "%zu beams in %zu layers", n_beams, n_layers);
     if (n_beams > kMaxInt || n_seqs > kMaxInt || n_seqs * n_beams > kv.n_seqs)

@@ -273,3 +273,31 @@ def test_joined_rows_of_an_offset_batch(jal, torch_cuda, act, cache):
     got = out[4:10, :512].view(6, 8, 64).double()
     ok = (got - ref[0][:6]).abs() <= lim[:6]
     assert ok[[0, 1, 2, 4, 5]].all() and (out[7, :512] == 7).all()  # (the third of three rows, of two at most)
+
+
+# ---- refusals ---------------------------------------------------------------------
+def test_index_arrays_off_their_alignment_are_refused(jal):
+    """Arrays that kernels read as 4-byte values: an address between two of them would fault."""
+    ok = dict(q=4096, out=8192, n_heads_q=4, scale=0.1, dtype=jal.F16)
+    groups = dict(group_start=4096, prefix_len=4096, n_groups=1, max_group=3, max_prefix_len=10)
+    beams = dict(logits=4096, cum=4096, scores=8192, parents=4096, tokens=4096, n_seqs=2, n_beams=3, vocab=100, k=3,
+                 workspace=4096, workspace_len=1 << 20)
+    append = dict(k=4096, v=4096, inv_freq=4096, dtype=jal.F16, rotary_dim=64)
+    order = dict(kv_len=4096, parents=4096, fresh_pages=4096, new_table=4096, new_len=8192, n_seqs=1, n_beams=3)
+    calls = [lambda f=f, v=v, b=b: f(jal, v, b) for f in (
+        lambda j, v, b: j.paged_attention(v, b, **ok),
+        lambda j, v, b: j.shared_prefix_attention(v, b, j.PrefixGroups(**groups), **ok),
+        lambda j, v, b: j.rope_kv_append(v, b, **append)) for v, b in (
+        (_view(jal, page_table=12290), _batch(jal)), (_view(jal), _batch(jal, q_start=16385)),
+        (_view(jal), _batch(jal, kv_len=20482)))]
+    calls += [lambda n=n: jal.shared_prefix_attention(_view(jal), _batch(jal), jal.PrefixGroups(**{**groups, n: 4098}), **ok)
+              for n in ("group_start", "prefix_len")]
+    calls.append(lambda: jal.rope_kv_append(_view(jal), _batch(jal), **{**append, "inv_freq": 4097}))
+    calls += [lambda n=n: jal.beam_select(**{**beams, n: 4098}) for n in ("cum", "scores", "parents", "tokens")]
+    calls += [lambda n=n: jal.beam_reorder(_view(jal), **{**order, n: 4098})
+              for n in ("kv_len", "parents", "fresh_pages", "new_table", "new_len")]
+    calls.append(lambda: jal.beam_reorder(_view(jal, page_table=12289), **order))
+    for i, call in enumerate(calls):
+        with pytest.raises(jal.K3Error) as e:
+            call()
+        assert e.value.code == jal.ERR_TENSOR_BOUNDS and "aligned" in str(e.value), (i, str(e.value))
