@@ -220,8 +220,9 @@ typedef struct jal_paged_kv {
  * the others at the positions before.  A sequence may have no row.  Rows
  * before q_start[0] and from q_start[n_seqs] on belong to none and are left
  * as they were, as are, in attention, a sequence's rows past the first
- * max_q_len.  A row before position 0 is not appended and sees nothing; one
- * past the table's last position is not appended and sees what that sees. */
+ * max_q_len.  A row before position 0 is not appended, its queries are not
+ * rotated, and it sees nothing; one past the table's last position is not
+ * appended and sees what that sees. */
 typedef struct jal_ragged_batch {
   const int32_t *q_start; /* [n_seqs + 1] */
   const int32_t *kv_len;  /* [n_seqs], the new rows included */

@@ -17,7 +17,7 @@ constexpr int kAppendThreads = 256;
 // cos and sin of pos * inv_freq with the product formed in 64 bits: at
 // position 10^5 a product rounded to f32 is off by 4e-3 radians.  The angle is
 // reduced to [-pi, pi] in 64 bits and rounded once, to f32.
-__device__ __forceinline__ float2 turn(int pos, float inv_freq) {
+__device__ __forceinline__ float2 turn(int64_t pos, float inv_freq) {
   const double a = (double)pos * (double)inv_freq;
   const double r = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
   float2 cs;
@@ -122,11 +122,13 @@ __global__ void __launch_bounds__(kWarps * 32, 7) k_rope_kv_append_pairs(const _
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   const int64_t pos64 = (int64_t)__ldg(p.kv_len + s) - (end - row);
-  if (pos64 < 0 || pos64 >= p.kv.cap) return;
-  const int pos = (int)pos64, hd = p.kv.hd, half = p.rotary / 2;
-  const int64_t at = slot_offset(p.kv, p.kv.table + (int64_t)s * p.kv.max_pages, 0, pos);
+  if (pos64 < 0) return;
+  const int hd = p.kv.hd, half = p.rotary / 2;
+  // (Past the table, and without a page, there is no place for the row's k and v; its
+  // queries are turned all the same.)
+  const int64_t at = pos64 >= p.kv.cap ? -1 : slot_offset(p.kv, p.kv.table + (int64_t)s * p.kv.max_pages, 0, (int)pos64);
   float2 *const cs = turns[warp];
-  for (int i = lane; i < half; i += 32) cs[i] = turn(pos, __ldg(p.inv_freq + i));
+  for (int i = lane; i < half; i += 32) cs[i] = turn(pos64, __ldg(p.inv_freq + i));
   __syncwarp();
   const int nq = p.q ? p.hq : 0, items = half / 8 + (hd - p.rotary) / 8, total = (nq + 2 * p.kv.hkv) * items;
   const int per = (total + parts - 1) / parts, stop = min(total, (part + 1) * per);
@@ -183,9 +185,8 @@ __global__ void __launch_bounds__(kAppendThreads) k_rope_kv_append(const AppendP
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   const int64_t pos64 = (int64_t)p.kv_len[s] - (end - row);
-  if (pos64 < 0 || pos64 >= p.kv.cap) return;
-  const int pos = (int)pos64;
-  for (int i = threadIdx.x; i < p.rotary / 2; i += kAppendThreads) cs[i] = turn(pos, p.inv_freq[i]);
+  if (pos64 < 0) return;
+  for (int i = threadIdx.x; i < p.rotary / 2; i += kAppendThreads) cs[i] = turn(pos64, p.inv_freq[i]);
   __syncthreads();
   // A head's row belongs to `lanes` neighbouring lanes, eight elements each.
   // Every lane has read what it needs (its partners' elements too) before any
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_rope_kv_append(const AppendP
     if (is_q) {
       store8((TA *)p.q_out + row * p.q_out_stride + h * hd + d, v);
     } else {
-      const int64_t at = slot_offset(p.kv, table, h, pos);
+      const int64_t at = pos64 >= p.kv.cap ? -1 : slot_offset(p.kv, table, h, (int)pos64);
       if (at >= 0) store8((TK *)(is_k ? p.kw : p.vw) + at + d, v);
     }
   }

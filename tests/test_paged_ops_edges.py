@@ -301,3 +301,33 @@ def test_index_arrays_off_their_alignment_are_refused(jal):
         with pytest.raises(jal.K3Error) as e:
             call()
         assert e.value.code == jal.ERR_TENSOR_BOUNDS and "aligned" in str(e.value), (i, str(e.value))
+
+
+# ---- append: rows past the table -----------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [64, 40])  # both kernels
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_past_the_table_still_turns_the_queries(jal, torch_cuda, rotary, in_place):
+    """A row past the table's last position is not appended, and its queries are turned by its position all the same."""
+    page, hd, hq = 4, 64, 3
+    pools = [torch.zeros(3, 1, page, hd, device=DEV) for _ in range(2)]
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    kv = jal.PagedKv(*pools, ints([[0, 1], [2, -1]]), dtype=jal.F32, n_pages=3, page_size=page, n_heads_kv=1, head_dim=hd,
+                     n_seqs=2, max_pages=2)
+    g = torch.Generator().manual_seed(rotary)
+    x, q = torch.randn(7, hd, generator=g), torch.randn(7, hq, hd, generator=g)
+    lens = [10, 6]  # positions 6 .. 9 of 8, and 4, 5 of which the page is missing
+    inv_freq = (10000.0 ** (-torch.arange(rotary // 2, dtype=torch.float64) / (rotary // 2))).float()
+    d_q = q.to(DEV)
+    q_out = d_q if in_place else torch.full((7, hq, hd), 7.0, device=DEV)
+    jal.rope_kv_append(kv, jal.RaggedBatch(ints([0, 4, 6]), ints(lens), 2, 7, 4, 10), x.to(DEV), x.to(DEV), inv_freq.to(DEV),
+                       dtype=jal.F32, rotary_dim=rotary, q=d_q, q_out=q_out, n_heads_q=hq)
+    rough = 2.0 ** -21 + 3 * 2.0 ** -24  # cos and sin within 2^-21, two products and an addition
+    for r, pos in enumerate([6, 7, 8, 9, 4, 5]):
+        want = turned(q[r], pos, inv_freq, rotary, False)
+        lim = rough * math.sqrt(2) * q[r].abs().amax() + half_step(torch.float32) * want.abs()
+        assert ((q_out[r].cpu().double() - want).abs() <= lim).all(), r
+    assert torch.equal(q_out[6].cpu(), q[6] if in_place else torch.full((hq, hd), 7.0))
+    want = torch.zeros(3, 1, page, hd)
+    want[1, 0, 2], want[1, 0, 3] = x[0], x[1]
+    assert torch.equal(pools[1].cpu(), want)
