@@ -250,7 +250,7 @@ typedef struct jal_prefix_groups {
  * rotate(q row).  k and v rows are [n_heads_kv][head_dim] of `dtype`, kv_stride
  * elements apart; q rows [n_heads_q][head_dim], q_stride / q_out_stride
  * elements apart (0 = dense; slices of one fused projection row are strided);
- * q_out may be q.  dtype is the cache's or JAL_F32.  The first rotary_dim
+ * q_out may be q with the same stride.  dtype is the cache's or JAL_F32.  The first rotary_dim
  * dims are rotated (0 = none, iRoPE layers): neox = 0 pairs (2i, 2i + 1), 1
  * pairs (i, i + rotary_dim / 2), by position * inv_freq[i] (device,
  * rotary_dim / 2 floats).  That angle is formed in 64 bits; jal_op_rope and
@@ -277,7 +277,7 @@ int jal_op_rope_kv_append(const jal_paged_kv *kv, const jal_ragged_batch *batch,
  * (bf16).  Over an f16 cache a weight is further off by up to 2^-36 of the
  * row's largest, which shows where one position lies 14 nats or more above the
  * ones that make the result.  n_heads_q is a multiple of n_heads_kv.  Strides
- * as in jal_op_rope_kv_append; out may be q.
+ * as in jal_op_rope_kv_append; out may be q with the same stride.
  * The workspace has to be as large as jal_op_paged_attention_workspace says
  * for the same arguments (JAL_ERR_TENSOR_BOUNDS), 16-byte aligned. */
 int jal_op_paged_attention(const jal_paged_kv *kv, const jal_ragged_batch *batch,

@@ -331,3 +331,19 @@ def test_append_past_the_table_still_turns_the_queries(jal, torch_cuda, rotary, 
     want = torch.zeros(3, 1, page, hd)
     want[1, 0, 2], want[1, 0, 3] = x[0], x[1]
     assert torch.equal(pools[1].cpu(), want)
+
+
+def test_results_over_inputs_of_another_shape_are_refused(jal):
+    """out may be q and scores may be cum where every block reads what it overwrites, and only there."""
+    ok = dict(q=4096, out=4096, n_heads_q=4, scale=0.1, dtype=jal.F16)
+    groups = jal.PrefixGroups(4096, 4096, 1, 3, 10)
+    for strides in (dict(q_stride=512), dict(out_stride=264), dict(q_stride=256, out_stride=512)):
+        for call in (lambda: jal.paged_attention(_view(jal), _batch(jal), **ok, **strides),
+                     lambda: jal.shared_prefix_attention(_view(jal), _batch(jal), groups, **ok, **strides)):
+            with pytest.raises(jal.K3Error) as e:
+                call()
+            assert e.value.code == jal.ERR_TENSOR_BOUNDS and "out is q" in str(e.value), str(e.value)
+    sizes = dict(n_seqs=2, n_beams=3, vocab=100, k=4)
+    with pytest.raises(jal.K3Error) as e:
+        jal.beam_select(4096, 4096, 4096, 8192, 12288, workspace=4096, workspace_len=jal.beam_select_workspace(**sizes), **sizes)
+    assert e.value.code == jal.ERR_TENSOR_BOUNDS and "scores" in str(e.value), str(e.value)
