@@ -241,6 +241,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(const __grid_c
   for (int w = 0; w < kJoinWarps; w++) top = fmaxf(top, red[w]);
   const float w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
   weight[tid] = w;
+  if (ml.y == 0.0f) weight[tid] = -1.0f;  // (not a weight of 0: what a piece far below the others holds may be NaN)
   float total = warp_sum(w * ml.y);
   __syncthreads();
   if (lane == 0) red[warp] = total;
@@ -256,11 +257,11 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(const __grid_c
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       const int piece = k + e * kJoinWarps;
-      c[e] = piece < n ? weight[piece] : 0.0f;
+      c[e] = piece < n ? weight[piece] : -1.0f;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         v[e][h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (c[e] != 0.0f && lane + 32 * h < chunks)
+        if (c[e] != -1.0f && lane + 32 * h < chunks)
           v[e][h] = *((const float4 *)(p.part_o + (piece * stride + at) * hd) + lane + 32 * h);
       }
     }

@@ -347,3 +347,20 @@ def test_results_over_inputs_of_another_shape_are_refused(jal):
     with pytest.raises(jal.K3Error) as e:
         jal.beam_select(4096, 4096, 4096, 8192, 12288, workspace=4096, workspace_len=jal.beam_select_workspace(**sizes), **sizes)
     assert e.value.code == jal.ERR_TENSOR_BOUNDS and "scores" in str(e.value), str(e.value)
+
+
+# ---- joining: pieces far below the others ---------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("new", [1, 70])
+def test_attention_poison_in_a_piece_of_no_weight(jal, torch_cuda, new, act, cache, bad):
+    """A value that a row sees reaches it even where its piece of the keys weighs less than f32 can hold."""
+    c = lift(flat_rows(act, cache, new, 4097), 0, 300.0)
+    c.pools[1].permute(c.perm)[int(c.table[0, 4000 // 64]), 0, 4000 % 64, 5] = bad
+    c.to_device(jal)
+    assert jal.paged_attention_workspace(c.kv, c.batch, c.hq, dtype=c.act_type)  # (cut into pieces)
+    got = attend(jal, c, 0.125)[:new, :c.hq * c.hd].view(new, c.hq, c.hd).float()
+    assert not got[:, :4, 5].isfinite().any()
+    got[:, :4, 5] = 0
+    assert (got == 0).all()  # e^-300 of the tail
