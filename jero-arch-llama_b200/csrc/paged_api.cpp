@@ -156,7 +156,7 @@ void check_grid(const AttnPlan &a, const jal_paged_kv &kv, const jal_ragged_batc
                 size_t hq) {
   const double blocks = (double)kv.n_heads_kv * ((double)a.tiles * a.splits * (double)b.n_seqs +
                                                  (g ? (double)a.prefix_tiles * a.prefix_splits * (double)g->n_groups : 0));
-  if (blocks > 2e9 || (!a.direct && (double)b.n_rows * (double)hq > 2e9))
+  if (blocks > 2e9 || (!a.direct && std::min((double)b.n_rows, (double)b.n_seqs * (double)b.max_q_len) * (double)hq > 2e9))
     fail(JAL_ERR_CAPABILITY_MISMATCH, "batch too large for one launch");
 }
 

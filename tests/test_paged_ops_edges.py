@@ -364,3 +364,14 @@ def test_attention_poison_in_a_piece_of_no_weight(jal, torch_cuda, new, act, cac
     assert not got[:, :4, 5].isfinite().any()
     got[:, :4, 5] = 0
     assert (got == 0).all()  # e^-300 of the tail
+
+
+def test_row_buffers_larger_than_the_batch_are_not_refused(jal):
+    """Row buffers may be as large as the largest step of a captured graph: work goes by the rows that a batch can have."""
+    kv = _view(jal, page_size=64, max_pages=4096, n_pages=1 << 16)
+    batch = _batch(jal, n_rows=1 << 25, max_kv_len=200000)
+    need = jal.paged_attention_workspace(kv, batch, 64, dtype=jal.F16)
+    assert need
+    with pytest.raises(jal.K3Error) as e:  # (the addresses are none)
+        jal.paged_attention(kv, batch, 4096, 4096, 64, 0.1, dtype=jal.F16, workspace=4096, workspace_len=need)
+    assert e.value.code != jal.ERR_CAPABILITY_MISMATCH, str(e.value)
