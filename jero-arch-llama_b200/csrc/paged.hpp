@@ -80,7 +80,7 @@ struct BeamParams {
 int beam_chunks(size_t n_rows, size_t vocab);
 size_t beam_workspace(size_t n_seqs, size_t n_beams, size_t vocab, size_t k);
 // Whether the joining block of one sequence can take that many lists.
-bool beam_fits(size_t n_beams, size_t vocab, size_t k, size_t n_rows);
+bool beam_fits(size_t n_beams, size_t vocab, size_t k);
 void launch_beam_select(const BeamParams &p, cudaStream_t s);
 
 struct ReorderParams {

@@ -357,7 +357,7 @@ static void check_beams(size_t n_seqs, size_t n_beams, size_t vocab, size_t k) {
     fail(JAL_ERR_CAPABILITY_MISMATCH, "%zu of %zu x %zu continuations (1 to 64)", k, n_beams, vocab);
   if (n_beams > 65535 || n_seqs > 65535 || n_seqs * n_beams > 65535)
     fail(JAL_ERR_CAPABILITY_MISMATCH, "%zu x %zu beams (65535 at most)", n_seqs, n_beams);
-  if (!beam_fits(n_beams, vocab, k, n_seqs * n_beams))
+  if (!beam_fits(n_beams, vocab, k))
     fail(JAL_ERR_CAPABILITY_MISMATCH, "%zu beams, %zu best of a vocabulary of %zu: too many candidates", n_beams, k,
          vocab);
 }

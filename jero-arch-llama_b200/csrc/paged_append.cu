@@ -64,7 +64,6 @@ __device__ __forceinline__ void rotated8(const TA *row, int d, int rotary, int n
 // come, which halves the warps an SM holds; 86 us with a block for each row).
 constexpr int kWarps = 4;
 
-template <class T>
 __device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2 *cs, int d, int half, int neox) {
 #pragma unroll
   for (int e = 0; e < 8; e++) {
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(kWarps * 32, 7) k_rope_kv_append_pairs(const _
       float a[8], b[8];
       ra[k].widen(a);
       rb[k].widen(b);
-      if (rotated && (is_q || is_k)) turn8<TA>(a, b, cs, d, half, p.neox);
+      if (rotated && (is_q || is_k)) turn8(a, b, cs, d, half, p.neox);
       if (is_q) {
         TA *const dst = (TA *)p.q_out + row * p.q_out_stride + h * hd;
         store8(dst + d, a);
