@@ -210,7 +210,7 @@ typedef struct jal_paged_kv {
   uint64_t head_dim; /* multiple of 8, at most 256 */
   uint64_t n_seqs, max_pages; /* max_pages * page_size < 2^31 - 2^16 */
   /* elements, multiples of 8; all three 0 = [page][kv_head][slot][head_dim],
-   * a layer of jal_kv_cache */
+   * as jal_kv_cache lays out a layer (its own pools are not handed out) */
   uint64_t page_stride, head_stride, slot_stride;
   int32_t dtype; /* JAL_F32, JAL_F16 or JAL_BF16 */
 } jal_paged_kv;
@@ -230,7 +230,7 @@ typedef struct jal_ragged_batch {
   uint64_t n_rows;        /* rows of the row buffers */
   uint64_t max_q_len;     /* no sequence has more new rows */
   uint64_t max_kv_len;    /* about the largest kv_len: how the work is cut up
-                             follows from it, results do not depend on it */
+                             follows from it, and results within their rounding */
 } jal_ragged_batch;
 
 /* Sequences that share a prefix: group g is the sequences [group_start[g],
@@ -269,8 +269,12 @@ int jal_op_rope_kv_append(const jal_paged_kv *kv, const jal_ragged_batch *batch,
  * position p sees t <= p; with sliding_window > 0 only t > p - sliding_window
  * and the first n_sink positions.  A row that sees nothing (no position, no
  * page) is 0, keys and values that a row does not see have no effect on it
- * whatever they hold, and a row that sees a NaN or an infinity follows the
- * formula (scores of -inf count as masked).  dtype (q and out): the
+ * whatever they hold, and a row that sees a NaN or an infinity is NaN or
+ * infinite where the formula is (scores of -inf count as masked; f32 rows over
+ * a 16-bit cache, which are carried in parts, may be NaN where they see an
+ * infinite key).  All sequences of a call go to the kernel, and to tiles, that
+ * its longest one asks for: long prompts beside single rows are better two
+ * calls.  dtype (q and out): the
  * cache's or JAL_F32.  Sums and softmax are f32; with 16-bit q the softmax
  * weights are rounded to that type for the product with V, and f32 q and
  * weights over a 16-bit cache are carried as parts of 22 bits (f16) or 24
@@ -311,8 +315,9 @@ int jal_op_shared_prefix_attention_workspace(const jal_paged_kv *kv,
  * sequence, scored cum[b] + log_softmax(logits[b])[t], the k best in
  * descending order; equal scores go to the lowest b * vocab + t.  logits:
  * [n_seqs * n_beams] rows of `dtype` (JAL_F32 / F16 / BF16), row_stride elements
- * apart (0 = vocab); cum: [n_seqs][n_beams].  Scores are formed and compared
- * in 64 bits, within a beam in the order of the logits.  A NaN logit counts as
+ * apart (0 = vocab); cum: [n_seqs][n_beams].  A row's log-sum-exp is made of
+ * f32 terms and partial sums; scores are formed from it and compared in 64
+ * bits, within a beam in the order of the logits.  A NaN logit counts as
  * -inf; a beam whose cum is not finite or whose logits hold +inf or nothing
  * above -inf scores -inf throughout (finished and empty beams).  k <= 64,
  * k <= n_beams * vocab, n_beams <= 256, n_beams * k <= 8192, vocab <= 2^20
@@ -337,9 +342,11 @@ int jal_op_beam_select_workspace(size_t n_seqs, size_t n_beams, size_t vocab,
  * is every row's, so that those positions stay masked.  Row r of a parent
  * outside [0, n_beams) becomes empty.  fresh_pages: [n_seqs * n_beams]
  * distinct pages that no row uses; the caller takes back those that new_table
- * does not name.  Layer i of the pools starts i * layer_stride elements
- * after the first (0 = n_pages * page_stride).  new_table and new_len must
- * not overlap the old ones. */
+ * does not name.  No two rows that are continued may have the same unfinished
+ * page: each one's first child keeps it, and both would append to it (of rows
+ * that start as copies of one prompt, let one be alive).  Layer i of the pools
+ * starts i * layer_stride elements after the first (0 = n_pages * page_stride).
+ * new_table and new_len must not overlap the old ones. */
 int jal_op_beam_reorder(const jal_paged_kv *kv, size_t n_layers,
                         size_t layer_stride, const int32_t *kv_len,
                         const int32_t *parents, const int32_t *fresh_pages,

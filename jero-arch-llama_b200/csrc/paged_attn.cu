@@ -334,8 +334,9 @@ void run_f32(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
 }
 template <class T, int NS, int HD>
 void run_16bit(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
-  // Prefixes on tcgen05 and a sequence's own keys on mma.sync: two launches
-  // that do not depend on each other.
+  // Prefixes on tcgen05 and a sequence's own keys on mma.sync: two launches that
+  // do not depend on each other.  (The second starts beside the first's last blocks:
+  // one of the first's fills the shared memory of an SM.)
   const int tc = plan.rows == kTcRows ? plan.prefix_rows != kMmaRows ? kBoth : kOwn : kPrefix;
   bool first = false;
   if constexpr (HD <= 128 && NS <= 2) {
@@ -364,8 +365,14 @@ void run_16bit_hd(const AttnParams &p, const AttnPlan &plan, cudaStream_t s) {
 // 101 us; 48 rows of up to 4100 keys of 8 KV heads in one piece 132 us, in three
 // 142 us; 128 rows of about 1100 keys of 4 KV heads in two pieces 119 us (with their
 // prefixes), in three 132 us.  An f32 cache's keys take longer, so a start is worth
-// fewer of them: the 48 rows 629 us with 256, 587 us with 48.
+// fewer of them: the 48 rows 627 us with 256, 588 us with 48; 64 sequences behind a
+// prefix 461 and 451; 131071 keys, eight groups and short calls the same with both.
 constexpr int64_t kApartKeys = 320;
+// Rows that share their keys from which on the tcgen05 kernel takes them.  Measured
+// with 2048 keys of 8 KV heads in us, mma.sync / tcgen05, for 32, 64 and 96 rows: one
+// sequence of f16 rows 15 / 17, 17 / 17, 21 / 19, of f32 rows 15 / 23, 19 / 23, 23 / 25;
+// 48 sequences of f16 rows 103 / 101, 183 / 102, 265 / 103, of f32 rows 134 / 171,
+// 246 / 173, 359 / 175.  So it is late for 33 to 64 rows of many sequences.
 constexpr int64_t kTcLeast = 64;
 // Blocks of the tcgen05 kernel fill an SM each and write 256 rows of partial
 // results, so its keys are cut only as far as that gives idle SMs work.

@@ -3,7 +3,7 @@
 //
 // A block takes 256 query rows of one KV head as two tiles of 128 and runs
 // over its keys in tiles of 128: S = Q K^T into tensor memory, softmax weights
-// P in registers (one thread a row), P back into tensor memory over S, and
+// P in registers (two threads a row), P back into tensor memory over S, and
 // O += P V with O in tensor memory.  The two row tiles take turns: while the
 // tensor cores work on one, a warpgroup forms the weights of the other, so a
 // K and a V tile are read once for 256 rows.  Per key tile the tensor cores
@@ -12,15 +12,15 @@
 // these follow one another: a key tile takes about 4400 cycles (scores, weights,
 // products, and the waits between the warps that make them; without the exponentials
 // it takes 8% less), and a block's start (rows, table, first K tile) and end 10000 and
-// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 238 to
-// 252 us, 0.65 PFLOP/s, with the tensor cores busy for 37% of the time.  (A quarter or half of the
-// exponentials as polynomials on the multiply-add units: 5 to 20 us slower.  Seven
+// 5500 more.  Ragged prompts behind a 1024-position window, 159 GFLOP: 239 to 254 us
+// by the box, 0.62 to 0.66 PFLOP/s, with the tensor cores busy for 35% of the time.
+// (A quarter or half of the exponentials as polynomials on the multiply-add units: 5 to 20 us slower.  Seven
 // loader warps, one softmax warpgroup a row tile, or the query rows asked for before the
 // first barrier: no faster.)
 //
 //   warps 0-15       softmax: four warpgroups, two for each row tile, each with
 //                    64 of the tile's 128 keys (warp w reads tensor-memory lanes
-//                    32 (w % 4) ..), and the result.  One thread a row and half:
+//                    32 (w % 4) ..), and the result.  One thread for a row's half:
 //                    one warp of a tile on a scheduler cannot hide its own
 //                    latencies
 //   warps 16-18      K and V rows from their pages into the ring, cp.async
