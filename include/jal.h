@@ -321,8 +321,8 @@ int jal_op_shared_prefix_attention_workspace(const jal_paged_kv *kv,
  * -inf; a beam whose cum is not finite or whose logits hold +inf or nothing
  * above -inf scores -inf throughout (finished and empty beams).  k <= 64,
  * k <= n_beams * vocab, n_beams <= 256, n_beams * k <= 8192, vocab <= 2^20
- * (JAL_ERR_CAPABILITY_MISMATCH).  Outputs [n_seqs][k]; with k = n_beams scores
- * may be cum. */
+ * (JAL_ERR_CAPABILITY_MISMATCH).  Outputs [n_seqs][k]; with k = n_beams, or
+ * for one sequence, scores may be cum. */
 int jal_op_beam_select(const void *logits, int dtype, size_t row_stride,
                        const float *cum, size_t n_seqs, size_t n_beams,
                        size_t vocab, size_t k, float *scores, int32_t *parents,

@@ -179,7 +179,8 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
   p.out_stride = row_stride(out_stride, hq * kv.head_dim, "out");
   aligned16(q, "q");
   aligned16(out, "out");
-  if (q == out && p.q_stride != p.out_stride) fail(JAL_ERR_TENSOR_BOUNDS, "out is q with another stride");
+  if (q == out && p.q_stride != p.out_stride && b.n_rows > 1)
+    fail(JAL_ERR_TENSOR_BOUNDS, "out is q with another stride");
   if (b.n_seqs == 0 || b.n_rows == 0 || b.max_q_len == 0) return;
   window = std::min<size_t>(window, kMaxInt);
   n_sink = std::min<size_t>(n_sink, kMaxInt);
@@ -386,7 +387,7 @@ int jal_op_beam_select(const void *logits, int dtype, size_t row_stride_in, cons
     NEED(workspace);
     aligned16(workspace, "workspace");
     if (workspace_len < need) fail(JAL_ERR_TENSOR_BOUNDS, "workspace of %zu bytes, %zu needed", workspace_len, need);
-    if (scores == cum && k != n_beams)
+    if (scores == cum && k != n_beams && n_seqs > 1)
       fail(JAL_ERR_TENSOR_BOUNDS, "scores are cum, with %zu best of %zu beams", k, n_beams);
     const int dev = current_device();
     on_device(logits, "logits", dev);

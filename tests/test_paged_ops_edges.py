@@ -375,3 +375,27 @@ def test_row_buffers_larger_than_the_batch_are_not_refused(jal):
     with pytest.raises(jal.K3Error) as e:  # (the addresses are none)
         jal.paged_attention(kv, batch, 4096, 4096, 64, 0.1, dtype=jal.F16, workspace=4096, workspace_len=need)
     assert e.value.code != jal.ERR_CAPABILITY_MISMATCH, str(e.value)
+
+
+def test_one_row_over_another_stride_is_not_refused(jal):
+    """One row, or one sequence's beams, has nothing to write over but itself."""
+    for call in (lambda: jal.paged_attention(_view(jal), _batch(jal, n_rows=1), 4096, 4096, 4, 0.1, dtype=jal.F16, q_stride=512),
+                 lambda: jal.beam_select(4096, 4096, 4096, 8192, 12288, 1, 1, 100, 4, workspace=4096, workspace_len=1 << 20)):
+        with pytest.raises(jal.K3Error) as e:  # (the addresses are none)
+            call()
+        assert e.value.code != jal.ERR_TENSOR_BOUNDS, str(e.value)
+
+
+@pytest.mark.gpu
+def test_one_sequence_selects_over_its_own_scores(jal, torch_cuda):
+    """The first step of a search: the k best of one beam, over the buffer that held its score."""
+    logits = torch.randn(2, 9001, generator=torch.Generator().manual_seed(1))
+    for beams, k in ((1, 8), (2, 7), (2, 1)):
+        cum = torch.zeros(8)
+        d_cum, need = cum.to(DEV), jal.beam_select_workspace(1, beams, 9001, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+        parents, tokens = (torch.zeros(1, k, dtype=torch.int32, device=DEV) for _ in range(2))
+        jal.beam_select(logits.to(DEV), d_cum, d_cum, parents, tokens, 1, beams, 9001, k, workspace=ws, workspace_len=need)
+        got = [d_cum[None, :k].cpu(), parents.cpu(), tokens.cpu()]
+        check_continuations(got, logits[:beams], cum[:beams], 1, beams, k)
+        assert not d_cum[max(k, beams):].any()
