@@ -353,6 +353,111 @@ int jal_op_beam_reorder(const jal_paged_kv *kv, size_t n_layers,
                         size_t n_seqs, size_t n_beams, int32_t *new_table,
                         int32_t *new_len, void *stream);
 
+/* ---- a paged cache of 8- or 4-bit codes ---------------------------------
+ * Of every position and KV head, K and V are held as head_dim codes and one
+ * f32 scale: element = scale * code.  8 bits: code is a signed byte.  4 bits: byte
+ * i holds dim 2 i in its low half and dim 2 i + 1 in its high half, each code + 8.
+ * Codes of (page, kv head, slot) lie at page * page_stride + head * head_stride +
+ * slot * slot_stride bytes of a pool, their scale at page * scale_page_stride + head
+ * * scale_head_stride + slot floats.  Pages and tables as in jal_paged_kv.  Scales
+ * may have either sign; finite ones are below 2^96. */
+typedef struct jal_quant_kv {
+  void *k, *v;               /* codes, 16-byte aligned */
+  float *k_scale, *v_scale;
+  const int32_t *page_table; /* [n_seqs][max_pages] */
+  uint64_t n_pages, page_size, n_heads_kv;
+  uint64_t head_dim; /* multiple of 16 (8 bits) or 32 (4 bits), at most 256 */
+  uint64_t n_seqs, max_pages; /* max_pages * page_size < 2^31 - 2^16 */
+  /* bytes, multiples of 16; all three 0 = [page][kv_head][slot][head_dim * bits / 8] */
+  uint64_t page_stride, head_stride, slot_stride;
+  /* floats; both 0 = [page][kv_head][slot] */
+  uint64_t scale_page_stride, scale_head_stride;
+  int32_t bits; /* 8 or 4 */
+} jal_quant_kv;
+
+/* jal_op_rope_kv_append into such a cache: arguments and rotation as there,
+ * dtype JAL_F32, JAL_F16 or JAL_BF16.  A head's row x (k rotated in 64 bits, rounded
+ * to f32 and not to dtype; v as it is) is stored with a = max |x|, m = 127 or 7, as
+ * scale = a / m and code = x * (m / a) to the nearest integer, each operation rounded
+ * to f32: an element is off by at most half a scale.  With a < 2^-100 scale
+ * and codes are 0; a row with an element that is not below 2^100 (a NaN and the
+ * infinities among them) is stored with scale NaN and reads as NaN. */
+int jal_op_quant_kv_append(const jal_quant_kv *kv, const jal_ragged_batch *batch,
+                           int dtype, const void *k, const void *v,
+                           size_t kv_stride, const float *inv_freq,
+                           size_t rotary_dim, int neox, const void *q,
+                           void *q_out, size_t n_heads_q, size_t q_stride,
+                           size_t q_out_stride, void *stream);
+
+/* jal_op_paged_attention over such a cache: the same rows, masks and results, with
+ * K[t] and V[t] what the codes stand for.  dtype (q and out): JAL_F32, JAL_F16 or
+ * JAL_BF16.  Codes enter the products exactly; scales multiply scores and weights
+ * in f32.  The weight times V's scale is rounded to f16 once (16-bit rows) or
+ * carried as two f16 parts, 22 bits (f32 rows), and is further off by up to 2^-33 of
+ * the largest such product that is possible for the keys at hand (the row's
+ * largest weight times the largest scale of V): that shows only where scales
+ * of V lie 10^6 apart or more, or one position 14 nats above those that make the
+ * result.  bf16 elements of q more than 2^27 below the row's largest lose bits, f32
+ * ones are carried as 22 bits of the row's largest.  Workspace as there, from
+ * jal_op_quant_kv_attention_workspace. */
+int jal_op_quant_kv_attention(const jal_quant_kv *kv,
+                              const jal_ragged_batch *batch, int dtype,
+                              const void *q, size_t n_heads_q, size_t q_stride,
+                              float scale, size_t sliding_window, size_t n_sink,
+                              void *out, size_t out_stride, void *workspace,
+                              size_t workspace_len, void *stream);
+int jal_op_quant_kv_attention_workspace(const jal_quant_kv *kv,
+                                        const jal_ragged_batch *batch, int dtype,
+                                        size_t n_heads_q, size_t sliding_window,
+                                        size_t n_sink, size_t *bytes);
+
+/* Reads positions back: of each sequence s < n_seqs, the positions [first[s],
+ * kv_len[s]) (first NULL = from 0; at most max_len of them) as scale * code into the
+ * same positions of `into`, rounded to its type.  `into` has tables, pages and a
+ * layout of its own, and the cache's heads and head_dim.  A position that either
+ * cache has no page or place for is left out; pages of `into` that two sequences
+ * share are written by both, so the two should hold the same there. */
+int jal_op_quant_kv_read(const jal_quant_kv *kv, const int32_t *first,
+                         const int32_t *kv_len, size_t n_seqs, size_t max_len,
+                         const jal_paged_kv *into, void *stream);
+
+/* Verification of drafted tokens.  The rows of `batch` are what the model was fed:
+ * tokens[q_start[s]] is sequence s's last sure token, the rows behind it its
+ * drafts.  Row r's logits, of `dtype` (JAL_F32 / F16 / BF16), row_stride elements
+ * apart (0 = vocab), are of the token behind row r; draft_logits (NULL: drafts come
+ * without probabilities) are the draft model's of the same, draft_stride apart, and
+ * not read at a sequence's last row.  With p = softmax(logits / temperature[s]) and
+ * q = softmax(draft_logits / draft_temperature[s]) (temperature NULL = 1;
+ * draft_temperature NULL = temperature), a draft x = tokens[r + 1] is accepted while
+ *   uniform[r] * q(x) < p(x),
+ * and at the first row r that refuses, the token behind it is drawn from max(p - q,
+ * 0), or at the last row from p: the first t whose running sum exceeds uniform[the
+ * sequence's last row] times the whole.  (uniform: one number in [0, 1) for each
+ * row.)  Every token is then distributed as p alone would have it.
+ * Without draft_logits, and where a draft row has no distribution, q is 1 at x.  A
+ * temperature not above 1e-5 (0, a NaN) puts all of p (or q) on the first of the
+ * largest logits.  A NaN logit counts as -inf; a row that holds +inf or nothing
+ * above -inf has no distribution: its draft is refused, and a token drawn from it is
+ * -1.  A draft outside the vocabulary is refused.  Where max(p - q, 0) is 0
+ * throughout, the token is drawn from p.
+ * Acceptance is decided from f32 sums of the exponentials, drawing from sums
+ * and exponentials in 64 bits.
+ * out_tokens (one for each row, not `tokens`): the accepted drafts from q_start[s]
+ * on, the drawn token, then -1; rows of no sequence are left as they were.
+ * n_accepted [n_seqs]: accepted drafts.  new_len (or NULL; may be batch's kv_len):
+ * kv_len[s] without the refused drafts' positions.  A sequence without rows
+ * accepts 0.  vocab < 2^30. */
+int jal_op_verify_drafts(const jal_ragged_batch *batch, const void *logits,
+                         int dtype, size_t row_stride, const void *draft_logits,
+                         size_t draft_stride, size_t vocab,
+                         const int32_t *tokens, const float *uniform,
+                         const float *temperature, const float *draft_temperature,
+                         int32_t *out_tokens, int32_t *n_accepted,
+                         int32_t *new_len, void *workspace, size_t workspace_len,
+                         void *stream);
+int jal_op_verify_drafts_workspace(const jal_ragged_batch *batch, size_t vocab,
+                                   size_t *bytes);
+
 /* ========================================================================
  * recipe.rs -- LlamaRecipe
  * ====================================================================== */

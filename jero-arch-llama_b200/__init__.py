@@ -142,6 +142,14 @@ class PrefixGroupsFields(C.Structure):
                 ("max_prefix_len", C.c_uint64)]
 
 
+class QuantKvFields(C.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("page_table", _P),
+                ("n_pages", C.c_uint64), ("page_size", C.c_uint64), ("n_heads_kv", C.c_uint64),
+                ("head_dim", C.c_uint64), ("n_seqs", C.c_uint64), ("max_pages", C.c_uint64),
+                ("page_stride", C.c_uint64), ("head_stride", C.c_uint64), ("slot_stride", C.c_uint64),
+                ("scale_page_stride", C.c_uint64), ("scale_head_stride", C.c_uint64), ("bits", C.c_int32)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "jal_last_error": (C.c_char_p, []),
@@ -174,6 +182,12 @@ _SIGS = {
     "jal_op_beam_select": (C.c_int, [_P, C.c_int, _SZ, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, _P, _P, _SZ, _P]),
     "jal_op_beam_select_workspace": (C.c_int, [_SZ, _SZ, _SZ, _SZ, C.POINTER(_SZ)]),
     "jal_op_beam_reorder": (C.c_int, [_P, _SZ, _SZ, _P, _P, _P, _SZ, _SZ, _P, _P, _P]),
+    "jal_op_quant_kv_append": (C.c_int, [_P, _P, C.c_int, _P, _P, _SZ, _P, _SZ, C.c_int, _P, _P, _SZ, _SZ, _SZ, _P]),
+    "jal_op_quant_kv_attention": (C.c_int, [_P, _P, C.c_int, _P, _SZ, _SZ, C.c_float, _SZ, _SZ, _P, _SZ, _P, _SZ, _P]),
+    "jal_op_quant_kv_attention_workspace": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, C.POINTER(_SZ)]),
+    "jal_op_quant_kv_read": (C.c_int, [_P, _P, _P, _SZ, _SZ, _P, _P]),
+    "jal_op_verify_drafts": (C.c_int, [_P, _P, C.c_int, _SZ, _P, _SZ, _SZ, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "jal_op_verify_drafts_workspace": (C.c_int, [_P, _SZ, C.POINTER(_SZ)]),
     "jal_recipe_new": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "jal_recipe_from_gguf": (C.c_int, [_P, _SZ, C.POINTER(_P)]),
     "jal_recipe_free": (None, [_P]),
@@ -508,6 +522,73 @@ def beam_reorder(kv: PagedKv, kv_len, parents, fresh_pages, new_table, new_len, 
     the unfinished pages of further children copied in every layer."""
     _check(lib().jal_op_beam_reorder(kv.ptr, n_layers, layer_stride, _ptr(kv_len), _ptr(parents), _ptr(fresh_pages),
                                      n_seqs, n_beams, _ptr(new_table), _ptr(new_len), _stream(stream)))
+
+
+class QuantKv:
+    """A paged cache of 8- or 4-bit codes (jal_quant_kv): device pools of codes
+    (bytes), their f32 scales, and the page table.  `strides`: (page, head, slot)
+    of the codes in bytes, `scale_strides`: (page, head) of the scales in floats;
+    None = [page][kv_head][slot]([head_dim * bits / 8])."""
+
+    def __init__(self, k, v, k_scale, v_scale, page_table, bits: int, n_pages: int, page_size: int, n_heads_kv: int,
+                 head_dim: int, n_seqs: int, max_pages: int, strides=None, scale_strides=None):
+        self._keep = (k, v, k_scale, v_scale, page_table)
+        self.fields = QuantKvFields(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), _ptr(page_table), n_pages,
+                                    page_size, n_heads_kv, head_dim, n_seqs, max_pages, *(strides or (0, 0, 0)),
+                                    *(scale_strides or (0, 0)), bits)
+        self.ptr = C.addressof(self.fields)
+
+
+def quant_kv_append(kv: QuantKv, batch: RaggedBatch, k, v, inv_freq, dtype: int, rotary_dim: int, neox: bool = False,
+                    kv_stride: int = 0, q=None, q_out=None, n_heads_q: int = 0, q_stride: int = 0,
+                    q_out_stride: int = 0, stream=None) -> None:
+    """Rotates the batch's k (and q) rows and appends k and v as codes."""
+    _check(lib().jal_op_quant_kv_append(kv.ptr, batch.ptr, dtype, _ptr(k), _ptr(v), kv_stride, _ptr(inv_freq),
+                                        rotary_dim, 1 if neox else 0, _ptr(q), _ptr(q_out), n_heads_q, q_stride,
+                                        q_out_stride, _stream(stream)))
+
+
+def quant_kv_attention(kv: QuantKv, batch: RaggedBatch, q, out, n_heads_q: int, scale: float, dtype: int,
+                       sliding_window: int = 0, n_sink: int = 0, q_stride: int = 0, out_stride: int = 0,
+                       workspace=None, workspace_len: int = 0, stream=None) -> None:
+    """paged_attention over a cache of codes."""
+    _check(lib().jal_op_quant_kv_attention(kv.ptr, batch.ptr, dtype, _ptr(q), n_heads_q, q_stride, scale,
+                                           sliding_window, n_sink, _ptr(out), out_stride, _ptr(workspace),
+                                           workspace_len, _stream(stream)))
+
+
+def quant_kv_attention_workspace(kv: QuantKv, batch: RaggedBatch, n_heads_q: int, dtype: int, sliding_window: int = 0,
+                                 n_sink: int = 0) -> int:
+    """Workspace bytes of the same quant_kv_attention call."""
+    n = _SZ()
+    _check(lib().jal_op_quant_kv_attention_workspace(kv.ptr, batch.ptr, dtype, n_heads_q, sliding_window, n_sink,
+                                                     C.byref(n)))
+    return n.value
+
+
+def quant_kv_read(kv: QuantKv, kv_len, into: PagedKv, n_seqs: int, max_len: int, first=None, stream=None) -> None:
+    """Positions [first, kv_len) of each sequence (at most max_len of them) into
+    the same positions of an unquantised paged cache."""
+    _check(lib().jal_op_quant_kv_read(kv.ptr, _ptr(first), _ptr(kv_len), n_seqs, max_len, into.ptr, _stream(stream)))
+
+
+def verify_drafts(batch: RaggedBatch, logits, tokens, uniform, out_tokens, n_accepted, vocab: int, dtype: int = F32,
+                  draft_logits=None, temperature=None, draft_temperature=None, new_len=None, row_stride: int = 0,
+                  draft_stride: int = 0, workspace=None, workspace_len: int = 0, stream=None) -> None:
+    """Which drafted tokens (int32, the batch's rows behind each sequence's first)
+    the target's logits accept, and the token drawn behind them: out_tokens int32
+    for each row, n_accepted int32 [n_seqs]."""
+    _check(lib().jal_op_verify_drafts(batch.ptr, _ptr(logits), dtype, row_stride, _ptr(draft_logits), draft_stride,
+                                      vocab, _ptr(tokens), _ptr(uniform), _ptr(temperature), _ptr(draft_temperature),
+                                      _ptr(out_tokens), _ptr(n_accepted), _ptr(new_len), _ptr(workspace),
+                                      workspace_len, _stream(stream)))
+
+
+def verify_drafts_workspace(batch: RaggedBatch, vocab: int) -> int:
+    """Workspace bytes of the same verify_drafts call."""
+    n = _SZ()
+    _check(lib().jal_op_verify_drafts_workspace(batch.ptr, vocab, C.byref(n)))
+    return n.value
 
 
 # ---- LlamaRecipe (recipe.rs:110-547) ----------------------------------------

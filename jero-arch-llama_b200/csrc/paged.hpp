@@ -26,6 +26,10 @@ struct PagedView {
   int32_t cap;  // max_pages * page_size: positions a table row has
 };
 
+// The arguments of the C entry points, checked, with their defaults filled in.
+jal_paged_kv checked_kv(const jal_paged_kv *in);
+PagedView view_of(const jal_paged_kv &kv);
+
 struct AttnParams {
   PagedView kv;
   const void *q;
@@ -54,6 +58,10 @@ struct AttnPlan {
 AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const jal_prefix_groups *g, size_t n_heads_q,
                         int act, size_t window, size_t n_sink);
 void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s);
+// Into how many pieces the keys of `blocks` blocks' rows go, and the kernel that
+// joins the pieces' results (launched behind the one that makes them).
+int attention_pieces(int64_t blocks, int64_t keys, int resident, int64_t start_keys, bool joined);
+void launch_attention_join(const AttnParams &p, int prefix_rows, cudaStream_t s);
 
 struct AppendParams {
   PagedView kv;

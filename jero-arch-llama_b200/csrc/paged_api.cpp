@@ -9,43 +9,12 @@
 #include "common.hpp"
 #include "jal.h"
 #include "paged.hpp"
+#include "paged_args.hpp"
 
 using namespace jal;
 
-namespace {
-
-constexpr uint64_t kMaxPositions = 0x7fffffffull - 65536;  // tiles run past the last position by less than 65536
-constexpr uint64_t kMaxInt = 0x7fffffffull;
-
-bool float_type(int t) { return t == JAL_F32 || t == JAL_F16 || t == JAL_BF16; }
-size_t type_bytes(int t) { return t == JAL_F32 ? 4 : 2; }
-
-// `p` is memory of the current device: a tensor of another device, or of the
-// host, would fault in the kernel.
-void on_device(const void *p, const char *what, int device) {
-  cudaPointerAttributes a = {};
-  JAL_CUDA(cudaPointerGetAttributes(&a, p));
-  if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
-    fail(JAL_ERR_INVALID_ARGUMENT, "%s is not device memory", what);
-  if (a.type == cudaMemoryTypeDevice && a.device != device)
-    fail(JAL_ERR_INVALID_ARGUMENT, "%s is on device %d, the current device is %d", what, a.device, device);
-}
-int current_device() {
-  int d = 0;
-  JAL_CUDA(cudaGetDevice(&d));
-  return d;
-}
-void aligned16(const void *p, const char *what) {
-  if ((uintptr_t)p % 16) fail(JAL_ERR_TENSOR_BOUNDS, "%s is not 16-byte aligned", what);
-}
-// Arrays that kernels read and write as 4-byte values: an address between two of
-// them would fault.
-void aligned4(const void *p, const char *what) {
-  if ((uintptr_t)p % 4) fail(JAL_ERR_TENSOR_BOUNDS, "%s is not 4-byte aligned", what);
-}
-
 // A cache view with its defaults filled in.
-jal_paged_kv checked_kv(const jal_paged_kv *in) {
+jal_paged_kv jal::checked_kv(const jal_paged_kv *in) {
   NEED(in);
   jal_paged_kv kv = *in;
   NEED(kv.k);
@@ -79,7 +48,7 @@ jal_paged_kv checked_kv(const jal_paged_kv *in) {
   return kv;
 }
 
-PagedView view_of(const jal_paged_kv &kv) {
+PagedView jal::view_of(const jal_paged_kv &kv) {
   PagedView v = {};
   v.k = kv.k;
   v.v = kv.v;
@@ -100,33 +69,12 @@ PagedView view_of(const jal_paged_kv &kv) {
   return v;
 }
 
-jal_ragged_batch checked_batch(const jal_ragged_batch *in, const jal_paged_kv &kv) {
-  NEED(in);
-  jal_ragged_batch b = *in;
-  NEED(b.q_start);
-  NEED(b.kv_len);
-  aligned4(b.q_start, "q_start");
-  aligned4(b.kv_len, "kv_len");
-  if (b.n_seqs > kv.n_seqs)
-    fail(JAL_ERR_TENSOR_BOUNDS, "batch of %llu sequences over a table of %llu", (unsigned long long)b.n_seqs,
-         (unsigned long long)kv.n_seqs);
-  if (b.n_rows > kMaxPositions) fail(JAL_ERR_TENSOR_BOUNDS, "batch of 2^31 rows or more");
-  if (b.max_q_len > b.n_rows) b.max_q_len = b.n_rows;
-  b.max_kv_len = std::min<uint64_t>(std::max<uint64_t>(b.max_kv_len, 1), kv.max_pages * kv.page_size);
-  return b;
-}
+namespace {
 
 void check_act(int dtype, const jal_paged_kv &kv) {
   if (!float_type(dtype) || (dtype != kv.dtype && dtype != JAL_F32))
     fail(JAL_ERR_CAPABILITY_MISMATCH, "rows of type %d over a cache of type %d (the cache's type or f32)", dtype,
          kv.dtype);
-}
-
-int64_t row_stride(size_t stride, size_t width, const char *what) {
-  if (stride == 0) stride = width;
-  if (stride < width || stride % 8 || stride > (1ull << 40))
-    fail(JAL_ERR_TENSOR_BOUNDS, "%s stride %zu: a multiple of 8, at least %zu", what, stride, width);
-  return (int64_t)stride;
 }
 
 void check_heads(size_t hq, const jal_paged_kv &kv, const jal_ragged_batch &b) {
@@ -164,7 +112,7 @@ void attention(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const j
                const void *q, size_t hq, size_t q_stride, float scale, size_t window, size_t n_sink, void *out,
                size_t out_stride, void *ws, size_t ws_len, void *stream) {
   const jal_paged_kv kv = checked_kv(kv_in);
-  const jal_ragged_batch b = checked_batch(batch, kv);
+  const jal_ragged_batch b = checked_batch(batch, kv.n_seqs, kv.max_pages * kv.page_size);
   jal_prefix_groups g = {};
   if (groups) g = checked_groups(groups, kv, b);
   check_act(dtype, kv);
@@ -241,7 +189,7 @@ int jal_op_rope_kv_append(const jal_paged_kv *kv_in, const jal_ragged_batch *bat
                           void *stream) {
   return guard([&] {
     const jal_paged_kv kv = checked_kv(kv_in);
-    const jal_ragged_batch b = checked_batch(batch, kv);
+    const jal_ragged_batch b = checked_batch(batch, kv.n_seqs, kv.max_pages * kv.page_size);
     check_act(dtype, kv);
     NEED(k);
     NEED(v);
@@ -322,7 +270,7 @@ int jal_op_shared_prefix_attention(const jal_paged_kv *kv, const jal_ragged_batc
 static size_t attention_bytes(const jal_paged_kv *kv_in, const jal_ragged_batch *batch, const jal_prefix_groups *groups,
                               int dtype, size_t hq, size_t window, size_t n_sink) {
   const jal_paged_kv kv = checked_kv(kv_in);
-  const jal_ragged_batch b = checked_batch(batch, kv);
+  const jal_ragged_batch b = checked_batch(batch, kv.n_seqs, kv.max_pages * kv.page_size);
   jal_prefix_groups g = {};
   if (groups) g = checked_groups(groups, kv, b);
   check_act(dtype, kv);

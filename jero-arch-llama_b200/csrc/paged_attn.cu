@@ -381,7 +381,9 @@ int tc_pieces(int64_t blocks, int64_t keys) {
   return (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
 }
 constexpr int64_t kBlockKeys = 256, kF32BlockKeys = 48, kJoinKeys = 256, kPieceKeys = 4, kLeastKeys = 64;
-int pieces(int64_t blocks, int64_t keys, int resident, int64_t start_keys, bool joined) {
+}  // namespace
+
+int attention_pieces(int64_t blocks, int64_t keys, int resident, int64_t start_keys, bool joined) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / kLeastKeys));
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= most; s++) {
@@ -395,8 +397,6 @@ int pieces(int64_t blocks, int64_t keys, int resident, int64_t start_keys, bool 
   }
   return (int)best;
 }
-
-}  // namespace
 
 AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const jal_prefix_groups *g, size_t hq,
                         int act, size_t window, size_t n_sink) {
@@ -417,8 +417,8 @@ AttnPlan plan_attention(const jal_paged_kv &kv, const jal_ragged_batch &b, const
   };
   auto pieces_for = [&](int rows, int64_t blocks, int64_t keys) {
     return rows == kTcRows ? tc_pieces(blocks, keys)
-                           : pieces(blocks, keys, mma_blocks((int)kv.head_dim),
-                                    kv.dtype == JAL_F32 ? kF32BlockKeys : kBlockKeys, g != nullptr);
+                           : attention_pieces(blocks, keys, mma_blocks((int)kv.head_dim),
+                                              kv.dtype == JAL_F32 ? kF32BlockKeys : kBlockKeys, g != nullptr);
   };
   a.rows = rows_for(pairs);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
@@ -455,10 +455,13 @@ void launch_paged_attention(AttnParams p, const AttnPlan &plan, cudaStream_t s) 
   } else {
     run_16bit_hd<__nv_bfloat16, 3>(p, plan, s);
   }
-  if (plan.direct) return;
+  if (!plan.direct) launch_attention_join(p, plan.prefix_rows, s);
+}
+
+void launch_attention_join(const AttnParams &p, int prefix_rows, cudaStream_t s) {
   const int64_t by_seq = (int64_t)p.n_seqs * p.max_q;
   launch(p.n_rows <= by_seq ? k_paged_attn_join<true> : k_paged_attn_join<false>,
-         std::min<int64_t>(p.n_rows, by_seq) * p.hq, kJoinThreads, 0, true, s, p, plan.prefix_rows);
+         std::min<int64_t>(p.n_rows, by_seq) * p.hq, kJoinThreads, 0, true, s, p, prefix_rows);
 }
 
 }  // namespace jal

@@ -1,0 +1,67 @@
+// Attention of a ragged batch over a paged cache of 8- or 4-bit codes: the plan of a
+// call and its launches.
+#include <algorithm>
+
+#include "common.hpp"
+#include "quant_attn_mma.cuh"
+
+namespace jal {
+
+namespace {
+
+using namespace paged;
+
+template <int BITS, int NS, int HD, int MT>
+void run_mma(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
+  const int64_t blocks = (int64_t)p.a.kv.hkv * p.a.splits * p.a.tiles * p.a.n_seqs;
+  constexpr int smem = QuantShape<BITS, NS, HD, MT>::smem;
+  JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_mma<BITS, NS, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  k_quant_attn_mma<BITS, NS, HD, MT><<<(unsigned)blocks, kMmaThreads, smem, s>>>(p, plan.direct);
+  JAL_CUDA(cudaGetLastError());
+}
+template <int BITS, int NS, int HD>
+void run_rows(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
+  if constexpr (HD <= 128) {
+    if (plan.rows == 32) return run_mma<BITS, NS, HD, 2>(p, plan, s);
+  }
+  run_mma<BITS, NS, HD, 1>(p, plan, s);
+}
+template <int BITS, int NS>
+void run_hd(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
+  if (p.a.kv.hd <= 64) run_rows<BITS, NS, 64>(p, plan, s);
+  else if (p.a.kv.hd <= 128) run_rows<BITS, NS, 128>(p, plan, s);
+  else run_rows<BITS, NS, 256>(p, plan, s);
+}
+template <int BITS>
+void run_type(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
+  if (p.a.act == JAL_F32) run_hd<BITS, 2>(p, plan, s);
+  else run_hd<BITS, 1>(p, plan, s);
+}
+
+constexpr int64_t kBlockKeys = 256;
+
+}  // namespace
+
+QuantAttnPlan plan_quant_attention(const jal_quant_kv &kv, const jal_ragged_batch &b, size_t hq, int act, size_t window,
+                                   size_t n_sink) {
+  QuantAttnPlan a = {};
+  const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv, pairs = (int64_t)b.max_q_len * G;
+  a.rows = pairs > 16 && kv.head_dim <= 128 ? 32 : 16;
+  a.tiles = (int)((pairs + a.rows - 1) / a.rows);
+  int64_t keys = (int64_t)b.max_kv_len;
+  if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
+  a.splits = attention_pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, quant_blocks((int)kv.head_dim, a.rows / 16),
+                              kBlockKeys, false);
+  a.direct = a.splits == 1;
+  if (!a.direct)
+    a.bytes = (size_t)a.splits * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;
+  return a;
+}
+
+void launch_quant_attention(const QuantAttnParams &p, int bits, const QuantAttnPlan &plan, cudaStream_t s) {
+  if (bits == 8) run_type<8>(p, plan, s);
+  else run_type<4>(p, plan, s);
+  if (!plan.direct) launch_attention_join(p.a, 0, s);
+}
+
+}  // namespace jal
