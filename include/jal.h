@@ -392,13 +392,10 @@ int jal_op_quant_kv_append(const jal_quant_kv *kv, const jal_ragged_batch *batch
 /* jal_op_paged_attention over such a cache: the same rows, masks and results, with
  * K[t] and V[t] what the codes stand for.  dtype (q and out): JAL_F32, JAL_F16 or
  * JAL_BF16.  Codes enter the products exactly; scales multiply scores and weights
- * in f32.  The weight times V's scale is rounded to f16 once (16-bit rows) or
- * carried as two f16 parts, 22 bits (f32 rows), and is further off by up to 2^-33 of
- * the largest such product that is possible for the keys at hand (the row's
- * largest weight times the largest scale of V): that shows only where scales
- * of V lie 10^6 apart or more, or one position 14 nats above those that make the
- * result.  bf16 elements of q more than 2^27 below the row's largest lose bits, f32
- * ones are carried as 22 bits of the row's largest.  Workspace as there, from
+ * in f32, and sums are f32 or exact.  Few rows: q is carried to 2^-16 of the row's
+ * largest element (f32 rows: 2^-31), weights times V's scale to 2^-14 of the largest
+ * of the 32 keys that are taken together (f32: 2^-30).  A row of q with a NaN or an
+ * infinity is NaN where it sees anything, one below 2^-100 counts as 0.  Workspace as there, from
  * jal_op_quant_kv_attention_workspace. */
 int jal_op_quant_kv_attention(const jal_quant_kv *kv,
                               const jal_ragged_batch *batch, int dtype,

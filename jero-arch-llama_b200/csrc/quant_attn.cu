@@ -11,20 +11,25 @@ namespace {
 
 using namespace paged;
 
-template <int BITS, int NS, int HD, int MT>
+// Tiles of eight rows of a block, by registers.
+constexpr int most_tiles(int hd, int ns) { return hd > 128 || (hd > 64 && ns > 1) ? 2 : 3; }
+
+template <int BITS, int NS, int HD, int R8>
 void run_mma(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
   const int64_t blocks = (int64_t)p.a.kv.hkv * p.a.splits * p.a.tiles * p.a.n_seqs;
-  constexpr int smem = QuantShape<BITS, NS, HD, MT>::smem;
-  JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_mma<BITS, NS, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  k_quant_attn_mma<BITS, NS, HD, MT><<<(unsigned)blocks, kMmaThreads, smem, s>>>(p, plan.direct);
+  constexpr int smem = QuantShape<BITS, NS, HD, R8>::smem;
+  static_assert(smem <= 232448 - 2048, "shared memory of a block");
+  JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_mma<BITS, NS, HD, R8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  k_quant_attn_mma<BITS, NS, HD, R8><<<(unsigned)blocks, kMmaThreads, smem, s>>>(p, plan.direct);
   JAL_CUDA(cudaGetLastError());
 }
 template <int BITS, int NS, int HD>
 void run_rows(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
-  if constexpr (HD <= 128) {
-    if (plan.rows == 32) return run_mma<BITS, NS, HD, 2>(p, plan, s);
+  if (plan.rows == 8) return run_mma<BITS, NS, HD, 1>(p, plan, s);
+  if constexpr (most_tiles(HD, NS) >= 3) {
+    if (plan.rows == 24) return run_mma<BITS, NS, HD, 3>(p, plan, s);
   }
-  run_mma<BITS, NS, HD, 1>(p, plan, s);
+  run_mma<BITS, NS, HD, 2>(p, plan, s);
 }
 template <int BITS, int NS>
 void run_hd(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
@@ -46,11 +51,12 @@ QuantAttnPlan plan_quant_attention(const jal_quant_kv &kv, const jal_ragged_batc
                                    size_t n_sink) {
   QuantAttnPlan a = {};
   const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv, pairs = (int64_t)b.max_q_len * G;
-  a.rows = pairs > 16 && kv.head_dim <= 128 ? 32 : 16;
+  const int ns = act == JAL_F32 ? 2 : 1;
+  a.rows = 8 * (int)std::min<int64_t>(most_tiles((int)kv.head_dim, ns), (pairs + 7) / 8);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
   int64_t keys = (int64_t)b.max_kv_len;
   if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
-  a.splits = attention_pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, quant_blocks((int)kv.head_dim, a.rows / 16),
+  a.splits = attention_pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, quant_blocks((int)kv.head_dim, a.rows / 8, ns),
                               kBlockKeys, false);
   a.direct = a.splits == 1;
   if (!a.direct)

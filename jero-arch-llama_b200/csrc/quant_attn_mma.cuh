@@ -1,89 +1,72 @@
 // Attention of few query rows over a paged cache of 8- or 4-bit codes on the
-// warp-level matrix instructions (mma.sync m16n8k16).  Included by quant_attn.cu.
+// warp-level integer matrix instructions (mma.sync m16n8k32).  Included by
+// quant_attn.cu.
 //
 //   out = sum_t softmax(scale * dk[t] * (q . ck[t])) * dv[t] * cv[t]
 //
-// with codes c and scales d.  Codes are whole numbers of at most 8 bits, which f16
-// holds exactly, so the products run over codes, and the scales multiply scores and
-// weights in f32: nothing of the cache is rounded.  q is carried as NS f16 parts of
-// the row times a power of two (one part for 16-bit rows, which is exact for f16 and for
-// bf16 down to 2^-27 of the row's largest; two, 22 bits, for f32 rows), and so are
-// the weights times dv.
+// with codes c and scales d.  Codes enter the products as they are stored: a warp that
+// widened them to f16 first spent three quarters of its instructions on that (one
+// row a sequence of 28 heads over 64 caches of up to 8192 4-bit positions: 138 us;
+// so: 63 us).  q, and the weights times dv, are whole numbers over a power of two (q:
+// over the row's largest), in balanced digits of 8 bits, v = sum_i 256^i digit_i with
+// digit_i in [-128, 127]: two digits for 16-bit rows, four for f32.  The products
+// of the digits are exact, and are put together in f32.
 //
-// A block takes MT tiles of 16 query rows of one KV head (the query heads of a
-// group, and neighbouring tokens); its four warps take 16 keys each in turn, and
+// A 16-row tile of the instruction holds eight query rows: rows i and i + 8 are the
+// upper and lower digit of row i, so one thread has both.  The weights of 32 keys
+// are numbers over the power of two below the largest of them, so their share is kept
+// however far below the row's maximum they lie, and their products are added to the
+// f32 output for each 32 keys.  An accumulator starts at 1.5 * 2^23 as f32 bits: read
+// as f32, it is that plus the sum, exactly.
+//
+// Errors: q is off by 2^-16 of the row's largest element (16-bit rows; f32: 2^-24 of
+// itself), a weight by 2^-15 (2^-30) of the largest of its 32 keys'.
+//
+// A block takes R8 tiles of eight query rows of one KV head (the query heads of a
+// group, and neighbouring tokens); its four warps take 32 keys each in turn, and
 // each is on its own until the end: it copies its keys' codes and scales with cp.async
 // into its own ring, and has its own running maxima, sums and output.
-//
-// A product's terms may be summed in any order, so the fragments of K take the dims
-// in the order in which a lane finds them in 16 bytes of a row, and q is laid out
-// to match; the columns of V's fragments are the dims that a lane has of one
-// row, and the result is put in order at the end.  A code becomes f16 by
-// being placed in the low mantissa bits of 1024 (its sum with 1024, exactly), from
-// which 1024 and the code's offset are subtracted.
 #pragma once
 
 #include "paged_attn_mma.cuh"
+#include "paged_attn_tc.cuh"
 #include "quant_kv.hpp"
 
 namespace jal {
 namespace paged {
 
-// f16 weights times dv refer to kQuantHeadroom less than the running maximum and to
-// the power of two below the largest |dv| so far: they stay below 2^15, and each
-// is off by 2^-25 beside its relative error.
-constexpr int kQuantHeadroom = 13;
+constexpr int kQuantKeys = 32;
+constexpr uint32_t kIntZero = 0x4B400000u;  // 1.5 * 2^23 as f32: an integer sum of 0
+constexpr float kIntZeroF = 12582912.0f;
 
-__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
-  uint32_t v;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+// Products of signed bytes with signed (BITS = 8) or unsigned (4) ones.
+template <int BITS>
+__device__ __forceinline__ void imma(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BITS == 8)
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two 16 x 16 tiles of bytes, transposed: lane 4 g + j gets of each tile the rows
+// 4 j .. 4 j + 3 of column g, and of column g + 8.  Lane i gives row i's address.
+__device__ __forceinline__ void ldsm_bytes(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t v;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(a), "r"(b), "r"(c));
+__device__ __forceinline__ pair_t pair_bits(uint32_t a, uint32_t b) {
+  pair_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
   return v;
-}
-constexpr uint32_t kH2_1024 = 0x64006400u, kH2_1032 = 0x64086408u, kH2_1152 = 0x64806480u, kH2_16th = 0x2C002C00u,
-                   kH2_m72 = 0xD480D480u;
-
-// Codes of one 32-bit word of a row as pairs of f16: 8 bits, 4 codes: (0, 1), (2, 3);
-// 4 bits, 8 codes: (0, 4), (1, 5), (2, 6), (3, 7).
-template <int BITS>
-__device__ __forceinline__ void row_pairs(uint32_t w, uint32_t *pair) {
-  if constexpr (BITS == 8) {
-    w ^= 0x80808080u;
-    pair[0] = h2_sub(__byte_perm(w, kH2_1024, 0x5150), kH2_1152);
-    pair[1] = h2_sub(__byte_perm(w, kH2_1024, 0x5352), kH2_1152);
-  } else {
-    const uint32_t u = w >> 8;
-    pair[0] = h2_sub((w & 0x000F000Fu) | kH2_1024, kH2_1032);
-    pair[1] = h2_fma((w & 0x00F000F0u) | kH2_1024, kH2_16th, kH2_m72);
-    pair[2] = h2_sub((u & 0x000F000Fu) | kH2_1024, kH2_1032);
-    pair[3] = h2_fma((u & 0x00F000F0u) | kH2_1024, kH2_16th, kH2_m72);
-  }
-}
-// The same dim of two rows as a pair, for the 4 or 8 codes of a word of each.
-template <int BITS>
-__device__ __forceinline__ void column_pairs(uint32_t a, uint32_t b, uint32_t *pair) {
-  uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a, b, 0x7632);
-  if constexpr (BITS == 8) {
-    lo ^= 0x80808080u;
-    hi ^= 0x80808080u;
-    pair[0] = h2_sub(__byte_perm(lo, kH2_1024, 0x5250), kH2_1152);
-    pair[1] = h2_sub(__byte_perm(lo, kH2_1024, 0x5351), kH2_1152);
-    pair[2] = h2_sub(__byte_perm(hi, kH2_1024, 0x5250), kH2_1152);
-    pair[3] = h2_sub(__byte_perm(hi, kH2_1024, 0x5351), kH2_1152);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const uint32_t w = i ? hi : lo, u = w >> 8;
-      pair[4 * i] = h2_sub((w & 0x000F000Fu) | kH2_1024, kH2_1032);
-      pair[4 * i + 1] = h2_fma((w & 0x00F000F0u) | kH2_1024, kH2_16th, kH2_m72);
-      pair[4 * i + 2] = h2_sub((u & 0x000F000Fu) | kH2_1024, kH2_1032);
-      pair[4 * i + 3] = h2_fma((u & 0x00F000F0u) | kH2_1024, kH2_16th, kH2_m72);
-    }
-  }
 }
 
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool there) {
@@ -93,46 +76,65 @@ template <int BYTES>
 __device__ __forceinline__ void lds(uint32_t addr, uint32_t *w) {
   if constexpr (BYTES == 16)
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
-  else if constexpr (BYTES == 8)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
   else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
 }
 
-// Blocks on an SM, by registers.
-constexpr int quant_blocks(int hd, int mt) { return hd > 128 || mt > 1 ? 2 : 3; }
+// The digits of four whole numbers v, byte i of word d the digit d of number i.  NS = 1:
+// v + 128 in the low 16 bits of each x; NS = 2: v.
+template <int NS>
+__device__ __forceinline__ void digits(const uint32_t (&x)[4], uint32_t (&word)[2 * NS]) {
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) y[i] = NS == 1 ? x[i] : x[i] + 0x00808080u;
+  const uint32_t a = __byte_perm(y[0], y[1], 0x5140), b = __byte_perm(y[2], y[3], 0x5140);  // bytes 0 and 1 of both
+  word[0] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+  word[1] = __byte_perm(a, b, 0x7632);
+  if constexpr (NS == 2) {
+    word[1] ^= 0x80808080u;
+    const uint32_t c = __byte_perm(y[0], y[1], 0x7362), d = __byte_perm(y[2], y[3], 0x7362);
+    word[2] = __byte_perm(c, d, 0x5410) ^ 0x80808080u;
+    word[3] = __byte_perm(c, d, 0x7632);
+  }
+}
 
-template <int BITS, int NS, int HD, int MT>
+// Blocks on an SM, by registers and shared memory.
+constexpr int quant_blocks(int hd, int r8, int ns) { return hd > 128 ? 1 : r8 * ns > 2 ? 2 : 3; }
+
+template <int BITS, int NS, int HD, int R8>
 struct QuantShape {
-  static constexpr int blocks = quant_blocks(HD, MT);
-  static constexpr int rows = 16 * MT;
+  static constexpr int blocks = quant_blocks(HD, R8, NS);
+  static constexpr int rows = 8 * R8;
   static constexpr int row_bytes = HD * BITS / 8;
-  static constexpr int chunks = row_bytes / 16;           // 16-byte pieces of a row
-  static constexpr int half = kMmaKeys * row_bytes;       // bytes of a stage's K (or V)
-  static constexpr int stage = 2 * half + 2 * kMmaKeys * 4;
-  static constexpr int stages = row_bytes <= 64 ? 6 : row_bytes == 128 ? 4 : 3;
+  static constexpr int chunks = row_bytes / 16;            // 16-byte pieces of a row
+  static constexpr int half = kQuantKeys * row_bytes;      // bytes of a stage's K (or V)
+  static constexpr int stage = 2 * half + 2 * kQuantKeys * 4;
+  static constexpr int stages = row_bytes <= 32 ? 6 : row_bytes == 64 ? 4 : 2;
   static constexpr int ring = kMmaWarps * stages * stage;
-  static constexpr int q_part = HD / 16 * 512;            // one part of 16 rows, as fragments
-  static constexpr int q_bytes = NS * MT * q_part;
-  static constexpr int out_row = HD + HD / 4;             // floats of a row where warps' results are joined
+  static constexpr int ksteps = HD / 32;
+  static constexpr int q_bytes = NS * R8 * ksteps * 512;   // fragments
+  static constexpr int out_row = HD + 4;                   // floats of a row where warps' results are joined
   static constexpr int merge = kMmaWarps * rows * out_row * 4;
   static constexpr int smem = q_bytes + (ring > merge ? ring : merge);
-  // Where 16-byte piece c of key r lies: conflict-free for the lanes' reads of K (a
-  // quarter warp: two neighbouring keys, four pieces) and of V (keys two apart).
+  // Where 16-byte piece c of K's row r and V's row r lies, without conflicts between
+  // the lanes that read together: of K two neighbouring rows, four pieces; of V the same
+  // piece of eight rows.
   static __device__ __forceinline__ uint32_t k_at(int r, int c) {
     return r * row_bytes + ((chunks >= 8 ? c ^ ((r & 1) << 2) : c) * 16);
   }
   static __device__ __forceinline__ uint32_t v_at(int r, int c) {
-    const int pos = (r >> 1) | ((r & 1) << 3);
-    const int x = chunks == 16 ? (pos & 1) | ((pos & 2) << 1) : chunks == 8 ? (pos & 3) << 1 : chunks == 4 ? pos & 2 : 0;
-    return pos * row_bytes + ((c ^ x) * 16);
+    const int x = chunks >= 8 ? r & 7 : chunks == 4 ? (r >> 1) & 3 : (r >> 2) & 1;
+    return r * row_bytes + ((c ^ x) * 16);
   }
+  // V's row for key i: a lane of the scores has keys 2 j, 2 j + 1 of every eight, and of
+  // the weights the rows 4 j .. 4 j + 3 of every sixteen.
+  static __device__ __forceinline__ int v_row(int i) { return (i & 16) | ((i & 6) << 1) | ((i & 8) >> 2) | (i & 1); }
 };
 
-template <int BITS, int NS, int HD, int MT>
-__global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, MT>::blocks)
+template <int BITS, int NS, int HD, int R8>
+__global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blocks)
     k_quant_attn_mma(const __grid_constant__ QuantAttnParams qp, const bool direct) {
-  using S = QuantShape<BITS, NS, HD, MT>;
+  using S = QuantShape<BITS, NS, HD, R8>;
   const AttnParams &p = qp.a;
   extern __shared__ __align__(128) char smem_raw[];
   __shared__ RowMask masks[S::rows];
@@ -141,38 +143,37 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, MT>::blo
   __shared__ uint32_t present[kMmaWarps][S::stages];
   pdl_trigger();
   Tile t;
-  if (!block_tile(p, kOwn, S::rows, kMmaWarps * kMmaKeys, t)) {
+  if (!block_tile(p, kOwn, S::rows, kMmaWarps * kQuantKeys, t)) {
     pdl_wait();
     return;
   }
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, hd = p.kv.hd;
-  const int n8 = lane / 4, j4 = lane % 4;  // this lane's key (or column), and quarter
+  const int g = lane / 4, j4 = lane % 4;  // this lane's row (or column), and quarter
   const uint32_t sq = smem_u32(smem_raw), ring = sq + S::q_bytes + warp * (S::stages * S::stage);
 
-  // This warp's keys: chunks of 16 of [u0, u1), every fourth.  Lanes i and i + 16
-  // look up where key i of a chunk lies, one chunk ahead of its copies.
-  const int n_chunks = (t.u1 - t.u0 + kMmaKeys - 1) / kMmaKeys;
+  // This warp's keys: chunks of 32 of [u0, u1), every fourth.  A lane looks up where
+  // its key of a chunk lies, one chunk ahead of the copies.
+  const int n_chunks = (t.u1 - t.u0 + kQuantKeys - 1) / kQuantKeys;
   auto locate = [&](int c) -> Slot {
-    const int u = t.u0 + c * kMmaKeys + lane % kMmaKeys;
+    const int u = t.u0 + c * kQuantKeys + lane;
     return c < n_chunks && u < t.u1 ? slot_of(p.kv, t, t.key(u)) : Slot{-1, 0};
   };
   auto copy = [&](const Slot &where, int stage) {
     const int64_t at = slot_offset(p.kv, where, t.head);
     const uint32_t dst = ring + stage * S::stage;
-    const uint32_t bits = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
+    const uint32_t bits = __ballot_sync(0xffffffffu, at >= 0);
     if (lane == 0) present[warp][stage] = bits;
-    {  // lane i: K's scale of key i; lane i + 16: V's
-      const int64_t e = at >= 0 ? (int64_t)where.page * qp.sc.s_page + t.head * qp.sc.s_head + where.slot : 0;
-      copy4(dst + 2 * S::half + lane * 4, (lane < kMmaKeys ? qp.sc.k : qp.sc.v) + e, at >= 0);
-    }
+    const int64_t e = at >= 0 ? (int64_t)where.page * qp.sc.s_page + t.head * qp.sc.s_head + where.slot : 0;
+    copy4(dst + 2 * S::half + lane * 4, qp.sc.k + e, at >= 0);
+    copy4(dst + 2 * S::half + kQuantKeys * 4 + lane * 4, qp.sc.v + e, at >= 0);
 #pragma unroll
-    for (int i = 0; i < S::chunks / 2; i++) {
+    for (int i = 0; i < S::chunks; i++) {
       const int r = (i * 32 + lane) / S::chunks, c = (i * 32 + lane) % S::chunks;
       const int64_t o = __shfl_sync(0xffffffffu, at, r);
       const bool there = o >= 0 && c * (128 / BITS) < hd;
-      const int64_t e = there ? o + c * 16 : 0;
-      copy16(dst + S::k_at(r, c), (const char *)p.kv.k + e, there);
-      copy16(dst + S::half + S::v_at(r, c), (const char *)p.kv.v + e, there);
+      const int64_t x = there ? o + c * 16 : 0;
+      copy16(dst + S::k_at(r, c), (const char *)p.kv.k + x, there);
+      copy16(dst + S::half + S::v_at(S::v_row(r), c), (const char *)p.kv.v + x, there);
     }
     copies_done();
   };
@@ -183,78 +184,108 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, MT>::blo
     next = locate(warp + (i + 1) * kMmaWarps);
     copy(at, i);
   }
-  // Query rows into shared memory as fragments: a row times 2^e, so that its
-  // largest element lies in [2^13, 2^14), in NS f16 parts.  Eight threads a row.
-#pragma unroll 1
-  for (int m = 0; m < MT; m++) {
-    const int r = tid / 8, j = m * 16 + r, sub = tid % 8;
-    const bool real = j < t.rows;
-    const int64_t qo = real ? q_offset(p, t, j) : 0;
-    constexpr int N = HD / 8;  // dims of a thread: fragments ks = sub, sub + 8, .. whole (16 dims each) or halves
-    float v[N];
-    float top = 0.0f;
+  // Query rows into shared memory as fragments of digits.  Sixteen threads a row; a
+  // thread has the four dims that make one word of a fragment.
+  {
+    const int r = tid / 16, sub = tid % 16;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      // Thread `sub` has the dims sub * 2 + (i / 2) * 16 + i % 2.
-      const int d = sub * 2 + (i / 2) * 16 + i % 2;
-      v[i] = real && d < hd ? load_as_f32(p.q, qo + d, p.act) : 0.0f;
-      if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
-    }
+    for (int m = 0; m < R8; m++) {
+      const int j = m * 8 + r;
+      const bool real = j < t.rows;
+      const int64_t qo = real ? q_offset(p, t, j) : 0;
+      constexpr int W = HD / 64;  // words of a thread
+      float v[W][4];
+      uint32_t top = 0;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = top > 0.0f ? 13 - ilogbf(top) : 0;
-    // in two steps: 2^e itself may lie outside f32's range
-    const float a = exp2f((float)(e / 2)), b = exp2f((float)(e - e / 2));
-    if (sub == 0) {
-      masks[j] = real ? row_mask(p, t, j) : RowMask{0, 0};
-      q_scale[j] = p.scale_log2 * ((1.0f / a) / b);
-    }
+      for (int w = 0; w < W; w++) {
+        // Word `sub + 16 w` of the row: fragment ks, quarter jj, half h; its dims as a lane
+        // finds them in 16 (or 8) bytes of a row of K.
+        const int at = sub + 16 * w, ks = at / 8, jj = at / 2 % 4, h = at % 2;
+        constexpr int per = (S::chunks >= 4 ? 128 : 64) / BITS;  // codes that a lane reads at once
+        const int piece = ks / (per / 8), x = ks % (per / 8);
+        const int base = (piece * 4 + jj) * per + x * 8;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int d = sub * 2 + (i / 2) * 16 + i % 2;
-      // Where the lanes find dim d in a row of K: quarter jj, word w of it, code c of
-      // the word; the word's pairs are halves of the fragments ks.
-      constexpr int codes = 32 / BITS, lane_bytes = S::chunks >= 4 ? 16 : 8, per_lane = lane_bytes * 8 / BITS;
-      const int piece = d / (4 * per_lane), jj = d / per_lane % 4, w = d % per_lane / codes, c = d % codes;
-      const int pr = BITS == 8 ? c / 2 : c % 4, h = BITS == 8 ? c % 2 : c / 4;
-      const int ks = piece * (per_lane / 4) + w * (codes / 4) + pr / 2, reg = (pr % 2) * 2 + (r >= 8 ? 1 : 0);
-      float x = v[i] * a * b;
+        for (int i = 0; i < 4; i++) {
+          const int d = BITS == 8 ? base + h * 4 + i : base + 2 * i + h;
+          v[w][i] = real && d < hd ? load_as_f32(p.q, qo + d, p.act) : 0.0f;
+          top = max(top, __float_as_uint(v[w][i]) & 0x7fffffffu);  // (a NaN's bits are above infinity's)
+        }
+      }
 #pragma unroll
-      for (int s = 0; s < NS; s++) {
-        const __half part = __float2half_rn(x);
-        x -= __half2float(part);
-        *(__half *)(smem_raw + (s * MT + m) * S::q_part + ks * 512 + ((r % 8) * 4 + jj) * 16 + reg * 4 + h * 2) = part;
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      constexpr float whole = NS == 1 ? 127.0f * 256.0f : 127.0f * 16777216.0f;
+      const float most = __uint_as_float(top);
+      const bool some = most >= kQuantLeast && most < INFINITY;
+      const float over = some ? whole / most : 0.0f;
+      if (sub == 0) {
+        masks[j] = real ? row_mask(p, t, j) : RowMask{0, 0};
+        // (A row with a NaN or an infinity has NaN scores.)
+        q_scale[j] = some ? p.scale_log2 * (most / whole) : most < INFINITY ? 0.0f : NAN;
+      }
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        const int at = sub + 16 * w, ks = at / 8, jj = at / 2 % 4, h = at % 2;
+        uint32_t x[4], word[2 * NS];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = some ? (uint32_t)__float2int_rn(v[w][i] * over) : 0u;
+        if (NS == 1)
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[i] += 128u;
+        digits<NS>(x, word);
+#pragma unroll
+        for (int s = 0; s < NS; s++) {  // fragment s: the digits 2 (NS - 1 - s) + 1 and below it
+          char *const f = smem_raw + ((s * R8 + m) * S::ksteps + ks) * 512 + (r * 4 + jj) * 16 + h * 8;
+          *(uint32_t *)f = word[2 * (NS - 1 - s) + 1];
+          *(uint32_t *)(f + 4) = word[2 * (NS - 1 - s)];
+        }
       }
     }
   }
   __syncthreads();
 
-  // Rows 16 m + lane / 4 and that + 8 are this lane's.
   // Rows that do not exist see everything: they have no say in what is masked.
   const RowSpan every = {0x7fffffff, 0, 0};
-  RowSpan span[MT][2];
-  float f[MT][2];
+  RowSpan span[R8];
+  float f[R8];
+  float top[R8], l[R8];  // running maxima, which the weights refer to, and their sums
+  pair_t o[R8][HD / 8];
+  // Where an accumulator of scores starts: 4-bit codes are stored with 8 added.
+  uint32_t start[R8][NS][2];
 #pragma unroll
-  for (int m = 0; m < MT; m++)
+  for (int m = 0; m < R8; m++) {
+    const int r = m * 8 + g;
+    span[m] = r < t.rows ? row_span(p, t, masks[r]) : every;
+    f[m] = q_scale[r];
+    top[m] = -INFINITY;
+    l[m] = 0.0f;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = m * 16 + h * 8 + n8;
-      span[m][h] = r < t.rows ? row_span(p, t, masks[r]) : every;
-      f[m][h] = q_scale[r];
-    }
-  float o[MT][HD / 8][4];
-  float top[MT][2], ref[MT][2], l[MT][2];  // running maxima, what the weights refer to, their sums
+    for (int i = 0; i < HD / 8; i++) o[m][i] = 0;
 #pragma unroll
-  for (int m = 0; m < MT; m++) {
+    for (int s = 0; s < NS; s++) {
+      uint32_t c[4] = {kIntZero, kIntZero, kIntZero, kIntZero};
+      if (BITS == 4) {
 #pragma unroll
-    for (int i = 0; i < HD / 8; i++) o[m][i][0] = o[m][i][1] = o[m][i][2] = o[m][i][3] = 0.0f;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      top[m][h] = ref[m][h] = -INFINITY;
-      l[m][h] = 0.0f;
+        for (int ks = 0; ks < S::ksteps; ks++) {
+          uint32_t a[4];
+          lds<16>(sq + ((s * R8 + m) * S::ksteps + ks) * 512 + lane * 16, a);
+          imma<8>(c, a, 0xF8F8F8F8u, 0xF8F8F8F8u);
+        }
+      }
+      start[m][s][0] = c[0];
+      start[m][s][1] = c[2];
     }
   }
-  int unit = 1;  // V's scales are taken over 2^(unit - 127)
+  const pair_t minus = pair(-kIntZeroF, -kIntZeroF), digit = pair(256.0f, 256.0f);
+  // What accumulators of the digits hold, in f32.
+  auto whole_pair = [&](const uint32_t (&c)[NS][4]) -> pair_t {
+    const pair_t hi = add2(pair_bits(c[0][0], c[0][1]), minus), lo = add2(pair_bits(c[0][2], c[0][3]), minus);
+    pair_t v = fma2(hi, digit, lo);
+    if constexpr (NS == 2) {
+      const pair_t hi1 = add2(pair_bits(c[1][0], c[1][1]), minus), lo1 = add2(pair_bits(c[1][2], c[1][3]), minus);
+      v = fma2(v, pair(65536.0f, 65536.0f), fma2(hi1, digit, lo1));
+    }
+    return v;
+  };
 
   int stage = 0;
 #pragma unroll 1
@@ -271,157 +302,141 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, MT>::blo
     __syncwarp();
     const uint32_t kb = ring + stage * S::stage, vb = kb + S::half, sb = vb + S::half;
     const uint32_t bits = present[warp][stage];
-    float s[MT][2][4] = {};
-    {
-      constexpr int lane_bytes = S::chunks >= 4 ? 16 : 8, words = lane_bytes / 4, codes = 32 / BITS;
-      constexpr int pieces = S::row_bytes / (4 * lane_bytes);
+    // Scores: the lane has keys 8 n + 2 j4 and the next one.
+    pair_t s[R8][4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      uint32_t acc[R8][NS][4];
+#pragma unroll
+      for (int m = 0; m < R8; m++)
+#pragma unroll
+        for (int q = 0; q < NS; q++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[m][q][e] = BITS == 4 ? start[m][q][e / 2] : kIntZero;
+      constexpr int lane_bytes = S::chunks >= 4 ? 16 : 8, words = lane_bytes / 4, pieces = S::row_bytes / (4 * lane_bytes);
 #pragma unroll
       for (int pc = 0; pc < pieces; pc++) {
-        uint32_t w[2][words];
+        uint32_t w[words];
+        if constexpr (lane_bytes == 16) lds<16>(kb + S::k_at(n * 8 + g, pc * 4 + j4), w);
+        else lds<8>(kb + S::k_at(n * 8 + g, 0) + j4 * 8, w);
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          if constexpr (lane_bytes == 16) lds<16>(kb + S::k_at(n * 8 + n8, pc * 4 + j4), w[n]);
-          else lds<8>(kb + S::k_at(n * 8 + n8, 0) + j4 * 8, w[n]);
-        }
+        for (int x = 0; x < words * 4 / BITS; x++) {
+          const int ks = pc * (words * 4 / BITS) + x;
+          const uint32_t b0 = BITS == 8 ? w[(2 * x) % words] : w[x % words] & 0x0F0F0F0Fu;
+          const uint32_t b1 = BITS == 8 ? w[(2 * x + 1) % words] : (w[x % words] >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-        for (int x = 0; x < words; x++) {
-          uint32_t b[2][codes / 2];
-          row_pairs<BITS>(w[0][x], b[0]);
-          row_pairs<BITS>(w[1][x], b[1]);
+          for (int m = 0; m < R8; m++)
 #pragma unroll
-          for (int k = 0; k < codes / 4; k++) {
-            const int ks = (pc * words + x) * (codes / 4) + k;
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-              for (int i = 0; i < NS; i++) {
-                uint32_t a[4];
-                lds<16>(sq + (i * MT + m) * S::q_part + ks * 512 + lane * 16, a);
-                mma16816<__half>(s[m][0], a, b[0][2 * k], b[0][2 * k + 1]);
-                mma16816<__half>(s[m][1], a, b[1][2 * k], b[1][2 * k + 1]);
-              }
-          }
+            for (int q = 0; q < NS; q++) {
+              uint32_t a[4];
+              lds<16>(sq + ((q * R8 + m) * S::ksteps + ks) * 512 + lane * 16, a);
+              imma<BITS>(acc[m][q], a, b0, b1);
+            }
         }
       }
+#pragma unroll
+      for (int m = 0; m < R8; m++) s[m][n] = whole_pair(acc[m]);
     }
-    // Scales of this lane's keys: 2 j4, 2 j4 + 1 and those + 8.
-    uint32_t dkw[2][2], dvw[2][2];
-    lds<8>(sb + j4 * 8, dkw[0]);
-    lds<8>(sb + 32 + j4 * 8, dkw[1]);
-    lds<8>(sb + 64 + j4 * 8, dvw[0]);
-    lds<8>(sb + 96 + j4 * 8, dvw[1]);
-    const int u = t.u0 + c * kMmaKeys;
-    bool whole = bits == 0xffffu;
+    const int u = t.u0 + c * kQuantKeys;
+    bool all = bits == 0xffffffffu;
 #pragma unroll
-    for (int m = 0; m < MT; m++) whole = whole && span[m][0].all(u, kMmaKeys) && span[m][1].all(u, kMmaKeys);
-    const bool masked = __any_sync(0xffffffffu, !whole);
-    uint32_t see[MT][2];
+    for (int m = 0; m < R8; m++) all = all && span[m].all(u, kQuantKeys);
+    const bool masked = __any_sync(0xffffffffu, !all);
+    uint32_t wa[R8][NS][4];
+    float unit[R8];  // what the whole numbers of the weights count
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int m = 0; m < R8; m++) {
+      float y[8];
 #pragma unroll
-      for (int h = 0; h < 2; h++) see[m][h] = masked ? bits & span[m][h].bits(u) : 0xffffffffu;
-    // A larger scale of V than any before: the output is taken over its power of two.
-    {
-      uint32_t most = 0;
+      for (int n = 0; n < 4; n++) {
+        uint32_t dk[2];
+        lds<8>(sb + n * 32 + j4 * 8, dk);
+        unpair(mul2(s[m][n], mul2(pair_bits(dk[0], dk[1]), pair(f[m], f[m]))), y[2 * n], y[2 * n + 1]);
+      }
+      if (masked) {
+        const uint32_t see = (bits & span[m].bits(u)) >> (2 * j4);
 #pragma unroll
-      for (int n = 0; n < 2; n++)
+        for (int i = 0; i < 8; i++)
+          if (!((see >> (i / 2 * 8 + i % 2)) & 1)) y[i] = -INFINITY;
+      }
+      float most = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(top[m], fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)));
+      if (__any_sync(0xffffffffu, most != top[m])) {
+        const float less = most == top[m] ? 1.0f : exp2_fast(top[m] - most);
+        top[m] = most;
+        l[m] *= less;
+#pragma unroll
+        for (int i = 0; i < HD / 8; i++) o[m][i] = mul2(o[m][i], pair(less, less));
+      }
+      const float ref = top[m] == -INFINITY ? 0.0f : top[m];
+      uint32_t big = 0;
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        uint32_t dv[2];
+        lds<8>(sb + kQuantKeys * 4 + n * 32 + j4 * 8, dv);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          const uint32_t x = dvw[n][e] & 0x7fffffffu;
-          most = max(most, x < 0x7f800000u ? x : 0u);
+          float &x = y[2 * n + e];
+          const bool seen = !masked || x != -INFINITY;  // (what a row does not see has no effect on it)
+          x = exp2_fast(x - ref);
+          l[m] += x;
+          x = seen ? x * __uint_as_float(dv[e]) : 0.0f;
+          big = max(big, __float_as_uint(x) & 0x7fffffffu);
         }
-      const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 23), 253);
-      if (e > unit) {
-        const float less = exp2f((float)(unit - e));
-        unit = e;
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int i = 0; i < HD / 8; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) o[m][i][q] *= less;
       }
-    }
-    const float over = __uint_as_float((uint32_t)(254 - unit) << 23);  // 2^(127 - unit)
-    uint32_t w[MT][NS][4];
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-      bool raise = false;
-      float now[2];
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // The weights over 2^(e - 13) (four digits: 2^(e - 29)), e the largest one's exponent.
+      constexpr int kShift = NS == 1 ? 13 : 29;
+      const int e = (int)(big >> 23);
+      const bool some = e > kShift;  // smaller ones than 2^(kShift - 127) count as 0
+      const float over = some ? __uint_as_float((uint32_t)min(254 + kShift - e, 254) << 23) : 0.0f;
+      unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - kShift) << 23) : 0.0f;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
+        uint32_t x[4], word[2 * NS];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int i = 0; i < 4; i++)
+          x[i] = NS == 1 ? __float_as_uint(fmaf(y[4 * h + i], over, kIntZeroF + 128.0f)) : (uint32_t)__float2int_rn(y[4 * h + i] * over);
+        digits<NS>(x, word);
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float &x = s[m][n][2 * h + e];
-            x = x * f[m][h] * __uint_as_float(dkw[n][e]);
-            if (masked && !((see[m][h] >> (n * 8 + j4 * 2 + e)) & 1)) x = -INFINITY;
-          }
-        float x = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        now[h] = fmaxf(top[m][h], fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)));
-        raise = raise || now[h] != top[m][h];
-      }
-      if (__any_sync(0xffffffffu, raise)) {
-        float less[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const float r = reference_of<kQuantHeadroom>(now[h]);
-          less[h] = now[h] == top[m][h] ? 1.0f : exp2_fast(ref[m][h] - r);
-          top[m][h] = now[h];
-          ref[m][h] = r;
-          l[m][h] *= less[h];
-        }
-#pragma unroll
-        for (int i = 0; i < HD / 8; i++)
-#pragma unroll
-          for (int q = 0; q < 4; q++) o[m][i][q] *= less[q / 2];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const float r = ref[m][h] == -INFINITY ? 0.0f : ref[m][h];
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          float x[2];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            x[e] = exp2_fast(s[m][n][2 * h + e] - r);
-            l[m][h] += x[e];
-            x[e] *= __uint_as_float(dvw[n][e]) * over;
-            // (What a row does not see has no effect on it, whatever its scale is.)
-            if (masked && !((see[m][h] >> (n * 8 + j4 * 2 + e)) & 1)) x[e] = 0.0f;
-          }
-          uint32_t part[NS];
-          split2<__half, NS>(x[0], x[1], part);
-#pragma unroll
-          for (int i = 0; i < NS; i++) w[m][i][2 * n + h] = part[i];
+        for (int q = 0; q < NS; q++) {
+          wa[m][q][2 * h] = word[2 * (NS - 1 - q) + 1];
+          wa[m][q][2 * h + 1] = word[2 * (NS - 1 - q)];
         }
       }
     }
-    {
-      // V: this lane's dims are n8 * (HD / 8) .., its keys 2 j4, 2 j4 + 1 and those + 8.
-      constexpr int lane_bytes = S::row_bytes / 8, step = lane_bytes < 16 ? lane_bytes : 16, codes = 32 / BITS;
+    // The output: the lane's columns are 2 j4, 2 j4 + 1 of every eight.
+    uint32_t first[R8][NS][4];
 #pragma unroll
-      for (int pc = 0; pc < lane_bytes / step; pc++) {
-        uint32_t x[4][step / 4];
+    for (int m = 0; m < R8; m++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int key = j4 * 2 + k % 2 + (k / 2) * 8, byte = n8 * lane_bytes + pc * 16;
-          lds<step>(vb + S::v_at(key, byte / 16) + byte % 16, x[k]);
-        }
+      for (int q = 0; q < NS; q++) {
+        first[m][q][0] = first[m][q][1] = first[m][q][2] = first[m][q][3] = kIntZero;
+        if (BITS == 4) imma<8>(first[m][q], wa[m][q], 0xF8F8F8F8u, 0xF8F8F8F8u);
+      }
 #pragma unroll
-        for (int y = 0; y < step / 4; y++) {
-          uint32_t b0[codes], b1[codes];
-          column_pairs<BITS>(x[0][y], x[1][y], b0);
-          column_pairs<BITS>(x[2][y], x[3][y], b1);
+    for (int ch = 0; ch < S::chunks; ch++) {
+      uint32_t b[4];
+      ldsm_bytes(b, vb + S::v_at(lane, ch));
 #pragma unroll
-          for (int k = 0; k < codes; k++)
+      for (int x = 0; x < 2 * 8 / BITS; x++) {
+        // 8 bits: columns 0 .. 7, 8 .. 15.  4 bits: the low, then the high halves of each.
+        const int h = BITS == 8 ? x : x / 2;
+        const uint32_t b0 = BITS == 8 ? b[h] : (b[h] >> (x % 2 * 4)) & 0x0F0F0F0Fu;
+        const uint32_t b1 = BITS == 8 ? b[h + 2] : (b[h + 2] >> (x % 2 * 4)) & 0x0F0F0F0Fu;
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+        for (int m = 0; m < R8; m++) {
+          uint32_t acc[NS][4];
 #pragma unroll
-              for (int i = 0; i < NS; i++)
-                mma16816<__half>(o[m][(pc * (step / 4) + y) * codes + k], w[m][i], b0[k], b1[k]);
+          for (int q = 0; q < NS; q++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[q][i] = first[m][q][i];
+            imma<BITS>(acc[q], wa[m][q], b0, b1);
+          }
+          pair_t &out = o[m][ch * (2 * 8 / BITS) + x];
+          out = fma2(whole_pair(acc), pair(unit[m], unit[m]), out);
         }
       }
     }
@@ -431,24 +446,29 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, MT>::blo
   copies_wait<0>();
   __syncthreads();  // no warp reads its ring any more
   pdl_wait();
-  // The four warps' results, joined through shared memory: element (i, n) of a row, dim
-  // n * (HD / 8) + i, at i * 8 + n + i / 4 * 8.
+  // The four warps' results, joined through shared memory.
   float *const merge = (float *)(smem_raw + S::q_bytes);
-  const float back = exp2f((float)(unit - 127));
 #pragma unroll
-  for (int m = 0; m < MT; m++)
+  for (int m = 0; m < R8; m++) {
+    float x = l[m];
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    x += __shfl_xor_sync(0xffffffffu, x, 2);
+    const int r = m * 8 + g;
+    if (j4 == 0) row_ml[warp][r] = make_float2(top[m], x);
+    float *const a = merge + (warp * S::rows + r) * S::out_row;
+    if constexpr (BITS == 8) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float x = l[m][h];
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      const int r = m * 16 + h * 8 + n8;
-      if (j4 == 0) row_ml[warp][r] = make_float2(ref[m][h], x);
-      float *const a = merge + (warp * S::rows + r) * S::out_row + j4 * 2;
+      for (int i = 0; i < HD / 8; i++) *(pair_t *)(a + i * 8 + j4 * 2) = o[m][i];
+    } else {
 #pragma unroll
-      for (int i = 0; i < HD / 8; i++)
-        *(float2 *)(a + i * 8 + i / 4 * 8) = make_float2(o[m][i][2 * h] * back, o[m][i][2 * h + 1] * back);
+      for (int i = 0; i < HD / 8; i += 2) {  // low and high halves: dims 4 j4, + 2 and + 1, + 3 of every sixteen
+        float x0, x1, x2, x3;
+        unpair(o[m][i], x0, x2);
+        unpair(o[m][i + 1], x1, x3);
+        *(float4 *)(a + i * 8 + j4 * 4) = make_float4(x0, x1, x2, x3);
+      }
     }
+  }
   __syncthreads();
   for (int i = tid; i < t.rows * (HD / 4); i += kMmaThreads) {
     const int j = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -457,32 +477,33 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, MT>::blo
 #pragma unroll
     for (int w = 0; w < kMmaWarps; w++) most = fmaxf(most, row_ml[w][j].x);
     const float safe = most == -INFINITY ? 0.0f : most;
-    float sum[4] = {};
-    const int n = d / (HD / 8), i0 = d % (HD / 8);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kMmaWarps; w++) {
       const float2 ml = row_ml[w][j];
       if (ml.y == 0.0f) continue;
       const float a = exp2f(ml.x - safe);
+      const float4 v = *(const float4 *)(merge + (w * S::rows + j) * S::out_row + d);
       sum_l = fmaf(a, ml.y, sum_l);
-      const float *const v = merge + (w * S::rows + j) * S::out_row + i0 * 8 + n + i0 / 4 * 8;
-#pragma unroll
-      for (int q = 0; q < 4; q++) sum[q] = fmaf(a, v[q * 8], sum[q]);
+      sum.x = fmaf(a, v.x, sum.x);
+      sum.y = fmaf(a, v.y, sum.y);
+      sum.z = fmaf(a, v.z, sum.z);
+      sum.w = fmaf(a, v.w, sum.w);
     }
     if (direct) {
       const float inv = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
       const int64_t oo = out_offset(p, t, j) + d;
       if (p.act == JAL_F32)
-        *(float4 *)((float *)p.out + oo) = make_float4(sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv);
+        *(float4 *)((float *)p.out + oo) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
       else if (p.act == JAL_F16)
-        *(uint2 *)((__half *)p.out + oo) = make_uint2(pack2<__half>(sum[0] * inv, sum[1] * inv), pack2<__half>(sum[2] * inv, sum[3] * inv));
+        *(uint2 *)((__half *)p.out + oo) = make_uint2(pack2<__half>(sum.x * inv, sum.y * inv), pack2<__half>(sum.z * inv, sum.w * inv));
       else
         *(uint2 *)((__nv_bfloat16 *)p.out + oo) =
-            make_uint2(pack2<__nv_bfloat16>(sum[0] * inv, sum[1] * inv), pack2<__nv_bfloat16>(sum[2] * inv, sum[3] * inv));
+            make_uint2(pack2<__nv_bfloat16>(sum.x * inv, sum.y * inv), pack2<__nv_bfloat16>(sum.z * inv, sum.w * inv));
     } else {
       const int64_t pi = part_index(p, t, j);
       if (d == 0) p.part_ml[pi] = make_float2(most, sum_l);
-      *(float4 *)(p.part_o + pi * hd + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      *(float4 *)(p.part_o + pi * hd + d) = sum;
     }
   }
 }

@@ -354,24 +354,37 @@ def test_scales_that_rows_must_not_meet(jal, torch_cuda, act, which, value, news
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("news", [2, 80])
 def test_scales_of_many_sizes(jal, torch_cuda, act, bits, news):
-    # Scales spread over 2^-16 .. 2^16, growing and shrinking along the keys.  2^-33 of the largest weight (at most 1)
-    # times V's largest scale, times 128 for a code, for each of the keys.
+    # Scales spread over 2^-16 .. 2^16 along the keys.
     c = QuantCase([700], [news], 2, 1, 64, act=act, bits=bits, page=16, spread=4.0).to_device(jal)
     ref = c.reference(1e-3)
-    far = float(torch.nan_to_num(c.scales[1]).max()) * 2.0 ** -33 * 128 * 700
-    _near(c, _attend(jal, c, 1e-3), ref, c.bound(ref, far))
+    _near(c, _attend(jal, c, 1e-3), ref, c.bound(ref))
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("news", [1, 80])
 def test_one_key_far_above_a_tail(jal, torch_cuda, news):
-    # Two codes at the ends: the tail's weights are 14 nats below one key's, and make the result's small part.
+    # One key takes nearly all of the weight and its value is 0: what is left of the result is the others', 17 nats
+    # below, which keep their share.
     c = QuantCase([3000], [news], 1, 1, 64, act="f16", bits=8, page=64)
-    c.set_scale(0, 0, 7, 0.0)
-    ref = c.reference(2.0)
+    for t in range(3000):
+        c.set_scale(0, 0, t, 0.0)
+    q = torch.randn(1, 1, 64, generator=torch.Generator().manual_seed(4)).to(c.act)
+    c.q_full[:] = q.reshape(1, 64)
+    c.q[:] = q
+    codes, scale = coded(q[0].float(), 8)
+    view = c.raw[0].permute([c.layout.index(x) for x in "phsd"])
+    at = 7
+    view[int(c.table[0, at // 64]), 0, at % 64] = packed(codes[0], 8)
+    c.set_scale(0, 0, at, float(17 / float((codes[0].double() * q[0, 0].double()).sum())))
+    c.set_scale(1, 0, at, 0.0)
+    ref = c.reference(1.0)
     c.to_device(jal)
-    far = float(torch.nan_to_num(c.scales[1]).max()) * 2.0 ** -33 * 128 * 3000
-    _near(c, _attend(jal, c, 2.0), ref, c.bound(ref, far))
+    out = _attend(jal, c, 1.0)
+    _near(c, out, ref, c.bound(ref))
+    # (the tail alone, to 2^-8 of its size)
+    tail = c.v[0].mean(0)[0] * 3000 * math.exp(-17) / (1 + 3000 * math.exp(-17))
+    got = out.cpu().double()[news - 1]
+    assert bool(((got - tail).abs() <= 2.0 ** -8 * tail.abs() + 2.0 ** -24).all())
 
 
 @pytest.mark.gpu
