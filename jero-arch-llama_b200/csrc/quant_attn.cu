@@ -4,6 +4,7 @@
 
 #include "common.hpp"
 #include "quant_attn_mma.cuh"
+#include "quant_attn_tc.cuh"
 
 namespace jal {
 
@@ -24,7 +25,18 @@ void run_mma(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s
   JAL_CUDA(cudaGetLastError());
 }
 template <int BITS, int NS, int HD>
+void run_tc(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
+  const int64_t blocks = (int64_t)p.a.kv.hkv * p.a.splits * p.a.tiles * p.a.n_seqs;
+  constexpr int smem = QuantTcShape<NS, HD>::smem;
+  JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_tc<BITS, NS, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  k_quant_attn_tc<BITS, NS, HD><<<(unsigned)blocks, kTcThreads, smem, s>>>(p, plan.direct);
+  JAL_CUDA(cudaGetLastError());
+}
+template <int BITS, int NS, int HD>
 void run_rows(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
+  if constexpr (HD <= 128) {
+    if (plan.rows == kTcRows) return run_tc<BITS, NS, HD>(p, plan, s);
+  }
   if (plan.rows == 8) return run_mma<BITS, NS, HD, 1>(p, plan, s);
   if constexpr (most_tiles(HD, NS) >= 3) {
     if (plan.rows == 24) return run_mma<BITS, NS, HD, 3>(p, plan, s);
@@ -44,6 +56,8 @@ void run_type(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t 
 }
 
 constexpr int64_t kBlockKeys = 256;
+// Rows that share their keys from which on the tcgen05 kernel takes them.
+constexpr int64_t kTcLeast = 64;
 
 }  // namespace
 
@@ -52,12 +66,19 @@ QuantAttnPlan plan_quant_attention(const jal_quant_kv &kv, const jal_ragged_batc
   QuantAttnPlan a = {};
   const int64_t G = (int64_t)(hq / kv.n_heads_kv), hkv = (int64_t)kv.n_heads_kv, pairs = (int64_t)b.max_q_len * G;
   const int ns = act == JAL_F32 ? 2 : 1;
-  a.rows = 8 * (int)std::min<int64_t>(most_tiles((int)kv.head_dim, ns), (pairs + 7) / 8);
+  a.rows = kv.head_dim <= 128 && pairs > kTcLeast
+               ? kTcRows
+               : 8 * (int)std::min<int64_t>(most_tiles((int)kv.head_dim, ns), (pairs + 7) / 8);
   a.tiles = (int)((pairs + a.rows - 1) / a.rows);
   int64_t keys = (int64_t)b.max_kv_len;
   if (window) keys = std::min<int64_t>(keys, (int64_t)(window + n_sink + b.max_q_len));
-  a.splits = attention_pieces(a.tiles * hkv * (int64_t)b.n_seqs, keys, quant_blocks((int)kv.head_dim, a.rows / 8, ns),
-                              kBlockKeys, false);
+  const int64_t blocks = a.tiles * hkv * (int64_t)b.n_seqs;
+  if (a.rows == kTcRows) {  // a block fills an SM: cut only as far as that gives idle ones work
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / (2 * kTcKeys)));
+    a.splits = (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
+  } else {
+    a.splits = attention_pieces(blocks, keys, quant_blocks((int)kv.head_dim, a.rows / 8, ns), kBlockKeys, false);
+  }
   a.direct = a.splits == 1;
   if (!a.direct)
     a.bytes = (size_t)a.splits * b.n_rows * hq * (kv.head_dim * sizeof(float) + sizeof(float2)) + 256;

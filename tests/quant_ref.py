@@ -102,11 +102,12 @@ class QuantCase(Case):
 
     def reference(self, scale, window=0, sinks=0):
         """Case's, and behind it, for every row: what an error of one part in the row's largest |q| makes of a score
-        at most, and what an error of one part in the largest weight (times V's scale) of its 32 keys makes of the
-        output.  Keys that the kernels take together are no further than 31 apart among those that a row sees."""
+        at most, and what errors of one part in the largest weight times V's scale of its 32 keys, and in the largest weight
+        times the largest scale of all keys, make of the output.  Keys that the kernels take together are no further than 31 apart among those that a row sees."""
         ref = super().reference(scale, window, sinks)
         off_q = torch.zeros(self.n_rows, self.hq, 1, dtype=torch.float64)
         off_w = torch.zeros(self.n_rows, self.hq, self.hd, dtype=torch.float64)
+        off_all = torch.zeros_like(off_w)
         group, row = self.hq // self.hkv, 0
         for s, (length, new) in enumerate(zip(self.lens, self.news)):
             for i in range(new):
@@ -120,28 +121,31 @@ class QuantCase(Case):
                         k, v = self.k[s][at, h // group].double(), self.v[s][at, h // group].double()
                         q = self.q[row, h].double()
                         off_q[row, h] = k.abs().sum(-1).max() * q.abs().max() * abs(scale)
-                        p = torch.softmax(k @ q * scale, 0) * dv[:, h // group]
+                        p = torch.softmax(k @ q * scale, 0)
+                        most = p.max() * dv[:, h // group].max()
+                        p = p * dv[:, h // group]
                         near = torch.nn.functional.max_pool1d(p[None, None], 63, 1, 31)[0, 0]
                         codes = v.abs() / dv[:, h // group].clamp(min=1e-300)[:, None]
-                        off_w[row, h] = near @ codes
+                        off_w[row, h], off_all[row, h] = near @ codes, most * codes.sum(0)
                 row += 1
-        return (*ref, off_q, off_w)
+        return (*ref, off_q, off_w, off_all)
 
     def bound(self, ref):
         """Largest difference that the kernels' roundings allow, from their count.  A score: hd + 8 roundings of its
         terms, four multiplications by scales; q as a whole number over its largest element, off by half of 1 / 32512
         (f32 rows: 2^-24 of the element and half of 2^-31 of the largest).  A weight: the score's error and the
         maximum's, each in the exponent, exp2's two units, three multiplications; and half of 2^-13 of the largest of
-        its 32 keys' (f32 rows: 2^-29).  f16 tiles of many rows: 2^-11 of itself instead.  The sums over n keys: n + 64
+        its 32 keys' (f32 rows: 2^-29).  tiles of many rows: 2^-11 of itself and 2^-35 of the row's
+        largest weight times V's largest scale.  The sums over n keys: n + 64
         additions above and below the quotient.  Then the result's rounding."""
-        out, mag, n, off, off_q, off_w = ref
+        out, mag, n, off, off_q, off_w, off_all = ref
         e = 2.0 ** -24
         wide = self.act == torch.float32
         score = (self.hd + 14) * e * off + (0.5 * 2.0 ** -30 if wide else 0.52 / 32512) * off_q
         weight = 2 * score * 1.5 + 14 * e + (2.0 ** -22 if wide else 2.0 ** -11)
         total = weight * 2 + 2 * (n + 64) * e
         tiny = torch.finfo(self.act).smallest_normal
-        own = total * mag + (2.0 ** -30 if wide else 2.0 ** -14) * (1 + total) * off_w
+        own = total * mag + (2.0 ** -30 if wide else 2.0 ** -14) * (1 + total) * off_w + 2.0 ** -34 * off_all
         return own + half_step(self.act) * (out.abs() + own) + tiny
 
 

@@ -257,6 +257,9 @@ SHAPES = [  # hq, hkv, hd, page, lens, news
     (8, 4, 256, 128, [300, 129], [2, 17]),
     (2, 1, 32, 1, [37, 12], [37, 3]),
     (16, 1, 64, 33, [90, 222], [64, 70]),
+    (8, 2, 128, 16, [200, 310, 9], [130, 40, 9]),
+    (4, 2, 96, 24, [260, 41], [47, 41]),
+    (2, 1, 128, 64, [513, 128, 600], [64, 40, 1]),
 ]
 
 
@@ -347,6 +350,22 @@ def test_scales_that_rows_must_not_meet(jal, torch_cuda, act, which, value, news
     c.to_device(jal)
     got = _attend(jal, c, 0.25, 5, 2).cpu()[:news].reshape(news, 4, 64).double()
     assert bool(((got - windowed[0][:news]).abs() <= bound[:news]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("news", [3, 30, 80, 200])
+def test_a_huge_value_behind_a_row_leaves_it_alone(jal, torch_cuda, act, news):
+    # Finite scales of 2^90 of K and of V at positions that some rows see and others do not.
+    c = QuantCase([210], [news], 2, 1, 64, act=act, bits=8, page=16)
+    clean = c.reference(0.25)
+    bound = c.bound(clean)
+    at = 208
+    c.set_scale(1, 0, at, 2.0 ** 90)
+    c.set_scale(0, 0, at, 2.0 ** 20)
+    c.to_device(jal)
+    got = _attend(jal, c, 0.25).cpu()[:news].reshape(news, 2, 64).double()
+    assert bool(((got - clean[0][:news]).abs() <= bound[:news])[:news - 2].all())
 
 
 @pytest.mark.gpu
