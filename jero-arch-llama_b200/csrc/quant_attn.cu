@@ -27,7 +27,7 @@ void run_mma(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s
 template <int BITS, int NS, int HD>
 void run_tc(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
   const int64_t blocks = (int64_t)p.a.kv.hkv * p.a.splits * p.a.tiles * p.a.n_seqs;
-  constexpr int smem = QuantTcShape<NS, HD>::smem;
+  constexpr int smem = QuantTcShape<BITS, NS, HD>::smem;
   JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_tc<BITS, NS, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   k_quant_attn_tc<BITS, NS, HD><<<(unsigned)blocks, kTcThreads, smem, s>>>(p, plan.direct);
   JAL_CUDA(cudaGetLastError());

@@ -46,17 +46,20 @@ struct QuantTcSync {
   alignas(16) float dk[8][128], dv[8][128];  // their scales (K's times the softmax's), 0 where there is no key
 };
 
-template <int NS, int HD>
+template <int BITS, int NS, int HD>
 struct QuantTcShape {
   static constexpr int tile = kTcKeys * HD * 2;  // bytes of a K or V tile
   static constexpr int q_tile = 128 * HD * 2;    // of one part of a row tile
   static constexpr int buffers = HD == 64 ? 6 : NS == 1 ? 4 : 2;
   // The query tiles; at the end 4 KB for each softmax warp.
   static constexpr int q_area = 2 * NS * q_tile > 65536 ? 2 * NS * q_tile : 65536;
-  static constexpr int ring = q_area, sync = q_area + buffers * tile, smem = sync + (int)sizeof(QuantTcSync);
+  // Codes on their way: of each loader the groups of eight rows that it has of a tile.
+  static constexpr int row_bytes = HD * BITS / 8, groups = (16 + kTcLoaders - 1) / kTcLoaders;
+  static constexpr int ring = q_area, raw = ring + buffers * tile, sync = raw + kTcLoaders * groups * 8 * row_bytes;
+  static constexpr int smem = sync + (int)sizeof(QuantTcSync);
 };
-static_assert(QuantTcShape<1, 128>::smem <= 232448 && QuantTcShape<2, 128>::smem <= 232448 &&
-                  QuantTcShape<2, 64>::smem <= 232448,
+static_assert(QuantTcShape<8, 1, 128>::smem <= 232448 && QuantTcShape<8, 2, 128>::smem <= 232448 &&
+                  QuantTcShape<8, 2, 64>::smem <= 232448,
               "shared memory of a block");
 
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
@@ -92,7 +95,7 @@ __device__ __forceinline__ void widen16(const uint32_t *w, uint32_t (&out)[8]) {
 
 template <int BITS, int NS, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_constant__ QuantAttnParams qp, const bool direct) {
-  using S = QuantTcShape<NS, HD>;
+  using S = QuantTcShape<BITS, NS, HD>;
   const AttnParams &p = qp.a;
   extern __shared__ __align__(1024) char smem_tc[];
   QuantTcSync &sy = *(QuantTcSync *)(smem_tc + S::sync);
@@ -110,7 +113,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
   // Loader: the 16 groups of 8 rows of a tile go round the warps; a lane looks up
   // two of its warp's (up to) 48 rows, one tile ahead, the first before anything else.
   const int w = warp - 16;
-  constexpr int kGroups = (16 + kTcLoaders - 1) / kTcLoaders;
+  constexpr int kGroups = S::groups;
   auto group = [&](int k) { return w + k * kTcLoaders; };
   auto locate = [&](int j, int k) -> Slot {
     const int gr = group(k + lane / 8), u = t.u0 + j * kTcKeys + gr * 8 + lane % 8;
@@ -160,65 +163,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < 16 + kTcLoaders) {
       // ---- the loader
+      // Codes come by cp.async, a group of eight rows at a time, and are widened from
+      // there into the ring while the ones behind them are on their way: V's of a tile while
+      // K's are widened, then K's of the next tile.
       // HD / 16 lanes widen a row, sixteen codes a lane: dims 16 c16 .., two pieces of 16
       // bytes in the swizzle.  (The upper four of eight lanes store their second piece
       // first, so that eight lanes store eight different ones.)
-      constexpr int kLanes = HD / 16, kRows = 32 / kLanes;  // lanes of a row; rows of a warp at once
-      constexpr int kSteps = 8 / kRows;                     // for a group of eight rows
+      constexpr int kLanes = HD / 16, kRows = 32 / kLanes;        // lanes of a row; rows of a warp at once
+      constexpr int kPieces = S::row_bytes / 16, kCopy = 32 / kPieces;  // of a row; rows of a warp's copy
       const int c16 = lane % kLanes, r0 = lane / kLanes, flip = c16 / 4;
-      const bool inside = c16 * 16 < hd;
+      const int cp = lane % kPieces, cr = lane / kPieces;
+      const bool inside = cp * (128 / BITS) < hd;
+      char *const raw = smem_tc + S::raw + w * (kGroups * 8 * S::row_bytes);
+      const uint32_t raw_s = smem_u32(raw);
       bool ok = true;
       int b = 0, parity = 1;  // of the buffer's "empty" phase before this use: the first use finds it free
-      auto load = [&](const void *pool, int64_t from, uint32_t (&x)[4]) {
-        x[0] = x[1] = x[2] = x[3] = BITS == 8 ? 0u : 0x88888888u;  // (codes of 0)
-        if (from < 0 || !inside) return;
-        const char *const src = (const char *)pool + from + c16 * (2 * BITS);
-        if constexpr (BITS == 8) {
-          const uint4 v = __ldg((const uint4 *)src);
-          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-        } else {
-          const uint2 v = __ldg((const uint2 *)src);
-          x[0] = v.x; x[1] = v.y;
+      // (Rows without a key are copied as zeros; 4-bit codes of 0 there stand for -8, with a
+      // scale of 0.)
+      auto ask = [&](const void *pool, const int64_t (&from)[2], int k) {
+        if (group(k) < 16) {
+#pragma unroll
+          for (int i = 0; i < (8 + kCopy - 1) / kCopy; i++) {
+            const int r = i * kCopy + cr;
+            const int64_t o = __shfl_sync(0xffffffffu, k < 4 ? from[0] : from[1], (k % 4) * 8 + r % 8);
+            const bool there = o >= 0 && inside;
+            if (r < 8) copy16(raw_s + (k * 8 + r) * S::row_bytes + cp * 16, (const char *)pool + (there ? o + cp * 16 : 0), there);
+          }
         }
+        copies_done();
       };
-      auto fill = [&](const void *pool, const int64_t (&from)[2]) {
-        // Rows of this warp's groups, kSteps steps a group; a batch of them is on its way
-        // while the one before is widened.
-        constexpr int kBatch = 4, kAll = kGroups * kSteps;
-        uint32_t x[2][kBatch][4];
-        auto ask = [&](int s0, int at) {
+      auto widen = [&](int k) {
+        copies_wait<kGroups - 1>();
+        __syncwarp();
+        if (group(k) >= 16) return;
+        char *const dst = base_p + S::ring + b * S::tile + c16 / 4 * (kTcKeys * 128) + group(k) * 1024;
 #pragma unroll
-          for (int i = 0; i < kBatch; i++) {
-            const int s = s0 + i;
-            if (s >= kAll) break;
-            const int k = s / kSteps, r = s % kSteps * kRows + r0;
-            const int64_t o = __shfl_sync(0xffffffffu, k < 4 ? from[0] : from[1], (k % 4) * 8 + r);
-            load(pool, group(k) < 16 ? o : -1, x[at][i]);
-          }
-        };
-        ask(0, 0);
-        ok = __all_sync(0xffffffffu, ok && wait(&sy.kv_empty[b], parity));
-        if (!ok) return;
-        char *const dst = base_p + S::ring + b * S::tile + c16 / 4 * (kTcKeys * 128);
-#pragma unroll
-        for (int s0 = 0; s0 < kAll; s0 += kBatch) {
-          const int at = s0 / kBatch % 2;
-          if (s0 + kBatch < kAll) ask(s0 + kBatch, at ^ 1);
-#pragma unroll
-          for (int i = 0; i < kBatch; i++) {
-            const int s = s0 + i;
-            if (s >= kAll) break;
-            const int k = s / kSteps, r = s % kSteps * kRows + r0;
-            if (group(k) >= 16) break;
-            uint32_t h[8];
-            widen16<BITS>(x[at][i], h);
-            char *const row = dst + group(k) * 1024 + r * 128;
-            const int c = c16 % 4 * 2;
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            *(uint4 *)(row + (((c + flip) ^ r) * 16)) = flip ? hi : lo;
-            *(uint4 *)(row + (((c + 1 - flip) ^ r) * 16)) = flip ? lo : hi;
-          }
+        for (int i = 0; i < 8 / kRows; i++) {
+          const int r = i * kRows + r0;
+          uint32_t x[4], h[8];
+          lds<2 * BITS>(raw_s + (k * 8 + r) * S::row_bytes + c16 * (2 * BITS), x);
+          widen16<BITS>(x, h);
+          char *const row = dst + r * 128;
+          const int c = c16 % 4 * 2;
+          const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+          *(uint4 *)(row + (((c + flip) ^ r) * 16)) = flip ? hi : lo;
+          *(uint4 *)(row + (((c + 1 - flip) ^ r) * 16)) = flip ? lo : hi;
         }
+        __syncwarp();  // every lane has read the group before it is filled again
+      };
+      auto begin = [&]() { return ok = __all_sync(0xffffffffu, ok && wait(&sy.kv_empty[b], parity)); };
+      auto end = [&]() {
         fence_proxy_async();  // the tensor cores read what was stored
         mbar_arrive(&sy.kv_full[b]);
         if (++b == S::buffers) {
@@ -226,33 +220,65 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
           parity ^= 1;
         }
       };
-#pragma unroll 1
-      for (int j = 0; j < n_tiles; j++) {
-        const int64_t at[2] = {slot_offset(p.kv, next0, t.head), slot_offset(p.kv, next1, t.head)};
-        const uint32_t bits0 = __ballot_sync(0xffffffffu, at[0] >= 0), bits1 = __ballot_sync(0xffffffffu, at[1] >= 0);
-        // The scales of this lane's rows.  (Tile j + 8 comes long after the softmax has read
-        // tile j's.)
+      // Where a tile's rows lie, which of them exist, and their scales.
+      int64_t at[2], ahead[2];
+      uint32_t bits[2];
+      float dk[2], dv[2];
+      auto look = [&](int64_t (&to)[2]) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const Slot &sl = e ? next1 : next0;
+          to[e] = slot_offset(p.kv, sl, t.head);
+          bits[e] = __ballot_sync(0xffffffffu, to[e] >= 0);
+          const bool there = to[e] >= 0;
+          const int64_t o = there ? (int64_t)sl.page * qp.sc.s_page + t.head * qp.sc.s_head + sl.slot : 0;
+          dk[e] = there ? __ldg(qp.sc.k + o) * p.scale_log2 : 0.0f;
+          dv[e] = there ? __ldg(qp.sc.v + o) : 0.0f;
+        }
+      };
+      if (n_tiles) {
+        look(ahead);
+        next0 = locate(1, 0);
+        next1 = locate(1, 4);
+#pragma unroll
+        for (int k = 0; k < kGroups; k++) ask(p.kv.k, ahead, k);
+      }
+#pragma unroll 1
+      for (int j = 0; j < n_tiles; j++) {
+        at[0] = ahead[0];
+        at[1] = ahead[1];
+        // (Tile j + 8 comes long after the softmax has read tile j's.)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
           const int gr = group(4 * e + lane / 8), key = gr * 8 + lane % 8;
           if (4 * e + lane / 8 < kGroups && gr < 16) {
-            const bool there = at[e] >= 0;
-            const int64_t o = there ? (int64_t)sl.page * qp.sc.s_page + t.head * qp.sc.s_head + sl.slot : 0;
-            sy.dk[j & 7][key] = there ? __ldg(qp.sc.k + o) * p.scale_log2 : 0.0f;
-            sy.dv[j & 7][key] = there ? __ldg(qp.sc.v + o) : 0.0f;
+            sy.dk[j & 7][key] = dk[e];
+            sy.dv[j & 7][key] = dv[e];
           }
         }
-        next0 = locate(j + 1, 0);
-        next1 = locate(j + 1, 4);
         if (lane < kGroups && group(lane) < 16)
-          sy.present[j & 7][group(lane)] = (uint8_t)((lane < 4 ? bits0 : bits1) >> (lane % 4 * 8));
+          sy.present[j & 7][group(lane)] = (uint8_t)((lane < 4 ? bits[0] : bits[1]) >> (lane % 4 * 8));
         __syncwarp();
         if (lane == 0) mbar_arrive(&sy.present_full[j & 7]);
-        fill(p.kv.k, at);
-        if (ok) fill(p.kv.v, at);
-        if (!ok) break;
+        if (!begin()) break;
+#pragma unroll 1
+        for (int k = 0; k < kGroups; k++) {
+          widen(k);
+          ask(p.kv.v, at, k);
+        }
+        end();
+        look(ahead);  // (of the last tile: no row)
+        next0 = locate(j + 2, 0);
+        next1 = locate(j + 2, 4);
+        if (!begin()) break;
+#pragma unroll 1
+        for (int k = 0; k < kGroups; k++) {
+          widen(k);
+          ask(p.kv.k, ahead, k);
+        }
+        end();
       }
+      copies_wait<0>();
     } else {
       // ---- the products: the whole warp runs the loop, so that addresses stay
       // uniform, and one lane issues
