@@ -43,7 +43,8 @@ struct QuantTcSync {
   uint8_t e[2][2][128];                // exponents of the largest scale of V that a row's halves see
   float m1[128];                       // at the end: what the weights of the second row tile refer to
   alignas(16) uint8_t present[8][16];  // which keys of tile j exist, a bit each, by j % 8
-  alignas(16) float dk[8][128], dv[8][128];  // their scales (K's times the softmax's), 0 where there is no key
+  alignas(16) float dk[8][128], dv[8][128];  // their scales (K's times the softmax's), 0 where there is
+                                             // no key; a V scale that is not finite is a NaN of K's
 };
 
 template <int BITS, int NS, int HD>
@@ -234,6 +235,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
           const int64_t o = there ? (int64_t)sl.page * qp.sc.s_page + t.head * qp.sc.s_head + sl.slot : 0;
           dk[e] = there ? __ldg(qp.sc.k + o) * p.scale_log2 : 0.0f;
           dv[e] = there ? __ldg(qp.sc.v + o) : 0.0f;
+          // (Weights of 0 times such a scale would be NaN in rows that do not see it.)
+          if (!(fabsf(dv[e]) < INFINITY)) {
+            dv[e] = 0.0f;
+            dk[e] = NAN;
+          }
         }
       };
       if (n_tiles) {
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
           for (int s = 0; s < NS; s++)
 #pragma unroll
             for (int k = 0; k < kTcKeys / 16; k++)
-              tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + (k / 4) * 64 + s * 32 + (k % 4) * 8,
+              tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + (k / 2) * 32 + s * 16 + (k % 2) * 8,
                         b + (uint32_t)(k * (2048 >> 4)), id_o, !first || s + k > 0);
         }
         __syncwarp();
@@ -440,46 +446,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
       ok = wait(&sy.s_full[i], turn & 1) && ok;
       __syncwarp();
       tc_fence_after();
-      float s[2][32];
-      tc_ld32(ts, (uint32_t *)s[0]);
-      tc_ld32(ts + 32, (uint32_t *)s[1]);
       const int u = t.u0 + j * kTcKeys + half * 64;
       const uint2 here = *(const uint2 *)&sy.present[j & 7][half * 8];
       const bool whole = (here.x & here.y) == 0xffffffffu && span.all(u, 64);
       const bool masked = !__all_sync(0xffffffffu, whole || !real);
       const float *const dk = sy.dk[j & 7] + half * 64, *const dv = sy.dv[j & 7] + half * 64;
-      tc_wait_ld();
-      // Scores over the row's factor.
+      // Scores over the row's factor, masked, back into tensor memory 32 at a time (64 in
+      // registers beside their scales are more than a thread has), with their maximum and
+      // the largest scale of V (its bits) that the row sees.
+      float mine = -INFINITY;
+      uint32_t largest = 0;
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        const float4 d = *(const float4 *)(dk + e);
-        float *const y = &s[e / 32][e % 32];
-        unpair(mul2(pair(y[0], y[1]), pair(d.x, d.y)), y[0], y[1]);
-        unpair(mul2(pair(y[2], y[3]), pair(d.z, d.w)), y[2], y[3]);
-      }
-      // The largest scale of V (its bits) among this half's keys that the row sees.
-      auto finite = [](uint32_t b) { b &= 0x7fffffffu; return b < 0x7f800000u ? b : 0u; };
-      uint32_t bits[2] = {0xffffffffu, 0xffffffffu}, largest = 0;
-      if (masked) {
-        bits[0] = here.x & span.bits(u);
-        bits[1] = here.y & span.bits(u + 32);
+      for (int c = 0; c < 2; c++) {
+        float s[32];
+        tc_ld32(ts + c * 32, (uint32_t *)s);
+        tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 64; e++) {
-          const bool seen = (bits[e / 32] >> (e % 32)) & 1;
-          if (!seen) s[e / 32][e % 32] = -INFINITY;
-          if (seen) largest = max(largest, finite(__float_as_uint(dv[e])));
+        for (int e = 0; e < 32; e += 4) {
+          const float4 d = *(const float4 *)(dk + c * 32 + e);
+          unpair(mul2(pair(s[e], s[e + 1]), pair(d.x, d.y)), s[e], s[e + 1]);
+          unpair(mul2(pair(s[e + 2], s[e + 3]), pair(d.z, d.w)), s[e + 2], s[e + 3]);
         }
-      } else {
-        const uint2 x = *(const uint2 *)(dv + lane * 2);
-        largest = __reduce_max_sync(0xffffffffu, max(finite(x.x), finite(x.y)));
+        if (masked) {
+          const uint32_t bits = (c ? here.y : here.x) & span.bits(u + c * 32);
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            if ((bits >> e) & 1) largest = max(largest, __float_as_uint(dv[c * 32 + e]) & 0x7fffffffu);
+            else s[e] = -INFINITY;
+          }
+        }
+        tc_st32(ts + c * 32, (uint32_t *)s);
+        float x[4] = {max3_nan(mine, s[0], s[1]), s[2], s[3], s[4]};
+#pragma unroll
+        for (int e = 5; e < 29; e += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++) x[k] = max3_nan(x[k], s[e + 2 * k], s[e + 2 * k + 1]);
+        mine = max3_nan(max3_nan(x[0], x[1], s[29]), max3_nan(x[2], x[3], s[30]), s[31]);
       }
-      float x[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
-#pragma unroll
-      for (int e = 4; e < 60; e += 8)
-#pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = max3_nan(x[k], s[(e + 2 * k) / 32][(e + 2 * k) % 32], s[(e + 2 * k + 1) / 32][(e + 2 * k + 1) % 32]);
-      const float mine = max3_nan(max3_nan(x[0], x[1], s[1][28]), max3_nan(x[2], x[3], s[1][29]),
-                                  max3_nan(s[1][30], s[1][31], s[1][31]));
+      if (!masked) {
+        const uint2 x = *(const uint2 *)(dv + lane * 2);
+        largest = __reduce_max_sync(0xffffffffu, max(x.x & 0x7fffffffu, x.y & 0x7fffffffu));
+      }
+      tc_wait_st();
       sy.x[i][half][r] = mine;
       sy.e[i][half][r] = (uint8_t)(largest >> 23);
       tile_sync();
@@ -507,29 +515,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
         }
       }
       const float ref = m == -INFINITY ? 0.0f : m;
-      // The weights, over this half's own scores: part q of the 64 keys' in the
-      // columns 32 q .. of the half.
+      // The weights, over this half's own scores: part q of 32 keys in 16 of the columns
+      // that held their scores.
       pair_t sum[2] = {0, 0};
       const pair_t scale2 = pair(scale, scale), ref2 = pair(-ref, -ref);
 #pragma unroll
       for (int c = 0; c < 2; c++) {
+        float s[32];
         uint32_t w[NS][16];
+        tc_ld32(ts + c * 32, (uint32_t *)s);
+        tc_wait_ld();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
           const float4 d = *(const float4 *)(dv + c * 32 + 2 * e);
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             float a, b;
-            const pair_t x2 = fma2(pair(s[c][2 * (e + h)], s[c][2 * (e + h) + 1]), scale2, ref2);
+            const pair_t x2 = fma2(pair(s[2 * (e + h)], s[2 * (e + h) + 1]), scale2, ref2);
             unpair(x2, a, b);
             a = exp2_fast(a);
             b = exp2_fast(b);
             sum[h] = add2(sum[h], pair(a, b));
             unpair(mul2(pair(a, b), h ? pair(d.z, d.w) : pair(d.x, d.y)), a, b);
-            if (masked) {  // (what a row does not see has no effect on it, whatever its scale is)
-              if (!((bits[c] >> (2 * (e + h))) & 1)) a = 0.0f;
-              if (!((bits[c] >> (2 * (e + h) + 1)) & 1)) b = 0.0f;
-            }
             uint32_t part2[NS];
             split2<__half, NS>(a, b, part2);
 #pragma unroll
@@ -537,7 +544,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
           }
         }
 #pragma unroll
-        for (int q = 0; q < NS; q++) tc_st16(ts + q * 32 + c * 16, w[q]);
+        for (int q = 0; q < NS; q++) tc_st16(ts + c * 32 + q * 16, w[q]);
       }
       {
         float a, b;
