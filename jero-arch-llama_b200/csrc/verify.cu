@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "paged_attn_tc.cuh"
 #include "paged_dev.cuh"
 #include "quant_kv.hpp"
 
@@ -26,11 +27,16 @@ namespace {
 using namespace paged;
 namespace cg = cooperative_groups;
 
-constexpr int kStatThreads = 256, kDrawThreads = 256, kDrawWarps = kDrawThreads / 32, kCluster = 8;
+constexpr int kStatThreads = 256, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kCluster = 8;
 constexpr float kCold = 1e-5f;  // temperatures up to this: all of the probability on the first largest logit
 constexpr float kLog2e = 1.4426950408889634f;
 
 // (An infinite temperature would make 0 x -inf of a logit of -inf.)
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
 __device__ __forceinline__ float temperature_of(const float *t, int s) {
   if (!t) return 1.0f;
   const float x = __ldg(t + s);
@@ -46,50 +52,54 @@ template <>
 __device__ __forceinline__ float logit<__half>(const __half *p) { return __half2float(__ldg(p)); }
 template <>
 __device__ __forceinline__ float logit<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(__ldg(p)); }
-// (A NaN counts as -inf.)
-__device__ __forceinline__ float known(float x) { return x == x ? x : -INFINITY; }
-
-// Elements [lo, hi) of a row by the block's threads, in pieces of 16 bytes where they
-// are aligned: f(index, values[N]).
+// Elements [lo, hi) of a row by the block's threads, kBatch pieces of 16 bytes at a time
+// where they are aligned: f(values[kBatch * N], first indexes of the pieces), a NaN as
+// -inf, and -inf where there is none.
+constexpr int kBatch = 4;
 template <class T, class F>
-__device__ __forceinline__ void each16(const T *row, int lo, int hi, F &&f) {
+__device__ __forceinline__ void each_batch(const T *row, int lo, int hi, F &&f) {
   constexpr int N = 16 / sizeof(T);
   const int skip = (int)((16 - ((uintptr_t)(row + lo) & 15)) & 15) / (int)sizeof(T);
   const int a = min(hi, lo + skip), n = (hi - a) / N, b = a + n * N;
-  for (int i = lo + threadIdx.x; i < a; i += kStatThreads) {
-    float x[N];
+  auto one = [&](int i) {
+    float x[kBatch * N];
+    int at[kBatch];
 #pragma unroll
-    for (int e = 0; e < N; e++) x[e] = -INFINITY;
-    x[0] = logit(row + i);
-    f(i, x);
-  }
-#pragma unroll 4
-  for (int k = threadIdx.x; k < n; k += kStatThreads) {
-    const uint4 w = ldg_stream16(row + a + k * N);
-    float x[N];
-    if constexpr (sizeof(T) == 4) {
-      x[0] = __uint_as_float(w.x);
-      x[1] = __uint_as_float(w.y);
-      x[2] = __uint_as_float(w.z);
-      x[3] = __uint_as_float(w.w);
-    } else {
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    for (int e = 0; e < kBatch * N; e++) x[e] = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) at[k] = i;
+    x[0] = fmaxf(logit(row + i), -INFINITY);
+    f(x, at);
+  };
+  for (int i = lo + threadIdx.x; i < a; i += kStatThreads) one(i);
+  for (int k0 = threadIdx.x; k0 < n; k0 += kStatThreads * kBatch) {
+    uint4 w[kBatch];
+    float x[kBatch * N];
+    int at[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      const int i = k0 + k * kStatThreads;
+      at[k] = a + i * N;
+      if (i < n) w[k] = ldg_stream16(row + at[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      const bool there = k0 + k * kStatThreads < n;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const float2 v = unpack2<T>(u[e]);
-        x[2 * e] = v.x;
-        x[2 * e + 1] = v.y;
+        if constexpr (sizeof(T) == 4) {
+          x[k * N + e] = there ? fmaxf(__uint_as_float(u[e]), -INFINITY) : -INFINITY;
+        } else {
+          const float2 v = unpack2<T>(u[e]);
+          x[k * N + 2 * e] = there ? fmaxf(v.x, -INFINITY) : -INFINITY;
+          x[k * N + 2 * e + 1] = there ? fmaxf(v.y, -INFINITY) : -INFINITY;
+        }
       }
     }
-    f(a + k * N, x);
+    f(x, at);
   }
-  for (int i = b + threadIdx.x; i < hi; i += kStatThreads) {
-    float x[N];
-#pragma unroll
-    for (int e = 0; e < N; e++) x[e] = -INFINITY;
-    x[0] = logit(row + i);
-    f(i, x);
-  }
+  for (int i = b + threadIdx.x; i < hi; i += kStatThreads) one(i);
 }
 
 // One piece of one row, target's or draft's: its largest logit with, of warm rows,
@@ -116,30 +126,45 @@ __global__ void __launch_bounds__(kStatThreads) k_verify_stats(const __grid_cons
   float m = -INFINITY, sum = 0.0f;
   int at = 0x7fffffff;
   if (is_cold(t)) {
-    each16(x, lo, hi, [&](int i, const float (&v)[N]) {
+    each_batch(x, lo, hi, [&](const float (&v)[kBatch * N], const int (&i)[kBatch]) {
 #pragma unroll
-      for (int e = 0; e < N; e++)
-        if (v[e] > m || (v[e] == m && i + e < at && m > -INFINITY)) {
-          m = v[e];
-          at = i + e;
-        }
+      for (int k = 0; k < kBatch; k++) {
+        float most = v[k * N];
+#pragma unroll
+        for (int e = 1; e < N; e++) most = fmaxf(most, v[k * N + e]);
+        if (most < m || most == -INFINITY) continue;
+        int first = 0x7fffffff;
+#pragma unroll
+        for (int e = N - 1; e >= 0; e--)
+          if (v[k * N + e] == most) first = i[k] + e;
+        at = most > m ? first : min(at, first);
+        m = most;
+      }
     });
   } else {
     const float c = kLog2e / t;
-    each16(x, lo, hi, [&](int, const float (&v)[N]) {
+    const pair_t c2 = pair(c, c);
+    each_batch(x, lo, hi, [&](const float (&v)[kBatch * N], const int (&)[kBatch]) {
       float most = v[0];
 #pragma unroll
-      for (int e = 1; e < N; e++) most = fmaxf(most, v[e]);
+      for (int e = 1; e < kBatch * N; e++) most = fmaxf(most, v[e]);
       if (most > m) {
-        sum *= exp2f((m - most) * c);  // (m = -inf: the sum is 0)
+        sum *= exp2_fast((m - most) * c);  // (m = -inf: the sum is 0)
         m = most;
       }
-      if (m > -INFINITY) {
+      if (m == -INFINITY) return;
+      const pair_t less = pair(-m, -m);
+      pair_t part[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < N; e++) sum += v[e] == v[e] ? exp2f((v[e] - m) * c) : 0.0f;
+      for (int e = 0; e < kBatch * N; e += 2) {
+        float y, z;
+        unpair(mul2(add2(pair(v[e], v[e + 1]), less), c2), y, z);
+        part[e / 2 % 2] = add2(part[e / 2 % 2], pair(exp2_fast(y), exp2_fast(z)));
       }
+      float y, z;
+      unpair(add2(part[0], part[1]), y, z);
+      sum += y + z;
     });
-    if (m == -INFINITY) sum = 0.0f;
   }
   // Threads, then warps.
   float most = warp_max(m);
@@ -205,42 +230,107 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// exp((x - m) / T) in 64 bits; 0 for -inf and NaN.
+// 2^y of kTogether numbers y <= 0 side by side (each is a chain of fifteen dependent
+// operations): to the nearest whole number in the exponent, the rest, at most 1/2, by its
+// power series; the first term left out is (ln 2 / 2)^11 / 11! = 2e-13 of the result.
+// 0 for y below -1000, and for -inf and NaN.
+constexpr int kTogether = 4;
+__device__ __forceinline__ void exp2_64(double (&y)[kTogether]) {
+  constexpr double series[11] = {1.0,  // (ln 2)^k / k!
+                                 6.931471805599453e-01, 2.402265069591007e-01, 5.5504108664821576e-02, 9.618129107628477e-03,
+                                 1.3333558146428441e-03, 1.5403530393381606e-04, 1.5252733804059838e-05, 1.3215486790144305e-06,
+                                 1.0178086009239696e-07, 7.054911620801121e-09};
+  double t[kTogether], p[kTogether];
+  bool some[kTogether];
+#pragma unroll
+  for (int i = 0; i < kTogether; i++) {
+    some[i] = y[i] > -1000.0;
+    y[i] = some[i] ? y[i] : 0.0;
+    t[i] = y[i] + 6755399441055744.0;  // 1.5 * 2^52
+    y[i] -= t[i] - 6755399441055744.0;
+    p[i] = series[10];
+  }
+#pragma unroll
+  for (int k = 9; k >= 0; k--)
+#pragma unroll
+    for (int i = 0; i < kTogether; i++) p[i] = fma(p[i], y[i], series[k]);
+#pragma unroll
+  for (int i = 0; i < kTogether; i++)
+    y[i] = some[i] ? __hiloint2double(__double2hiint(p[i]) + (__double2loint(t[i]) << 20), __double2loint(p[i])) : 0.0;
+}
+
+// exp((x - m) / T) in 64 bits, as a power of two.
 struct Weight {
-  double m, inv;
+  double m, c;
+  __device__ __forceinline__ Weight() {}
+  __device__ __forceinline__ Weight(float m, float t) : m(m), c(1.4426950408889634 / (double)t) {}
+  __device__ __forceinline__ double power(float x) const { return ((double)x - m) * c; }
   __device__ __forceinline__ double operator()(float x) const {
-    return x > -INFINITY ? exp(((double)x - m) * inv) : 0.0;
+    double y[kTogether] = {power(x)};
+    exp2_64(y);
+    return y[0];
   }
 };
 
-// What the row that emits draws from: exp((x_t - m) / T) / sum, less the draft's.
+// What the row that emits draws from: p, or what of p is above q, each summed apart:
+// the token's weight is p / zx - q / zy where that is positive.
 template <class T>
 struct Drawn {
   const T *x, *y;  // target's logits; the draft's, or null
   Weight wx, wy;
-  double zx, zy;   // 1 / sums
+  double border;   // p > q where the exponents of the two differ by more than this
   int one;         // the token that the draft was sure of, or -1
-  __device__ __forceinline__ double p(int t) const { return wx(logit(x + t)) * zx; }
-  __device__ __forceinline__ double rest(int t, double px) const {
-    if (t == one) return 0.0;
-    return y ? fmax(px - wy(logit(y + t)) * zy, 0.0) : px;
+  // Of the tokens at[] below `end`: p and q over their sums' scale, and whether they are
+  // drawn from.
+  __device__ __forceinline__ void get(const int (&at)[kTogether], int end, double (&px)[kTogether], double (&qx)[kTogether],
+                                      bool (&in)[kTogether]) const {
+    float a[kTogether], b[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; i++) {
+      a[i] = at[i] < end ? logit(x + at[i]) : -INFINITY;
+      b[i] = y && at[i] < end ? logit(y + at[i]) : -INFINITY;
+    }
+    double gap[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; i++) {
+      px[i] = wx.power(a[i]);
+      qx[i] = 0.0;
+      gap[i] = px[i];
+    }
+    exp2_64(px);
+    if (y) {
+#pragma unroll
+      for (int i = 0; i < kTogether; i++) {
+        qx[i] = wy.power(b[i]);
+        gap[i] -= qx[i];
+      }
+      exp2_64(qx);
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; i++)
+      in[i] = px[i] > 0.0 && (y ? qx[i] == 0.0 || gap[i] > border : at[i] != one);
   }
 };
 
+struct PartSums {
+  double zx, zy, px, qx;  // sums of p and q over a warp's part of the vocabulary; of p and q where p > q
+};
 struct DrawShared {
-  double zx, zy;                         // this block's sums of exponentials
-  double rest[kDrawWarps], p[kDrawWarps];  // each warp's sums over its part of the vocabulary
+  PartSums part[kDrawWarps];
   int stop;
   RowStats target, draft;
 };
 
 template <class T>
 __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_constant__ VerifyParams p) {
+  constexpr int most_parts = kCluster * kDrawWarps;  // of the vocabulary, one a warp
+  constexpr int kOfLane = most_parts / 32;           // parts that a lane looks at
   __shared__ DrawShared sh;
-  constexpr int parts = kCluster * kDrawWarps;  // of the vocabulary, one a warp
-  __shared__ double red[2][kDrawWarps], part_rest[parts], part_p[parts];
+  __shared__ PartSums all[most_parts];
+  __shared__ double slice[kDrawWarps];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), s = blockIdx.x / kCluster;
+  const int blocks = (int)cluster.num_blocks(), parts = blocks * kDrawWarps;
+  const int rank = (int)cluster.block_rank(), s = blockIdx.x / blocks;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
@@ -262,13 +352,13 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
     bool take = false;
     if (x >= 0 && x < p.vocab) {
       const RowStats a = row_stats(p, r, t);
-      const float lx = known(logit((const T *)p.logits + r * p.stride + x));
+      const float lx = logit((const T *)p.logits + r * p.stride + x);
       double px = 0.0, qx = 1.0;
-      if (!a.none()) px = is_cold(t) ? (double)(a.at == x) : Weight{a.m, 1.0 / t}(lx) / a.sum;
+      if (!a.none()) px = is_cold(t) ? (double)(a.at == x) : Weight(a.m, t)(lx) / a.sum;
       if (p.draft) {
         const RowStats b = row_stats(p, p.n_rows + r, td);
-        const float ly = known(logit((const T *)p.draft + r * p.draft_stride + x));
-        if (!b.none()) qx = is_cold(td) ? (double)(b.at == x) : Weight{b.m, 1.0 / td}(ly) / b.sum;
+        const float ly = logit((const T *)p.draft + r * p.draft_stride + x);
+        if (!b.none()) qx = is_cold(td) ? (double)(b.at == x) : Weight(b.m, td)(ly) / b.sum;
       }
       take = (double)__ldg(p.uniform + r) * qx < px;
     }
@@ -291,118 +381,154 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
   if (!a.none() && is_cold(t)) {
     token = a.at;
   } else if (!a.none()) {
-    Drawn<T> d = {};
+    Drawn<T> d;
     d.x = (const T *)p.logits + stop * p.stride;
-    d.wx = Weight{a.m, 1.0 / t};
+    d.y = nullptr;
+    d.wx = Weight(a.m, t);
     d.one = -1;
     if (!sure) {
       const int x = __ldg(p.tokens + stop + 1);
       if (p.draft && !sh.draft.none() && !is_cold(td)) {
         d.y = (const T *)p.draft + stop * p.draft_stride;
-        d.wy = Weight{sh.draft.m, 1.0 / td};
+        d.wy = Weight(sh.draft.m, td);
+        // (From the sums in f32: a token that falls on the wrong side has p and q within
+        // 2^-20 of each other, and a weight of next to nothing.)
+        d.border = (double)log2f(a.sum) - (double)log2f(sh.draft.sum);
       } else {
         d.one = p.draft && !sh.draft.none() ? sh.draft.at : x;
       }
     }
     // This warp's part of the vocabulary, a whole number of 32.
     const int per = (p.vocab + parts * 32 - 1) / (parts * 32) * 32;
-    const int mine = rank * kDrawWarps + warp;
-    const int lo = (int)min((int64_t)p.vocab, (int64_t)mine * per), hi = (int)min((int64_t)p.vocab, (int64_t)lo + per);
-    double zx = 0.0, zy = 0.0;
-#pragma unroll 4
-    for (int i = lo + lane; i < hi; i += 32) {
-      zx += d.wx(logit(d.x + i));
-      if (d.y) zy += d.wy(logit(d.y + i));
-    }
-    zx = warp_sum64(zx);
-    zy = warp_sum64(zy);
-    if (lane == 0) {
-      red[0][warp] = zx;
-      red[1][warp] = zy;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      sh.zx = sh.zy = 0.0;
-      for (int w = 0; w < kDrawWarps; w++) {
-        sh.zx += red[0][w];
-        sh.zy += red[1][w];
+    const int lo = (int)min((int64_t)p.vocab, (int64_t)(rank * kDrawWarps + warp) * per);
+    const int hi = (int)min((int64_t)p.vocab, (int64_t)lo + per);
+    PartSums mine = {0.0, 0.0, 0.0, 0.0};
+    for (int i0 = lo + lane; i0 < hi; i0 += 32 * kTogether) {
+      double px[kTogether], qx[kTogether];
+      bool in[kTogether];
+      int at[kTogether];
+#pragma unroll
+      for (int i = 0; i < kTogether; i++) at[i] = i0 + 32 * i;
+      d.get(at, hi, px, qx, in);
+#pragma unroll
+      for (int i = 0; i < kTogether; i++) {
+        mine.zx += px[i];
+        mine.px += in[i] ? px[i] : 0.0;
+        if (d.y) {
+          mine.zy += qx[i];
+          mine.qx += in[i] ? qx[i] : 0.0;
+        }
       }
     }
+    mine.zx = warp_sum64(mine.zx);
+    mine.px = warp_sum64(mine.px);
+    if (d.y) {
+      mine.zy = warp_sum64(mine.zy);
+      mine.qx = warp_sum64(mine.qx);
+    }
+    if (lane == 0) sh.part[warp] = mine;
     cluster.sync();
-    zx = zy = 0.0;
-    for (int k = 0; k < kCluster; k++) {
-      const DrawShared *const o = cluster.map_shared_rank(&sh, k);
-      zx += o->zx;
-      zy += o->zy;
-    }
-    d.zx = 1.0 / zx;
-    d.zy = d.y ? 1.0 / zy : 0.0;
-    double rest = 0.0, whole = 0.0;
-#pragma unroll 4
-    for (int i = lo + lane; i < hi; i += 32) {
-      const double px = d.p(i);
-      whole += px;
-      rest += d.rest(i, px);
-    }
-    rest = warp_sum64(rest);
-    whole = warp_sum64(whole);
-    if (lane == 0) {
-      sh.rest[warp] = rest;
-      sh.p[warp] = whole;
-    }
-    cluster.sync();
-    if (tid < parts) {
-      const DrawShared *const o = cluster.map_shared_rank(&sh, tid / kDrawWarps);
-      part_rest[tid] = o->rest[tid % kDrawWarps];
-      part_p[tid] = o->p[tid % kDrawWarps];
-    }
-    __syncthreads();
+    if (tid < parts) all[tid] = cluster.map_shared_rank(&sh, tid / kDrawWarps)->part[tid % kDrawWarps];
     cluster.sync();  // no block leaves while others read its sums
-    // Every warp goes through the parts in order, with the same numbers: the part
+    // Every warp goes through the parts, kOfLane a lane, with the same numbers: the part
     // in which the running sum first exceeds `want`, or the last one with any weight
     // where rounding (or a number that is not below 1) leaves none.
-    double total = 0.0;
-    for (int k = 0; k < parts; k++) total += part_rest[k];
+    PartSums of[kOfLane];
+    double zx = 0.0, zy = 0.0;
+#pragma unroll
+    for (int k = 0; k < kOfLane; k++) {
+      of[k] = PartSums{0.0, 0.0, 0.0, 0.0};
+      if (kOfLane * lane + k < parts) of[k] = all[kOfLane * lane + k];
+      zx += of[k].zx;
+      zy += of[k].zy;
+    }
+    const double ix = 1.0 / warp_sum64(zx), iy = d.y ? 1.0 / warp_sum64(zy) : 0.0;
+    double w[kOfLane], sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kOfLane; k++) sum += w[k] = fmax(of[k].px * ix - of[k].qx * iy, 0.0);
+    double total = warp_sum64(sum);
     const bool from_p = !(total > 0.0);
-    const double *const part = from_p ? part_p : part_rest;
     if (from_p) {
-      total = 0.0;
-      for (int k = 0; k < parts; k++) total += part[k];
+      sum = 0.0;
+#pragma unroll
+      for (int k = 0; k < kOfLane; k++) sum += w[k] = of[k].zx * ix;
+      total = warp_sum64(sum);
     }
     const double want = (double)__ldg(p.uniform + end - 1) * total;
-    int chosen = -1;
-    bool over = false;
-    double run = 0.0, before = 0.0;
-    for (int k = 0; k < parts && !over; k++) {
-      if (!(part[k] > 0.0)) continue;
-      chosen = k;
-      before = run;
-      run += part[k];
-      over = run > want;
+    double upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const double n = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += n;
     }
-    if (mine != max(chosen, 0)) return;
-    writes = true;
-    int pick = -1, some = -1;
-    for (int i0 = lo; i0 < hi && pick < 0; i0 += 32) {
-      const int i = i0 + lane;
-      double w = 0.0;
-      if (i < hi) {
-        const double px = d.p(i);
-        w = from_p ? px : d.rest(i, px);
+    double run = upto - sum, before = run;  // before: of this lane's first part past `want`, or its last one
+    int over = 0x7fffffff, last = -1;
+#pragma unroll
+    for (int k = 0; k < kOfLane; k++) {
+      if (w[k] > 0.0 && over == 0x7fffffff) {
+        last = kOfLane * lane + k;
+        before = run;
+        if (run + w[k] > want) over = last;
       }
-      double sum = w;
+      run += w[k];
+    }
+    int chosen = __reduce_min_sync(0xffffffffu, over);
+    if (chosen == 0x7fffffff) chosen = max(__reduce_max_sync(0xffffffffu, last), 0);
+    before = __shfl_sync(0xffffffffu, before, chosen / kOfLane);
+    if (rank != chosen / kDrawWarps) return;
+    // The block that has the part goes through it, kTogether tokens a lane at a time.
+    const int c_lo = (int)min((int64_t)p.vocab, (int64_t)chosen * per), c_hi = (int)min((int64_t)p.vocab, (int64_t)c_lo + per);
+    int some = -1;  // the last token with any weight
+    for (int base = c_lo; base < c_hi && token < 0; base += kDrawThreads * kTogether) {
+      double px[kTogether], qx[kTogether], w[kTogether], sum = 0.0;
+      bool in[kTogether];
+      int at[kTogether];
+      const int first = base + tid * kTogether;
+#pragma unroll
+      for (int e = 0; e < kTogether; e++) at[e] = first + e;
+      d.get(at, c_hi, px, qx, in);
+#pragma unroll
+      for (int e = 0; e < kTogether; e++) sum += w[e] = from_p ? px[e] * ix : in[e] ? fmax(px[e] * ix - qx[e] * iy, 0.0) : 0.0;
+      // Sums up to this lane, of the warps, and up to this warp.
+      upto = sum;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
-        const double n = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += n;
+        const double n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, w > 0.0 && before + sum > want);
-      const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0);
-      if (past) pick = i0 + __ffs(past) - 1;
-      if (any) some = i0 + 31 - __clz(any);
-      before += __shfl_sync(0xffffffffu, sum, 31);
+      __syncthreads();  // (the slices of the round before have been read)
+      if (lane == 31) slice[warp] = upto;
+      __syncthreads();
+      double start = before;
+      for (int k = 0; k < warp; k++) start += slice[k];
+      for (int k = 0; k < kDrawWarps; k++) before += slice[k];
+      start += upto - sum;
+      int pick = 0x7fffffff, last = -1;
+#pragma unroll
+      for (int e = 0; e < kTogether; e++) {
+        start += w[e];
+        if (w[e] > 0.0) {
+          last = first + e;
+          if (start > want) pick = min(pick, first + e);
+        }
+      }
+      if (tid == 0) {
+        sh.stop = 0x7fffffff;
+        sh.target.at = -1;
+      }
+      __syncthreads();
+      pick = __reduce_min_sync(0xffffffffu, pick);
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (lane == 0) {
+        if (pick != 0x7fffffff) atomicMin(&sh.stop, pick);
+        atomicMax(&sh.target.at, last);
+      }
+      __syncthreads();
+      if (sh.stop != 0x7fffffff) token = sh.stop;
+      some = max(some, sh.target.at);
     }
-    token = pick >= 0 ? pick : some;
+    if (token < 0) token = some;
+    writes = warp == 0;
   }
   if (!writes) return;
   for (int r = beg + lane; r < end; r += 32) p.out_tokens[r] = r < stop ? __ldg(p.tokens + r + 1) : r == stop ? token : -1;
@@ -420,12 +546,16 @@ void run(const VerifyParams &p, cudaStream_t s) {
     JAL_CUDA(cudaGetLastError());
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.n_seqs * kCluster);
+  // Blocks of a sequence: parts of 128 tokens a warp at least.
+  unsigned cluster = 1;
+  while (cluster < kCluster && p.vocab > (int)(cluster * kDrawWarps * 128)) cluster *= 2;
+  cfg.gridDim = dim3((unsigned)p.n_seqs * cluster);
   cfg.blockDim = dim3(kDrawThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {kCluster, 1, 1};
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
