@@ -230,33 +230,38 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// 2^y of kTogether numbers y <= 0 side by side (each is a chain of fifteen dependent
-// operations): to the nearest whole number in the exponent, the rest, at most 1/2, by its
-// power series; the first term left out is (ln 2 / 2)^11 / 11! = 2e-13 of the result.
-// 0 for y below -1000, and for -inf and NaN.
+// 2^y of kTogether numbers y <= 0 side by side (each is a chain of dependent
+// operations): to the nearest 32nd in the exponent, whose power comes from a table, and
+// the rest, at most 1/64, by its power series; the first term left out is (ln 2 / 64)^5
+// / 5! = 1.2e-12 of the result.  0 for y below -1000, and for -inf and NaN.
 constexpr int kTogether = 4;
-__device__ __forceinline__ void exp2_64(double (&y)[kTogether]) {
-  constexpr double series[11] = {1.0,  // (ln 2)^k / k!
-                                 6.931471805599453e-01, 2.402265069591007e-01, 5.5504108664821576e-02, 9.618129107628477e-03,
-                                 1.3333558146428441e-03, 1.5403530393381606e-04, 1.5252733804059838e-05, 1.3215486790144305e-06,
-                                 1.0178086009239696e-07, 7.054911620801121e-09};
-  double t[kTogether], p[kTogether];
+struct Powers {
+  double of[32];  // 2^(i / 32)
+};
+__device__ __forceinline__ void exp2_64(const Powers &table, double (&y)[kTogether]) {
+  constexpr double series[5] = {1.0, 6.931471805599453e-01, 2.402265069591007e-01, 5.5504108664821576e-02,
+                                9.618129107628477e-03};  // (ln 2)^k / k!
+  double p[kTogether];
+  int n[kTogether];
   bool some[kTogether];
 #pragma unroll
   for (int i = 0; i < kTogether; i++) {
     some[i] = y[i] > -1000.0;
     y[i] = some[i] ? y[i] : 0.0;
-    t[i] = y[i] + 6755399441055744.0;  // 1.5 * 2^52
-    y[i] -= t[i] - 6755399441055744.0;
-    p[i] = series[10];
+    const double t = y[i] + 211106232532992.0;  // 1.5 * 2^47: the low word counts 32nds
+    n[i] = __double2loint(t);
+    y[i] -= t - 211106232532992.0;
+    p[i] = series[4];
   }
 #pragma unroll
-  for (int k = 9; k >= 0; k--)
+  for (int k = 3; k >= 0; k--)
 #pragma unroll
     for (int i = 0; i < kTogether; i++) p[i] = fma(p[i], y[i], series[k]);
 #pragma unroll
-  for (int i = 0; i < kTogether; i++)
-    y[i] = some[i] ? __hiloint2double(__double2hiint(p[i]) + (__double2loint(t[i]) << 20), __double2loint(p[i])) : 0.0;
+  for (int i = 0; i < kTogether; i++) {
+    p[i] *= table.of[n[i] & 31];
+    y[i] = some[i] ? __hiloint2double(__double2hiint(p[i]) + (n[i] >> 5 << 20), __double2loint(p[i])) : 0.0;
+  }
 }
 
 // exp((x - m) / T) in 64 bits, as a power of two.
@@ -265,9 +270,9 @@ struct Weight {
   __device__ __forceinline__ Weight() {}
   __device__ __forceinline__ Weight(float m, float t) : m(m), c(1.4426950408889634 / (double)t) {}
   __device__ __forceinline__ double power(float x) const { return ((double)x - m) * c; }
-  __device__ __forceinline__ double operator()(float x) const {
+  __device__ __forceinline__ double operator()(const Powers &table, float x) const {
     double y[kTogether] = {power(x)};
-    exp2_64(y);
+    exp2_64(table, y);
     return y[0];
   }
 };
@@ -282,7 +287,7 @@ struct Drawn {
   int one;         // the token that the draft was sure of, or -1
   // Of the tokens at[] below `end`: p and q over their sums' scale, and whether they are
   // drawn from.
-  __device__ __forceinline__ void get(const int (&at)[kTogether], int end, double (&px)[kTogether], double (&qx)[kTogether],
+  __device__ __forceinline__ void get(const Powers &table, const int (&at)[kTogether], int end, double (&px)[kTogether], double (&qx)[kTogether],
                                       bool (&in)[kTogether]) const {
     float a[kTogether], b[kTogether];
 #pragma unroll
@@ -297,14 +302,14 @@ struct Drawn {
       qx[i] = 0.0;
       gap[i] = px[i];
     }
-    exp2_64(px);
+    exp2_64(table, px);
     if (y) {
 #pragma unroll
       for (int i = 0; i < kTogether; i++) {
         qx[i] = wy.power(b[i]);
         gap[i] -= qx[i];
       }
-      exp2_64(qx);
+      exp2_64(table, qx);
     }
 #pragma unroll
     for (int i = 0; i < kTogether; i++)
@@ -315,8 +320,16 @@ struct Drawn {
 struct PartSums {
   double zx, zy, px, qx;  // sums of p and q over a warp's part of the vocabulary; of p and q where p > q
 };
+struct Choice {
+  double ix, iy;  // 1 / sums
+  double want;    // what the running sum has to exceed
+  double before;  // the running sum ahead of the part
+  int part;
+  bool from_p;
+};
 struct DrawShared {
   PartSums part[kDrawWarps];
+  Choice choice;
   int stop;
   RowStats target, draft;
 };
@@ -328,6 +341,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
   __shared__ DrawShared sh;
   __shared__ PartSums all[most_parts];
   __shared__ double slice[kDrawWarps];
+  __shared__ Powers table;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), parts = blocks * kDrawWarps;
   const int rank = (int)cluster.block_rank(), s = blockIdx.x / blocks;
@@ -336,6 +350,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   const float t = temperature_of(p.temperature, s), td = temperature_of(p.draft_temperature, s);
   if (tid == 0) sh.stop = end - 1;
+  if (tid < 32) table.of[tid] = exp2((double)tid / 32.0);
   __syncthreads();
   pdl_wait();
   if (beg == end) {
@@ -354,11 +369,11 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       const RowStats a = row_stats(p, r, t);
       const float lx = logit((const T *)p.logits + r * p.stride + x);
       double px = 0.0, qx = 1.0;
-      if (!a.none()) px = is_cold(t) ? (double)(a.at == x) : Weight(a.m, t)(lx) / a.sum;
+      if (!a.none()) px = is_cold(t) ? (double)(a.at == x) : Weight(a.m, t)(table, lx) / a.sum;
       if (p.draft) {
         const RowStats b = row_stats(p, p.n_rows + r, td);
         const float ly = logit((const T *)p.draft + r * p.draft_stride + x);
-        if (!b.none()) qx = is_cold(td) ? (double)(b.at == x) : Weight(b.m, td)(ly) / b.sum;
+        if (!b.none()) qx = is_cold(td) ? (double)(b.at == x) : Weight(b.m, td)(table, ly) / b.sum;
       }
       take = (double)__ldg(p.uniform + r) * qx < px;
     }
@@ -409,7 +424,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       int at[kTogether];
 #pragma unroll
       for (int i = 0; i < kTogether; i++) at[i] = i0 + 32 * i;
-      d.get(at, hi, px, qx, in);
+      d.get(table, at, hi, px, qx, in);
 #pragma unroll
       for (int i = 0; i < kTogether; i++) {
         mine.zx += px[i];
@@ -430,51 +445,60 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
     cluster.sync();
     if (tid < parts) all[tid] = cluster.map_shared_rank(&sh, tid / kDrawWarps)->part[tid % kDrawWarps];
     cluster.sync();  // no block leaves while others read its sums
-    // Every warp goes through the parts, kOfLane a lane, with the same numbers: the part
-    // in which the running sum first exceeds `want`, or the last one with any weight
-    // where rounding (or a number that is not below 1) leaves none.
-    PartSums of[kOfLane];
-    double zx = 0.0, zy = 0.0;
+    // The first warp goes through the parts, kOfLane a lane: the part in which the
+    // running sum first exceeds `want`, or the last one with any weight where
+    // rounding (or a number that is not below 1) leaves none.  (Every block does so, with
+    // the same numbers.)
+    if (warp == 0) {
+      PartSums of[kOfLane];
+      double zx = 0.0, zy = 0.0;
 #pragma unroll
-    for (int k = 0; k < kOfLane; k++) {
-      of[k] = PartSums{0.0, 0.0, 0.0, 0.0};
-      if (kOfLane * lane + k < parts) of[k] = all[kOfLane * lane + k];
-      zx += of[k].zx;
-      zy += of[k].zy;
-    }
-    const double ix = 1.0 / warp_sum64(zx), iy = d.y ? 1.0 / warp_sum64(zy) : 0.0;
-    double w[kOfLane], sum = 0.0;
-#pragma unroll
-    for (int k = 0; k < kOfLane; k++) sum += w[k] = fmax(of[k].px * ix - of[k].qx * iy, 0.0);
-    double total = warp_sum64(sum);
-    const bool from_p = !(total > 0.0);
-    if (from_p) {
-      sum = 0.0;
-#pragma unroll
-      for (int k = 0; k < kOfLane; k++) sum += w[k] = of[k].zx * ix;
-      total = warp_sum64(sum);
-    }
-    const double want = (double)__ldg(p.uniform + end - 1) * total;
-    double upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const double n = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += n;
-    }
-    double run = upto - sum, before = run;  // before: of this lane's first part past `want`, or its last one
-    int over = 0x7fffffff, last = -1;
-#pragma unroll
-    for (int k = 0; k < kOfLane; k++) {
-      if (w[k] > 0.0 && over == 0x7fffffff) {
-        last = kOfLane * lane + k;
-        before = run;
-        if (run + w[k] > want) over = last;
+      for (int k = 0; k < kOfLane; k++) {
+        of[k] = PartSums{0.0, 0.0, 0.0, 0.0};
+        if (kOfLane * lane + k < parts) of[k] = all[kOfLane * lane + k];
+        zx += of[k].zx;
+        zy += of[k].zy;
       }
-      run += w[k];
+      const double ix = 1.0 / warp_sum64(zx), iy = d.y ? 1.0 / warp_sum64(zy) : 0.0;
+      double w[kOfLane], sum = 0.0;
+#pragma unroll
+      for (int k = 0; k < kOfLane; k++) sum += w[k] = fmax(of[k].px * ix - of[k].qx * iy, 0.0);
+      double total = warp_sum64(sum);
+      const bool from_p = !(total > 0.0);
+      if (from_p) {
+        sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < kOfLane; k++) sum += w[k] = of[k].zx * ix;
+        total = warp_sum64(sum);
+      }
+      const double want = (double)__ldg(p.uniform + end - 1) * total;
+      double upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const double n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
+      }
+      double run = upto - sum, before = run;  // before: of this lane's first part past `want`, or its last one
+      int over = 0x7fffffff, last = -1;
+#pragma unroll
+      for (int k = 0; k < kOfLane; k++) {
+        if (w[k] > 0.0 && over == 0x7fffffff) {
+          last = kOfLane * lane + k;
+          before = run;
+          if (run + w[k] > want) over = last;
+        }
+        run += w[k];
+      }
+      int chosen = __reduce_min_sync(0xffffffffu, over);
+      if (chosen == 0x7fffffff) chosen = max(__reduce_max_sync(0xffffffffu, last), 0);
+      before = __shfl_sync(0xffffffffu, before, chosen / kOfLane);
+      if (lane == 0) sh.choice = Choice{ix, iy, want, before, chosen, from_p};
     }
-    int chosen = __reduce_min_sync(0xffffffffu, over);
-    if (chosen == 0x7fffffff) chosen = max(__reduce_max_sync(0xffffffffu, last), 0);
-    before = __shfl_sync(0xffffffffu, before, chosen / kOfLane);
+    __syncthreads();
+    const double ix = sh.choice.ix, iy = sh.choice.iy, want = sh.choice.want;
+    double before = sh.choice.before;
+    const int chosen = sh.choice.part;
+    const bool from_p = sh.choice.from_p;
     if (rank != chosen / kDrawWarps) return;
     // The block that has the part goes through it, kTogether tokens a lane at a time.
     const int c_lo = (int)min((int64_t)p.vocab, (int64_t)chosen * per), c_hi = (int)min((int64_t)p.vocab, (int64_t)c_lo + per);
@@ -486,11 +510,11 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       const int first = base + tid * kTogether;
 #pragma unroll
       for (int e = 0; e < kTogether; e++) at[e] = first + e;
-      d.get(at, c_hi, px, qx, in);
+      d.get(table, at, c_hi, px, qx, in);
 #pragma unroll
       for (int e = 0; e < kTogether; e++) sum += w[e] = from_p ? px[e] * ix : in[e] ? fmax(px[e] * ix - qx[e] * iy, 0.0) : 0.0;
       // Sums up to this lane, of the warps, and up to this warp.
-      upto = sum;
+      double upto = sum;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
         const double n = __shfl_up_sync(0xffffffffu, upto, o);
@@ -567,7 +591,7 @@ void run(const VerifyParams &p, cudaStream_t s) {
 
 int verify_chunks(size_t n_rows, size_t vocab) {
   // Pieces of 4096 logits at least, blocks enough for every SM several times over.
-  const size_t most = std::max<size_t>(1, vocab / 4096), want = (size_t)kPagedSMs * 8 / n_rows + 1;
+  const size_t most = std::max<size_t>(1, vocab / 4096), want = (size_t)kPagedSMs * 6 / n_rows + 1;
   return (int)std::min<size_t>(64, std::min(most, want));
 }
 
