@@ -12,14 +12,31 @@ namespace {
 
 using namespace paged;
 
-// cos and sin of pos * inv_freq in 64 bits, the angle reduced to [-pi, pi] by
-// 2 pi in two parts.  Codes go by values next to a border, so what is quantised is
-// the rotated value to the last bit of f32.
+// cos and sin of pos * inv_freq in 64 bits: the angle less the nearest multiple of
+// pi / 2 (in two parts), their power series there (the first terms left out are (pi /
+// 4)^16 / 16! = 1e-15 and (pi / 4)^15 / 15! = 2e-14), and the quarter turns.  Codes go by
+// values next to a border, so what is quantised is the rotated value to the last bit of
+// f32.
 __device__ __forceinline__ double2 turn64(int64_t pos, float inv_freq) {
-  const double a = (double)pos * (double)inv_freq, n = rint(a * 0.15915494309189535);
-  const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
-  double2 cs;
-  sincos(r, &cs.y, &cs.x);
+  const double a = (double)pos * (double)inv_freq, n = rint(a * 0.6366197723675814);
+  const double r = fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, a)), z = r * r;
+  double c = -1.0 / 87178291200.0, s = 1.0 / 6227020800.0;
+  c = fma(c, z, 1.0 / 479001600.0);
+  s = fma(s, z, -1.0 / 39916800.0);
+  c = fma(c, z, -1.0 / 3628800.0);
+  s = fma(s, z, 1.0 / 362880.0);
+  c = fma(c, z, 1.0 / 40320.0);
+  s = fma(s, z, -1.0 / 5040.0);
+  c = fma(c, z, -1.0 / 720.0);
+  s = fma(s, z, 1.0 / 120.0);
+  c = fma(c, z, 1.0 / 24.0);
+  s = fma(s, z, -1.0 / 6.0);
+  c = fma(c, z, -0.5);
+  s = fma(s * z, r, r);
+  c = fma(c, z, 1.0);
+  const int quarter = (int)(long long)n & 3;
+  double2 cs = quarter & 1 ? make_double2(-s, c) : make_double2(c, s);
+  if (quarter & 2) cs = make_double2(-cs.x, -cs.y);
   return cs;
 }
 
@@ -54,6 +71,53 @@ __device__ __forceinline__ void store_codes8(uint8_t *row, int d, const float (&
   }
 }
 
+// Eight elements as they are in memory.
+template <class T>
+struct Raw8 {
+  uint4 w;
+  __device__ __forceinline__ void load(const T *p) { w = *(const uint4 *)p; }
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = unpack2<T>(u[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+template <>
+struct Raw8<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float *p) { load8(p, v); }
+  __device__ __forceinline__ void widen(float (&o)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = v[i];
+  }
+};
+
+// The pairs of eight dims at d and the eight half a rotation further on, turned in T2's
+// type (k in 64 bits; q, which is rounded to its own type, in f32).
+template <class T2, class T1>
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const T2 *cs, int d, int half, int neox) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    if (neox) {
+      const T2 t = cs[d + e];
+      const T1 x = a[e], y = b[e];
+      a[e] = (float)(x * t.x - y * t.y);
+      b[e] = (float)(x * t.y + y * t.x);
+    } else if (e % 2 == 0) {
+      const T2 t = cs[(d + e) / 2], u = cs[(d + half + e) / 2];
+      const T1 x = a[e], y = a[e + 1], z = b[e], w = b[e + 1];
+      a[e] = (float)(x * t.x - y * t.y);
+      a[e + 1] = (float)(x * t.y + y * t.x);
+      b[e] = (float)(z * u.x - w * u.y);
+      b[e + 1] = (float)(z * u.y + w * u.x);
+    }
+  }
+}
+
 constexpr int kWarps = 4;
 
 // A warp takes part of a token row's heads, `lanes` neighbouring lanes a head.
@@ -63,10 +127,13 @@ constexpr int kWarps = 4;
 // its partners' elements.  Every lane has read what it needs before any lane of
 // the head writes, so q_out may be q.
 template <int BITS, class TA, bool PAIRS>
-__global__ void __launch_bounds__(kWarps * 32) k_quant_kv_append(const __grid_constant__ QuantAppendParams qp,
-                                                                 const int parts, const int lanes) {
+__global__ void __launch_bounds__(kWarps * 32, 5) k_quant_kv_append(const __grid_constant__ QuantAppendParams qp,
+                                                                    const int parts, const int lanes) {
   const AppendParams &p = qp.a;
+  constexpr int kItems = !PAIRS ? 1 : sizeof(TA) == 4 ? 2 : 4;  // heads of a lane on their way at a time
   __shared__ double2 turns[kWarps][kPagedMaxHeadDim / 2];
+  __shared__ float2 turns_q[kWarps][kPagedMaxHeadDim / 2];
+  pdl_wait();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
   const int row = (int)(unit / parts), part = (int)(unit - (int64_t)row * parts);
@@ -87,70 +154,81 @@ __global__ void __launch_bounds__(kWarps * 32) k_quant_kv_append(const __grid_co
     at = slot_offset(p.kv, sl, 0);
     s_at = (int64_t)sl.page * qp.s_page + sl.slot;
   }
-  double2 *const cs = turns[warp];
-  for (int i = lane; i < half; i += 32) cs[i] = turn64(pos64, __ldg(p.inv_freq + i));
-  __syncwarp();
   const int nq = p.q ? p.hq : 0, heads = nq + 2 * p.kv.hkv;
-  const int per = (heads + parts - 1) / parts, stop = min(heads, (part + 1) * per);
-  const int c = lane % lanes;
+  const int per = (heads + parts - 1) / parts, stop = min(heads, (part + 1) * per), step = 32 / lanes;
+  const int c = lane % lanes, mine = lane / lanes;
   // The eight dims of this lane, and where their partners are.
   const bool rotated = PAIRS ? c < half / 8 : false;
   const int d = PAIRS ? (rotated ? c * 8 : p.rotary + (c - half / 8) * 8) : c * 8;
-  for (int base = part * per; base < stop; base += 32 / lanes) {
-    const int head = base + lane / lanes;
-    const bool mine = head < stop && d < hd;
+  const bool inside = d < hd;
+  auto source = [&](int head) {
     const bool is_q = head < nq, is_k = !is_q && head < nq + p.kv.hkv;
     const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
-    const TA *const src = (const TA *)(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.q_stride : p.kv_stride) + h * hd;
-    float a[8] = {}, b[8] = {};
-    if (mine) {
-      load8(src + d, a);
-      if (rotated) load8(src + d + half, b);
-      if constexpr (PAIRS) {
-        if (rotated && (is_q || is_k)) {
+    return (const TA *)(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.q_stride : p.kv_stride) + h * hd;
+  };
+  double2 *const cs = turns[warp];
+  float2 *const cq = turns_q[warp];
+  bool turned = false;
+  for (int base = part * per; base < stop; base += step * kItems) {
+    Raw8<TA> ra[kItems], rb[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; k++) {
+      const int head = base + k * step + mine;
+      if (head >= stop || !inside) continue;
+      const TA *const src = source(head);
+      ra[k].load(src + d);
+      if (rotated) rb[k].load(src + d + half);
+    }
+    if (!turned) {  // (while the first rows are on their way)
+      for (int i = lane; i < half; i += 32) {
+        const double2 t = turn64(pos64, __ldg(p.inv_freq + i));
+        cs[i] = t;
+        cq[i] = make_float2((float)t.x, (float)t.y);
+      }
+      __syncwarp();
+      turned = true;
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; k++) {
+      const int head = base + k * step + mine;
+      const bool there = head < stop && inside;
+      const bool is_q = head < nq, is_k = !is_q && head < nq + p.kv.hkv;
+      const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
+      float a[8] = {}, b[8] = {};
+      if (there) {
+        ra[k].widen(a);
+        if (rotated) rb[k].widen(b);
+        if constexpr (PAIRS) {
+          if (rotated && is_q) turn8<float2, float>(a, b, cq, d, half, p.neox);
+          if (rotated && is_k) turn8<double2, double>(a, b, cs, d, half, p.neox);
+        } else if (is_q || is_k) {
+          const TA *const src = source(head);
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            if (p.neox) {
-              const double2 t = cs[d + e];
-              const double x = a[e], y = b[e];
-              a[e] = (float)(x * t.x - y * t.y);
-              b[e] = (float)(x * t.y + y * t.x);
-            } else if (e % 2 == 0) {
-              const double2 t = cs[(d + e) / 2], u = cs[(d + half + e) / 2];
-              const double x = a[e], y = a[e + 1], z = b[e], w = b[e + 1];
-              a[e] = (float)(x * t.x - y * t.y);
-              a[e + 1] = (float)(x * t.y + y * t.x);
-              b[e] = (float)(z * u.x - w * u.y);
-              b[e + 1] = (float)(z * u.y + w * u.x);
-            }
+            const int i = d + e;
+            if (i >= p.rotary) continue;
+            const bool low = p.neox ? i < half : i % 2 == 0;
+            const int other = p.neox ? (low ? i + half : i - half) : i ^ 1;
+            const double2 t = cs[p.neox ? (low ? i : i - half) : i / 2];
+            const double y = load_as_f32(src, other, p.act), x = load_as_f32(src, i, p.act);
+            a[e] = (float)(low ? x * t.x - y * t.y : y * t.y + x * t.x);
           }
         }
-      } else if (is_q || is_k) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int i = d + e;
-          if (i >= p.rotary) continue;
-          const bool low = p.neox ? i < half : i % 2 == 0;
-          const int other = p.neox ? (low ? i + half : i - half) : i ^ 1;
-          const double2 t = cs[p.neox ? (low ? i : i - half) : i / 2];
-          const double y = load_as_f32(src, other, p.act), x = load_as_f32(src, i, p.act);
-          a[e] = (float)(low ? x * t.x - y * t.y : y * t.y + x * t.x);
-        }
       }
-    }
-    // The largest magnitude of the head, by its bits: a NaN's are above infinity's.
-    uint32_t top = 0;
+      if (!PAIRS) __syncwarp();
+      if (there && is_q) {
+        TA *const dst = (TA *)p.q_out + row * p.q_out_stride + h * hd;
+        store8(dst + d, a);
+        if (rotated) store8(dst + d + half, b);
+      }
+      if (!__any_sync(0xffffffffu, there && !is_q)) continue;
+      // The largest magnitude of the head, by its bits: a NaN's are above infinity's.
+      uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
-    for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    __syncwarp();
-    if (!mine) continue;
-    if (is_q) {
-      TA *const dst = (TA *)p.q_out + row * p.q_out_stride + h * hd;
-      store8(dst + d, a);
-      if (rotated) store8(dst + d + half, b);
-    } else if (at >= 0) {
+      for (int e = 0; e < 8; e++)
+        top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
+      for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!there || is_q || at < 0) continue;
       const float m = __uint_as_float(top);
       const bool none = m < kQuantLeast, bad = !(m < kQuantMost);
       const float per_unit = none || bad ? 0.0f : __fdiv_rn(Codes<BITS>::most, m);
@@ -177,10 +255,8 @@ void run_append(const QuantAppendParams &p, cudaStream_t s) {
   const int heads = (p.a.q ? p.a.hq : 0) + 2 * p.a.kv.hkv, most = std::max(1, heads / (32 / lanes));
   const int64_t rows = p.a.n_rows;
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 32 * kPagedSMs / rows));
-  const unsigned blocks = (unsigned)((rows * parts + kWarps - 1) / kWarps);
-  if (pairs) k_quant_kv_append<BITS, TA, true><<<blocks, kWarps * 32, 0, s>>>(p, parts, lanes);
-  else k_quant_kv_append<BITS, TA, false><<<blocks, kWarps * 32, 0, s>>>(p, parts, lanes);
-  JAL_CUDA(cudaGetLastError());
+  launch_beside(pairs ? k_quant_kv_append<BITS, TA, true> : k_quant_kv_append<BITS, TA, false>,
+                (rows * parts + kWarps - 1) / kWarps, kWarps * 32, 0, s, p, parts, lanes);
 }
 template <int BITS>
 void run_append(const QuantAppendParams &p, cudaStream_t s) {
@@ -190,52 +266,83 @@ void run_append(const QuantAppendParams &p, cudaStream_t s) {
 }
 
 // ---- reading back -----------------------------------------------------------
-// A block takes kReadSlots positions of one sequence and KV head; a thread has eight
-// dims of kReadItems of them, K and V.  Bound by memory.
+// A block takes kReadSlots positions of one sequence and KV head: its first threads
+// look up where they lie and their scales, then a thread has eight dims of a position at
+// a time, K and V.  Bound by memory.
 constexpr int kReadThreads = 256, kReadSlots = 64;
 
+// Eight codes as they are in memory.
 template <int BITS>
-__device__ __forceinline__ void widen_codes8(const uint8_t *row, int d, float (&v)[8]) {
-  if constexpr (BITS == 8) {
-    const uint2 w = *(const uint2 *)(row + d);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e % 4)));
-  } else {
-    const uint32_t w = *(const uint32_t *)(row + d / 2);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = (float)((int)((w >> (4 * e)) & 15u) - 8);
+struct RawCodes8 {
+  uint32_t w[BITS / 4];
+  __device__ __forceinline__ void load(const uint8_t *row, int d) {
+    if constexpr (BITS == 8) {
+      const uint2 x = __ldg((const uint2 *)(row + d));
+      w[0] = x.x;
+      w[1] = x.y;
+    } else {
+      w[0] = __ldg((const uint32_t *)(row + d / 2));
+    }
   }
-}
+  __device__ __forceinline__ void widen(float scale, float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      // The code in the low mantissa bits of 2^23, which is taken off with its offset.
+      const uint32_t c = BITS == 8 ? __byte_perm(w[e / 4] ^ 0x80808080u, 0x4B000000u, 0x7440 + e % 4)
+                                   : ((w[0] >> (4 * e)) & 15u) | 0x4B000000u;
+      v[e] = __fmul_rn(__uint_as_float(c) - (BITS == 8 ? 8388736.0f : 8388616.0f), scale);
+    }
+  }
+};
 
 template <int BITS, class TO>
 __global__ void __launch_bounds__(kReadThreads) k_quant_kv_read(const __grid_constant__ QuantReadParams p, const int tiles) {
+  __shared__ int64_t from_at[kReadSlots], into_at[kReadSlots];
+  __shared__ float k_scale[kReadSlots], v_scale[kReadSlots];
+  pdl_wait();
   const int tile = blockIdx.x % tiles, rest = blockIdx.x / tiles, head = rest % p.from.hkv, s = rest / p.from.hkv;
   const int beg = p.first ? max(__ldg(p.first + s), 0) : 0;
   const int64_t most = min((int64_t)beg + p.max_len, (int64_t)min(p.from.cap, p.into.cap));
   const int end = (int)min((int64_t)__ldg(p.kv_len + s), most);
   const int64_t t64 = (int64_t)beg + (int64_t)tile * kReadSlots;
   if (t64 >= end) return;
-  const int t0 = (int)t64;
-  const int n8 = p.from.hd / 8, total = min(kReadSlots, end - t0) * n8;
-  const int32_t *const from = p.from.table + (int64_t)s * p.from.max_pages, *const into = p.into.table + (int64_t)s * p.into.max_pages;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < total; i += kReadThreads) {
-    const int t = t0 + i / n8, d = (i % n8) * 8;
-    const Slot a = slot_of(p.from, from, t), b = slot_of(p.into, into, t);
-    const int64_t at = slot_offset(p.from, a, head), to = slot_offset(p.into, b, head);
-    if (at < 0 || to < 0) continue;
-    const int64_t s_at = (int64_t)a.page * p.sc.s_page + head * p.sc.s_head + a.slot;
-    const float ks = __ldg(p.sc.k + s_at), vs = __ldg(p.sc.v + s_at);
-    float k[8], v[8];
-    widen_codes8<BITS>((const uint8_t *)p.from.k + at, d, k);
-    widen_codes8<BITS>((const uint8_t *)p.from.v + at, d, v);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      k[e] = __fmul_rn(k[e], ks);
-      v[e] = __fmul_rn(v[e], vs);
+  const int t0 = (int)t64, n = min(kReadSlots, end - t0);
+  if (threadIdx.x < n) {
+    const int i = threadIdx.x;
+    const Slot a = slot_of(p.from, p.from.table + (int64_t)s * p.from.max_pages, t0 + i),
+               b = slot_of(p.into, p.into.table + (int64_t)s * p.into.max_pages, t0 + i);
+    const int64_t at = slot_offset(p.from, a, head);
+    from_at[i] = at;
+    into_at[i] = at < 0 ? -1 : slot_offset(p.into, b, head);  // -1: left out
+    if (at >= 0) {
+      const int64_t s_at = (int64_t)a.page * p.sc.s_page + head * p.sc.s_head + a.slot;
+      k_scale[i] = __ldg(p.sc.k + s_at);
+      v_scale[i] = __ldg(p.sc.v + s_at);
     }
-    store8((TO *)p.kw + to + d, k);
-    store8((TO *)p.vw + to + d, v);
+  }
+  __syncthreads();
+  const int n8 = p.from.hd / 8, total = n * n8;
+  // (A lane's pieces of a round, asked for together.)
+  constexpr int kRound = 4;
+  for (int i0 = threadIdx.x; i0 < total; i0 += kReadThreads * kRound) {
+    RawCodes8<BITS> k[kRound], v[kRound];
+#pragma unroll
+    for (int r = 0; r < kRound; r++) {
+      const int i = i0 + r * kReadThreads, t = i / n8, d = (i - t * n8) * 8;
+      if (i >= total || into_at[t] < 0) continue;
+      k[r].load((const uint8_t *)p.from.k + from_at[t], d);
+      v[r].load((const uint8_t *)p.from.v + from_at[t], d);
+    }
+#pragma unroll
+    for (int r = 0; r < kRound; r++) {
+      const int i = i0 + r * kReadThreads, t = i / n8, d = (i - t * n8) * 8;
+      if (i >= total || into_at[t] < 0) continue;
+      float x[8];
+      k[r].widen(k_scale[t], x);
+      store8((TO *)p.kw + into_at[t] + d, x);
+      v[r].widen(v_scale[t], x);
+      store8((TO *)p.vw + into_at[t] + d, x);
+    }
   }
 }
 
@@ -243,10 +350,9 @@ template <int BITS>
 void run_read(const QuantReadParams &p, cudaStream_t s) {
   const int64_t tiles = (p.max_len + kReadSlots - 1) / kReadSlots, blocks = tiles * p.from.hkv * p.n_seqs;
   if (blocks > 2000000000) fail(JAL_ERR_CAPABILITY_MISMATCH, "too many positions for one launch");
-  if (p.into.dtype == JAL_F32) k_quant_kv_read<BITS, float><<<(unsigned)blocks, kReadThreads, 0, s>>>(p, (int)tiles);
-  else if (p.into.dtype == JAL_F16) k_quant_kv_read<BITS, __half><<<(unsigned)blocks, kReadThreads, 0, s>>>(p, (int)tiles);
-  else k_quant_kv_read<BITS, __nv_bfloat16><<<(unsigned)blocks, kReadThreads, 0, s>>>(p, (int)tiles);
-  JAL_CUDA(cudaGetLastError());
+  if (p.into.dtype == JAL_F32) launch_beside(k_quant_kv_read<BITS, float>, blocks, kReadThreads, 0, s, p, (int)tiles);
+  else if (p.into.dtype == JAL_F16) launch_beside(k_quant_kv_read<BITS, __half>, blocks, kReadThreads, 0, s, p, (int)tiles);
+  else launch_beside(k_quant_kv_read<BITS, __nv_bfloat16>, blocks, kReadThreads, 0, s, p, (int)tiles);
 }
 
 }  // namespace

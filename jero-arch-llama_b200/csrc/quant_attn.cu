@@ -21,16 +21,14 @@ void run_mma(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s
   constexpr int smem = QuantShape<BITS, NS, HD, R8>::smem;
   static_assert(smem <= 232448 - 2048, "shared memory of a block");
   JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_mma<BITS, NS, HD, R8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  k_quant_attn_mma<BITS, NS, HD, R8><<<(unsigned)blocks, kMmaThreads, smem, s>>>(p, plan.direct);
-  JAL_CUDA(cudaGetLastError());
+  launch_beside(k_quant_attn_mma<BITS, NS, HD, R8>, blocks, kMmaThreads, smem, s, p, plan.direct);
 }
 template <int BITS, int NS, int HD>
 void run_tc(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {
   const int64_t blocks = (int64_t)p.a.kv.hkv * p.a.splits * p.a.tiles * p.a.n_seqs;
   constexpr int smem = QuantTcShape<BITS, NS, HD>::smem;
   JAL_CUDA(cudaFuncSetAttribute(k_quant_attn_tc<BITS, NS, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  k_quant_attn_tc<BITS, NS, HD><<<(unsigned)blocks, kTcThreads, smem, s>>>(p, plan.direct);
-  JAL_CUDA(cudaGetLastError());
+  launch_beside(k_quant_attn_tc<BITS, NS, HD>, blocks, kTcThreads, smem, s, p, plan.direct);
 }
 template <int BITS, int NS, int HD>
 void run_rows(const QuantAttnParams &p, const QuantAttnPlan &plan, cudaStream_t s) {

@@ -141,12 +141,10 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
   __shared__ float q_scale[S::rows];
   __shared__ float2 row_ml[kMmaWarps][S::rows];
   __shared__ uint32_t present[kMmaWarps][S::stages];
+  pdl_wait();
   pdl_trigger();
   Tile t;
-  if (!block_tile(p, kOwn, S::rows, kMmaWarps * kQuantKeys, t)) {
-    pdl_wait();
-    return;
-  }
+  if (!block_tile(p, kOwn, S::rows, kMmaWarps * kQuantKeys, t)) return;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, hd = p.kv.hd;
   const int g = lane / 4, j4 = lane % 4;  // this lane's row (or column), and quarter
   const uint32_t sq = smem_u32(smem_raw), ring = sq + S::q_bytes + warp * (S::stages * S::stage);
@@ -445,7 +443,6 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
   }
   copies_wait<0>();
   __syncthreads();  // no warp reads its ring any more
-  pdl_wait();
   // The four warps' results, joined through shared memory.
   float *const merge = (float *)(smem_raw + S::q_bytes);
 #pragma unroll

@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
   const AttnParams &p = qp.a;
   extern __shared__ __align__(1024) char smem_tc[];
   QuantTcSync &sy = *(QuantTcSync *)(smem_tc + S::sync);
+  pdl_wait();
   pdl_trigger();
   Tile t;
   if (!block_tile(p, kOwn, kTcRows, kTcKeys, t)) return;

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kStatThreads) k_verify_stats(const __grid_cons
   constexpr int N = 16 / sizeof(T);
   __shared__ float red_m[kStatThreads / 32], red_s[kStatThreads / 32];
   __shared__ int red_i[kStatThreads / 32];
+  pdl_wait();
   pdl_trigger();
   const int chunk = blockIdx.x % p.chunks, which = blockIdx.x / p.chunks, row = which % p.n_rows;
   const bool draft = which >= p.n_rows;
@@ -566,8 +567,7 @@ template <class T>
 void run(const VerifyParams &p, cudaStream_t s) {
   if (p.n_rows) {
     const int64_t blocks = (int64_t)p.n_rows * p.chunks * (p.draft ? 2 : 1);
-    k_verify_stats<T><<<(unsigned)blocks, kStatThreads, 0, s>>>(p);
-    JAL_CUDA(cudaGetLastError());
+    launch_beside(k_verify_stats<T>, blocks, kStatThreads, 0, s, p);
   }
   cudaLaunchConfig_t cfg = {};
   // Blocks of a sequence: parts of 128 tokens a warp at least.

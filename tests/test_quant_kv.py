@@ -175,11 +175,16 @@ def test_append_is_the_definition(jal, torch_cuda, act, bits, hd, rotary, neox, 
         assert torch.equal(got.cpu(), want)
     for got, want in ((c.d_ks, sc[0]), (c.d_vs, sc[1])):
         assert _same(got.cpu(), want)
-    # queries: the rotation in 64 bits, rounded to f32 and then to the type, in place; other rows as they were
+    # queries, in place: rotated in f32, each of x cos and y sin off by 2 roundings and their sum by one, which is at most
+    # 3 (|x cos| + |y sin|) <= 3 sqrt 2 |(x, y)| times 2^-24; then the type's rounding.  Other rows as they were.
     got = c.d_q.cpu()
     n = sum(c.news)
     back = got[:, :c.hq * hd].reshape(c.n_rows, c.hq, hd).double()
-    off = (2.0 ** -23 + half_step(c.act)) * q.abs() + torch.finfo(c.act).smallest_normal
+    i0 = torch.arange(rotary // 2) if neox else torch.arange(0, rotary, 2)
+    i1 = i0 + (rotary // 2 if neox else 1)
+    size = q.abs()
+    size[..., i0] = size[..., i1] = torch.hypot(q[..., i0], q[..., i1])
+    off = 3 * 2 ** 0.5 * 2.0 ** -24 * size + half_step(c.act) * (q.abs() + 2.0 ** -21 * size) + torch.finfo(c.act).smallest_normal
     assert bool(((back - q).abs() <= off)[:n].all())
     assert torch.equal(got[n:], c.q_full[n:]) and torch.equal(got[:, c.hq * hd:], c.q_full[:, c.hq * hd:])
 
