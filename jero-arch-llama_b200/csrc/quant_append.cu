@@ -96,24 +96,26 @@ struct Raw8<float> {
   }
 };
 
-// The pairs of eight dims at d and the eight half a rotation further on, turned in T2's
-// type (k in 64 bits; q, which is rounded to its own type, in f32).
-template <class T2, class T1>
-__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const T2 *cs, int d, int half, int neox) {
+// The pairs of eight dims at d and the eight half a rotation further on, turned: t[i]
+// is pair i's cosine and sine.  (k in 64 bits; q, which is rounded to its own type, in f32.)
+template <class T1, class T2>
+__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const T2 (&t)[8], int neox) {
+  if (neox) {
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    if (neox) {
-      const T2 t = cs[d + e];
+    for (int e = 0; e < 8; e++) {
       const T1 x = a[e], y = b[e];
-      a[e] = (float)(x * t.x - y * t.y);
-      b[e] = (float)(x * t.y + y * t.x);
-    } else if (e % 2 == 0) {
-      const T2 t = cs[(d + e) / 2], u = cs[(d + half + e) / 2];
+      a[e] = (float)(x * t[e].x - y * t[e].y);
+      b[e] = (float)(x * t[e].y + y * t[e].x);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
       const T1 x = a[e], y = a[e + 1], z = b[e], w = b[e + 1];
-      a[e] = (float)(x * t.x - y * t.y);
-      a[e + 1] = (float)(x * t.y + y * t.x);
-      b[e] = (float)(z * u.x - w * u.y);
-      b[e + 1] = (float)(z * u.y + w * u.x);
+      const T2 f = t[e / 2], g = t[4 + e / 2];
+      a[e] = (float)(x * f.x - y * f.y);
+      a[e + 1] = (float)(x * f.y + y * f.x);
+      b[e] = (float)(z * g.x - w * g.y);
+      b[e + 1] = (float)(z * g.y + w * g.x);
     }
   }
 }
@@ -131,8 +133,8 @@ __global__ void __launch_bounds__(kWarps * 32, 5) k_quant_kv_append(const __grid
                                                                     const int parts, const int lanes) {
   const AppendParams &p = qp.a;
   constexpr int kItems = !PAIRS ? 1 : sizeof(TA) == 4 ? 2 : 4;  // heads of a lane on their way at a time
+  constexpr int kKvItems = kItems > 2 ? 2 : 1;
   __shared__ double2 turns[kWarps][kPagedMaxHeadDim / 2];
-  __shared__ float2 turns_q[kWarps][kPagedMaxHeadDim / 2];
   pdl_wait();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
@@ -161,74 +163,112 @@ __global__ void __launch_bounds__(kWarps * 32, 5) k_quant_kv_append(const __grid
   const bool rotated = PAIRS ? c < half / 8 : false;
   const int d = PAIRS ? (rotated ? c * 8 : p.rotary + (c - half / 8) * 8) : c * 8;
   const bool inside = d < hd;
-  auto source = [&](int head) {
-    const bool is_q = head < nq, is_k = !is_q && head < nq + p.kv.hkv;
-    const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
-    return (const TA *)(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.q_stride : p.kv_stride) + h * hd;
-  };
   double2 *const cs = turns[warp];
-  float2 *const cq = turns_q[warp];
-  bool turned = false;
-  for (int base = part * per; base < stop; base += step * kItems) {
-    Raw8<TA> ra[kItems], rb[kItems];
+  for (int i = lane; i < half; i += 32) cs[i] = turn64(pos64, __ldg(p.inv_freq + i));
+  __syncwarp();
+  // This lane's pair i: d + i (split halves); d / 2 + i and (d + half) / 2 + i - 4 (neighbours).
+  auto pair_of = [&](int i) { return p.neox ? d + i : i < 4 ? d / 2 + i : (d + half) / 2 + i - 4; };
+  // Without PAIRS: element i of a head's row with its partner, wherever that is.
+  auto turn1 = [&](const TA *src, int i) -> float {
+    const bool low = p.neox ? i < half : i % 2 == 0;
+    const int other = p.neox ? (low ? i + half : i - half) : i ^ 1;
+    const double2 t = cs[p.neox ? (low ? i : i - half) : i / 2];
+    const double y = load_as_f32(src, other, p.act), x = load_as_f32(src, i, p.act);
+    return (float)(low ? x * t.x - y * t.y : y * t.y + x * t.x);
+  };
+  int base = part * per;
+  const int q_stop = min(stop, nq);
+  if (base < q_stop) {
+    const TA *const src = (const TA *)p.q + row * p.q_stride + d;
+    TA *const dst = (TA *)p.q_out + row * p.q_out_stride + d;
+    float2 t[8];
 #pragma unroll
-    for (int k = 0; k < kItems; k++) {
-      const int head = base + k * step + mine;
-      if (head >= stop || !inside) continue;
-      const TA *const src = source(head);
-      ra[k].load(src + d);
-      if (rotated) rb[k].load(src + d + half);
-    }
-    if (!turned) {  // (while the first rows are on their way)
-      for (int i = lane; i < half; i += 32) {
-        const double2 t = turn64(pos64, __ldg(p.inv_freq + i));
-        cs[i] = t;
-        cq[i] = make_float2((float)t.x, (float)t.y);
+    for (int i = 0; i < 8; i++) {
+      t[i] = make_float2(1.0f, 0.0f);
+      if (rotated) {
+        const double2 x = cs[pair_of(i)];
+        t[i] = make_float2((float)x.x, (float)x.y);
       }
-      __syncwarp();
-      turned = true;
+    }
+    for (; base < q_stop; base += step * kItems) {
+      Raw8<TA> ra[kItems], rb[kItems];
+#pragma unroll
+      for (int k = 0; k < kItems; k++) {
+        const int head = base + k * step + mine;
+        if (head >= q_stop || !inside) continue;
+        ra[k].load(src + head * hd);
+        if (rotated) rb[k].load(src + head * hd + half);
+      }
+#pragma unroll
+      for (int k = 0; k < kItems; k++) {
+        const int head = base + k * step + mine;
+        const bool there = head < q_stop && inside;
+        float a[8], b[8];
+        if (there) {
+          ra[k].widen(a);
+          if constexpr (PAIRS) {
+            if (rotated) {
+              rb[k].widen(b);
+              turn8<float>(a, b, t, p.neox);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              if (d + e < p.rotary) a[e] = turn1(src - d + head * hd, d + e);
+          }
+        }
+        if (!PAIRS) __syncwarp();
+        if (there) {
+          store8(dst + head * hd, a);
+          if (rotated) store8(dst + head * hd + half, b);
+        }
+      }
+    }
+    base = q_stop;
+  }
+  for (; base < stop; base += step * kKvItems) {
+    Raw8<TA> ra[kKvItems], rb[kKvItems];
+#pragma unroll
+    for (int k = 0; k < kKvItems; k++) {
+      const int i = base + k * step + mine - nq;
+      if (i >= stop - nq || !inside) continue;
+      const bool is_k = i < p.kv.hkv;
+      const TA *const src = (const TA *)(is_k ? p.k : p.v) + row * p.kv_stride + (is_k ? i : i - p.kv.hkv) * hd + d;
+      ra[k].load(src);
+      if (rotated) rb[k].load(src + half);
     }
 #pragma unroll
-    for (int k = 0; k < kItems; k++) {
-      const int head = base + k * step + mine;
-      const bool there = head < stop && inside;
-      const bool is_q = head < nq, is_k = !is_q && head < nq + p.kv.hkv;
-      const int h = is_q ? head : head - nq - (is_k ? 0 : p.kv.hkv);
+    for (int k = 0; k < kKvItems; k++) {
+      const int i = base + k * step + mine - nq;
+      const bool there = i < stop - nq && inside, is_k = i < p.kv.hkv;
+      const int h = is_k ? i : i - p.kv.hkv;
       float a[8] = {}, b[8] = {};
       if (there) {
         ra[k].widen(a);
         if (rotated) rb[k].widen(b);
-        if constexpr (PAIRS) {
-          if (rotated && is_q) turn8<float2, float>(a, b, cq, d, half, p.neox);
-          if (rotated && is_k) turn8<double2, double>(a, b, cs, d, half, p.neox);
-        } else if (is_q || is_k) {
-          const TA *const src = source(head);
+        if (is_k) {
+          if constexpr (PAIRS) {
+            if (rotated) {
+              double2 t[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const int i = d + e;
-            if (i >= p.rotary) continue;
-            const bool low = p.neox ? i < half : i % 2 == 0;
-            const int other = p.neox ? (low ? i + half : i - half) : i ^ 1;
-            const double2 t = cs[p.neox ? (low ? i : i - half) : i / 2];
-            const double y = load_as_f32(src, other, p.act), x = load_as_f32(src, i, p.act);
-            a[e] = (float)(low ? x * t.x - y * t.y : y * t.y + x * t.x);
+              for (int e = 0; e < 8; e++) t[e] = cs[pair_of(e)];
+              turn8<double>(a, b, t, p.neox);
+            }
+          } else {
+            const TA *const src = (const TA *)p.k + row * p.kv_stride + h * hd;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              if (d + e < p.rotary) a[e] = turn1(src, d + e);
           }
         }
       }
-      if (!PAIRS) __syncwarp();
-      if (there && is_q) {
-        TA *const dst = (TA *)p.q_out + row * p.q_out_stride + h * hd;
-        store8(dst + d, a);
-        if (rotated) store8(dst + d + half, b);
-      }
-      if (!__any_sync(0xffffffffu, there && !is_q)) continue;
       // The largest magnitude of the head, by its bits: a NaN's are above infinity's.
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 8; e++)
         top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
       for (int o = lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!there || is_q || at < 0) continue;
+      if (!there || at < 0) continue;
       const float m = __uint_as_float(top);
       const bool none = m < kQuantLeast, bad = !(m < kQuantMost);
       const float per_unit = none || bad ? 0.0f : __fdiv_rn(Codes<BITS>::most, m);
