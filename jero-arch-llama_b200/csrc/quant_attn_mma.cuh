@@ -39,17 +39,17 @@ constexpr int kQuantKeys = 32;
 constexpr uint32_t kIntZero = 0x4B400000u;  // 1.5 * 2^23 as f32: an integer sum of 0
 constexpr float kIntZeroF = 12582912.0f;
 
-// Products of signed bytes with signed (BITS = 8) or unsigned (4) ones.
+// d = c + products of signed bytes with signed (BITS = 8) or unsigned (4) ones.
 template <int BITS>
-__device__ __forceinline__ void imma(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void imma(uint32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const uint32_t (&c)[4]) {
   if constexpr (BITS == 8)
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
   else
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 // Two 16 x 16 tiles of bytes, transposed: lane 4 g + j gets of each tile the rows
 // 4 j .. 4 j + 3 of column g, and of column g + 8.  Lane i gives row i's address.
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
   float top[R8], l[R8];  // running maxima, which the weights refer to, and their sums
   pair_t o[R8][HD / 8];
   // Where an accumulator of scores starts: 4-bit codes are stored with 8 added.
-  uint32_t start[R8][NS][2];
+  uint32_t start[R8][NS][4];
 #pragma unroll
   for (int m = 0; m < R8; m++) {
     const int r = m * 8 + g;
@@ -266,13 +266,14 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
         for (int ks = 0; ks < S::ksteps; ks++) {
           uint32_t a[4];
           lds<16>(sq + ((s * R8 + m) * S::ksteps + ks) * 512 + lane * 16, a);
-          imma<8>(c, a, 0xF8F8F8F8u, 0xF8F8F8F8u);
+          imma<8>(c, a, 0xF8F8F8F8u, 0xF8F8F8F8u, c);
         }
       }
-      start[m][s][0] = c[0];
-      start[m][s][1] = c[2];
+      start[m][s][0] = start[m][s][1] = c[0];
+      start[m][s][2] = start[m][s][3] = c[2];
     }
   }
+  uint32_t zero[4] = {kIntZero, kIntZero, kIntZero, kIntZero};
   const pair_t minus = pair(-kIntZeroF, -kIntZeroF), digit = pair(256.0f, 256.0f);
   // What accumulators of the digits hold, in f32.
   auto whole_pair = [&](const uint32_t (&c)[NS][4]) -> pair_t {
@@ -302,38 +303,40 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
     const uint32_t bits = present[warp][stage];
     // Scores: the lane has keys 8 n + 2 j4 and the next one.
     pair_t s[R8][4];
-#pragma unroll
-    for (int n = 0; n < 4; n++) {
-      uint32_t acc[R8][NS][4];
-#pragma unroll
-      for (int m = 0; m < R8; m++)
-#pragma unroll
-        for (int q = 0; q < NS; q++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[m][q][e] = BITS == 4 ? start[m][q][e / 2] : kIntZero;
+    {
       constexpr int lane_bytes = S::chunks >= 4 ? 16 : 8, words = lane_bytes / 4, pieces = S::row_bytes / (4 * lane_bytes);
+      constexpr int steps = words * 4 / BITS;  // of a piece
+      uint32_t acc[4][R8][NS][4];
 #pragma unroll
       for (int pc = 0; pc < pieces; pc++) {
-        uint32_t w[words];
-        if constexpr (lane_bytes == 16) lds<16>(kb + S::k_at(n * 8 + g, pc * 4 + j4), w);
-        else lds<8>(kb + S::k_at(n * 8 + g, 0) + j4 * 8, w);
+        uint32_t w[4][words];
 #pragma unroll
-        for (int x = 0; x < words * 4 / BITS; x++) {
-          const int ks = pc * (words * 4 / BITS) + x;
-          const uint32_t b0 = BITS == 8 ? w[(2 * x) % words] : w[x % words] & 0x0F0F0F0Fu;
-          const uint32_t b1 = BITS == 8 ? w[(2 * x + 1) % words] : (w[x % words] >> 4) & 0x0F0F0F0Fu;
+        for (int n = 0; n < 4; n++) {
+          if constexpr (lane_bytes == 16) lds<16>(kb + S::k_at(n * 8 + g, pc * 4 + j4), w[n]);
+          else lds<8>(kb + S::k_at(n * 8 + g, 0) + j4 * 8, w[n]);
+        }
+#pragma unroll
+        for (int x = 0; x < steps; x++) {
+          const int ks = pc * steps + x;
 #pragma unroll
           for (int m = 0; m < R8; m++)
 #pragma unroll
             for (int q = 0; q < NS; q++) {
               uint32_t a[4];
               lds<16>(sq + ((q * R8 + m) * S::ksteps + ks) * 512 + lane * 16, a);
-              imma<BITS>(acc[m][q], a, b0, b1);
+#pragma unroll
+              for (int n = 0; n < 4; n++) {
+                const uint32_t b0 = BITS == 8 ? w[n][(2 * x) % words] : w[n][x % words] & 0x0F0F0F0Fu;
+                const uint32_t b1 = BITS == 8 ? w[n][(2 * x + 1) % words] : (w[n][x % words] >> 4) & 0x0F0F0F0Fu;
+                imma<BITS>(acc[n][m][q], a, b0, b1, ks ? acc[n][m][q] : start[m][q]);
+              }
             }
         }
       }
 #pragma unroll
-      for (int m = 0; m < R8; m++) s[m][n] = whole_pair(acc[m]);
+      for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int m = 0; m < R8; m++) s[m][n] = whole_pair(acc[n][m]);
     }
     const int u = t.u0 + c * kQuantKeys;
     bool all = bits == 0xffffffffu;
@@ -411,8 +414,7 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
     for (int m = 0; m < R8; m++)
 #pragma unroll
       for (int q = 0; q < NS; q++) {
-        first[m][q][0] = first[m][q][1] = first[m][q][2] = first[m][q][3] = kIntZero;
-        if (BITS == 4) imma<8>(first[m][q], wa[m][q], 0xF8F8F8F8u, 0xF8F8F8F8u);
+        if constexpr (BITS == 4) imma<8>(first[m][q], wa[m][q], 0xF8F8F8F8u, 0xF8F8F8F8u, zero);
       }
 #pragma unroll
     for (int ch = 0; ch < S::chunks; ch++) {
@@ -428,11 +430,7 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
         for (int m = 0; m < R8; m++) {
           uint32_t acc[NS][4];
 #pragma unroll
-          for (int q = 0; q < NS; q++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[q][i] = first[m][q][i];
-            imma<BITS>(acc[q], wa[m][q], b0, b1);
-          }
+          for (int q = 0; q < NS; q++) imma<BITS>(acc[q], wa[m][q], b0, b1, BITS == 4 ? first[m][q] : zero);
           pair_t &out = o[m][ch * (2 * 8 / BITS) + x];
           out = fma2(whole_pair(acc), pair(unit[m], unit[m]), out);
         }
