@@ -291,7 +291,7 @@ static size_t verify_bytes(const jal_ragged_batch &b, size_t vocab) {
   const size_t chunks = b.n_rows ? (size_t)verify_chunks(b.n_rows, vocab) : 1;
   if (2 * b.n_rows * chunks > kMaxInt)
     fail(JAL_ERR_CAPABILITY_MISMATCH, "batch of %llu rows too large for one launch", (unsigned long long)b.n_rows);
-  return 2 * b.n_rows * chunks * sizeof(float2);
+  return verify_workspace(b.n_seqs, b.n_rows, vocab, nullptr, nullptr);
 }
 
 int jal_op_verify_drafts(const jal_ragged_batch *batch, const void *logits, int dtype, size_t stride,
@@ -355,7 +355,7 @@ int jal_op_verify_drafts(const jal_ragged_batch *batch, const void *logits, int 
     p.out_tokens = out_tokens;
     p.n_accepted = n_accepted;
     p.new_len = new_len;
-    p.part = (float2 *)ws;
+    verify_workspace(b.n_seqs, b.n_rows, vocab, &p, ws);
     p.n_seqs = (int32_t)b.n_seqs;
     p.n_rows = (int32_t)b.n_rows;
     p.vocab = (int32_t)vocab;

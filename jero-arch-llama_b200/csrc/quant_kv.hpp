@@ -67,17 +67,24 @@ struct QuantReadParams {
 };
 void launch_quant_kv_read(const QuantReadParams &p, int bits, cudaStream_t s);
 
+struct VerifySums {
+  double zx, zy, px, qx;  // sums of p and q over a part of the vocabulary; of p and q where p > q
+};
 struct VerifyParams {
   const void *logits, *draft;  // draft: null where drafts have no probabilities
   int64_t stride, draft_stride;
   const int32_t *q_start, *kv_len, *tokens;
   const float *uniform, *temperature, *draft_temperature;
   int32_t *out_tokens, *n_accepted, *new_len;
-  float2 *part;  // [2][n_rows][chunks]: target's, then draft's
+  VerifySums *parts;  // [n_seqs][parts of the vocabulary]
+  float2 *part;       // [2][n_rows][chunks]: target's, then draft's
+  int32_t *arrived;   // [n_seqs]: blocks that have left their sums
   int32_t n_seqs, n_rows, vocab, chunks, dtype;
 };
 // Pieces a row of logits is cut into.
 int verify_chunks(size_t n_rows, size_t vocab);
+// Bytes of the workspace; its places into p, where that is given.
+size_t verify_workspace(size_t n_seqs, size_t n_rows, size_t vocab, VerifyParams *p, void *ws);
 void launch_verify_drafts(const VerifyParams &p, cudaStream_t s);
 
 }  // namespace jal

@@ -3,17 +3,17 @@
 //
 // Two kernels.  The first reads every row of logits once, in pieces: the largest
 // logit m and sum exp((x - m) / T) of each piece (of greedy rows the first of the
-// largest).  The second has a cluster of blocks for each sequence: the pieces give
-// p(x) and q(x) of every draft, hence the row that emits a token; of that row alone
-// the probabilities are formed again, in 64 bits, summed in the order of the
-// vocabulary, and searched for the random number.
+// largest).  The second has a few blocks for each sequence: the pieces give p(x) and
+// q(x) of every draft, hence the row that emits a token; of that row alone the
+// probabilities are formed again, in 64 bits, and summed over parts of the vocabulary;
+// the sequence's last block to be done with that finds the part, and in it the token, in
+// which the running sum passes the random number.
 //
 // The sums of the drawn row are in 64 bits because a token is where a number falls
 // among up to 2^17 sums: with relative errors of 2^-24 in them, one draw in a hundred
 // would be another token.
-#include <cooperative_groups.h>
-
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "paged_attn_tc.cuh"
@@ -25,18 +25,12 @@ namespace jal {
 namespace {
 
 using namespace paged;
-namespace cg = cooperative_groups;
 
-constexpr int kStatThreads = 256, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kCluster = 8;
+constexpr int kStatThreads = 256, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawBlocks = 8;  // kDrawBlocks: of a sequence, at most
 constexpr float kCold = 1e-5f;  // temperatures up to this: all of the probability on the first largest logit
 constexpr float kLog2e = 1.4426950408889634f;
 
 // (An infinite temperature would make 0 x -inf of a logit of -inf.)
-__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
-  pair_t v;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
 __device__ __forceinline__ float temperature_of(const float *t, int s) {
   if (!t) return 1.0f;
   const float x = __ldg(t + s);
@@ -52,9 +46,31 @@ template <>
 __device__ __forceinline__ float logit<__half>(const __half *p) { return __half2float(__ldg(p)); }
 template <>
 __device__ __forceinline__ float logit<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(__ldg(p)); }
+// The larger of two words' values (a NaN is passed over), and a word's values.
+template <class T>
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+template <>
+__device__ __forceinline__ uint32_t word_max<__half>(uint32_t a, uint32_t b) {
+  uint32_t v;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+  return v;
+}
+template <>
+__device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t v;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+  return v;
+}
+template <class T>
+constexpr uint32_t kLowest = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+
 // Elements [lo, hi) of a row by the block's threads, kBatch pieces of 16 bytes at a time
-// where they are aligned: f(values[kBatch * N], first indexes of the pieces), a NaN as
-// -inf, and -inf where there is none.
+// where they are aligned: f(words, first indexes of the pieces), -inf where there is no
+// element.
 constexpr int kBatch = 4;
 template <class T, class F>
 __device__ __forceinline__ void each_batch(const T *row, int lo, int hi, F &&f) {
@@ -62,51 +78,105 @@ __device__ __forceinline__ void each_batch(const T *row, int lo, int hi, F &&f) 
   const int skip = (int)((16 - ((uintptr_t)(row + lo) & 15)) & 15) / (int)sizeof(T);
   const int a = min(hi, lo + skip), n = (hi - a) / N, b = a + n * N;
   auto one = [&](int i) {
-    float x[kBatch * N];
+    uint32_t w[kBatch * 4];
     int at[kBatch];
 #pragma unroll
-    for (int e = 0; e < kBatch * N; e++) x[e] = -INFINITY;
+    for (int e = 0; e < kBatch * 4; e++) w[e] = kLowest<T>;
 #pragma unroll
     for (int k = 0; k < kBatch; k++) at[k] = i;
-    x[0] = fmaxf(logit(row + i), -INFINITY);
-    f(x, at);
+    if constexpr (sizeof(T) == 4) w[0] = __ldg((const uint32_t *)row + i);
+    else w[0] = __byte_perm(__ldg((const uint16_t *)row + i), kLowest<T>, 0x5410);
+    f(w, at);
   };
   for (int i = lo + threadIdx.x; i < a; i += kStatThreads) one(i);
   for (int k0 = threadIdx.x; k0 < n; k0 += kStatThreads * kBatch) {
-    uint4 w[kBatch];
-    float x[kBatch * N];
+    uint32_t w[kBatch * 4];
     int at[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; k++) {
       const int i = k0 + k * kStatThreads;
       at[k] = a + i * N;
-      if (i < n) w[k] = ldg_stream16(row + at[k]);
+      uint4 x = make_uint4(kLowest<T>, kLowest<T>, kLowest<T>, kLowest<T>);
+      if (i < n) x = ldg_stream16(row + at[k]);
+      w[4 * k] = x.x;
+      w[4 * k + 1] = x.y;
+      w[4 * k + 2] = x.z;
+      w[4 * k + 3] = x.w;
     }
-#pragma unroll
-    for (int k = 0; k < kBatch; k++) {
-      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-      const bool there = k0 + k * kStatThreads < n;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        if constexpr (sizeof(T) == 4) {
-          x[k * N + e] = there ? fmaxf(__uint_as_float(u[e]), -INFINITY) : -INFINITY;
-        } else {
-          const float2 v = unpack2<T>(u[e]);
-          x[k * N + 2 * e] = there ? fmaxf(v.x, -INFINITY) : -INFINITY;
-          x[k * N + 2 * e + 1] = there ? fmaxf(v.y, -INFINITY) : -INFINITY;
-        }
-      }
-    }
-    f(x, at);
+    f(w, at);
   }
   for (int i = b + threadIdx.x; i < hi; i += kStatThreads) one(i);
+}
+template <class T>
+__device__ __forceinline__ float word_top(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else {
+    const float2 v = unpack2<T>(w);
+    return fmaxf(v.x, v.y);
+  }
+}
+
+// Largest logit and sum of a thread's elements.  Quickly: the exponentials are
+// 2^(x c - k), with k the whole number above the largest x c so far, so x c - k is
+// rounded once, and the sum is brought to the largest logit at the end.  False where that
+// does not do: a NaN (which makes the sum one), or x c that no longer has a fraction.
+template <class T>
+__device__ __forceinline__ bool sum_up(const T *x, int lo, int hi, float c, float &m, float &sum) {
+  float k = -INFINITY;
+  m = -INFINITY;
+  sum = 0.0f;
+  const pair_t c2 = pair(c, c);
+  each_batch(x, lo, hi, [&](uint32_t (&w)[kBatch * 4], const int (&)[kBatch]) {
+    uint32_t top = word_max<T>(w[0], kLowest<T>);
+#pragma unroll
+    for (int e = 1; e < kBatch * 4; e++) top = word_max<T>(top, w[e]);
+    const float most = word_top<T>(top);
+    if (most > m) {
+      m = most;
+      const float next = ceilf(m * c);
+      sum *= exp2_fast(k - next);  // (k = -inf: the sum is 0)
+      k = next;
+    }
+    if (m == -INFINITY) return;
+    const pair_t less = pair(-k, -k);
+    pair_t part[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < kBatch * 4; e += sizeof(T) / 2) {
+      float2 v;
+      if constexpr (sizeof(T) == 4) v = make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1]));
+      else v = unpack2<T>(w[e]);
+      float y, z;
+      unpair(fma2(pair(v.x, v.y), c2, less), y, z);
+      part[e / 2 % 2] = add2(part[e / 2 % 2], pair(exp2_fast(y), exp2_fast(z)));
+    }
+    float y, z;
+    unpair(add2(part[0], part[1]), y, z);
+    sum += y + z;
+  });
+  if (m == -INFINITY || m == INFINITY) return true;
+  sum *= exp2f(fmaf(-m, c, k));
+  return sum == sum && fabsf(k) < 4194304.0f;
+}
+// The same for any logits: NaNs passed over, exponents of differences.
+template <class T>
+__device__ __noinline__ void sum_up_any(const T *x, int lo, int hi, float c, float &m_out, float &sum_out) {
+  float m = -INFINITY, sum = 0.0f;
+  for (int i = lo + threadIdx.x; i < hi; i += kStatThreads) {
+    const float v = fmaxf(logit(x + i), -INFINITY);
+    if (v > m) {
+      sum *= exp2f((m - v) * c);
+      m = v;
+    }
+    if (v > -INFINITY) sum += exp2f((v - m) * c);
+  }
+  m_out = m;
+  sum_out = sum;
 }
 
 // One piece of one row, target's or draft's: its largest logit with, of warm rows,
 // the sum of the exponentials relative to it, of cold ones the first index of it.
 template <class T>
 __global__ void __launch_bounds__(kStatThreads) k_verify_stats(const __grid_constant__ VerifyParams p) {
-  constexpr int N = 16 / sizeof(T);
   __shared__ float red_m[kStatThreads / 32], red_s[kStatThreads / 32];
   __shared__ int red_i[kStatThreads / 32];
   pdl_wait();
@@ -124,48 +194,37 @@ __global__ void __launch_bounds__(kStatThreads) k_verify_stats(const __grid_cons
   const int lo = (int)min((int64_t)p.vocab, (int64_t)chunk * per), hi = (int)min((int64_t)p.vocab, (int64_t)lo + per);
   const T *const x = (const T *)(draft ? p.draft : p.logits) + row * (draft ? p.draft_stride : p.stride);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0 && chunk == 0 && row == beg && !draft) p.arrived[s] = 0;
   float m = -INFINITY, sum = 0.0f;
   int at = 0x7fffffff;
   if (is_cold(t)) {
-    each_batch(x, lo, hi, [&](const float (&v)[kBatch * N], const int (&i)[kBatch]) {
+    each_batch(x, lo, hi, [&](uint32_t (&w)[kBatch * 4], const int (&i)[kBatch]) {
 #pragma unroll
       for (int k = 0; k < kBatch; k++) {
-        float most = v[k * N];
+        uint32_t top = word_max<T>(w[4 * k], kLowest<T>);
 #pragma unroll
-        for (int e = 1; e < N; e++) most = fmaxf(most, v[k * N + e]);
+        for (int e = 1; e < 4; e++) top = word_max<T>(top, w[4 * k + e]);
+        const float most = word_top<T>(top);
         if (most < m || most == -INFINITY) continue;
         int first = 0x7fffffff;
 #pragma unroll
-        for (int e = N - 1; e >= 0; e--)
-          if (v[k * N + e] == most) first = i[k] + e;
+        for (int e = 3; e >= 0; e--) {
+          if constexpr (sizeof(T) == 4) {
+            if (__uint_as_float(w[4 * k + e]) == most) first = i[k] + e;
+          } else {
+            const float2 v = unpack2<T>(w[4 * k + e]);
+            if (v.y == most) first = i[k] + 2 * e + 1;
+            if (v.x == most) first = i[k] + 2 * e;
+          }
+        }
         at = most > m ? first : min(at, first);
         m = most;
       }
     });
   } else {
     const float c = kLog2e / t;
-    const pair_t c2 = pair(c, c);
-    each_batch(x, lo, hi, [&](const float (&v)[kBatch * N], const int (&)[kBatch]) {
-      float most = v[0];
-#pragma unroll
-      for (int e = 1; e < kBatch * N; e++) most = fmaxf(most, v[e]);
-      if (most > m) {
-        sum *= exp2_fast((m - most) * c);  // (m = -inf: the sum is 0)
-        m = most;
-      }
-      if (m == -INFINITY) return;
-      const pair_t less = pair(-m, -m);
-      pair_t part[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < kBatch * N; e += 2) {
-        float y, z;
-        unpair(mul2(add2(pair(v[e], v[e + 1]), less), c2), y, z);
-        part[e / 2 % 2] = add2(part[e / 2 % 2], pair(exp2_fast(y), exp2_fast(z)));
-      }
-      float y, z;
-      unpair(add2(part[0], part[1]), y, z);
-      sum += y + z;
-    });
+    const bool done = sum_up(x, lo, hi, c, m, sum);
+    if (__syncthreads_or(!done)) sum_up_any(x, lo, hi, c, m, sum);
   }
   // Threads, then warps.
   float most = warp_max(m);
@@ -235,11 +294,9 @@ __device__ __forceinline__ double warp_sum64(double v) {
 // operations): to the nearest 32nd in the exponent, whose power comes from a table, and
 // the rest, at most 1/64, by its power series; the first term left out is (ln 2 / 64)^5
 // / 5! = 1.2e-12 of the result.  0 for y below -1000, and for -inf and NaN.
+// All lanes of a warp together: lane i holds the table's entry i.
 constexpr int kTogether = 4;
-struct Powers {
-  double of[32];  // 2^(i / 32)
-};
-__device__ __forceinline__ void exp2_64(const Powers &table, double (&y)[kTogether]) {
+__device__ __forceinline__ void exp2_64(double entry, double (&y)[kTogether]) {
   constexpr double series[5] = {1.0, 6.931471805599453e-01, 2.402265069591007e-01, 5.5504108664821576e-02,
                                 9.618129107628477e-03};  // (ln 2)^k / k!
   double p[kTogether];
@@ -260,7 +317,7 @@ __device__ __forceinline__ void exp2_64(const Powers &table, double (&y)[kTogeth
     for (int i = 0; i < kTogether; i++) p[i] = fma(p[i], y[i], series[k]);
 #pragma unroll
   for (int i = 0; i < kTogether; i++) {
-    p[i] *= table.of[n[i] & 31];
+    p[i] *= __shfl_sync(0xffffffffu, entry, n[i]);  // (of the lane n % 32)
     y[i] = some[i] ? __hiloint2double(__double2hiint(p[i]) + (n[i] >> 5 << 20), __double2loint(p[i])) : 0.0;
   }
 }
@@ -271,9 +328,9 @@ struct Weight {
   __device__ __forceinline__ Weight() {}
   __device__ __forceinline__ Weight(float m, float t) : m(m), c(1.4426950408889634 / (double)t) {}
   __device__ __forceinline__ double power(float x) const { return ((double)x - m) * c; }
-  __device__ __forceinline__ double operator()(const Powers &table, float x) const {
+  __device__ __forceinline__ double operator()(double entry, float x) const {
     double y[kTogether] = {power(x)};
-    exp2_64(table, y);
+    exp2_64(entry, y);
     return y[0];
   }
 };
@@ -288,7 +345,7 @@ struct Drawn {
   int one;         // the token that the draft was sure of, or -1
   // Of the tokens at[] below `end`: p and q over their sums' scale, and whether they are
   // drawn from.
-  __device__ __forceinline__ void get(const Powers &table, const int (&at)[kTogether], int end, double (&px)[kTogether], double (&qx)[kTogether],
+  __device__ __forceinline__ void get(double entry, const int (&at)[kTogether], int end, double (&px)[kTogether], double (&qx)[kTogether],
                                       bool (&in)[kTogether]) const {
     float a[kTogether], b[kTogether];
 #pragma unroll
@@ -303,14 +360,14 @@ struct Drawn {
       qx[i] = 0.0;
       gap[i] = px[i];
     }
-    exp2_64(table, px);
+    exp2_64(entry, px);
     if (y) {
 #pragma unroll
       for (int i = 0; i < kTogether; i++) {
         qx[i] = wy.power(b[i]);
         gap[i] -= qx[i];
       }
-      exp2_64(table, qx);
+      exp2_64(entry, qx);
     }
 #pragma unroll
     for (int i = 0; i < kTogether; i++)
@@ -318,9 +375,12 @@ struct Drawn {
   }
 };
 
-struct PartSums {
-  double zx, zy, px, qx;  // sums of p and q over a warp's part of the vocabulary; of p and q where p > q
-};
+using PartSums = VerifySums;
+// (Written by other blocks: past the first-level cache.)
+__device__ __forceinline__ PartSums load_sums(const PartSums *p) {
+  const double *const d = (const double *)p;
+  return {__ldcg(d), __ldcg(d + 1), __ldcg(d + 2), __ldcg(d + 3)};
+}
 struct Choice {
   double ix, iy;  // 1 / sums
   double want;    // what the running sum has to exceed
@@ -329,29 +389,25 @@ struct Choice {
   bool from_p;
 };
 struct DrawShared {
-  PartSums part[kDrawWarps];
   Choice choice;
   int stop;
+  bool last;  // of the sequence's blocks
   RowStats target, draft;
 };
 
 template <class T>
-__global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_constant__ VerifyParams p) {
-  constexpr int most_parts = kCluster * kDrawWarps;  // of the vocabulary, one a warp
+__global__ void __launch_bounds__(kDrawThreads, 2) k_verify_draw(const __grid_constant__ VerifyParams p, const int blocks) {
+  constexpr int most_parts = kDrawBlocks * kDrawWarps;  // of the vocabulary, one a warp
   constexpr int kOfLane = most_parts / 32;           // parts that a lane looks at
   __shared__ DrawShared sh;
-  __shared__ PartSums all[most_parts];
   __shared__ double slice[kDrawWarps];
-  __shared__ Powers table;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = (int)cluster.num_blocks(), parts = blocks * kDrawWarps;
-  const int rank = (int)cluster.block_rank(), s = blockIdx.x / blocks;
+  const int parts = blocks * kDrawWarps, s = blockIdx.x / blocks, rank = blockIdx.x - s * blocks;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   const float t = temperature_of(p.temperature, s), td = temperature_of(p.draft_temperature, s);
   if (tid == 0) sh.stop = end - 1;
-  if (tid < 32) table.of[tid] = exp2((double)tid / 32.0);
+  const double entry = exp2((double)lane / 32.0);
   __syncthreads();
   pdl_wait();
   if (beg == end) {
@@ -359,7 +415,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       p.n_accepted[s] = 0;
       if (p.new_len) p.new_len[s] = p.kv_len[s];
     }
-    return;  // (the whole cluster)
+    return;
   }
   // Every block finds the row that emits: a warp for each draft.
   for (int r = beg + warp; r < end - 1; r += kDrawWarps) {
@@ -370,11 +426,11 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       const RowStats a = row_stats(p, r, t);
       const float lx = logit((const T *)p.logits + r * p.stride + x);
       double px = 0.0, qx = 1.0;
-      if (!a.none()) px = is_cold(t) ? (double)(a.at == x) : Weight(a.m, t)(table, lx) / a.sum;
+      if (!a.none()) px = is_cold(t) ? (double)(a.at == x) : Weight(a.m, t)(entry, lx) / a.sum;
       if (p.draft) {
         const RowStats b = row_stats(p, p.n_rows + r, td);
         const float ly = logit((const T *)p.draft + r * p.draft_stride + x);
-        if (!b.none()) qx = is_cold(td) ? (double)(b.at == x) : Weight(b.m, td)(table, ly) / b.sum;
+        if (!b.none()) qx = is_cold(td) ? (double)(b.at == x) : Weight(b.m, td)(entry, ly) / b.sum;
       }
       take = (double)__ldg(p.uniform + r) * qx < px;
     }
@@ -419,13 +475,13 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
     const int lo = (int)min((int64_t)p.vocab, (int64_t)(rank * kDrawWarps + warp) * per);
     const int hi = (int)min((int64_t)p.vocab, (int64_t)lo + per);
     PartSums mine = {0.0, 0.0, 0.0, 0.0};
-    for (int i0 = lo + lane; i0 < hi; i0 += 32 * kTogether) {
+    for (int i0 = lo; i0 < hi; i0 += 32 * kTogether) {
       double px[kTogether], qx[kTogether];
       bool in[kTogether];
       int at[kTogether];
 #pragma unroll
-      for (int i = 0; i < kTogether; i++) at[i] = i0 + 32 * i;
-      d.get(table, at, hi, px, qx, in);
+      for (int i = 0; i < kTogether; i++) at[i] = i0 + 32 * i + lane;
+      d.get(entry, at, hi, px, qx, in);
 #pragma unroll
       for (int i = 0; i < kTogether; i++) {
         mine.zx += px[i];
@@ -442,21 +498,27 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       mine.zy = warp_sum64(mine.zy);
       mine.qx = warp_sum64(mine.qx);
     }
-    if (lane == 0) sh.part[warp] = mine;
-    cluster.sync();
-    if (tid < parts) all[tid] = cluster.map_shared_rank(&sh, tid / kDrawWarps)->part[tid % kDrawWarps];
-    cluster.sync();  // no block leaves while others read its sums
+    // The sequence's last block to get here goes on with what all have found.
+    if (lane == 0) p.parts[(int64_t)s * parts + rank * kDrawWarps + warp] = mine;
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      sh.last = atomicAdd(p.arrived + s, 1) == blocks - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    const VerifySums *const all = p.parts + (int64_t)s * parts;
     // The first warp goes through the parts, kOfLane a lane: the part in which the
     // running sum first exceeds `want`, or the last one with any weight where
-    // rounding (or a number that is not below 1) leaves none.  (Every block does so, with
-    // the same numbers.)
+    // rounding (or a number that is not below 1) leaves none.
     if (warp == 0) {
       PartSums of[kOfLane];
       double zx = 0.0, zy = 0.0;
 #pragma unroll
       for (int k = 0; k < kOfLane; k++) {
         of[k] = PartSums{0.0, 0.0, 0.0, 0.0};
-        if (kOfLane * lane + k < parts) of[k] = all[kOfLane * lane + k];
+        if (kOfLane * lane + k < parts) of[k] = load_sums(all + kOfLane * lane + k);
         zx += of[k].zx;
         zy += of[k].zy;
       }
@@ -500,8 +562,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
     double before = sh.choice.before;
     const int chosen = sh.choice.part;
     const bool from_p = sh.choice.from_p;
-    if (rank != chosen / kDrawWarps) return;
-    // The block that has the part goes through it, kTogether tokens a lane at a time.
+    // The block goes through the part, kTogether tokens a lane at a time.
     const int c_lo = (int)min((int64_t)p.vocab, (int64_t)chosen * per), c_hi = (int)min((int64_t)p.vocab, (int64_t)c_lo + per);
     int some = -1;  // the last token with any weight
     for (int base = c_lo; base < c_hi && token < 0; base += kDrawThreads * kTogether) {
@@ -511,7 +572,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
       const int first = base + tid * kTogether;
 #pragma unroll
       for (int e = 0; e < kTogether; e++) at[e] = first + e;
-      d.get(table, at, c_hi, px, qx, in);
+      d.get(entry, at, c_hi, px, qx, in);
 #pragma unroll
       for (int e = 0; e < kTogether; e++) sum += w[e] = from_p ? px[e] * ix : in[e] ? fmax(px[e] * ix - qx[e] * iy, 0.0) : 0.0;
       // Sums up to this lane, of the warps, and up to this warp.
@@ -563,28 +624,21 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_draw(const __grid_const
   }
 }
 
+// Blocks of a sequence: parts of 128 tokens a warp at least.
+int draw_blocks(int vocab) {
+  int n = 1;
+  while (n < kDrawBlocks && vocab > n * kDrawWarps * 128) n *= 2;
+  return n;
+}
+
 template <class T>
 void run(const VerifyParams &p, cudaStream_t s) {
   if (p.n_rows) {
     const int64_t blocks = (int64_t)p.n_rows * p.chunks * (p.draft ? 2 : 1);
     launch_beside(k_verify_stats<T>, blocks, kStatThreads, 0, s, p);
   }
-  cudaLaunchConfig_t cfg = {};
-  // Blocks of a sequence: parts of 128 tokens a warp at least.
-  unsigned cluster = 1;
-  while (cluster < kCluster && p.vocab > (int)(cluster * kDrawWarps * 128)) cluster *= 2;
-  cfg.gridDim = dim3((unsigned)p.n_seqs * cluster);
-  cfg.blockDim = dim3(kDrawThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.n_rows ? 2 : 1;
-  JAL_CUDA(cudaLaunchKernelEx(&cfg, k_verify_draw<T>, p));
+  const int blocks = draw_blocks(p.vocab);
+  launch_beside(k_verify_draw<T>, (int64_t)p.n_seqs * blocks, kDrawThreads, 0, s, p, blocks);
 }
 
 }  // namespace
@@ -593,6 +647,18 @@ int verify_chunks(size_t n_rows, size_t vocab) {
   // Pieces of 4096 logits at least, blocks enough for every SM several times over.
   const size_t most = std::max<size_t>(1, vocab / 4096), want = (size_t)kPagedSMs * 6 / n_rows + 1;
   return (int)std::min<size_t>(64, std::min(most, want));
+}
+
+size_t verify_workspace(size_t n_seqs, size_t n_rows, size_t vocab, VerifyParams *p, void *ws) {
+  // Sums of the parts (whole 32 bytes first), the pieces of the rows, the counters.
+  const size_t parts = n_seqs * (size_t)draw_blocks((int)vocab) * kDrawWarps * sizeof(VerifySums);
+  const size_t pieces = 2 * n_rows * (n_rows ? (size_t)verify_chunks(n_rows, vocab) : 1) * sizeof(float2);
+  if (p) {
+    p->parts = (VerifySums *)ws;
+    p->part = (float2 *)((char *)ws + parts);
+    p->arrived = (int32_t *)((char *)ws + parts + pieces);
+  }
+  return n_rows ? parts + pieces + n_seqs * sizeof(int32_t) : 0;
 }
 
 void launch_verify_drafts(const VerifyParams &p, cudaStream_t s) {
