@@ -26,7 +26,7 @@ namespace {
 
 using namespace paged;
 
-constexpr int kStatThreads = 256, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawBlocks = 8;  // kDrawBlocks: of a sequence, at most
+constexpr int kStatThreads = 256, kDrawThreads = 256, kDrawWarps = kDrawThreads / 32, kDrawBlocks = 32;  // kDrawBlocks: of a sequence, at most
 constexpr float kCold = 1e-5f;  // temperatures up to this: all of the probability on the first largest logit
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -322,12 +322,19 @@ __device__ __forceinline__ void exp2_64(double entry, double (&y)[kTogether]) {
   }
 }
 
+// An f32 number in 64 bits by its bits (integer operations, where the conversion would
+// take the pipe of the 64-bit ones); zeros and subnormals become numbers of at most
+// 2^-126, infinities 2^128, and a NaN is taken for -inf.
+__device__ __forceinline__ double wide(float x) {
+  const uint32_t u = __float_as_uint(fmaxf(x, -INFINITY));
+  return __hiloint2double((int)((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(u << 29));
+}
 // exp((x - m) / T) in 64 bits, as a power of two.
 struct Weight {
   double m, c;
   __device__ __forceinline__ Weight() {}
   __device__ __forceinline__ Weight(float m, float t) : m(m), c(1.4426950408889634 / (double)t) {}
-  __device__ __forceinline__ double power(float x) const { return ((double)x - m) * c; }
+  __device__ __forceinline__ double power(float x) const { return (wide(x) - m) * c; }
   __device__ __forceinline__ double operator()(double entry, float x) const {
     double y[kTogether] = {power(x)};
     exp2_64(entry, y);
@@ -396,7 +403,7 @@ struct DrawShared {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kDrawThreads, 2) k_verify_draw(const __grid_constant__ VerifyParams p, const int blocks) {
+__global__ void __launch_bounds__(kDrawThreads, 4) k_verify_draw(const __grid_constant__ VerifyParams p, const int blocks) {
   constexpr int most_parts = kDrawBlocks * kDrawWarps;  // of the vocabulary, one a warp
   constexpr int kOfLane = most_parts / 32;           // parts that a lane looks at
   __shared__ DrawShared sh;
@@ -624,11 +631,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_verify_draw(const __grid_co
   }
 }
 
-// Blocks of a sequence: parts of 128 tokens a warp at least.
-int draw_blocks(int vocab) {
-  int n = 1;
-  while (n < kDrawBlocks && vocab > n * kDrawWarps * 128) n *= 2;
-  return n;
+// Blocks of a sequence: parts of 128 tokens a warp at least, and all blocks on the SMs
+// at once, four on each, where that leaves one for a sequence.
+int draw_blocks(size_t n_seqs, size_t vocab) {
+  const size_t fit = 4 * kPagedSMs / std::max<size_t>(1, n_seqs), work = (vocab + kDrawWarps * 128 - 1) / (kDrawWarps * 128);
+  return (int)std::max<size_t>(1, std::min<size_t>(kDrawBlocks, std::min(fit, work)));
 }
 
 template <class T>
@@ -637,7 +644,7 @@ void run(const VerifyParams &p, cudaStream_t s) {
     const int64_t blocks = (int64_t)p.n_rows * p.chunks * (p.draft ? 2 : 1);
     launch_beside(k_verify_stats<T>, blocks, kStatThreads, 0, s, p);
   }
-  const int blocks = draw_blocks(p.vocab);
+  const int blocks = draw_blocks(p.n_seqs, p.vocab);
   launch_beside(k_verify_draw<T>, (int64_t)p.n_seqs * blocks, kDrawThreads, 0, s, p, blocks);
 }
 
@@ -651,7 +658,7 @@ int verify_chunks(size_t n_rows, size_t vocab) {
 
 size_t verify_workspace(size_t n_seqs, size_t n_rows, size_t vocab, VerifyParams *p, void *ws) {
   // Sums of the parts (whole 32 bytes first), the pieces of the rows, the counters.
-  const size_t parts = n_seqs * (size_t)draw_blocks((int)vocab) * kDrawWarps * sizeof(VerifySums);
+  const size_t parts = n_seqs * (size_t)draw_blocks(n_seqs, vocab) * kDrawWarps * sizeof(VerifySums);
   const size_t pieces = 2 * n_rows * (n_rows ? (size_t)verify_chunks(n_rows, vocab) : 1) * sizeof(float2);
   if (p) {
     p->parts = (VerifySums *)ws;
