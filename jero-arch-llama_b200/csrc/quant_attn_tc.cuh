@@ -73,6 +73,11 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(a), "r"(b), "r"(c));
   return v;
 }
+__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
 // Sixteen codes, in order, as f16: a code is placed in the low mantissa bits of 1024 (its
 // sum with 1024, exactly), from which 1024 and the code's offset are subtracted.
 template <int BITS>
@@ -165,53 +170,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < 16 + kTcLoaders) {
       // ---- the loader
-      // Codes come by cp.async, a group of eight rows at a time, and are widened from
-      // there into the ring while the ones behind them are on their way: V's of a tile while
-      // K's are widened, then K's of the next tile.
+      // Codes come by cp.async, two groups of eight rows at a time, and are widened from there into the ring while the ones behind them are on their way:
+      // V's of a tile while K's are widened, then K's of the next tile.  Rows without a
+      // key are left as they are: whatever the bytes are, they are codes, and weigh
+      // nothing.
       // HD / 16 lanes widen a row, sixteen codes a lane: dims 16 c16 .., two pieces of 16
-      // bytes in the swizzle.  (The upper four of eight lanes store their second piece
-      // first, so that eight lanes store eight different ones.)
-      constexpr int kLanes = HD / 16, kRows = 32 / kLanes;        // lanes of a row; rows of a warp at once
-      constexpr int kPieces = S::row_bytes / 16, kCopy = 32 / kPieces;  // of a row; rows of a warp's copy
+      // bytes in the swizzle.  (The upper four of eight lanes have their pieces the other
+      // way round, so that eight lanes store eight different ones.)
+      constexpr int kLanes = HD / 16, kRows = 32 / kLanes;  // lanes of a row; rows of a warp at once
+      constexpr int kUnits = kGroups / 2;
+      static_assert(kGroups % 2 == 0 && kUnits <= 4, "units of two groups");
       const int c16 = lane % kLanes, r0 = lane / kLanes, flip = c16 / 4;
-      const int cp = lane % kPieces, cr = lane / kPieces;
-      const bool inside = cp * (128 / BITS) < hd;
       char *const raw = smem_tc + S::raw + w * (kGroups * 8 * S::row_bytes);
       const uint32_t raw_s = smem_u32(raw);
       bool ok = true;
       int b = 0, parity = 1;  // of the buffer's "empty" phase before this use: the first use finds it free
-      // (Rows without a key are copied as zeros; 4-bit codes of 0 there stand for -8, with a
-      // scale of 0.)
-      auto ask = [&](const void *pool, const int64_t (&from)[2], int k) {
-        if (group(k) < 16) {
+      constexpr int kPieces = S::row_bytes / 16, kCopy = 32 / kPieces;  // of a row; rows of a warp's copy
+      const int cp = lane % kPieces, cr = lane / kPieces;
+      const bool inside = cp * 16 < hd * BITS / 8;
+      // Lanes 0 .. 15 (unit 1: 16 .. 31) have the places of a unit's rows.
+      auto ask = [&](const void *pool, const int64_t (&from)[2], int unit, bool any) {
 #pragma unroll
-          for (int i = 0; i < (8 + kCopy - 1) / kCopy; i++) {
-            const int r = i * kCopy + cr;
-            const int64_t o = __shfl_sync(0xffffffffu, k < 4 ? from[0] : from[1], (k % 4) * 8 + r % 8);
-            const bool there = o >= 0 && inside;
-            if (r < 8) copy16(raw_s + (k * 8 + r) * S::row_bytes + cp * 16, (const char *)pool + (there ? o + cp * 16 : 0), there);
-          }
+        for (int i = 0; i < 16 / kCopy; i++) {
+          const int r = i * kCopy + cr;
+          const int64_t o = __shfl_sync(0xffffffffu, unit < 2 ? from[0] : from[1], unit % 2 * 16 + r);
+          if (any && o >= 0 && inside) copy16(raw_s + (unit * 16 + r) * S::row_bytes + cp * 16, (const char *)pool + o + cp * 16, true);
         }
         copies_done();
       };
-      auto widen = [&](int k) {
-        copies_wait<kGroups - 1>();
+      auto widen = [&](int unit) {
+        copies_wait<kUnits - 1>();
         __syncwarp();
-        if (group(k) >= 16) return;
-        char *const dst = base_p + S::ring + b * S::tile + c16 / 4 * (kTcKeys * 128) + group(k) * 1024;
+        char *const dst = base_p + S::ring + b * S::tile + c16 / 4 * (kTcKeys * 128);
+        constexpr int kSteps = 16 / kRows;
+        const int c = c16 % 4 * 2;
+        uint32_t x[kSteps][BITS / 2];
 #pragma unroll
-        for (int i = 0; i < 8 / kRows; i++) {
-          const int r = i * kRows + r0;
-          uint32_t x[4], h[8];
-          lds<2 * BITS>(raw_s + (k * 8 + r) * S::row_bytes + c16 * (2 * BITS), x);
-          widen16<BITS>(x, h);
-          char *const row = dst + r * 128;
-          const int c = c16 % 4 * 2;
-          const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-          *(uint4 *)(row + (((c + flip) ^ r) * 16)) = flip ? hi : lo;
-          *(uint4 *)(row + (((c + 1 - flip) ^ r) * 16)) = flip ? lo : hi;
+        for (int i = 0; i < kSteps; i++) {
+          const uint32_t at = raw_s + (unit * 16 + i * kRows + r0) * S::row_bytes + c16 * (2 * BITS);
+          if constexpr (BITS == 8) {
+            lds<8>(at + flip * 8, x[i]);
+            lds<8>(at + 8 - flip * 8, x[i] + 2);
+          } else {
+            x[i][0] = lds4(at + flip * 4);
+            x[i][1] = lds4(at + 4 - flip * 4);
+          }
         }
-        __syncwarp();  // every lane has read the group before it is filled again
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+          const int gr = group(unit * 2 + i * kRows / 8), r = (i * kRows + r0) % 8;
+          if (gr >= 16) break;
+          uint32_t h[8];
+          widen16<BITS>(x[i], h);
+          char *const row = dst + gr * 1024 + r * 128;
+          *(uint4 *)(row + (((c + flip) ^ r) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *(uint4 *)(row + (((c + 1 - flip) ^ r) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        __syncwarp();  // every lane has read the unit before it is filled again
       };
       auto begin = [&]() { return ok = __all_sync(0xffffffffu, ok && wait(&sy.kv_empty[b], parity)); };
       auto end = [&]() {
@@ -248,7 +263,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
         next0 = locate(1, 0);
         next1 = locate(1, 4);
 #pragma unroll
-        for (int k = 0; k < kGroups; k++) ask(p.kv.k, ahead, k);
+        for (int k = 0; k < kUnits; k++) ask(p.kv.k, ahead, k, true);
       }
 #pragma unroll 1
       for (int j = 0; j < n_tiles; j++) {
@@ -268,20 +283,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(&sy.present_full[j & 7]);
         if (!begin()) break;
-#pragma unroll 1
-        for (int k = 0; k < kGroups; k++) {
+#pragma unroll
+        for (int k = 0; k < kUnits; k++) {
           widen(k);
-          ask(p.kv.v, at, k);
+          ask(p.kv.v, at, k, true);
         }
         end();
         look(ahead);  // (of the last tile: no row)
         next0 = locate(j + 2, 0);
         next1 = locate(j + 2, 4);
         if (!begin()) break;
-#pragma unroll 1
-        for (int k = 0; k < kGroups; k++) {
+#pragma unroll
+        for (int k = 0; k < kUnits; k++) {
           widen(k);
-          ask(p.kv.k, ahead, k);
+          ask(p.kv.k, ahead, k, j + 1 < n_tiles);
         }
         end();
       }
