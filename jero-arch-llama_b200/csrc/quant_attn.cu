@@ -75,7 +75,7 @@ QuantAttnPlan plan_quant_attention(const jal_quant_kv &kv, const jal_ragged_batc
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kPagedMaxSplits, keys / (2 * kTcKeys)));
     a.splits = (int)std::min(most, std::max<int64_t>(1, kPagedSMs / std::max<int64_t>(1, blocks)));
   } else {
-    a.splits = attention_pieces(blocks, keys, quant_blocks((int)kv.head_dim, a.rows / 8, ns), kBlockKeys, false);
+    a.splits = attention_pieces(blocks, keys, quant_blocks(kv.bits, (int)kv.head_dim, a.rows / 8, ns), kBlockKeys, false);
   }
   a.direct = a.splits == 1;
   if (!a.direct)

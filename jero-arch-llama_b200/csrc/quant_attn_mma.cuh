@@ -98,18 +98,22 @@ __device__ __forceinline__ void digits(const uint32_t (&x)[4], uint32_t (&word)[
   }
 }
 
-// Blocks on an SM, by registers and shared memory.
-constexpr int quant_blocks(int hd, int r8, int ns) { return hd > 128 ? 1 : r8 * ns > 2 ? 2 : 3; }
+// Blocks on an SM, by registers and shared memory.  (Eight 16-bit rows over 4-bit codes:
+// four blocks with three stages 73 us where three with four take 75; over 8-bit codes
+// 131071 keys 56 and 52.)
+constexpr int quant_blocks(int bits, int hd, int r8, int ns) {
+  return hd > 128 ? 1 : r8 * ns > 2 ? 2 : bits == 4 && hd > 64 && r8 * ns == 1 ? 4 : 3;
+}
 
 template <int BITS, int NS, int HD, int R8>
 struct QuantShape {
-  static constexpr int blocks = quant_blocks(HD, R8, NS);
+  static constexpr int blocks = quant_blocks(BITS, HD, R8, NS);
   static constexpr int rows = 8 * R8;
   static constexpr int row_bytes = HD * BITS / 8;
   static constexpr int chunks = row_bytes / 16;            // 16-byte pieces of a row
   static constexpr int half = kQuantKeys * row_bytes;      // bytes of a stage's K (or V)
   static constexpr int stage = 2 * half + 2 * kQuantKeys * 4;
-  static constexpr int stages = row_bytes <= 32 ? 6 : row_bytes == 64 ? 4 : 2;
+  static constexpr int stages = row_bytes <= 32 ? 6 : row_bytes == 64 ? (blocks == 4 ? 3 : 4) : 2;
   static constexpr int ring = kMmaWarps * stages * stage;
   static constexpr int ksteps = HD / 32;
   static constexpr int q_bytes = NS * R8 * ksteps * 512;   // fragments
@@ -164,14 +168,26 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
     const int64_t e = at >= 0 ? (int64_t)where.page * qp.sc.s_page + t.head * qp.sc.s_head + where.slot : 0;
     copy4(dst + 2 * S::half + lane * 4, qp.sc.k + e, at >= 0);
     copy4(dst + 2 * S::half + kQuantKeys * 4 + lane * 4, qp.sc.v + e, at >= 0);
+    // (Rows that lie one behind the other, as within a page, need not be passed round.)
+    const int64_t first = __shfl_sync(0xffffffffu, at, 0);
+    if (__all_sync(0xffffffffu, at >= 0 && at == first + lane * S::row_bytes) && hd == HD) {
+      const char *const ks = (const char *)p.kv.k + first + lane * 16, *const vs = (const char *)p.kv.v + first + lane * 16;
 #pragma unroll
-    for (int i = 0; i < S::chunks; i++) {
-      const int r = (i * 32 + lane) / S::chunks, c = (i * 32 + lane) % S::chunks;
-      const int64_t o = __shfl_sync(0xffffffffu, at, r);
-      const bool there = o >= 0 && c * (128 / BITS) < hd;
-      const int64_t x = there ? o + c * 16 : 0;
-      copy16(dst + S::k_at(r, c), (const char *)p.kv.k + x, there);
-      copy16(dst + S::half + S::v_at(S::v_row(r), c), (const char *)p.kv.v + x, there);
+      for (int i = 0; i < S::chunks; i++) {
+        const int r = (i * 32 + lane) / S::chunks, c = lane % S::chunks;
+        copy16(dst + S::k_at(r, c), ks + i * 512, true);
+        copy16(dst + S::half + S::v_at(S::v_row(r), c), vs + i * 512, true);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::chunks; i++) {
+        const int r = (i * 32 + lane) / S::chunks, c = lane % S::chunks;
+        const int64_t o = __shfl_sync(0xffffffffu, at, r);
+        const bool there = o >= 0 && c * (128 / BITS) < hd;
+        const int64_t x = there ? o + c * 16 : 0;
+        copy16(dst + S::k_at(r, c), (const char *)p.kv.k + x, there);
+        copy16(dst + S::half + S::v_at(S::v_row(r), c), (const char *)p.kv.v + x, there);
+      }
     }
     copies_done();
   };
@@ -343,17 +359,20 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
 #pragma unroll
     for (int m = 0; m < R8; m++) all = all && span[m].all(u, kQuantKeys);
     const bool masked = __any_sync(0xffffffffu, !all);
+    uint32_t dk[4][2], dv[4][2];  // scales of this lane's keys
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      lds<8>(sb + n * 32 + j4 * 8, dk[n]);
+      lds<8>(sb + kQuantKeys * 4 + n * 32 + j4 * 8, dv[n]);
+    }
     uint32_t wa[R8][NS][4];
     float unit[R8];  // what the whole numbers of the weights count
 #pragma unroll
     for (int m = 0; m < R8; m++) {
       float y[8];
 #pragma unroll
-      for (int n = 0; n < 4; n++) {
-        uint32_t dk[2];
-        lds<8>(sb + n * 32 + j4 * 8, dk);
-        unpair(mul2(s[m][n], mul2(pair_bits(dk[0], dk[1]), pair(f[m], f[m]))), y[2 * n], y[2 * n + 1]);
-      }
+      for (int n = 0; n < 4; n++)
+        unpair(mul2(s[m][n], mul2(pair_bits(dk[n][0], dk[n][1]), pair(f[m], f[m]))), y[2 * n], y[2 * n + 1]);
       if (masked) {
         const uint32_t see = (bits & span[m].bits(u)) >> (2 * j4);
 #pragma unroll
@@ -374,15 +393,13 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
       uint32_t big = 0;
 #pragma unroll
       for (int n = 0; n < 4; n++) {
-        uint32_t dv[2];
-        lds<8>(sb + kQuantKeys * 4 + n * 32 + j4 * 8, dv);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           float &x = y[2 * n + e];
           const bool seen = !masked || x != -INFINITY;  // (what a row does not see has no effect on it)
           x = exp2_fast(x - ref);
           l[m] += x;
-          x = seen ? x * __uint_as_float(dv[e]) : 0.0f;
+          x = seen ? x * __uint_as_float(dv[n][e]) : 0.0f;
           big = max(big, __float_as_uint(x) & 0x7fffffffu);
         }
       }

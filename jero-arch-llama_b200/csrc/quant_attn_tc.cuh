@@ -230,7 +230,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
       };
       auto begin = [&]() { return ok = __all_sync(0xffffffffu, ok && wait(&sy.kv_empty[b], parity)); };
       auto end = [&]() {
-        fence_proxy_async();  // the tensor cores read what was stored
         mbar_arrive(&sy.kv_full[b]);
         if (++b == S::buffers) {
           b = 0;
@@ -342,6 +341,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
       // K tile j is copy 2 j, V tile j copy 2 j + 1; copies go round the buffers.
       auto there = [&](int g) {
         const bool ok = wait(&sy.kv_full[g % S::buffers], (g / S::buffers) & 1);
+        // (The fence stands here and not behind the stores: there it would wait for the
+        // loader's copies that are on their way.)
+        fence_proxy_async();
         tc_fence_after();
         return ok;
       };
