@@ -436,13 +436,13 @@ int jal_op_quant_kv_read(const jal_quant_kv *kv, const int32_t *first,
  * row.)  Every token is then distributed as p alone would have it.
  * Without draft_logits, and where a draft row has no distribution, q is 1 at x.  A
  * temperature not above 1e-5 (0, a NaN) puts all of p (or q) on the first of the
- * largest logits.  A NaN logit counts as -inf; a row that holds +inf or nothing
+ * largest logits, one above 1e30 counts as that.  A NaN logit counts as -inf; a row that holds +inf or nothing
  * above -inf has no distribution: its draft is refused, and a token drawn from it is
  * -1.  A draft outside the vocabulary is refused.  Where max(p - q, 0) is 0
  * throughout, the token is drawn from p.
  * Acceptance is decided from f32 sums of the exponentials, drawing from sums
  * and exponentials in 64 bits.
- * out_tokens (one for each row, not `tokens`): the accepted drafts from q_start[s]
+ * out_tokens (one for each row, apart from `tokens`): the accepted drafts from q_start[s]
  * on, the drawn token, then -1; rows of no sequence are left as they were.
  * n_accepted [n_seqs]: accepted drafts.  new_len (or NULL; may be batch's kv_len):
  * kv_len[s] without the refused drafts' positions.  A sequence without rows

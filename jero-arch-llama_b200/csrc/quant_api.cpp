@@ -321,7 +321,9 @@ int jal_op_verify_drafts(const jal_ragged_batch *batch, const void *logits, int 
     aligned4(out_tokens, "out_tokens");
     aligned4(n_accepted, "n_accepted");
     aligned4(new_len, "new_len");
-    if (out_tokens == tokens) fail(JAL_ERR_TENSOR_BOUNDS, "out_tokens cannot be tokens");
+    // (Blocks of a sequence read tokens while another writes.)
+    const uintptr_t in = (uintptr_t)tokens, to = (uintptr_t)out_tokens, bytes = b.n_rows * sizeof(int32_t);
+    if (to == in || (to < in + bytes && in < to + bytes)) fail(JAL_ERR_TENSOR_BOUNDS, "out_tokens overlaps tokens");
     if (b.n_seqs == 0) return;
     if (need) {
       NEED(ws);

@@ -604,3 +604,70 @@ def test_codes_of_the_reference_form_round_to_nearest():
     assert torch.equal(unpacked(packed(codes[:, :4], 8), 8), codes[:, :4])
     codes, _ = coded(x, 4)
     assert torch.equal(unpacked(packed(codes, 4), 4), codes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,news", [(8, [2, 1, 0, 5]), (4, [40, 1, 0, 33])])
+def test_a_captured_run_of_all(jal, torch_cuda, bits, news):
+    """Append, attention, reading back and verification captured together, in a padded batch: replays give what the calls
+    gave one by one, over other lengths too, and rows behind the last sequence stay as they were."""
+    hq, hkv, hd, vocab = 8, 2, 64, 500
+    c = QuantCase([700, 90, 0, 64], news, hq, hkv, hd, act="f16", bits=bits, page=16).to_device(jal)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n, m = c.n_rows, 4
+    k, v = (torch.randn(n, hkv * hd, generator=g, device=DEV).half() for _ in range(2))
+    inv = 10000.0 ** (-torch.arange(hd // 2, device=DEV) / (hd // 2)).float()
+    head = torch.randn(hq * hd, vocab, generator=g, device=DEV).half()
+    tokens = torch.randint(0, vocab, (n,), generator=g, device=DEV).int()
+    u = torch.rand(n, generator=g, device=DEV)
+    wide = jal.RaggedBatch(c.d_q_start, c.d_kv_len, n_seqs=m, n_rows=n, max_q_len=max(news) + 9, max_kv_len=c.width * 16)
+    need = jal.quant_kv_attention_workspace(c.kv, wide, hq, dtype=jal.F16)
+    need_v = jal.verify_drafts_workspace(wide, vocab)
+    ws, ws_v = (torch.empty(max(x, 16), dtype=torch.uint8, device=DEV) for x in (need, need_v))
+    pools = [torch.empty(c.n_pages, hkv, 16, hd, dtype=torch.float16, device=DEV) for _ in range(2)]
+    into = jal.PagedKv(*pools, c.d_table, dtype=jal.F16, n_pages=c.n_pages, page_size=16, n_heads_kv=hkv, head_dim=hd,
+                       n_seqs=m, max_pages=c.width)
+    q, out = torch.empty(n, hq * hd, dtype=torch.float16, device=DEV), torch.empty(n, hq * hd, dtype=torch.float16, device=DEV)
+    logits = torch.empty(n, vocab, dtype=torch.float16, device=DEV)
+    told, took, lens = (torch.empty(x, dtype=torch.int32, device=DEV) for x in (n, m, m))
+    written = [c.d_k, c.d_v, c.d_ks, c.d_vs, *pools, q, out, logits, told, took, lens]
+    at_first = [x.clone() for x in written[:4]]
+
+    def reset():
+        for x, y in zip(written, at_first):
+            x.copy_(y)
+        for x in written[4:]:
+            x.fill_(-9)
+
+    def run(stream):
+        jal.quant_kv_append(c.kv, wide, k, v, inv, dtype=jal.F16, rotary_dim=hd, q=c.d_q, q_out=q, n_heads_q=hq,
+                            q_stride=c.q_stride, stream=stream)
+        jal.quant_kv_attention(c.kv, wide, q, out, hq, 0.125, dtype=jal.F16, workspace=ws, workspace_len=need,
+                               stream=stream)
+        jal.quant_kv_read(c.kv, c.d_kv_len, into, m, 800, stream=stream)
+        jal.verify_drafts(wide, logits, tokens, u, told, took, vocab, dtype=jal.F16, new_len=lens, workspace=ws_v,
+                          workspace_len=need_v, stream=stream)
+
+    def filled():  # (the product between attention and verification is not part of the graph)
+        reset()
+        logits.copy_((c.d_q[:, :hq * hd] @ head) * 0.02)
+        torch.cuda.synchronize()
+
+    filled()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run(side)
+    for now in ([700, 90, 0, 64], [650, 60, 0, 40], [700, 90, 0, 64]):
+        c.d_kv_len.copy_(torch.tensor(now, dtype=torch.int32))
+        filled()
+        run(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        want = [x.clone() for x in written]
+        filled()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(written, want):
+            assert _same(a.cpu(), b.cpu())
+        rows = sum(news)
+        assert bool((told[rows:] == -9).all()) and bool((out[rows:] == -9).all()) and bool((q[rows:] == -9).all())
+        assert bool(out[:rows].isfinite().all()) and bool((told[:rows] >= -1).all())

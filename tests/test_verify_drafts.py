@@ -251,3 +251,59 @@ def test_in_place_lengths_streams_and_graphs(jal, torch_cuda):
         torch.cuda.synchronize()
         assert args["out_tokens"].tolist() == want[0] and args["n_accepted"].tolist() == want[1]
         assert d.d_len.tolist() == want[2]  # the batch's own lengths
+
+
+def test_overlapping_tokens_are_refused(jal):
+    b = _batch(jal)
+    need = jal.verify_drafts_workspace(b, 100)
+    for out in (8192 - 16, 8192 - 4, 8192 + 4, 8192 + 16):  # five tokens at 8192
+        with pytest.raises(jal.K3Error) as e:
+            jal.verify_drafts(b, logits=4096, tokens=8192, uniform=4096, out_tokens=out, n_accepted=4096, vocab=100,
+                              workspace=4096, workspace_len=need)
+        assert e.value.code == jal.ERR_TENSOR_BOUNDS and "overlaps" in str(e.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("drafted", [True, False])
+def test_logits_at_the_ends_of_the_type(jal, torch_cuda, act, drafted):
+    # Sums whose exponents leave no fraction in 32 bits, all logits as large as they can be, and large ones near each
+    # other (whole steps of the type apart, at a temperature of two steps).
+    news, vocab, most = [4, 4, 4, 4, 1], 3000, torch.finfo(NAMES[act]).max
+    base = {"f32": 2.0 ** 22, "f16": 32768.0, "bf16": 2.0 ** 22}[act]
+    step = base * torch.finfo(NAMES[act]).eps
+    for temps in ([1.0, 1.0, 1.0, 2 * step, 1.0], [1e-3, 50.0, 2e-5, 3 * step, 1e30]):
+        d = Drafts(news, vocab, act=act, drafted=drafted, seed=31)
+        d.logits[0:4] = most
+        d.logits[4:8] = -most
+        d.logits[8:12, ::3] = most
+        d.logits[8:12, 1::3] = -most
+        g = torch.Generator().manual_seed(32)
+        d.logits[12:16] = (base + step * torch.randint(0, 12, (4, vocab), generator=g)).to(NAMES[act])
+        d.logits[16, 100:200] = most
+        if drafted:
+            d.draft[0:16] = d.logits[0:16]
+            d.draft[5, 7], d.draft[13, :50] = most, base
+        for r in range(15):
+            d.tokens[r + 1] = int(torch.randint(0, vocab, (1,), generator=g))
+        d.t = torch.tensor(temps)
+        d.check(jal)
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(jal, torch_cuda):
+    both = [Drafts([6, 1, 3], 70001, seed=41), Drafts([2] * 40, 5000, act="bf16", drafted=False, seed=42)]
+    kept = [{}, {}]
+    for d, k in zip(both, kept):
+        d.run(jal, keep=k)
+    streams = [torch.cuda.Stream() for _ in both]
+    for k in kept:
+        k["args"]["out_tokens"].fill_(-9)
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s, k in zip(streams, kept):
+            jal.verify_drafts(k["batch"], **k["args"], stream=s)
+    torch.cuda.synchronize()
+    for d, k in zip(both, kept):
+        assert (k["args"]["out_tokens"].tolist(), k["args"]["n_accepted"].tolist()) == d.wanted()[:2]
