@@ -100,6 +100,16 @@ __device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+  pair_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ pair_t pair_bits(uint32_t a, uint32_t b) {
+  pair_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float v;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));

@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "paged_attn_tc.cuh"
 #include "paged_dev.cuh"
 #include "quant_kv.hpp"
 
@@ -324,19 +325,31 @@ struct RawCodes8 {
       w[0] = __ldg((const uint32_t *)(row + d / 2));
     }
   }
+  // A code in the mantissa of 2^23 (4 bits: where it lies in its half word, as 16^i codes),
+  // from which that and the code's offset are taken off; then times the scale.
   __device__ __forceinline__ void widen(float scale, float (&v)[8]) const {
+    const pair_t by = pair(scale, scale);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      // The code in the low mantissa bits of 2^23, which is taken off with its offset.
-      const uint32_t c = BITS == 8 ? __byte_perm(w[e / 4] ^ 0x80808080u, 0x4B000000u, 0x7440 + e % 4)
-                                   : ((w[0] >> (4 * e)) & 15u) | 0x4B000000u;
-      v[e] = __fmul_rn(__uint_as_float(c) - (BITS == 8 ? 8388736.0f : 8388616.0f), scale);
+    for (int e = 0; e < 8; e += 2) {
+      pair_t x;
+      if constexpr (BITS == 8) {
+        const uint32_t u = w[e / 4] ^ 0x80808080u;
+        x = pair_bits(__byte_perm(u, 0x4B000000u, 0x7440 + e % 4), __byte_perm(u, 0x4B000000u, 0x7441 + e % 4));
+        x = add2(x, pair(-8388736.0f, -8388736.0f));
+      } else {
+        const uint32_t u = e < 4 ? w[0] : w[0] >> 16, low = 15u << (4 * (e % 4)), high = low << 4;
+        const float a = e % 4 ? 1.0f / 256.0f : 1.0f, b = a / 16.0f;
+        x = pair_bits((u & low) | 0x4B000000u, (u & high) | 0x4B000000u);
+        x = fma2(x, pair(a, b), pair(-8388608.0f * a - 8.0f, -8388608.0f * b - 8.0f));
+      }
+      unpair(mul2(x, by), v[e], v[e + 1]);
     }
   }
 };
 
 template <int BITS, class TO>
-__global__ void __launch_bounds__(kReadThreads) k_quant_kv_read(const __grid_constant__ QuantReadParams p, const int tiles) {
+__global__ void __launch_bounds__(kReadThreads) k_quant_kv_read(const __grid_constant__ QuantReadParams p, const int tiles,
+                                                                   const uint32_t over_n8) {
   __shared__ int64_t from_at[kReadSlots], into_at[kReadSlots];
   __shared__ float k_scale[kReadSlots], v_scale[kReadSlots];
   pdl_wait();
@@ -361,6 +374,7 @@ __global__ void __launch_bounds__(kReadThreads) k_quant_kv_read(const __grid_con
     }
   }
   __syncthreads();
+  // (over_n8 = 2^32 / n8 and a little: quotients of numbers below 2^16 are exact.)
   const int n8 = p.from.hd / 8, total = n * n8;
   // (A lane's pieces of a round, asked for together.)
   constexpr int kRound = 4;
@@ -368,14 +382,14 @@ __global__ void __launch_bounds__(kReadThreads) k_quant_kv_read(const __grid_con
     RawCodes8<BITS> k[kRound], v[kRound];
 #pragma unroll
     for (int r = 0; r < kRound; r++) {
-      const int i = i0 + r * kReadThreads, t = i / n8, d = (i - t * n8) * 8;
+      const int i = i0 + r * kReadThreads, t = (int)__umulhi((uint32_t)i, over_n8), d = (i - t * n8) * 8;
       if (i >= total || into_at[t] < 0) continue;
       k[r].load((const uint8_t *)p.from.k + from_at[t], d);
       v[r].load((const uint8_t *)p.from.v + from_at[t], d);
     }
 #pragma unroll
     for (int r = 0; r < kRound; r++) {
-      const int i = i0 + r * kReadThreads, t = i / n8, d = (i - t * n8) * 8;
+      const int i = i0 + r * kReadThreads, t = (int)__umulhi((uint32_t)i, over_n8), d = (i - t * n8) * 8;
       if (i >= total || into_at[t] < 0) continue;
       float x[8];
       k[r].widen(k_scale[t], x);
@@ -390,9 +404,10 @@ template <int BITS>
 void run_read(const QuantReadParams &p, cudaStream_t s) {
   const int64_t tiles = (p.max_len + kReadSlots - 1) / kReadSlots, blocks = tiles * p.from.hkv * p.n_seqs;
   if (blocks > 2000000000) fail(JAL_ERR_CAPABILITY_MISMATCH, "too many positions for one launch");
-  if (p.into.dtype == JAL_F32) launch_beside(k_quant_kv_read<BITS, float>, blocks, kReadThreads, 0, s, p, (int)tiles);
-  else if (p.into.dtype == JAL_F16) launch_beside(k_quant_kv_read<BITS, __half>, blocks, kReadThreads, 0, s, p, (int)tiles);
-  else launch_beside(k_quant_kv_read<BITS, __nv_bfloat16>, blocks, kReadThreads, 0, s, p, (int)tiles);
+  const uint32_t over_n8 = 0xFFFFFFFFu / (uint32_t)(p.from.hd / 8) + 1;
+  if (p.into.dtype == JAL_F32) launch_beside(k_quant_kv_read<BITS, float>, blocks, kReadThreads, 0, s, p, (int)tiles, over_n8);
+  else if (p.into.dtype == JAL_F16) launch_beside(k_quant_kv_read<BITS, __half>, blocks, kReadThreads, 0, s, p, (int)tiles, over_n8);
+  else launch_beside(k_quant_kv_read<BITS, __nv_bfloat16>, blocks, kReadThreads, 0, s, p, (int)tiles, over_n8);
 }
 
 }  // namespace

@@ -6,8 +6,8 @@
 //
 // with codes c and scales d.  Codes enter the products as they are stored: a warp that
 // widened them to f16 first spent three quarters of its instructions on that (one
-// row a sequence of 28 heads over 64 caches of up to 8192 4-bit positions: 138 us;
-// so: 63 us).  q, and the weights times dv, are whole numbers over a power of two (q:
+// row a sequence of 28 heads, 4 KV heads of 128, over 64 caches of up to 8192 4-bit
+// positions: 138 us; so: 73 us).  q, and the weights times dv, are whole numbers over a power of two (q:
 // over the row's largest), in balanced digits of 8 bits, v = sum_i 256^i digit_i with
 // digit_i in [-128, 127]: two digits for 16-bit rows, four for f32.  The products
 // of the digits are exact, and are put together in f32.
@@ -26,6 +26,14 @@
 // group, and neighbouring tokens); its four warps take 32 keys each in turn, and
 // each is on its own until the end: it copies its keys' codes and scales with cp.async
 // into its own ring, and has its own running maxima, sums and output.
+//
+// What bounds it is instructions: with eight rows a warp issues two products and
+// a dozen others on scores and weights for each key and row pair that it has, so an
+// SM works where its loads could wait.  Read once, codes and scales would take 33 us of
+// the 73 above; 48 sequences of 4 to 6 rows of 32 heads (8 KV heads of 128, up to 12288
+// 8-bit positions) take 228 us, 99 for their bytes; one sequence of 131071 positions 52,
+// 42 for its bytes.  With all row tiles of a KV head in one block, codes are read
+// once for all heads of the group and all drafted tokens.
 #pragma once
 
 #include "paged_attn_mma.cuh"
@@ -57,16 +65,6 @@ __device__ __forceinline__ void ldsm_bytes(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
-}
-__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
-  pair_t v;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
-__device__ __forceinline__ pair_t pair_bits(uint32_t a, uint32_t b) {
-  pair_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
-  return v;
 }
 
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool there) {
