@@ -129,6 +129,12 @@ constexpr int kWarps = 4;
 // one lane whichever way they are paired.  Otherwise a lane has eight dims and reads
 // its partners' elements.  Every lane has read what it needs before any lane of
 // the head writes, so q_out may be q.
+// Queries come first, then keys and values, with a lane's turns in registers: as one
+// loop over all heads each head read them from shared memory again (78 us where it then was
+// 70, and is 67: 7 prompts of up to 2048 tokens of 32 and 8 heads of 128, bf16, 4 bits, with
+// the new positions read back; memory alone 43).  What is left is instructions: the 64-bit
+// rotation of K, the widening and packing of 16-bit rows.  Five blocks an SM: four, six and
+// seven were slower.
 template <int BITS, class TA, bool PAIRS>
 __global__ void __launch_bounds__(kWarps * 32, 5) k_quant_kv_append(const __grid_constant__ QuantAppendParams qp,
                                                                     const int parts, const int lanes) {
@@ -309,8 +315,11 @@ void run_append(const QuantAppendParams &p, cudaStream_t s) {
 // ---- reading back -----------------------------------------------------------
 // A block takes kReadSlots positions of one sequence and KV head: its first threads
 // look up where they lie and their scales, then a thread has eight dims of a position at
-// a time, K and V.  Bound by memory.
-constexpr int kReadThreads = 256, kReadSlots = 64;
+// a time, K and V.  Bound by memory, then by instructions on its way there: 16 sequences of
+// up to 4096 4-bit positions of 8 heads of 128 into bf16 take 48 us, 5.6 TB/s (widened one
+// by one 54; blocks of 256 threads 49.5, since a block's chain of lengths, table and scales
+// comes before its first code; 32 or 128 positions a block are the same).
+constexpr int kReadThreads = 128, kReadSlots = 64;
 
 // Eight codes as they are in memory.
 template <int BITS>
