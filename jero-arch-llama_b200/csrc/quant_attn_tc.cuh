@@ -47,6 +47,7 @@ struct QuantTcSync {
   // multiplied by ([256]).  Barriers lie between these uses.
   float x[2][2][128];
   uint8_t e[2][2][128];                // exponents of the largest scale of V that a row's halves see
+  bool bad[2][128];                    // rows of q with a NaN or an infinity
   float m1[128];                       // at the end: what the weights of the second row tile refer to
   alignas(16) uint8_t present[8][16];  // which keys of tile j exist, a bit each, by j % 8
   alignas(16) float dk[8][128], dv[8][128];  // their scales (K's times the softmax's), 0 where there is
@@ -426,18 +427,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
       for (int k = 0; k < CH / 2; k++) {
         const int kr = (k * 32 + lane) / CH, c = lane % CH;
         const int64_t o = __shfl_sync(0xffffffffu, qt, kr);
-        float v[8] = {}, top = 0.0f;
+        float v[8] = {};
         if (o >= 0 && c * 8 < hd) {
           if (NS == 2) load8((const float *)p.q + o + c * 8, v);
           else if (p.act == JAL_F16) load8((const __half *)p.q + o + c * 8, v);
           else load8((const __nv_bfloat16 *)p.q + o + c * 8, v);
         }
+        uint32_t most = 0;  // (a NaN's bits are above infinity's)
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (fabsf(v[e]) < INFINITY) top = fmaxf(top, fabsf(v[e]));
+        for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
 #pragma unroll
-        for (int x = CH / 2; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const int e = top > 0.0f ? 13 - ilogbf(top) : 0;
+        for (int x = CH / 2; x > 0; x >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+        const float top = __uint_as_float(most);
+        // A row with a NaN or an infinity goes in as 0, and its result is made NaN at the end: an
+        // infinite element's scores may all be -inf, as if the row saw nothing.
+        const bool bad = !(top < INFINITY);
+        if (bad) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] = 0.0f;
+        }
+        const int e = top > 0.0f && !bad ? 13 - ilogbf(top) : 0;
         // in two steps: 2^e itself may lie outside f32's range
         const float a = exp2f((float)(e / 2)), b = exp2f((float)(e - e / 2));
         uint32_t part2[4][NS];
@@ -447,7 +456,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
         for (int s = 0; s < NS; s++)
           *(uint4 *)(dst + s * S::q_tile + (c / 8) * (128 * 128) + (first + kr) * 128 + (((c % 8) ^ (kr & 7)) * 16)) =
               make_uint4(part2[0][s], part2[1][s], part2[2][s], part2[3][s]);
-        if (c == 0) (&sy.x[0][0][0])[i * 128 + first + kr] = (1.0f / a) / b;
+        if (c == 0) {
+          (&sy.x[0][0][0])[i * 128 + first + kr] = (1.0f / a) / b;
+          sy.bad[i][first + kr] = bad;
+        }
       }
       fence_proxy_async();
       mbar_arrive(&sy.q_full);
@@ -586,6 +598,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
     if (!has0) ok = wait(&sy.q_full, 0) && ok;
     __syncwarp();
     tc_fence_after();
+    if (sy.bad[i][r] && l != 0.0f) l = NAN;  // (its scores are 0, so that l counts the keys that it sees)
     sy.x[i][half][r] = l;
     if (i == 1 && half == 0) sy.m1[r] = m;
     if (twice) asm volatile("bar.sync 3, 512;" ::: "memory");
