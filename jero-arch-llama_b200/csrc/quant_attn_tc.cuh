@@ -440,13 +440,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
         for (int x = CH / 2; x > 0; x >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
         const float top = __uint_as_float(most);
         // A row with a NaN or an infinity goes in as 0, and its result is made NaN at the end: an
-        // infinite element's scores may all be -inf, as if the row saw nothing.
-        const bool bad = !(top < INFINITY);
-        if (bad) {
+        // infinite element's scores may all be -inf, as if the row saw nothing.  One that is next to
+        // nothing goes in as 0 too: the inverse of its power of two may lie below f32's range, and
+        // the -inf of a masked key times 0 is NaN.
+        const bool bad = !(top < INFINITY), some = !bad && top >= kQuantLeast;
+        if (!some) {
 #pragma unroll
           for (int e = 0; e < 8; e++) v[e] = 0.0f;
         }
-        const int e = top > 0.0f && !bad ? 13 - ilogbf(top) : 0;
+        const int e = some ? 13 - ilogbf(top) : 0;
         // in two steps: 2^e itself may lie outside f32's range
         const float a = exp2f((float)(e / 2)), b = exp2f((float)(e - e / 2));
         uint32_t part2[4][NS];

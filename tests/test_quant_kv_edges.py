@@ -4,7 +4,7 @@ import math
 import pytest
 
 from quant_ref import QuantCase
-from test_quant_kv import _attend
+from test_quant_kv import _attend, _near
 
 # Rows of one sequence; with two heads a KV head they go to tiles of 8 and 24 rows, to one tile of 128, to two of
 # 128, and to several blocks.
@@ -38,3 +38,29 @@ def test_query_rows_with_a_nan_or_an_infinity(jal, torch_cuda, act, bits, value,
     assert bool(got[bad].isnan().all())
     assert bool(((got - ref[0][:2 * n]).abs() <= bound[:2 * n])[good].all())
     assert bool((got[n:n + 2] == 0).all())
+
+
+def _small_rows(jal, bits, n):
+    # f32 rows whose largest element is 2^e, over scales of K of 2^91, so that rows down to 2^-100 have scores of their
+    # own; smaller ones count as 0.  From position 0 on: there are masked keys.
+    size = [0.0, 2.0 ** -149, 2.0 ** -140, 2.0 ** -137, 2.0 ** -126, 2.0 ** -101, 2.0 ** -100, 2.0 ** -99, 2.0 ** -98, 2.0 ** -97]
+    c = QuantCase([n], [n], 2, 1, 64, act="f32", bits=bits, page=16, seed=n)
+    for t in range(n):
+        c.set_scale(0, 0, t, 2.0 ** 91)
+    unit = (c.q / c.q.abs().amax(-1, keepdim=True)).clone()
+    for r in range(c.n_rows):
+        for h in range(2):
+            c.q[r, h] = unit[r, h] * size[(2 * r + h) % len(size)]
+    given = c.q_full.clone()
+    c.q[c.q.abs().amax(-1) < 2.0 ** -100] = 0.0
+    ref = c.reference(1.0)
+    c.q_full.copy_(given)
+    c.to_device(jal)
+    _near(c, _attend(jal, c, 1.0), ref, c.bound(ref))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", [40, 80, 300])
+def test_query_rows_next_to_nothing_of_many(jal, torch_cuda, bits, n):
+    _small_rows(jal, bits, n)
