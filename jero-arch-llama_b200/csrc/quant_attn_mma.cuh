@@ -225,7 +225,8 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      constexpr float whole = NS == 1 ? 127.0f * 256.0f : 127.0f * 16777216.0f;
+      // (The lower two of four digits count as a fraction: whole / most stays in f32's range.)
+      constexpr float whole = 127.0f * 256.0f;
       const float most = __uint_as_float(top);
       const bool some = most >= kQuantLeast && most < INFINITY;
       const float over = some ? whole / most : 0.0f;
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
         const int at = sub + 16 * w, ks = at / 8, jj = at / 2 % 4, h = at % 2;
         uint32_t x[4], word[2 * NS];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = some ? (uint32_t)__float2int_rn(v[w][i] * over) : 0u;
+        for (int i = 0; i < 4; i++) x[i] = some ? (uint32_t)__float2int_rn(v[w][i] * over * (NS == 1 ? 1.0f : 65536.0f)) : 0u;
         if (NS == 1)
 #pragma unroll
           for (int i = 0; i < 4; i++) x[i] += 128u;
@@ -289,13 +290,13 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
   }
   uint32_t zero[4] = {kIntZero, kIntZero, kIntZero, kIntZero};
   const pair_t minus = pair(-kIntZeroF, -kIntZeroF), digit = pair(256.0f, 256.0f);
-  // What accumulators of the digits hold, in f32.
+  // What accumulators of the digits hold, in f32; of four digits, over 2^16.
   auto whole_pair = [&](const uint32_t (&c)[NS][4]) -> pair_t {
     const pair_t hi = add2(pair_bits(c[0][0], c[0][1]), minus), lo = add2(pair_bits(c[0][2], c[0][3]), minus);
     pair_t v = fma2(hi, digit, lo);
     if constexpr (NS == 2) {
       const pair_t hi1 = add2(pair_bits(c[1][0], c[1][1]), minus), lo1 = add2(pair_bits(c[1][2], c[1][3]), minus);
-      v = fma2(v, pair(65536.0f, 65536.0f), fma2(hi1, digit, lo1));
+      v = fma2(fma2(hi1, digit, lo1), pair(0x1p-16f, 0x1p-16f), v);
     }
     return v;
   };
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
       const int e = (int)(big >> 23);
       const bool some = e > kShift;  // smaller ones than 2^(kShift - 127) count as 0
       const float over = some ? __uint_as_float((uint32_t)min(254 + kShift - e, 254) << 23) : 0.0f;
-      unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - kShift) << 23) : 0.0f;
+      unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - kShift + (NS == 1 ? 0 : 16)) << 23) : 0.0f;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         uint32_t x[4], word[2 * NS];

@@ -64,3 +64,10 @@ def _small_rows(jal, bits, n):
 @pytest.mark.parametrize("n", [40, 80, 300])
 def test_query_rows_next_to_nothing_of_many(jal, torch_cuda, bits, n):
     _small_rows(jal, bits, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", [3, 12, 30])
+def test_query_rows_next_to_nothing_of_few(jal, torch_cuda, bits, n):
+    _small_rows(jal, bits, n)
