@@ -12,10 +12,12 @@
 //     be rounded to 11 bits twice, nothing but the weights is.
 //   - q is carried as f16 parts of the row times a power of two, whatever its type
 //     (one part for 16-bit rows; two, 22 bits, for f32).
-//   - The weights refer to the row's maximum plus E less kQuantHeadroom, with 2^E
-//     the power of two below the largest |dv| that the row has seen: weight times dv
-//     stays below 2^15, and each is off by 2^-35 of the row's largest weight times its
-//     largest dv beside its relative error.
+//   - The weights and their sum refer to the row's maximum alone; weight times dv, which
+//     goes to the product with V, over 2^(E - kQuantHeadroom) too, with 2^E the power
+//     of two below the largest |dv| that the row has seen.  It stays below 2^15, and each is
+//     off by 2^-35 of the row's largest weight times its largest dv beside its relative
+//     error.  (One reference for both would lose the sum's earlier part as soon as E grows by
+//     more than f32's range, and costs f32 rows bits of the weights' exponents.)
 //
 // 2048 rows of 32 heads (8 KV heads of 128) behind 6144 cached 8-bit positions take 449
 // us (the same over a bf16 cache 258).  What is dearer here: three loader warps widen
@@ -48,7 +50,7 @@ struct QuantTcSync {
   float x[2][2][128];
   uint8_t e[2][2][128];                // exponents of the largest scale of V that a row's halves see
   bool bad[2][128];                    // rows of q with a NaN or an infinity
-  float m1[128];                       // at the end: what the weights of the second row tile refer to
+  float m1[128], unit1[128];           // at the end, of the second row tile: what its weights refer to, what O counts
   alignas(16) uint8_t present[8][16];  // which keys of tile j exist, a bit each, by j % 8
   alignas(16) float dk[8][128], dv[8][128];  // their scales (K's times the softmax's), 0 where there is
                                              // no key; a V scale that is not finite is a NaN of K's
@@ -475,6 +477,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
     const RowSpan span = row_span(p, t, mk);
     float m = -INFINITY, l = 0.0f;  // m: what the weights refer to, base 2; l: this half's sum
     int high = kQuantLeastE;        // E: the power of two below V's largest scale that the row has seen
+    auto power = [](int e) -> float { return __uint_as_float((uint32_t)(127 + e) << 23); };
     bool ok = true;
     int turn = 0;  // of this row tile
 #pragma unroll 1
@@ -529,17 +532,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
       sy.x[i][half][r] = mine;
       sy.e[i][half][r] = (uint8_t)(largest >> 23);
       tile_sync();
+      const int was = high;
       high = max(high, max((int)(largest >> 23), (int)sy.e[i][half ^ 1][r]) - 127);
       const float top = max3_nan(mine, sy.x[i][half ^ 1][r], mine) * scale;
       // A NaN or an infinite score makes the row NaN, as the formula does.
       if (!(top < INFINITY)) l = NAN;
       // Raise the reference of the rows that need it (the first tile's all).
       // O is at rest: its products up to tile j - 1 were done before S.
-      const bool raise = top + (float)high - m > (float)(kQuantSlack + kQuantHeadroom);  // (m = -inf: any score)
+      const bool raise = top - m > (float)kQuantSlack || high > was;  // (m = -inf: any score)
       if (__any_sync(0xffffffffu, raise)) {
-        const float next = raise ? reference_of<kQuantHeadroom>(top + (float)high) : m, c = raise ? exp2_fast(m - next) : 1.0f;
+        const float next = raise ? fmaxf(m, top) : m, less = next == m ? 0.0f : m - next, c = exp2_fast(less + (float)(was - high));
         m = next;
-        l *= c;
+        l *= exp2_fast(less);
         if (turn > 0) {  // this half of O's columns
 #pragma unroll 1
           for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 32) {
@@ -556,7 +560,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
       // The weights, over this half's own scores: part q of 32 keys in 16 of the columns
       // that held their scores.
       pair_t sum[2] = {0, 0};
-      const pair_t scale2 = pair(scale, scale), ref2 = pair(-ref, -ref);
+      const float lift = power(kQuantHeadroom - high);
+      const pair_t scale2 = pair(scale, scale), ref2 = pair(-ref, -ref), lift2 = pair(lift, lift);
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         float s[32];
@@ -574,7 +579,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
             a = exp2_fast(a);
             b = exp2_fast(b);
             sum[h] = add2(sum[h], pair(a, b));
-            unpair(mul2(pair(a, b), h ? pair(d.z, d.w) : pair(d.x, d.y)), a, b);
+            unpair(mul2(pair(a, b), mul2(h ? pair(d.z, d.w) : pair(d.x, d.y), lift2)), a, b);
             uint32_t part2[NS];
             split2<__half, NS>(a, b, part2);
 #pragma unroll
@@ -602,7 +607,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
     tc_fence_after();
     if (sy.bad[i][r] && l != 0.0f) l = NAN;  // (its scores are 0, so that l counts the keys that it sees)
     sy.x[i][half][r] = l;
-    if (i == 1 && half == 0) sy.m1[r] = m;
+    float unit = power(high - kQuantHeadroom);  // what O counts
+    if (i == 1 && half == 0) {
+      sy.m1[r] = m;
+      sy.unit1[r] = unit;
+    }
     if (twice) asm volatile("bar.sync 3, 512;" ::: "memory");
     else tile_sync();
     if (!twice || i == 0) {
@@ -615,6 +624,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
         c1 = m1 == -INFINITY ? 0.0f : exp2_fast(m1 - top);
         l = l * c0 + l1 * c1;
         m = top;
+        c0 *= unit;
+        c1 *= sy.unit1[r];
+        unit = 1.0f;
       }
       if (*given_up) l = NAN;
       // 32 dims at a time through the warp's 4 KB of the query tiles' memory
@@ -645,7 +657,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_quant_attn_tc(const __grid_co
           }
         }
 #pragma unroll
-        for (int e = 0; e < 32; e++) o[e] *= inv;
+        for (int e = 0; e < 32; e++) o[e] = o[e] * inv * unit;
       };
       const int first = half * (HD / 2);
       __syncwarp();

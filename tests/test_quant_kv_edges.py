@@ -71,3 +71,19 @@ def test_query_rows_next_to_nothing_of_many(jal, torch_cuda, bits, n):
 @pytest.mark.parametrize("n", [3, 12, 30])
 def test_query_rows_next_to_nothing_of_few(jal, torch_cuda, bits, n):
     _small_rows(jal, bits, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("length,n", [(90, 2), (384, 40), (384, 100), (1500, 40), (1500, 1)])
+@pytest.mark.parametrize("first,scales", [(128, (0.0, 2.0 ** 40)), (256, (2.0 ** -96, 2.0 ** 40)), (64, (2.0 ** 40, 0.0)),
+                                          (700, (2.0 ** -90, 2.0 ** 90)), (128, (0.0, 2.0 ** 95))])
+def test_scales_of_v_far_apart_in_a_rows_sight(jal, torch_cuda, act, length, n, first, scales):
+    # Values of the first keys next to nothing beside the others', or the other way round, at scores near each other: the
+    # sum of the weights counts all of them.  One piece and several, one row tile and two.
+    c = QuantCase([length], [n], 2, 1, 64, act=act, bits=8, page=16)
+    for t in range(length):
+        c.set_scale(1, 0, t, scales[0] if t < first else scales[1])
+    ref = c.reference(1e-3)
+    c.to_device(jal)
+    _near(c, _attend(jal, c, 1e-3), ref, c.bound(ref))
