@@ -404,12 +404,12 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
       }
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // The weights over 2^(e - 13) (four digits: 2^(e - 29)), e the largest one's exponent.
-      constexpr int kShift = NS == 1 ? 13 : 29;
-      const int e = (int)(big >> 23);
-      const bool some = e > kShift;  // smaller ones than 2^(kShift - 127) count as 0
-      const float over = some ? __uint_as_float((uint32_t)min(254 + kShift - e, 254) << 23) : 0.0f;
-      unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - kShift + (NS == 1 ? 0 : 16)) << 23) : 0.0f;
+      // The weights over 2^(e - 13) (four digits: 2^(e - 29)), e the largest one's exponent;
+      // over 2^-126, where that is more.
+      const int e = (int)(big >> 23), shift = min(NS == 1 ? 13 : 29, e - 1);
+      const bool some = e > 0;  // (smaller than 2^-126, all: they count as 0)
+      const float over = some ? __uint_as_float((uint32_t)(254 + shift - e) << 23) : 0.0f;
+      unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - shift + (NS == 1 ? 0 : 16)) << 23) : 0.0f;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         uint32_t x[4], word[2 * NS];

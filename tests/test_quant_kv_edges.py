@@ -2,8 +2,9 @@
 import math
 
 import pytest
+import torch
 
-from quant_ref import QuantCase
+from quant_ref import QuantCase, coded, packed
 from test_quant_kv import _attend, _near
 
 # Rows of one sequence; with two heads a KV head they go to tiles of 8 and 24 rows, to one tile of 128, to two of
@@ -87,3 +88,50 @@ def test_scales_of_v_far_apart_in_a_rows_sight(jal, torch_cuda, act, length, n, 
     ref = c.reference(1e-3)
     c.to_device(jal)
     _near(c, _attend(jal, c, 1e-3), ref, c.bound(ref))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", NEWS)
+def test_small_scales_of_v(jal, torch_cuda, act, bits, n):
+    # The smallest scale that an append leaves is 2^-107 (4 bits: 2^-103).
+    c = QuantCase([n + 40], [n], 2, 1, 64, act=act, bits=bits, page=16)
+    for t in range(n + 40):
+        c.set_scale(1, 0, t, 2.0 ** -107 * (1 + t % 5))
+    ref = c.reference(0.25)
+    c.to_device(jal)
+    _near(c, _attend(jal, c, 0.25), ref, c.bound(ref))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("n,small", [(1, 2.0 ** -107), (1, 2.0 ** -90)])
+def test_one_key_far_above_a_tail_of_small_values(jal, torch_cuda, act, n, small):
+    # One key takes nearly all of the weight and its value is 0: the result is the others', 17 nats below, over small
+    # scales of V (2^-107: the smallest that an append leaves).
+    c = QuantCase([3000], [n], 1, 1, 64, act=act, bits=8, page=64)
+    for t in range(3000):
+        c.set_scale(0, 0, t, 0.0)
+        c.set_scale(1, 0, t, small)
+    q = torch.randn(1, 1, 64, generator=torch.Generator().manual_seed(4)).to(c.act)
+    c.q_full[:] = q.reshape(1, 64)
+    codes, _ = coded(q[0].float(), 8)
+    view = c.raw[0].permute([c.layout.index(x) for x in "phsd"])
+    view[int(c.table[0, 0]), 0, 7] = packed(codes[0], 8)
+    c.set_scale(0, 0, 7, float(17 / float((codes[0].double() * q[0, 0].double()).sum())))
+    c.set_scale(1, 0, 7, 0.0)
+    c.to_device(jal)
+    got = _rows(c, _attend(jal, c, 1.0), n)
+    seen = torch.arange(3000)[None] <= torch.arange(3000 - n, 3000)[:, None]
+    weight = torch.where(seen, math.exp(-17), 0.0).double()
+    weight[:, 7] = 1.0
+    tail = weight @ c.v[0][:, 0].double() / weight.sum(-1, keepdim=True)
+    # 2^-8 of the tail's size: weights to 2^-11, the score of 17 and f32's 3000 sums in the exponent and beside, bf16's
+    # result, and results below f32's normal numbers.  Few rows: each weight times its scale, beside, to 2^-126, where
+    # those end: the tail's are 2^-24.5 of the scale.
+    size = weight @ c.v[0][:, 0].abs().double() / weight.sum(-1, keepdim=True)
+    off = 2.0 ** -8 * size + 2.0 ** -126
+    if n == 1:
+        off = off + 2.0 ** -126 * size / (math.exp(-17) * small)
+    assert bool(((got[:, 0] - tail).abs() <= off).all())
