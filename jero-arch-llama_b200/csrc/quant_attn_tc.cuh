@@ -35,7 +35,7 @@
 namespace jal {
 namespace paged {
 
-constexpr int kQuantSlack = 4, kQuantHeadroom = 10, kQuantLeastE = -96;
+constexpr int kQuantSlack = 4, kQuantHeadroom = 10, kQuantLeastE = -107;  // (an append leaves no smaller scale)
 
 struct QuantTcSync {
   uint64_t q_full;

@@ -106,7 +106,7 @@ def test_small_scales_of_v(jal, torch_cuda, act, bits, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ["f32", "bf16"])
-@pytest.mark.parametrize("n,small", [(1, 2.0 ** -107), (1, 2.0 ** -90)])
+@pytest.mark.parametrize("n,small", [(1, 2.0 ** -107), (1, 2.0 ** -90), (80, 2.0 ** -107), (80, 2.0 ** -90)])
 def test_one_key_far_above_a_tail_of_small_values(jal, torch_cuda, act, n, small):
     # One key takes nearly all of the weight and its value is 0: the result is the others', 17 nats below, over small
     # scales of V (2^-107: the smallest that an append leaves).
