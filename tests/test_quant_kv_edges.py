@@ -135,3 +135,37 @@ def test_one_key_far_above_a_tail_of_small_values(jal, torch_cuda, act, n, small
     if n == 1:
         off = off + 2.0 ** -126 * size / (math.exp(-17) * small)
     assert bool(((got[:, 0] - tail).abs() <= off).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("softmax_scale", [0.25, -0.25])
+@pytest.mark.parametrize("n", [3, 30, 80])
+def test_an_infinite_scale_of_k(jal, torch_cuda, act, value, softmax_scale, n):
+    # A score of +inf makes the row NaN; one of -inf leaves the key out (or the row NaN).  Rows before the position are
+    # as they were.
+    length = 90
+    at = length - 2
+    c = QuantCase([length], [n], 4, 2, 64, act=act, bits=8, page=16)
+    clean = c.reference(softmax_scale)
+    clean_bound = c.bound(clean)
+    sign = torch.stack([torch.stack([(c.q[r, h].double() * c.k[0][at, h // 2].double()).sum() for h in range(4)])
+                        for r in range(n)]) * value * softmax_scale
+    c.set_scale(0, 0, at, 0.0)
+    c.mapped = lambda s, t: t != at
+    without = c.reference(softmax_scale)
+    bound = c.bound(without)
+    del c.mapped
+    c.set_scale(0, 0, at, value)
+    c.to_device(jal)
+    got = _rows(c, _attend(jal, c, softmax_scale), n)
+    free = n - 2  # rows before the position
+    assert bool(((got - clean[0][:n]).abs() <= clean_bound[:n])[:free].all())
+    for r in range(free, n):
+        for h in range(4):
+            if sign[r, h] > 0:
+                assert bool(got[r, h].isnan().all())
+            else:
+                near = (got[r, h] - without[0][r, h]).abs() <= bound[r, h]
+                assert bool((near | got[r, h].isnan()).all())
