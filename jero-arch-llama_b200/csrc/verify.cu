@@ -396,14 +396,50 @@ struct Choice {
   double want;    // what the running sum has to exceed
   double before;  // the running sum ahead of the part
   int part;
-  bool from_p;
+  bool from_p, close;
 };
+// What of p = px ix is above q = qx iy; 0 where that is within their rounding.  (No product
+// is left unrounded, so that it is 0 where the two are the same.)
+__device__ __forceinline__ double above(double px, double ix, double qx, double iy) {
+  const double p = __dmul_rn(px, ix), w = __dsub_rn(p, __dmul_rn(qx, iy));
+  return w > 0x1p-36 * p ? w : 0.0;
+}
+// Where less than this of p is above q, the two may be nearly the same at nearly all tokens, and
+// the border from sums in f32 (2^-20 of p at most is on its wrong side) does not do.
+constexpr double kClose = 0x1p-10;
 struct DrawShared {
   Choice choice;
   int stop;
   bool last;  // of the sequence's blocks
   RowStats target, draft;
 };
+
+// What of p is above q at the tokens [lo, hi), by one warp.
+template <class T>
+__device__ __noinline__ double sum_above(const T *x, const T *y, float m, float t, float my, float ty, int lo, int hi, double ix,
+                                         double iy) {
+  const int lane = threadIdx.x % 32;
+  const double entry = exp2((double)lane / 32.0);
+  Drawn<T> d;
+  d.x = x;
+  d.y = y;
+  d.wx = Weight(m, t);
+  d.wy = Weight(my, ty);
+  d.border = 0.0;
+  d.one = -1;
+  double sum = 0.0;
+  for (int i0 = lo; i0 < hi; i0 += 32 * kTogether) {
+    double px[kTogether], qx[kTogether];
+    bool in[kTogether];
+    int at[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; i++) at[i] = i0 + 32 * i + lane;
+    d.get(entry, at, hi, px, qx, in);
+#pragma unroll
+    for (int i = 0; i < kTogether; i++) sum += above(px[i], ix, qx[i], iy);
+  }
+  return warp_sum64(sum);
+}
 
 // Bound by instructions: a token of the drawn row costs some 40, a quarter of them
 // in 64 bits.  128256 tokens of p and of q for each of 32 sequences take 19 us,
@@ -414,7 +450,7 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_draw(const __grid_co
   constexpr int most_parts = kDrawBlocks * kDrawWarps;  // of the vocabulary, one a warp
   constexpr int kOfLane = most_parts / 32;           // parts that a lane looks at
   __shared__ DrawShared sh;
-  __shared__ double slice[kDrawWarps];
+  __shared__ double slice[kDrawWarps], weight[most_parts];
   const int parts = blocks * kDrawWarps, s = blockIdx.x / blocks, rank = blockIdx.x - s * blocks;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int beg, end;
@@ -478,7 +514,8 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_draw(const __grid_co
         d.y = (const T *)p.draft + stop * p.draft_stride;
         d.wy = Weight(sh.draft.m, td);
         // (From the sums in f32: a token that falls on the wrong side has p and q within
-        // 2^-20 of each other, and a weight of next to nothing.)
+        // 2^-20 of each other, and a weight of next to nothing.  Where that is all there is,
+        // the weights are summed again, below.)
         d.border = (double)log2f(a.sum) - (double)log2f(sh.draft.sum);
       } else {
         d.one = p.draft && !sh.draft.none() ? sh.draft.at : x;
@@ -523,109 +560,132 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_draw(const __grid_co
     __syncthreads();
     if (!sh.last) return;
     const VerifySums *const all = p.parts + (int64_t)s * parts;
-    // The first warp goes through the parts, kOfLane a lane: the part in which the
-    // running sum first exceeds `want`, or the last one with any weight where
-    // rounding (or a number that is not below 1) leaves none.
-    if (warp == 0) {
-      PartSums of[kOfLane];
-      double zx = 0.0, zy = 0.0;
-#pragma unroll
-      for (int k = 0; k < kOfLane; k++) {
-        of[k] = PartSums{0.0, 0.0, 0.0, 0.0};
-        if (kOfLane * lane + k < parts) of[k] = load_sums(all + kOfLane * lane + k);
-        zx += of[k].zx;
-        zy += of[k].zy;
-      }
-      const double ix = 1.0 / warp_sum64(zx), iy = d.y ? 1.0 / warp_sum64(zy) : 0.0;
-      double w[kOfLane], sum = 0.0;
-#pragma unroll
-      for (int k = 0; k < kOfLane; k++) sum += w[k] = fmax(of[k].px * ix - of[k].qx * iy, 0.0);
-      double total = warp_sum64(sum);
-      const bool from_p = !(total > 0.0);
-      if (from_p) {
-        sum = 0.0;
-#pragma unroll
-        for (int k = 0; k < kOfLane; k++) sum += w[k] = of[k].zx * ix;
-        total = warp_sum64(sum);
-      }
-      const double want = (double)__ldg(p.uniform + end - 1) * total;
-      double upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const double n = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += n;
-      }
-      double run = upto - sum, before = run;  // before: of this lane's first part past `want`, or its last one
-      int over = 0x7fffffff, last = -1;
-#pragma unroll
-      for (int k = 0; k < kOfLane; k++) {
-        if (w[k] > 0.0 && over == 0x7fffffff) {
-          last = kOfLane * lane + k;
-          before = run;
-          if (run + w[k] > want) over = last;
-        }
-        run += w[k];
-      }
-      int chosen = __reduce_min_sync(0xffffffffu, over);
-      if (chosen == 0x7fffffff) chosen = max(__reduce_max_sync(0xffffffffu, last), 0);
-      before = __shfl_sync(0xffffffffu, before, chosen / kOfLane);
-      if (lane == 0) sh.choice = Choice{ix, iy, want, before, chosen, from_p};
-    }
-    __syncthreads();
-    const double ix = sh.choice.ix, iy = sh.choice.iy, want = sh.choice.want;
-    double before = sh.choice.before;
-    const int chosen = sh.choice.part;
-    const bool from_p = sh.choice.from_p;
-    // The block goes through the part, kTogether tokens a lane at a time.
-    const int c_lo = (int)min((int64_t)p.vocab, (int64_t)chosen * per), c_hi = (int)min((int64_t)p.vocab, (int64_t)c_lo + per);
     int some = -1;  // the last token with any weight
-    for (int base = c_lo; base < c_hi && token < 0; base += kDrawThreads * kTogether) {
-      double px[kTogether], qx[kTogether], w[kTogether], sum = 0.0;
-      bool in[kTogether];
-      int at[kTogether];
-      const int first = base + tid * kTogether;
-#pragma unroll
-      for (int e = 0; e < kTogether; e++) at[e] = first + e;
-      d.get(entry, at, c_hi, px, qx, in);
-#pragma unroll
-      for (int e = 0; e < kTogether; e++) sum += w[e] = from_p ? px[e] * ix : in[e] ? fmax(px[e] * ix - qx[e] * iy, 0.0) : 0.0;
-      // Sums up to this lane, of the warps, and up to this warp.
-      double upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const double n = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += n;
-      }
-      __syncthreads();  // (the slices of the round before have been read)
-      if (lane == 31) slice[warp] = upto;
-      __syncthreads();
-      double start = before;
-      for (int k = 0; k < warp; k++) start += slice[k];
-      for (int k = 0; k < kDrawWarps; k++) before += slice[k];
-      start += upto - sum;
-      int pick = 0x7fffffff, last = -1;
-#pragma unroll
-      for (int e = 0; e < kTogether; e++) {
-        start += w[e];
-        if (w[e] > 0.0) {
-          last = first + e;
-          if (start > want) pick = min(pick, first + e);
+    // The first turn takes the parts' weights from what the blocks have summed; the second, where p and q
+    // are close (or the first has found no token), from the tokens' own.
+    for (int turn = 0; turn < 2; turn++) {
+      if (turn) {
+        const double ix = sh.choice.ix, iy = sh.choice.iy;
+        for (int part = warp; part < parts; part += kDrawWarps) {
+          const int p_lo = (int)min((int64_t)p.vocab, (int64_t)part * per), p_hi = (int)min((int64_t)p.vocab, (int64_t)p_lo + per);
+          const double sum = sum_above(d.x, d.y, a.m, t, sh.draft.m, td, p_lo, p_hi, ix, iy);
+          if (lane == 0) weight[part] = sum;
         }
+        __syncthreads();
       }
-      if (tid == 0) {
-        sh.stop = 0x7fffffff;
-        sh.target.at = -1;
+      // The first warp goes through the parts, kOfLane a lane: the part in which the
+      // running sum first exceeds `want`, or the last one with any weight where
+      // rounding (or a number that is not below 1) leaves none.
+      if (warp == 0) {
+        double w[kOfLane], sum = 0.0, ix, iy;
+        if (turn == 0) {
+          PartSums of[kOfLane];
+          double zx = 0.0, zy = 0.0;
+#pragma unroll
+          for (int k = 0; k < kOfLane; k++) {
+            of[k] = PartSums{0.0, 0.0, 0.0, 0.0};
+            if (kOfLane * lane + k < parts) of[k] = load_sums(all + kOfLane * lane + k);
+            zx += of[k].zx;
+            zy += of[k].zy;
+          }
+          ix = 1.0 / warp_sum64(zx);
+          iy = d.y ? 1.0 / warp_sum64(zy) : 0.0;
+#pragma unroll
+          for (int k = 0; k < kOfLane; k++) sum += w[k] = fmax(of[k].px * ix - of[k].qx * iy, 0.0);
+        } else {
+          ix = sh.choice.ix;
+          iy = sh.choice.iy;
+#pragma unroll
+          for (int k = 0; k < kOfLane; k++) sum += w[k] = kOfLane * lane + k < parts ? weight[kOfLane * lane + k] : 0.0;
+        }
+        double total = warp_sum64(sum);
+        const bool close = turn == 0 && d.y && total < kClose, from_p = !close && !(total > 0.0);
+        if (from_p) {
+          sum = 0.0;
+#pragma unroll
+          for (int k = 0; k < kOfLane; k++) sum += w[k] = kOfLane * lane + k < parts ? __ldcg(&all[kOfLane * lane + k].zx) * ix : 0.0;
+          total = warp_sum64(sum);
+        }
+        const double want = (double)__ldg(p.uniform + end - 1) * total;
+        double upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const double n = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += n;
+        }
+        double run = upto - sum, before = run;  // before: of this lane's first part past `want`, or its last one
+        int over = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int k = 0; k < kOfLane; k++) {
+          if (w[k] > 0.0 && over == 0x7fffffff) {
+            last = kOfLane * lane + k;
+            before = run;
+            if (run + w[k] > want) over = last;
+          }
+          run += w[k];
+        }
+        int chosen = __reduce_min_sync(0xffffffffu, over);
+        if (chosen == 0x7fffffff) chosen = max(__reduce_max_sync(0xffffffffu, last), 0);
+        before = __shfl_sync(0xffffffffu, before, chosen / kOfLane);
+        if (lane == 0) sh.choice = Choice{ix, iy, want, before, chosen, from_p, close};
       }
       __syncthreads();
-      pick = __reduce_min_sync(0xffffffffu, pick);
-      last = __reduce_max_sync(0xffffffffu, last);
-      if (lane == 0) {
-        if (pick != 0x7fffffff) atomicMin(&sh.stop, pick);
-        atomicMax(&sh.target.at, last);
+      if (sh.choice.close) continue;
+      const double ix = sh.choice.ix, iy = sh.choice.iy, want = sh.choice.want;
+      double before = sh.choice.before;
+      const int chosen = sh.choice.part;
+      const bool from_p = sh.choice.from_p;
+      // The block goes through the part, kTogether tokens a lane at a time.
+      const int c_lo = (int)min((int64_t)p.vocab, (int64_t)chosen * per), c_hi = (int)min((int64_t)p.vocab, (int64_t)c_lo + per);
+      for (int base = c_lo; base < c_hi && token < 0; base += kDrawThreads * kTogether) {
+        double px[kTogether], qx[kTogether], w[kTogether], sum = 0.0;
+        bool in[kTogether];
+        int at[kTogether];
+        const int first = base + tid * kTogether;
+#pragma unroll
+        for (int e = 0; e < kTogether; e++) at[e] = first + e;
+        d.get(entry, at, c_hi, px, qx, in);
+#pragma unroll
+        for (int e = 0; e < kTogether; e++) sum += w[e] = from_p ? px[e] * ix : turn || in[e] ? above(px[e], ix, qx[e], iy) : 0.0;
+        // Sums up to this lane, of the warps, and up to this warp.
+        double upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const double n = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += n;
+        }
+        __syncthreads();  // (the slices of the round before have been read)
+        if (lane == 31) slice[warp] = upto;
+        __syncthreads();
+        double start = before;
+        for (int k = 0; k < warp; k++) start += slice[k];
+        for (int k = 0; k < kDrawWarps; k++) before += slice[k];
+        start += upto - sum;
+        int pick = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int e = 0; e < kTogether; e++) {
+          start += w[e];
+          if (w[e] > 0.0) {
+            last = first + e;
+            if (start > want) pick = min(pick, first + e);
+          }
+        }
+        if (tid == 0) {
+          sh.stop = 0x7fffffff;
+          sh.target.at = -1;
+        }
+        __syncthreads();
+        pick = __reduce_min_sync(0xffffffffu, pick);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0) {
+          if (pick != 0x7fffffff) atomicMin(&sh.stop, pick);
+          atomicMax(&sh.target.at, last);
+        }
+        __syncthreads();
+        if (sh.stop != 0x7fffffff) token = sh.stop;
+        some = max(some, sh.target.at);
       }
-      __syncthreads();
-      if (sh.stop != 0x7fffffff) token = sh.stop;
-      some = max(some, sh.target.at);
+      if (token >= 0 || some >= 0 || !d.y) break;
     }
     if (token < 0) token = some;
     writes = warp == 0;

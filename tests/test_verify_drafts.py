@@ -307,3 +307,30 @@ def test_two_calls_at_once(jal, torch_cuda):
     torch.cuda.synchronize()
     for d, k in zip(both, kept):
         assert (k["args"]["out_tokens"].tolist(), k["args"]["n_accepted"].tolist()) == d.wanted()[:2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1, 7, 500, 5000, 70001])
+def test_distributions_that_are_the_same(jal, torch_cuda, vocab):
+    # The draft's logits are the target's and a constant: max(p - q, 0) is 0 throughout, and behind a draft that is no
+    # token the next one is drawn from p.  (Logits are multiples of 2^-10, so that their differences are exact; sums of
+    # their exponentials in 32 bits still differ.)
+    n = 40
+    d = Drafts([2] * n, vocab, seed=51, noise=0.0)
+    d.logits = (d.logits * 1024).round() / 1024
+    shift = torch.arange(d.n)[:, None] * 0.375 - 5
+    d.draft = d.logits + shift
+    assert torch.equal((d.draft.double() - d.logits.double()), shift.double().expand_as(d.logits))
+    d.tokens[1::2] = torch.where(torch.arange(len(d.tokens[1::2])) % 2 == 0, -1, vocab).int()
+    d.check(jal)
+
+
+@pytest.mark.gpu
+def test_distributions_next_to_each_other(jal, torch_cuda):
+    # Draft's logits less their log-sum-exp, rounded: p and q are within 1e-6 of each other at every token, and what of p
+    # is above q is drawn from all the same behind a draft that is no token.
+    n, vocab = 40, 6000
+    d = Drafts([2] * n, vocab, seed=52, noise=0.0)
+    d.draft = torch.log_softmax(d.logits.double(), -1).float()
+    d.tokens[1::2] = -1
+    d.check(jal)
