@@ -393,8 +393,9 @@ int jal_op_quant_kv_append(const jal_quant_kv *kv, const jal_ragged_batch *batch
  * K[t] and V[t] what the codes stand for.  dtype (q and out): JAL_F32, JAL_F16 or
  * JAL_BF16.  Codes enter the products exactly; scales multiply scores and weights
  * in f32, and sums are f32 or exact.  Few rows: q is carried to 2^-16 of the row's
- * largest element (f32 rows: 2^-31), weights times V's scale to 2^-14 of the largest
- * of the 32 keys that are taken together (f32: 2^-30).  Many rows: q to 2^-11 (f32:
+ * largest element (f32 rows: 2^-31 of that and 2^-24 of itself), weights times V's scale
+ * to 2^-15.98 of the largest of the 32 keys that are taken together (f32: 2^-30), or to
+ * 2^-126.  Many rows: q to 2^-11 (f32:
  * 2^-22) of the element, those weights to 2^-12 (2^-22) of themselves and 2^-35 of the
  * row's largest weight times V's largest scale.  A row of q with a NaN or an
  * infinity is NaN where it sees anything, one below 2^-100 counts as 0; a row that sees

@@ -14,13 +14,15 @@
 //
 // A 16-row tile of the instruction holds eight query rows: rows i and i + 8 are the
 // upper and lower digit of row i, so one thread has both.  The weights of 32 keys
-// are numbers over the power of two below the largest of them, so their share is kept
-// however far below the row's maximum they lie, and their products are added to the
-// f32 output for each 32 keys.  An accumulator starts at 1.5 * 2^23 as f32 bits: read
+// are numbers over a 32512th of the largest of them (four digits: 2^-29 of the power of two
+// below it), so their share is kept however far below the row's maximum they lie, and their
+// products are added to the f32 output for each 32 keys.  An accumulator starts at 1.5 * 2^23 as f32 bits: read
 // as f32, it is that plus the sum, exactly.
 //
 // Errors: q is off by 2^-16 of the row's largest element (16-bit rows; f32: 2^-24 of
-// itself), a weight by 2^-15 (2^-30) of the largest of its 32 keys'.
+// itself and 2^-31 of that), a weight times V's scale by 2^-16 (2^-30) of the largest of its
+// 32 keys', or by 2^-126 where that is more.  (Over the power of two below the largest, one or
+// two bits fewer, the 64 caches above were a fifth further from the formula, in the same time.)
 //
 // A block takes R8 tiles of eight query rows of one KV head (the query heads of a
 // group, and neighbouring tokens); its four warps take 32 keys each in turn, and
@@ -76,6 +78,13 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t *w) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
   else
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+
+// 1 / x by the special-function unit: relative error 2^-23.
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // The digits of four whole numbers v, byte i of word d the digit d of number i.  NS = 1:
@@ -404,12 +413,19 @@ __global__ void __launch_bounds__(kMmaThreads, QuantShape<BITS, NS, HD, R8>::blo
       }
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // The weights over 2^(e - 13) (four digits: 2^(e - 29)), e the largest one's exponent;
-      // over 2^-126, where that is more.
-      const int e = (int)(big >> 23), shift = min(NS == 1 ? 13 : 29, e - 1);
-      const bool some = e > 0;  // (smaller than 2^-126, all: they count as 0)
-      const float over = some ? __uint_as_float((uint32_t)(254 + shift - e) << 23) : 0.0f;
-      unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - shift + (NS == 1 ? 0 : 16)) << 23) : 0.0f;
+      // The weights as whole numbers over `unit`: the largest one's 32512th; four digits: 2^-29 of the
+      // power of two below it; over 2^-126, where that is more.
+      float over;
+      if constexpr (NS == 1) {
+        const float most = __uint_as_float(max(big, 0x08000000u));  // (2^-111)
+        over = 32512.0f * rcp_fast(most);
+        unit[m] = big >= 0x7F800000u ? NAN : most * (1.0f / 32512.0f);
+      } else {
+        const int e = (int)(big >> 23), shift = min(29, e - 1);
+        const bool some = e > 0;  // (smaller than 2^-126, all: they count as 0)
+        over = some ? __uint_as_float((uint32_t)(254 + shift - e) << 23) : 0.0f;
+        unit[m] = e == 255 ? NAN : some ? __uint_as_float((uint32_t)(e - shift + 16) << 23) : 0.0f;
+      }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         uint32_t x[4], word[2 * NS];

@@ -169,3 +169,30 @@ def test_an_infinite_scale_of_k(jal, torch_cuda, act, value, softmax_scale, n):
             else:
                 near = (got[r, h] - without[0][r, h]).abs() <= bound[r, h]
                 assert bool((near | got[r, h].isnan()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("below", [12.3, 14.6, 15.4, 17.0])
+def test_weights_far_below_the_largest_of_their_keys(jal, torch_cuda, act, bits, below):
+    # 32 keys: one with nearly all of the weight and a value of 0, the others 2^-below of it with values of one sign.  A
+    # weight times V's scale is off by half of 1 / 32512 of the largest, 2^-15.98; the other terms are the case's bound's.
+    c = QuantCase([32], [1], 1, 1, 64, act=act, bits=bits, page=16)
+    q = c.q[0, 0].float()
+    codes, _ = coded(q[None], bits)
+    for t in range(32):
+        page, slot = int(c.table[0, t // 16]), t % 16
+        view = c.raw[1].permute([c.layout.index(x) for x in "phsd"])
+        high = 127 if bits == 8 else 7
+        v = torch.full((64,), 0 if t == 7 else high - t % 3, dtype=torch.int32)
+        view[page, 0, slot] = packed(v[None], bits)[0]
+        c.set_scale(1, 0, t, 1.0)
+        if t == 7:
+            c.raw[0].permute([c.layout.index(x) for x in "phsd"])[page, 0, slot] = packed(codes, bits)[0]
+        c.set_scale(0, 0, t, 0.0)
+    c.set_scale(0, 0, 7, float(below * math.log(2) / float((codes[0].double() * q.double()).sum())))
+    ref = c.reference(1.0)
+    bound = c.bound(ref) - (2.0 ** -14 - 2.0 ** -15.98) * ref[5]
+    c.to_device(jal)
+    _near(c, _attend(jal, c, 1.0), ref, bound)
