@@ -395,10 +395,9 @@ int jal_op_quant_kv_append(const jal_quant_kv *kv, const jal_ragged_batch *batch
  * in f32, and sums are f32 or exact.  Few rows: q is carried to 2^-16 of the row's
  * largest element (f32 rows: 2^-31 of that and 2^-24 of itself), weights times V's scale
  * to 2^-15.98 of the largest of the 32 keys that are taken together (f32: 2^-30), or to
- * 2^-126.  Many rows: q to 2^-11 (f32:
- * 2^-22) of the element, those weights to 2^-12 (2^-22) of themselves and 2^-35 of the
- * row's largest weight times V's largest scale.  A row of q with a NaN or an
- * infinity is NaN where it sees anything, one below 2^-100 counts as 0; a row that sees
+ * 2^-126.  Many rows: q to 2^-11 (f32: 2^-22) of the element, those weights to 2^-12
+ * (2^-22) of themselves and 2^-35 of the row's largest weight times V's largest scale
+ * (of 2^-107, where that is more).  A row of q with a NaN or an infinity is NaN where it sees anything, one below 2^-100 counts as 0; a row that sees
  * a scale that is not finite may be NaN where the formula is infinite.  Workspace as there, from
  * jal_op_quant_kv_attention_workspace. */
 int jal_op_quant_kv_attention(const jal_quant_kv *kv,
@@ -442,7 +441,7 @@ int jal_op_quant_kv_read(const jal_quant_kv *kv, const int32_t *first,
  * -1.  A draft outside the vocabulary is refused.  Where max(p - q, 0) is 0
  * throughout, the token is drawn from p.
  * Acceptance is decided from f32 sums of the exponentials, drawing from sums
- * and exponentials in 64 bits.
+ * and exponentials in 64 bits, where p that is within 2^-36 of q is not above it.
  * out_tokens (one for each row, apart from `tokens`): the accepted drafts from q_start[s]
  * on, the drawn token, then -1; rows of no sequence are left as they were.
  * n_accepted [n_seqs]: accepted drafts.  new_len (or NULL; may be batch's kv_len):

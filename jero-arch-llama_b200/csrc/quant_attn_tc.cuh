@@ -19,8 +19,8 @@
 //     error.  (One reference for both would lose the sum's earlier part as soon as E grows by
 //     more than f32's range, and costs f32 rows bits of the weights' exponents.)
 //
-// 2048 rows of 32 heads (8 KV heads of 128) behind 6144 cached 8-bit positions take 449
-// us (the same over a bf16 cache 258).  What is dearer here: three loader warps widen
+// 2048 rows of 32 heads (8 KV heads of 128) behind 6144 cached 8-bit positions take 446
+// us (the same over a bf16 cache 258; f32 rows 565).  What is dearer here: three loader warps widen
 // 128 x 128 codes a tile (without that, in a private copy, 373), and scales are
 // fetched and multiplied with each score and weight (without that too 292).  The 256 blocks are 1.73 rounds of
 // 148 SMs; cut into pieces they would have to be joined, 40 us for four.

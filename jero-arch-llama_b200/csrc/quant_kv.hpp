@@ -19,8 +19,8 @@ struct QuantScales {
 };
 
 // Launches a kernel that may start while the launch before it still runs: every block
-// begins with pdl_wait() before it looks at memory, so what is saved is the way of the
-// launch itself (about 1.5 us of a short call).
+// waits (pdl_wait()) before it looks at what that can have written, so what is saved is the
+// way of the launch itself (about 1.5 us of a short call).
 template <class F, class... A>
 void launch_beside(F kernel, int64_t blocks, int threads, int smem, cudaStream_t s, const A &...args) {
   cudaLaunchConfig_t cfg = {};

@@ -444,7 +444,9 @@ __device__ __noinline__ double sum_above(const T *x, const T *y, float m, float 
 // Bound by instructions: a token of the drawn row costs some 40, a quarter of them
 // in 64 bits.  128256 tokens of p and of q for each of 32 sequences take 19 us,
 // finding the emitting row 6 before that, finding the token 6 behind it.  The sequence's last block goes on by itself: a cluster of 16 blocks that met for it held the
-// SMs longer (64 sequences of 152064: the call 75 us, so 67).
+// SMs longer (64 sequences of 152064: the call 75 us, where it then was 67, and is 62).  A call
+// with a sequence whose p and q are nearly the same (kClose) waits for one block's way through
+// its row: 32 such sequences of 128256 tokens take 257 us where others take 55.
 template <class T>
 __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_draw(const __grid_constant__ VerifyParams p, const int blocks) {
   constexpr int most_parts = kDrawBlocks * kDrawWarps;  // of the vocabulary, one a warp
@@ -453,6 +455,8 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_draw(const __grid_co
   __shared__ double slice[kDrawWarps], weight[most_parts];
   const int parts = blocks * kDrawWarps, s = blockIdx.x / blocks, rank = blockIdx.x - s * blocks;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  // (Read ahead of the wait: the first kernel's blocks have waited for whatever wrote these before
+  // they let this one begin.  Without rows there is no first kernel, and they have no say.)
   int beg, end;
   seq_rows(p.q_start, p.n_rows, s, beg, end);
   const float t = temperature_of(p.temperature, s), td = temperature_of(p.draft_temperature, s);
