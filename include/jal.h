@@ -397,8 +397,9 @@ int jal_op_quant_kv_append(const jal_quant_kv *kv, const jal_ragged_batch *batch
  * to 2^-15.98 of the largest of the 32 keys that are taken together (f32: 2^-30), or to
  * 2^-126.  Many rows: q to 2^-11 (f32: 2^-22) of the element, those weights to 2^-12
  * (2^-22) of themselves and 2^-35 of the row's largest weight times V's largest scale
- * (of 2^-107, where that is more).  A row of q with a NaN or an infinity is NaN where it sees anything, one below 2^-100 counts as 0; a row that sees
- * a scale that is not finite may be NaN where the formula is infinite.  Workspace as there, from
+ * (of 2^-107, where that is more).  A row of q with a NaN or an infinity is NaN
+ * where it sees anything, one below 2^-100 counts as 0; a row that sees a scale that
+ * is not finite may be NaN where the formula is infinite.  Workspace as there, from
  * jal_op_quant_kv_attention_workspace. */
 int jal_op_quant_kv_attention(const jal_quant_kv *kv,
                               const jal_ragged_batch *batch, int dtype,
