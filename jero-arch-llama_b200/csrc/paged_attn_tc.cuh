@@ -502,7 +502,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_paged_attn_tc(const __grid_co
           if (c == 0) (&sy.x[0][0][0])[i * 128 + first + kr] = (1.0f / fabsf(a)) / b;
         }
         tile_sync();
-        scale *= (&sy.x[0][0][0])[i * 128 + r];
+        // (Positive, however small the row: the -inf of a masked key times 0 is NaN.  Scores below 2^37
+        // times 2^-126 are as good as 0.)
+        scale = fmaxf(scale * (&sy.x[0][0][0])[i * 128 + r], 0x1p-126f);
       }
       int lo = real ? mk.lim : 0x7fffffff, wl = real ? mk.wlo : 0x7fffffff, wh = real ? mk.wlo : 0;
       lo = __reduce_min_sync(0xffffffffu, lo);

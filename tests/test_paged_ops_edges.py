@@ -399,3 +399,20 @@ def test_one_sequence_selects_over_its_own_scores(jal, torch_cuda):
         got = [d_cum[None, :k].cpu(), parents.cpu(), tokens.cpu()]
         check_continuations(got, logits[:beams], cum[:beams], 1, beams, k)
         assert not d_cum[max(k, beams):].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [3, 30, 100, 300])
+def test_query_rows_next_to_nothing(jal, torch_cuda, cache, hd, n):
+    # f32 rows whose largest element is 2^e, down to the smallest number: scores next to 0, and the mean of the values that
+    # a row sees.  From position 0 on: there are masked keys.
+    size = [0.0, 2.0 ** -149, 2.0 ** -140, 2.0 ** -137, 2.0 ** -126, 2.0 ** -120, 2.0 ** -100, 2.0 ** -20, 1.0]
+    c = Case([n], [n], 2, 1, hd, act="f32", cache=cache, page=16, seed=n)
+    unit = (c.q / c.q.abs().amax(-1, keepdim=True)).clone()
+    for r in range(c.n_rows):
+        for h in range(2):
+            c.q[r, h] = unit[r, h] * size[(2 * r + h) % len(size)]
+    c.to_device(jal)
+    check(c, attend(jal, c, 0.125), 0.125)
